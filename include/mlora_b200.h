@@ -39,6 +39,10 @@ extern "C" {
 #define MLORA_STATUS_INDPTR 0x4u        /* seg_indptr decreasing or past the row count */
 #define MLORA_STATUS_SCATTER_RANGE 0x8u /* scatter descriptor outside its buffers */
 #define MLORA_STATUS_TIMEOUT 0x10u      /* a bounded wait for an async copy gave up */
+#define MLORA_STATUS_LENGTH 0x20u       /* a length or count is negative or past its table or buffer (clamped) */
+#define MLORA_STATUS_EXHAUSTED 0x40u    /* the free list ended before every request had its blocks */
+#define MLORA_STATUS_KV_RANGE 0x80u     /* a slot or a block-table entry outside the cache (skipped; read as zeros) */
+#define MLORA_STATUS_DRAFT_RANGE 0x100u /* a drafted token outside the vocabulary (refused) */
 
 /*
  * Segment routing of one step; mirrors KernelInputMetaData
@@ -288,6 +292,109 @@ int mlora_row_parallel_apply_p2p(const void* x, int64_t rows, int64_t in_shard, 
                                  const mlora_kernel_input_metadata_t* meta, void* y, int64_t y_row_stride,
                                  const mlora_peer_exchange_t* xchg, int32_t phase, int32_t dtype, uint32_t* status,
                                  void* stream);
+
+/*
+ * The paged serving step: block tables and slots from request lengths, the
+ * write of new keys and values, attention over the cache, and the verification
+ * of drafted tokens. The reference leaves its cache and sampling to the
+ * model library (one dense row of positions per request); these entry points
+ * have no counterpart there.
+ *
+ * Blocks, slots, positions and tokens of one step. Request i has ctx_lens[i]
+ * tokens in the cache, gets new_lens[i] more, and holds held_blocks[i] blocks
+ * (entries of its block-table row, max_blocks wide). It is granted
+ *   max(min(ceil((ctx + new) / block_size), max_blocks) - held, 0)
+ * more blocks, taken from free_blocks[*free_head ..] in request order until the
+ * list ends, and written behind the held entries of its row.
+ *   q_indptr   [requests + 1]  prefix of new_lens (usable as seg_indptr)
+ *   kv_lens    [requests]      ctx + new
+ *   held_out   [requests]      blocks held now (may be held_blocks itself)
+ *   free_head_out [1]          first free entry now (may be free_head itself)
+ *   positions, slot_map [max_tokens]  position in the request, and
+ *              block * block_size + offset; -1 for a token without a block.
+ *              Past the last token: 0 and -1.
+ *   ticket     one device word, zero before the first call; calls that share
+ *              it must not overlap on the GPU.
+ * requests <= 8192. The launch does not overlap the kernels that follow it.
+ */
+int mlora_plan_paged_step(const int32_t* ctx_lens, const int32_t* new_lens, const int32_t* held_blocks,
+                          int64_t requests, const int32_t* free_blocks, int64_t num_free, const int32_t* free_head,
+                          int32_t* block_tables, int64_t table_row_stride, int64_t max_blocks, int32_t block_size,
+                          int32_t* q_indptr, int32_t* kv_lens, int32_t* held_out, int32_t* free_head_out,
+                          int32_t* positions, int32_t* slot_map, int64_t max_tokens, uint32_t* ticket,
+                          uint32_t* status, void* stream);
+
+/*
+ * A paged cache: element d of head h of slot s of block b lies at
+ *   k + b * k_block_stride + s * k_slot_stride + h * k_head_stride + d
+ * (strides in elements, the last one 1), and the same for v.
+ */
+typedef struct mlora_paged_cache {
+  void* k;
+  void* v;
+  int64_t num_blocks;
+  int32_t block_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t dtype;
+  int64_t k_block_stride, k_slot_stride, k_head_stride;
+  int64_t v_block_stride, v_slot_stride, v_head_stride;
+} mlora_paged_cache_t;
+
+/*
+ * cache[slot_map[t]] = (k[t], v[t]) for every t < tokens with slot_map[t] >= 0.
+ * k, v: [tokens, kv_heads, head_dim] of the cache's dtype, token and head
+ * strides in elements (slices of a fused projection are read in place). No two
+ * tokens may have the same slot.
+ */
+int mlora_write_paged_kv(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                         int64_t v_token_stride, int64_t v_head_stride, int64_t tokens,
+                         const mlora_paged_cache_t* cache, const int32_t* slot_map, uint32_t* status, void* stream);
+
+/*
+ * out[t, h] = softmax(scale * q[t, h] . K^T) V over the keys that token t of
+ * request i sees: its position is pos = kv_lens[i] - (q_indptr[i+1] -
+ * q_indptr[i]) + (t - q_indptr[i]), and it sees keys j <= pos, with window > 0
+ * only j > pos - window. Query head h reads key head h / (q_heads / kv_heads).
+ * fp32 scores, sums and statistics. A query that sees no key, and rows past
+ * q_indptr[requests], give zeros.
+ *   q, out     [tokens, q_heads, head_dim] of the cache's dtype, head_dim
+ *              <= 256 and a multiple of 8; token and head strides in elements
+ *   block_tables [requests, max_blocks] (rows table_row_stride apart)
+ *   max_q_len  the longest request's new tokens, or more (host value)
+ *   workspace  mlora_paged_attention_workspace_bytes() bytes, zero before the
+ *              first call; calls that share it must not overlap on the GPU
+ */
+int mlora_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,
+                          int32_t q_heads, const mlora_paged_cache_t* cache, const int32_t* block_tables,
+                          int64_t table_row_stride, int64_t max_blocks, const int32_t* kv_lens,
+                          const int32_t* q_indptr, int64_t requests, int64_t max_q_len, float scale, int32_t window,
+                          void* out, int64_t out_token_stride, int64_t out_head_stride, void* workspace,
+                          size_t workspace_bytes, uint32_t* status, void* stream);
+size_t mlora_paged_attention_workspace_bytes(void);
+
+/*
+ * Speculative verification. Request i has n + 1 rows row_indptr[i] ..
+ * row_indptr[i+1] - 1 of target probabilities and n <= max_drafts drafts; draft
+ * j is kept while accept_u[i, j] * q_j(x_j) < p_j(x_j). One more token is
+ * drawn by inversion at sample_u[i]: from the positive part of p - q at the
+ * first refusal, from p behind n kept drafts (weights in 40-bit fixed point,
+ * so the result does not depend on the order of summation; -1 where the row
+ * has no probability).
+ *   target        [rows, vocab] of `dtype`, row stride in elements
+ *   draft         [requests, max_drafts, vocab] of `dtype`, or NULL: every
+ *                 draft counts as certain (q(x) = 1)
+ *   draft_tokens  int64 [requests, max_drafts], contiguous
+ *   accept_u, sample_u  fp32 [requests, max_drafts], [requests], in [0, 1)
+ *   tokens        int64 [requests, max_drafts + 1]: kept drafts, the drawn
+ *                 token, then -1
+ *   num_emitted   [requests]: kept drafts + 1; 0 for a request without rows
+ */
+int mlora_verify_draft(const void* target, int64_t rows, int64_t vocab, int64_t target_row_stride, const void* draft,
+                       int64_t draft_request_stride, int64_t draft_row_stride, const int64_t* draft_tokens,
+                       const int32_t* row_indptr, int64_t requests, int32_t max_drafts, const float* accept_u,
+                       const float* sample_u, int64_t* tokens, int32_t* num_emitted, int32_t dtype, uint32_t* status,
+                       void* stream);
 
 /* Programmatic dependent launch (on by default; env MLORA_PDL=0 turns it off). */
 void mlora_set_pdl(int enable);

@@ -57,6 +57,21 @@ class MetadataT(ctypes.Structure):
     ]
 
 
+class PagedCacheT(ctypes.Structure):
+    """ctypes mirror of ``mlora_paged_cache_t``."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("num_blocks", ctypes.c_int64),
+        ("block_size", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        *[(f"{side}_{name}_stride", ctypes.c_int64) for side in "kv" for name in ("block", "slot", "head")],
+    ]
+
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
@@ -86,6 +101,14 @@ CAPI_SIGNATURES = {
     "mlora_peer_buffer_destroy": (_I32, [_P]),
     "mlora_row_parallel_apply_p2p": (_I32, [_P, _I64, _I64, _I64, _P, _P, _I64, _I64, ctypes.POINTER(MetadataT), _P,
                                             _I64, _P, _I32, _I32, _P, _P]),
+    "mlora_plan_paged_step": (_I32, [_P, _P, _P, _I64, _P, _I64, _P, _P, _I64, _I64, _I32, _P, _P, _P, _P, _P, _P, _I64,
+                                     _P, _P, _P]),
+    "mlora_write_paged_kv": (_I32, [_P, _I64, _I64, _P, _I64, _I64, _I64, ctypes.POINTER(PagedCacheT), _P, _P, _P]),
+    "mlora_paged_attention": (_I32, [_P, _I64, _I64, _I64, _I32, ctypes.POINTER(PagedCacheT), _P, _I64, _I64, _P, _P,
+                                     _I64, _I64, ctypes.c_float, _I32, _P, _I64, _I64, _P, ctypes.c_size_t, _P, _P]),
+    "mlora_paged_attention_workspace_bytes": (ctypes.c_size_t, []),
+    "mlora_verify_draft": (_I32, [_P, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I32, _P, _P, _P, _P, _I32, _P,
+                                  _P]),
     "mlora_set_pdl": (None, [ctypes.c_int]),
     "mlora_get_pdl": (ctypes.c_int, []),
     "mlora_last_error": (ctypes.c_char_p, []),

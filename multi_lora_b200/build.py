@@ -3,7 +3,7 @@
 * ``libmlora_b200.so`` — every CUDA kernel plus the C ABI of
   ``include/mlora_b200.h``; compiled by nvcc for sm_100a only, static cudart,
   no torch dependency.
-* ``_mlora_torch.so`` — the ``torch.ops.mlora`` binding (torch_ops.cpp),
+* ``_mlora_torch.so`` — the ``torch.ops.mlora`` binding (torch_ops*.cpp),
   linked against ``libmlora_b200.so`` through an ``$ORIGIN`` rpath.
 
 Both land next to this file so that they travel with the source tree. A
@@ -91,8 +91,8 @@ def build_cuda_lib(force: bool = False, verbose: bool = False) -> Path:
 
 
 def build_torch_lib(force: bool = False, verbose: bool = False) -> Path:
-    src = CSRC / "torch_ops.cpp"
-    if not force and not _stale(TORCH_LIB, [src, CUDA_LIB, ROOT / "include" / "mlora_b200.h"]):
+    srcs = sorted(CSRC.glob("torch_ops*.cpp"))
+    if not force and not _stale(TORCH_LIB, [*srcs, CUDA_LIB, ROOT / "include" / "mlora_b200.h"]):
         return TORCH_LIB
     import torch
     import torch.utils.cpp_extension as ext
@@ -100,10 +100,17 @@ def build_torch_lib(force: bool = False, verbose: bool = False) -> Path:
     incs = ext.include_paths("cuda")
     libs = ext.library_paths("cuda")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    OBJ.mkdir(exist_ok=True)
+    cxx = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+           "-DTORCH_API_INCLUDE_EXTENSION_H", *[f"-I{p}" for p in incs]]
+    objs = [OBJ / (src.stem + ".o") for src in srcs]
+    jobs = [[*cxx, "-c", str(src), "-o", str(obj)] for src, obj in zip(srcs, objs)
+            if force or _stale(obj, [src, ROOT / "include" / "mlora_b200.h"])]
+    with cf.ThreadPoolExecutor(max_workers=max(1, len(jobs))) as ex:
+        for done in [ex.submit(_run, c) for c in jobs]:
+            done.result()
     cmd = [
-        os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
-        f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_API_INCLUDE_EXTENSION_H",
-        *[f"-I{p}" for p in incs], str(src), "-o", str(TORCH_LIB.with_suffix(".so.tmp")),
+        os.environ.get("CXX", "g++"), "-shared", *map(str, objs), "-o", str(TORCH_LIB.with_suffix(".so.tmp")),
         *[f"-L{p}" for p in libs], f"-L{PKG}",
         "-lmlora_b200", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
         "-Wl,-rpath,$ORIGIN",
