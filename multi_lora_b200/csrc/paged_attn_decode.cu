@@ -1,0 +1,463 @@
+// Attention over the paged cache for few query rows: decode steps and drafts.
+//
+// The G = q_heads / kv_heads query heads of a key head and the request's new
+// tokens form one block of rows (row r: token r / G, head r % G; at most 64),
+// so K and V are read once for all of them. What bounds it is that read: with
+// R rows there are R operations a byte, far under what the tensor cores
+// need to be the limit. Everything else serves keeping loads in flight:
+//   * a producer warp fetches tiles of 64 keys by TMA, one box of a page
+//     (gcd(block size, 64) rows of 64 columns) a lane, through a ring of
+//     stages of K and V; a box behind the keys is a coordinate out of range,
+//     which reads zeros and no memory;
+//   * consumer warps take 16 rows and 16 or 32 of the 64 keys each on mma.sync
+//     tiles and keep their own running maximum, sum and 16 x D output sums over
+//     the whole item, with no exchange between warps until its end; scores and sums are fp32, the probabilities are rounded to
+//     the cache's type for the second product (their fp32 values make the sum);
+//   * key tiles are dealt evenly over the CTAs (paged_sched.cuh).
+// Keys outside [first, kv) may hold anything: scores are replaced, not added
+// to, and their V fragments are cleared before the product, since 0 * NaN is NaN.
+#include <mutex>
+
+#include "kernels.h"
+#include "mma.cuh"
+#include "paged_sched.cuh"
+#include "paged_tma.h"
+#include "tc.cuh"
+
+namespace mlora {
+
+constexpr int kDecTile = 64;  // keys a stage
+
+struct DecodeArgs {
+  CUtensorMap k_map, v_map;
+  PagedAttnArgs a;
+  int box;     // rows of a TMA box
+};
+
+template <int D, int MT>
+struct DecodeCfg {
+  static constexpr int KG = MT == 4 ? 2 : 4;      // key groups: warps that share 16 rows
+  static constexpr int kSub = kDecTile / 16 / KG; // groups of 16 keys that a warp takes of a tile
+  static constexpr int kWarps = KG * MT;
+  static constexpr int kThreads = kWarps * 32 + 32;
+  static constexpr int kPerSm = MT == 1 ? 2 : 1;
+  static constexpr int kSide = kDecTile * D * 2;  // bytes of K (or V) in a stage
+  static constexpr int kStages = (MT == 1 ? 96 : 160) * 1024 / (2 * kSide);
+  static constexpr int kRowF = D + 4;             // floats of a row in the merge buffer
+  static constexpr int kMerge = MT * 16 * kRowF * 4;
+  static constexpr int kSmem = kStages * 2 * kSide + kMerge + 1024;
+};
+
+// One item's description, the same in every warp.
+struct DecodeItem {
+  int req, head, q0, qn, kv, first, tile0, n;
+};
+
+template <int MT>
+__device__ __forceinline__ void decode_load(const PagedAttnArgs& p, DecodeItem& it, int req, int group) {
+  const PagedRequest r = paged_request(p, req, false);
+  it.req = req;
+  it.q0 = r.q0;
+  it.qn = r.qn;
+  it.kv = r.kv;
+  it.first = paged_first_key(p, r.kv - r.qn);
+  it.tile0 = it.first / kDecTile;
+  it.n = r.qn > 0 && r.qn <= 16 * MT / group ? max(1, (r.kv + kDecTile - 1) / kDecTile - it.tile0) : 0;
+}
+
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(DecodeCfg<D, MT>::kThreads, DecodeCfg<D, MT>::kPerSm)
+paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
+  using C = DecodeCfg<D, MT>;
+  constexpr bool kTwoTerms = Num<T>::is_bf16;
+  constexpr int NS = C::kStages, SIDE = C::kSide, HALF = kDecTile * 128;
+  extern __shared__ __align__(1024) unsigned char s_raw[];
+  __shared__ __align__(8) uint64_t full[NS], empty[NS];
+  __shared__ float s_m[C::kWarps][16], s_l[C::kWarps][16];
+  __shared__ int s_last;
+  const PagedAttnArgs& p = args.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~uintptr_t(1023));
+  float* merge = reinterpret_cast<float*>(smem + NS * 2 * SIDE);
+  const int group = p.q_heads / p.kv_heads;
+
+  if (tid == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], C::kWarps);
+    }
+    fence_barrier_init();
+  }
+  if (warp == C::kWarps && lane == 0) {
+    tma_prefetch_map(&args.k_map);
+    tma_prefetch_map(&args.v_map);
+  }
+  pdl_wait();
+  pdl_trigger();
+
+  PagedSplit split;
+  DecodeItem it;
+  long long before;
+  int req;
+  paged_find<C::kThreads>(
+      p.requests,
+      [&](int i) {
+        const PagedRequest r = paged_request(p, i, blockIdx.x == 0);
+        // rows beyond what the caller said: reported, and not computed
+        if (blockIdx.x == 0 && r.qn > p.max_q_len) flag_error(p.status, kErrLength);
+        if (r.qn == 0 || r.qn > 16 * MT / group) return 0ll;
+        const int t0 = paged_first_key(p, r.kv - r.qn) / kDecTile;
+        return (long long)max(1, (r.kv + kDecTile - 1) / kDecTile - t0) * p.kv_heads;
+      },
+      split, req, before);
+  paged_zero_rest<T>(p);
+  long long pos = split.start(blockIdx.x);
+  const long long end = split.start(blockIdx.x + 1);
+  if (pos >= end) return;
+  decode_load<MT>(p, it, req, group);
+  int tile = (int)((pos - before) % it.n);
+  it.head = (int)((pos - before) / it.n);
+  auto next_item = [&]() {
+    tile = 0;
+    if (++it.head == p.kv_heads) {
+      it.head = 0;
+      for (int i = it.req + 1; i < p.requests; ++i) {
+        decode_load<MT>(p, it, i, group);
+        if (it.n > 0) break;
+      }
+    }
+  };
+  bool ok = true;
+
+  if (warp == C::kWarps) {  // ---- producer ----
+    const int boxes = kDecTile / args.box, jobs = boxes * (D / 64) * 2;
+    const int b = lane % boxes, half = (lane / boxes) % (D / 64), side = lane / (boxes * (D / 64));
+    int stage = 0, round = 0;
+    while (pos < end) {
+      const int len = (int)min((long long)(it.n - tile), end - pos);
+      const int32_t* table = p.tables + it.req * p.table_stride;
+      for (int k = 0; k < len; ++k) {
+        const int j = (it.tile0 + tile + k) * kDecTile + b * args.box;
+        int block = (int)p.num_blocks, off = 0;  // out of range: zeros
+        if (lane < jobs && j < it.kv && j + args.box > it.first) {
+          const int e = __ldcg(table + j / p.block_size);
+          off = j % p.block_size;
+          if (e >= 0 && e < p.num_blocks) block = e;
+          else flag_error(p.status, kErrKvRange);
+        }
+        if (round > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait(&empty[stage], (round - 1) & 1, p.status));
+        if (ok) {
+          if (lane == 0) mbar_arrive_expect_tx(&full[stage], 2 * SIDE);
+          __syncwarp();
+          if (lane < jobs)
+            tma_load_4d(smem + stage * 2 * SIDE + side * SIDE + half * HALF + b * args.box * 128,
+                        side == 0 ? &args.k_map : &args.v_map, half * 64, off, it.head, block, &full[stage]);
+        }
+        if (++stage == NS) {
+          stage = 0;
+          ++round;
+        }
+      }
+      pos += len;
+      if (pos < end) next_item();
+    }
+    return;
+  }
+
+  // ---- consumers: warp = (16 rows mt, 16 keys of each tile kg) ----
+  const int mt = warp / C::KG, kg = warp % C::KG;
+  const float sl = p.scale * 1.4426950408889634f;  // scores in powers of two
+  int stage = 0, phase = 0;
+  uint32_t* tickets = static_cast<uint32_t*>(p.workspace);
+  float* parts = reinterpret_cast<float*>(tickets + kPagedTickets);
+  constexpr int PART = MT * 16 * (D + 2);  // floats of a piece: sums, maxima, totals
+  while (pos < end) {
+    const int len = (int)min((long long)(it.n - tile), end - pos);
+    const int rows = it.qn * group;
+    // Q fragments: rows lane / 4 and + 8, columns (lane % 4) * 2 (+ 8) of each 16
+    uint32_t qf[D / 16][4];
+    int limit[2], floor_[2];  // keys below `limit` and at or above `floor_` are seen
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = mt * 16 + (lane >> 2) + e * 8;
+      const int t = r / group;
+      const int pq = it.kv - it.qn + t;
+      limit[e] = r < rows ? pq + 1 : 0;
+      floor_[e] = paged_first_key(p, pq);
+      const T* src = static_cast<const T*>(p.q) + (it.q0 + t) * p.q_token +
+                     (it.head * group + r - t * group) * p.q_head + (lane & 3) * 2;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        qf[k][e] = r < rows ? __ldcg(reinterpret_cast<const unsigned int*>(src + k * 16)) : 0u;
+        qf[k][2 + e] = r < rows ? __ldcg(reinterpret_cast<const unsigned int*>(src + k * 16 + 8)) : 0u;
+      }
+    }
+    float o[D / 8][4];
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    for (int k = 0; k < len; ++k) {
+      ok = ok && mbar_wait(&full[stage], phase, p.status);
+      __syncwarp();
+#pragma unroll
+      for (int sub = 0; sub < C::kSub; ++sub) {
+        const int k0 = (kg * C::kSub + sub) * 16, j0 = (it.tile0 + tile + k) * kDecTile + k0;  // 16 keys
+        if (mt * 16 < rows && j0 < it.kv && j0 + 16 > it.first) {
+          const uint32_t ks = smem_addr(smem + stage * 2 * SIDE), vs = ks + SIDE;
+          float s[2][4];
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+            const int key = k0 + n * 8 + (lane & 7);
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {  // 32 columns: two k steps
+              const int chunk = c * 4 + (lane >> 3);
+              uint32_t b0, b1, b2, b3;
+              ldsm_x4(ks + (chunk >> 3) * HALF + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), b0, b1, b2, b3);
+              mma_16816<T>(s[n], qf[2 * c][0], qf[2 * c][1], qf[2 * c][2], qf[2 * c][3], b0, b1);
+              mma_16816<T>(s[n], qf[2 * c + 1][0], qf[2 * c + 1][1], qf[2 * c + 1][2], qf[2 * c + 1][3], b2, b3);
+            }
+          }
+          const bool edge = j0 + 16 > it.kv - it.qn + 1 || j0 < paged_first_key(p, it.kv - 1);  // not all seen by all rows
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              s[n][e] *= sl;
+              if (edge) {
+                const int j = j0 + n * 8 + (lane & 3) * 2 + (e & 1);
+                if (j >= limit[e >> 1] || j < floor_[e >> 1]) s[n][e] = -INFINITY;
+              }
+            }
+          uint32_t pf[4], pr[4];
+          float fix[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float m_new = fmaxf(m[e], top), ref = m_new == -INFINITY ? 0.f : m_new;
+            fix[e] = exp2_fast(m[e] - ref);
+            m[e] = m_new;
+            const float p0 = exp2_fast(s[0][2 * e] - ref), p1 = exp2_fast(s[0][2 * e + 1] - ref);
+            const float p2 = exp2_fast(s[1][2 * e] - ref), p3 = exp2_fast(s[1][2 * e + 1] - ref);
+            l[e] = l[e] * fix[e] + ((p0 + p1) + (p2 + p3));
+            pf[e] = pack_round2<T>(p0, p1);
+            pf[2 + e] = pack_round2<T>(p2, p3);
+            if constexpr (kTwoTerms) {
+              pr[e] = pack_round2<T>(p0 - Pack2<T>::lo(pf[e]), p1 - Pack2<T>::hi(pf[e]));
+              pr[2 + e] = pack_round2<T>(p2 - Pack2<T>::lo(pf[2 + e]), p3 - Pack2<T>::hi(pf[2 + e]));
+            }
+          }
+          if (__any_sync(0xffffffffu, fix[0] != 1.f || fix[1] != 1.f)) {
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) {
+              o[n][0] *= fix[0];
+              o[n][1] *= fix[0];
+              o[n][2] *= fix[1];
+              o[n][3] *= fix[1];
+            }
+          }
+          // V: keys of this thread's fragments are (lane % 4) * 2 + {0, 1} and + 8
+          uint32_t clear0 = 0xffffffffu, clear1 = 0xffffffffu;
+          const bool partial = j0 + 16 > it.kv || j0 < it.first;
+          if (partial) {
+            const int j = j0 + (lane & 3) * 2;
+            auto keep = [&](int x) { return x < it.kv && x >= it.first; };
+            clear0 = (keep(j) ? 0xffffu : 0u) | (keep(j + 1) ? 0xffff0000u : 0u);
+            clear1 = (keep(j + 8) ? 0xffffu : 0u) | (keep(j + 9) ? 0xffff0000u : 0u);
+          }
+          const int key = k0 + (lane & 15);
+#pragma unroll
+          for (int n = 0; n < D / 16; ++n) {  // 16 columns of V
+            const int chunk = n * 2 + (lane >> 4);
+            uint32_t b0, b1, b2, b3;
+            ldsm_x4_trans(vs + (chunk >> 3) * HALF + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), b0, b1, b2, b3);
+            if (partial) {
+              b0 &= clear0;
+              b1 &= clear1;
+              b2 &= clear0;
+              b3 &= clear1;
+            }
+            mma_16816<T>(o[2 * n], pf[0], pf[1], pf[2], pf[3], b0, b1);
+            mma_16816<T>(o[2 * n + 1], pf[0], pf[1], pf[2], pf[3], b2, b3);
+            if constexpr (kTwoTerms) {
+              mma_16816<T>(o[2 * n], pr[0], pr[1], pr[2], pr[3], b0, b1);
+              mma_16816<T>(o[2 * n + 1], pr[0], pr[1], pr[2], pr[3], b2, b3);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[stage]);
+      if (++stage == NS) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+
+    // ---- join the key groups of each 16 rows ----
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+      if ((lane & 3) == 0) {
+        s_m[warp][(lane >> 2) + e * 8] = m[e];
+        s_l[warp][(lane >> 2) + e * 8] = l[e];
+      }
+    }
+    named_barrier(1, C::kWarps * 32);
+    float scale_own[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = (lane >> 2) + e * 8;
+      float top = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < C::KG; ++g) top = fmaxf(top, s_m[mt * C::KG + g][r]);
+      scale_own[e] = top == -INFINITY ? 0.f : exp2_fast(m[e] - top);
+    }
+    for (int g = 0; g < C::KG; ++g) {
+      if (kg == g) {
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float2* d = reinterpret_cast<float2*>(merge + (mt * 16 + (lane >> 2) + e * 8) * C::kRowF + n * 8 + (lane & 3) * 2);
+            float2 v = make_float2(o[n][2 * e] * scale_own[e], o[n][2 * e + 1] * scale_own[e]);
+            if (g > 0) {
+              const float2 u = *d;
+              v.x += u.x;
+              v.y += u.y;
+            }
+            *d = v;
+          }
+      }
+      named_barrier(1, C::kWarps * 32);
+    }
+    const bool begins = tile == 0, ends = tile + len == it.n, whole = begins && ends;
+    auto row_stat = [&](int r, float& top, float& sum) {  // over the key groups of row r
+      const int w = (r >> 4) * C::KG, i = r & 15;
+      top = s_m[w][i];
+#pragma unroll
+      for (int g = 1; g < C::KG; ++g) top = fmaxf(top, s_m[w + g][i]);
+      sum = 0.f;
+#pragma unroll
+      for (int g = 0; g < C::KG; ++g) sum += top == -INFINITY ? 0.f : s_l[w + g][i] * exp2_fast(s_m[w + g][i] - top);
+    };
+    auto store = [&](int r, int c, const float* v, float inv) {  // 8 columns of row r
+      const int t = r / group;
+      T* dst = static_cast<T*>(p.out) + (it.q0 + t) * p.out_token + (it.head * group + r - t * group) * p.out_head + c;
+      uint4 u;
+      u.x = pack_round2<T>(v[0] * inv, v[1] * inv);
+      u.y = pack_round2<T>(v[2] * inv, v[3] * inv);
+      u.z = pack_round2<T>(v[4] * inv, v[5] * inv);
+      u.w = pack_round2<T>(v[6] * inv, v[7] * inv);
+      *reinterpret_cast<uint4*>(dst) = u;
+    };
+    float* part = parts + ((long long)blockIdx.x * 2 + (begins ? 1 : 0)) * PART;
+    for (int e = tid; e < rows * (D / 8); e += C::kWarps * 32) {
+      const int r = e / (D / 8), c = (e % (D / 8)) * 8;
+      float top, sum;
+      row_stat(r, top, sum);
+      const float4 v0 = *reinterpret_cast<const float4*>(merge + r * C::kRowF + c);
+      const float4 v1 = *reinterpret_cast<const float4*>(merge + r * C::kRowF + c + 4);
+      if (whole) {
+        const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+        store(r, c, v, sum > 0.f || sum != sum ? 1.f / sum : 0.f);
+      } else {
+        __stcg(reinterpret_cast<float4*>(part + r * D + c), v0);
+        __stcg(reinterpret_cast<float4*>(part + r * D + c + 4), v1);
+        if (c == 0) {
+          __stcg(part + MT * 16 * D + r, top);
+          __stcg(part + MT * 16 * (D + 1) + r, sum);
+        }
+      }
+    }
+    if (!whole) {
+      const long long item0 = pos - tile;
+      const int c0 = split.owner(item0), c1 = split.owner(item0 + it.n - 1);
+      __threadfence();
+      named_barrier(1, C::kWarps * 32);
+      if (tid == 0) {
+        const bool last = atomicAdd(tickets + c0, 1u) == (uint32_t)(c1 - c0);
+        if (last) tickets[c0] = 0u;
+        __threadfence();
+        s_last = last;
+      }
+      named_barrier(1, C::kWarps * 32);
+      if (s_last) {
+        auto piece = [&](int c) { return parts + ((long long)c * 2 + (c == c0 ? 1 : 0)) * PART; };
+        for (int e = tid; e < rows * (D / 8); e += C::kWarps * 32) {
+          const int r = e / (D / 8), c = (e % (D / 8)) * 8;
+          float top = -INFINITY, sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          for (int x = c0; x <= c1; ++x) top = fmaxf(top, __ldcg(piece(x) + MT * 16 * D + r));
+          if (top != -INFINITY) {
+#pragma unroll 4
+            for (int x = c0; x <= c1; ++x) {
+              const float* src = piece(x);
+              const float w = exp2_fast(__ldcg(src + MT * 16 * D + r) - top);
+              sum = fmaf(__ldcg(src + MT * 16 * (D + 1) + r), w, sum);
+              const float4 v0 = __ldcg(reinterpret_cast<const float4*>(src + r * D + c));
+              const float4 v1 = __ldcg(reinterpret_cast<const float4*>(src + r * D + c + 4));
+              v[0] = fmaf(v0.x, w, v[0]);
+              v[1] = fmaf(v0.y, w, v[1]);
+              v[2] = fmaf(v0.z, w, v[2]);
+              v[3] = fmaf(v0.w, w, v[3]);
+              v[4] = fmaf(v1.x, w, v[4]);
+              v[5] = fmaf(v1.y, w, v[5]);
+              v[6] = fmaf(v1.z, w, v[6]);
+              v[7] = fmaf(v1.w, w, v[7]);
+            }
+          }
+          store(r, c, v, sum > 0.f || sum != sum ? 1.f / sum : 0.f);
+        }
+      }
+    }
+    named_barrier(1, C::kWarps * 32);  // the merge buffer and s_last are free again
+    pos += len;
+    if (pos < end) next_item();
+  }
+}
+
+namespace {
+
+template <typename T, int D, int MT>
+cudaError_t launch_decode(const DecodeArgs& a, cudaStream_t st, bool pdl) {
+  using C = DecodeCfg<D, MT>;
+  auto kern = paged_attention_decode_kernel<T, D, MT>;
+  static const cudaError_t attr =
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  if (attr != cudaSuccess) return attr;
+  const int ctas = paged_sm_count() * C::kPerSm;
+  static_assert(C::kSmem <= 227 * 1024, "shared memory");
+  if (ctas > kPagedTickets ||
+      (size_t)ctas * 2 * MT * 16 * (D + 2) * 4 + kPagedTickets * 4 > kPagedWorkspaceBytes)
+    return cudaErrorNotSupported;
+  return launch_kernel(kern, dim3(ctas), dim3(C::kThreads), C::kSmem, st, pdl, a);
+}
+
+template <typename T, int D>
+cudaError_t launch_decode_m(const DecodeArgs& a, int rows, cudaStream_t st, bool pdl) {
+  if (rows <= 16) return launch_decode<T, D, 1>(a, st, pdl);
+  if (rows <= 32) return launch_decode<T, D, 2>(a, st, pdl);
+  return launch_decode<T, D, 4>(a, st, pdl);
+}
+
+}  // namespace
+
+cudaError_t launch_paged_attention_decode(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl) {
+  if ((dtype != kBF16 && dtype != kF16) || (a.dim != 64 && a.dim != 128)) return cudaErrorNotSupported;
+  DecodeArgs d{};
+  d.a = a;
+  d.box = paged_box(a.block_size, kDecTile);
+  if (d.box < 8 || !paged_maps(a, dtype, d.box, &d.k_map, &d.v_map)) return cudaErrorNotSupported;
+  const long long all = (long long)a.max_q_len * (a.q_heads / a.kv_heads);
+  const int rows = all > kDecodeMaxRows ? kDecodeMaxRows : (int)all;
+  if (dtype == kBF16)
+    return a.dim == 64 ? launch_decode_m<__nv_bfloat16, 64>(d, rows, st, pdl)
+                       : launch_decode_m<__nv_bfloat16, 128>(d, rows, st, pdl);
+  return a.dim == 64 ? launch_decode_m<__half, 64>(d, rows, st, pdl) : launch_decode_m<__half, 128>(d, rows, st, pdl);
+}
+
+}  // namespace mlora

@@ -203,9 +203,13 @@ int mlora_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
   const bool vec = pieces(q, es, q_token_stride, q_head_stride) && pieces(out, es, out_token_stride, out_head_stride) &&
                    pieces(c.k, es, c.k_block_stride, c.k_slot_stride, c.k_head_stride) &&
                    pieces(c.v, es, c.v_block_stride, c.v_slot_stride, c.v_head_stride);
-  return launched(
-      mlora::launch_paged_attention_general(a, c.dtype, vec, (cudaStream_t)stream, mlora_get_pdl() != 0),
-      "paged attention launch");
+  const bool pdl = mlora_get_pdl() != 0;
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (vec && es == 2 && max_q_len * (q_heads / c.kv_heads) <= mlora::kDecodeMaxRows) {
+    const cudaError_t e = mlora::launch_paged_attention_decode(a, c.dtype, st, pdl);
+    if (e != cudaErrorNotSupported) return launched(e, "paged attention launch");
+  }
+  return launched(mlora::launch_paged_attention_general(a, c.dtype, vec, st, pdl), "paged attention launch");
 }
 
 int mlora_verify_draft(const void* target, int64_t rows, int64_t vocab, int64_t target_row_stride, const void* draft,

@@ -1,0 +1,127 @@
+// What the paged attention kernels share: a request's lengths with their
+// checks, the split of all key tiles over the CTAs, and the tensor maps' limits.
+//
+// The work of a launch is a sequence of items (request, key head, and for long
+// chunks a tile of query rows), each a run of key tiles. CTA c of G takes the
+// c-th G-th of all tiles, wherever item boundaries fall: every CTA reads the
+// same number of keys whatever the lengths are, and a single long request spreads over the
+// whole GPU. An item inside one CTA is finished there; of an item that
+// several CTAs share each writes its unnormalised sums, maximum and total to
+// the workspace, and the CTA that counts itself last joins them in CTA order
+// (the same order, so the same bits, every time). A CTA has at most two such
+// pieces: the rest of an item that an earlier CTA began (slot 0), and the
+// beginning of one that a later CTA ends (slot 1).
+#pragma once
+
+#include "common.cuh"
+#include "paged.h"
+
+namespace mlora {
+
+struct PagedRequest {
+  int q0, qn, kv;  // first row, rows, keys
+};
+
+__device__ __forceinline__ PagedRequest paged_request(const PagedAttnArgs& p, int i, bool report) {
+  PagedRequest r;
+  r.q0 = __ldcg(p.q_indptr + i);
+  const int q1 = __ldcg(p.q_indptr + i + 1);
+  r.kv = __ldcg(p.kv_lens + i);
+  r.qn = q1 - r.q0;
+  if (r.q0 < 0 || q1 < r.q0 || q1 > p.tokens) {
+    if (report) flag_error(p.status, kErrIndptr);
+    r.q0 = r.qn = 0;
+  }
+  const long long cap = (long long)p.width * p.block_size;
+  if (r.kv < 0 || r.kv > cap) {
+    if (report) flag_error(p.status, kErrLength);
+    r.kv = r.kv < 0 ? 0 : (int)cap;
+  }
+  return r;
+}
+
+// First key that query row `pos` of a request sees.
+__device__ __forceinline__ int paged_first_key(const PagedAttnArgs& p, int pos) {
+  return p.window > 0 ? max(0, pos - p.window + 1) : 0;
+}
+
+struct PagedSplit {
+  long long total, base, rem;  // CTA c has base tiles, the first `rem` CTAs one more
+  __device__ void set(long long tiles, int ctas) {
+    total = tiles;
+    base = tiles / ctas;
+    rem = tiles - base * ctas;
+  }
+  __device__ long long start(long long c) const { return c * base + min(c, rem); }
+  __device__ int owner(long long tile) const {
+    const long long wide = rem * (base + 1);
+    return (int)(tile < wide ? tile / (base + 1) : rem + (tile - wide) / base);
+  }
+};
+
+// Whole block of NT threads: the split over the grid, the request that this CTA's first
+// tile lies in, and the tiles before that request. `tiles(i)`: tiles of request i.
+template <int NT, typename F>
+__device__ __forceinline__ void paged_find(int requests, F tiles, PagedSplit& split, int& req, long long& before) {
+  __shared__ long long s_warp[NT / 32];
+  __shared__ long long s_before;
+  __shared__ int s_req;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (requests + NT - 1) / NT;
+  const int r0 = min(requests, tid * per), r1 = min(requests, r0 + per);
+  long long mine = 0;
+  for (int i = r0; i < r1; ++i) mine += tiles(i);
+  long long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += u;
+  }
+  if (lane == 31) s_warp[warp] = incl;
+  if (tid == 0) s_req = requests;
+  __syncthreads();
+  long long total = 0, upto = incl - mine;
+#pragma unroll
+  for (int w = 0; w < NT / 32; ++w) {
+    const long long u = s_warp[w];
+    upto += w < warp ? u : 0;
+    total += u;
+  }
+  split.set(total, gridDim.x);
+  const long long a = split.start(blockIdx.x);
+  if (a >= upto && a < upto + mine) {
+    int i = r0;
+    for (long long n = tiles(i); a >= upto + n; n = tiles(++i)) upto += n;
+    s_req = i;
+    s_before = upto;
+  }
+  __syncthreads();
+  req = s_req;
+  before = s_before;
+}
+
+// Rows behind the last request's give zeros; all CTAs share them.
+template <typename T>
+__device__ __forceinline__ void paged_zero_rest(const PagedAttnArgs& p) {
+  const int last = p.requests > 0 ? __ldcg(p.q_indptr + p.requests) : 0;
+  if (last < 0 || last >= p.tokens) return;
+  const int64_t pieces = p.dim / 8, n = (int64_t)(p.tokens - last) * p.q_heads * pieces;
+  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < n; e += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t row = e / pieces;
+    T* o = static_cast<T*>(p.out) + (last + row / p.q_heads) * p.out_token + (row % p.q_heads) * p.out_head +
+           (e % pieces) * 8;
+    *reinterpret_cast<uint4*>(o) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// 2^x on the special function unit; 0 for -infinity.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+constexpr int kPagedTickets = 1024;  // words at the start of the workspace, zero between calls
+constexpr size_t kPagedWorkspaceBytes = (size_t)64 << 20;
+
+}  // namespace mlora

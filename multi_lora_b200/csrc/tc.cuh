@@ -27,6 +27,17 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
+// 4-D tiled load (coordinates innermost first, c0 aligned as for tma_load_2d; a
+// coordinate past its dimension reads zeros).
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_addr(bar))
+      : "memory");
+}
+
 // 2-D tiled store of a shared-memory box to global (coordinates as for
 // tma_load_2d; c0 * element size a multiple of 16 bytes, c0, c1 >= 0). Part
 // of the bulk group that bulk_commit() closes.
