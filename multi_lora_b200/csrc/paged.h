@@ -69,10 +69,12 @@ struct PagedAttnArgs {
 cudaError_t launch_paged_attention_general(const PagedAttnArgs& a, int dtype, bool vec, cudaStream_t st, bool pdl);
 
 // 16-bit caches with head_dim 64 or 128, block size a multiple of 8, 16-byte pieces
-// everywhere. `decode`: requests with q_len * (q_heads / kv_heads) <= 64 rows; every
-// other request is left alone. cudaErrorNotSupported: the shape is not one of these.
+// everywhere. Decode: up to kDecodeMaxRows rows (max_q_len * q_heads / kv_heads);
+// chunk: any number. cudaErrorNotSupported: the shape is not one of these.
 cudaError_t launch_paged_attention_decode(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl);
 constexpr int kDecodeMaxRows = 64;
+
+cudaError_t launch_paged_attention_chunk(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl);
 
 struct VerifyArgs {
   const void* target;         // [rows, vocab]

@@ -1,0 +1,645 @@
+// Attention over the paged cache for chunks of new tokens, on the fifth-
+// generation tensor cores.
+//
+// The rows of a (request, key head) are its new tokens times the G query heads
+// of the key head (row r: token r / G, head r % G), so that one pass over K and
+// V serves the whole group. A CTA takes 256 of them, as two tiles of 128, over
+// a run of 128-key tiles (the even split of paged_sched.cuh):
+//   S = Q K^T   (tcgen05.mma, both operands from shared memory, S in TMEM)
+//   P = exp2(scale' S - m)  by one warpgroup a tile, a thread a row: a row's
+//               128 scores in registers, P written over S in TMEM
+//   O += P V    (tcgen05.mma, P from TMEM, V from shared memory as it lies, with
+//               the columns as the contiguous dimension; O in TMEM, 2 x 128 fp32 columns)
+// The two tiles run half a period apart: while one warpgroup works on its
+// scores, the tensor cores do the other tile's products. S and P share their TMEM
+// columns (2 x 128 for S/P and 2 x D for O fill the 512), so the scores of the
+// next key tile wait for the product that reads P.
+//
+// The running maximum that P is taken against is raised only when a row's
+// scores exceed it by 2^8 (O is rescaled in TMEM then, rarely after the first
+// tiles); P stays below 2^8 and everything is normalised at the end by the sum of P
+// in fp32. An f16 P is rounded once (11 bits). A bf16 P goes in as two terms,
+// its rounding and the rounding's remainder (16 bits): one term of 8 bits would add as much
+// error as the result's own rounding. The second term is one more product of the same size.
+//
+// What bounds it: the exponentials (16 a cycle and SM: 2048 cycles for two
+// 128 x 128 tiles) and the tensor cores (4096 multiply-adds a cycle: 2048
+// cycles for f16, 3072 for bf16 with its second term, at D = 128).
+//
+// Keys behind the cache's end may hold anything: their scores are replaced,
+// and their rows of V are cleared in shared memory, since 0 * NaN is NaN.
+#include "kernels.h"
+#include "paged_sched.cuh"
+#include "paged_tma.h"
+#include "tc.cuh"
+
+namespace mlora {
+
+constexpr int kChunkKeys = 128;   // keys a tile
+constexpr int kChunkRows = 256;   // query rows an item: two tiles of 128
+constexpr int kChunkThreads = 384;
+
+struct ChunkArgs {
+  CUtensorMap k_map, v_map;
+  PagedAttnArgs a;
+  int box;
+};
+
+template <int D>
+struct ChunkCfg {
+  static constexpr int kSlot = kChunkKeys * D * 2;       // K or V of a tile
+  static constexpr int kQ = 128 * D * 2;                 // one tile of Q
+  static constexpr int kSlots = 160 * 1024 / kSlot;
+  static constexpr int kSmem = 2 * kQ + kSlots * kSlot + 1024;
+  static constexpr int kPart = 128 * (D + 2);            // floats of a tile's piece
+};
+
+struct ChunkItem {
+  int req, head, rt, q0, qn, kv, rows;  // rows: of the whole request
+  int first, end;                       // keys that some row of the item sees
+  int tile0, n;
+};
+
+__device__ __forceinline__ void chunk_span(const PagedAttnArgs& p, ChunkItem& it, int group) {
+  const int r0 = it.rt * kChunkRows, r1 = min(it.rows, r0 + kChunkRows);
+  const int base = it.kv - it.qn;
+  it.first = paged_first_key(p, base + r0 / group);
+  it.end = max(0, base + (r1 - 1) / group + 1);
+  it.tile0 = it.first / kChunkKeys;
+  it.n = max(1, (it.end + kChunkKeys - 1) / kChunkKeys - it.tile0);
+}
+
+// False for a request without rows.
+__device__ __forceinline__ bool chunk_request(const PagedAttnArgs& p, ChunkItem& it, int req, int group, bool report) {
+  const PagedRequest r = paged_request(p, req, report);
+  it.req = req;
+  it.q0 = r.q0;
+  it.qn = r.qn;
+  it.kv = r.kv;
+  it.rows = r.qn * group;
+  return r.qn > 0;
+}
+
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// Ties registers of an asynchronous load to this point: nothing that uses them moves before it.
+__device__ __forceinline__ void tie32(uint32_t (&r)[32]) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31]));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]: A's row in its lane, two 16-bit elements a column.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Descriptor of V as it lies: rows of 64 columns (128 bytes, 128B swizzle), the
+// next 64 columns `col_bytes` on (leading offset), the next 8 rows 1024 bytes on.
+__device__ __forceinline__ uint64_t umma_desc_rows(const void* tile, uint32_t col_bytes) {
+  return (uint64_t)((smem_addr(tile) >> 4) & 0x3FFFu) | ((uint64_t)(col_bytes >> 4) << 16) | (64ull << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+
+template <int N>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kChunkThreads, 1)
+paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
+  using C = ChunkCfg<D>;
+  constexpr int NS = C::kSlots, HALF = kChunkKeys * 128;
+  constexpr bool kTwoTerms = Num<T>::is_bf16;
+  constexpr uint32_t S_COL = 0, O_COL = 256;
+  extern __shared__ __align__(1024) unsigned char s_raw[];
+  __shared__ __align__(8) uint64_t full[NS], empty[NS], q_ready[2], s_full[2], p_ready[2], pv_done[2];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_last[2];
+  const PagedAttnArgs& p = args.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* ring = smem + 2 * C::kQ;
+  const int group = p.q_heads / p.kv_heads;
+
+  if (tid == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int q = 0; q < 2; ++q) {
+      mbar_init(&q_ready[q], 4);
+      mbar_init(&s_full[q], 1);
+      mbar_init(&p_ready[q], 4);
+      mbar_init(&pv_done[q], 1);
+    }
+    fence_barrier_init();
+    tma_prefetch_map(&args.k_map);
+    tma_prefetch_map(&args.v_map);
+  }
+  if (warp == 1) tmem_alloc(&s_tmem, 512);
+  tc_fence_before();
+  pdl_wait();
+  pdl_trigger();
+
+  PagedSplit split;
+  ChunkItem it;
+  long long before;
+  int req;
+  paged_find<kChunkThreads>(
+      p.requests,
+      [&](int i) {
+        ChunkItem x;
+        if (!chunk_request(p, x, i, group, blockIdx.x == 0)) return 0ll;
+        long long n = 0;
+        for (x.rt = 0; x.rt * kChunkRows < x.rows; ++x.rt) {
+          chunk_span(p, x, group);
+          n += x.n;
+        }
+        return n * p.kv_heads;
+      },
+      split, req, before);
+  paged_zero_rest<T>(p);
+  tc_fence_after();  // the barriers inside paged_find have made s_tmem visible
+  const uint32_t tmem = s_tmem;
+  long long pos = split.start(blockIdx.x);
+  const long long end = split.start(blockIdx.x + 1);
+  int tile = 0;
+  auto item_of_request = [&](long long rel) {  // the item that holds tile `rel` of request it.req
+    long long per_head = 0;
+    for (it.rt = 0; it.rt * kChunkRows < it.rows; ++it.rt) {
+      chunk_span(p, it, group);
+      per_head += it.n;
+    }
+    it.head = (int)(rel / per_head);
+    rel -= it.head * per_head;
+    for (it.rt = 0;; ++it.rt) {
+      chunk_span(p, it, group);
+      if (rel < it.n) break;
+      rel -= it.n;
+    }
+    tile = (int)rel;
+  };
+  auto next_item = [&]() {
+    tile = 0;
+    if (++it.rt * kChunkRows >= it.rows) {
+      it.rt = 0;
+      if (++it.head == p.kv_heads) {
+        it.head = 0;
+        for (int i = it.req + 1; i < p.requests; ++i)
+          if (chunk_request(p, it, i, group, false)) break;
+      }
+    }
+    chunk_span(p, it, group);
+  };
+  if (pos < end) {
+    chunk_request(p, it, req, group, false);
+    item_of_request(pos - before);
+  }
+  bool ok = true;
+
+  // Registers: 384 threads are launched with 168 each (64512); the four warps of
+  // the producer and the tensor cores keep 72, the softmax warps take 216: 128 * 72
+  // + 256 * 216 = 64512.
+  if (warp < 4) {
+    regs_down<72>();
+    if (warp == 0) {  // ---- producer: K and V of each tile, a box of a page a lane ----
+      const int boxes = kChunkKeys / args.box, jobs = boxes * (D / 64);
+      const int b = lane % boxes, half = lane / boxes;
+      int slot = 0, round = 0;
+      while (pos < end) {
+        const int len = (int)min((long long)(it.n - tile), end - pos);
+        const int32_t* table = p.tables + it.req * p.table_stride;
+        for (int k = 0; k < len; ++k) {
+          const int j = (it.tile0 + tile + k) * kChunkKeys + b * args.box;
+          int block = (int)p.num_blocks, off = 0;  // out of range: zeros
+          if (lane < jobs && j < it.end && j + args.box > it.first) {
+            const int e = __ldcg(table + j / p.block_size);
+            off = j % p.block_size;
+            if (e >= 0 && e < p.num_blocks) block = e;
+            else flag_error(p.status, kErrKvRange);
+          }
+#pragma unroll
+          for (int side = 0; side < 2; ++side) {
+            if (round > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait(&empty[slot], (round - 1) & 1, p.status));
+            if (ok) {
+              if (lane == 0) mbar_arrive_expect_tx(&full[slot], C::kSlot);
+              __syncwarp();
+              if (lane < jobs)
+                tma_load_4d(ring + slot * C::kSlot + half * HALF + b * args.box * 128,
+                            side == 0 ? &args.k_map : &args.v_map, half * 64, off, it.head, block, &full[slot]);
+            }
+            if (++slot == NS) {
+              slot = 0;
+              ++round;
+            }
+          }
+        }
+        pos += len;
+        if (pos < end) next_item();
+      }
+    } else if (warp == 1) {  // ---- tensor cores ----
+      constexpr uint32_t idesc_s = umma_idesc_f16(Num<T>::is_bf16, 128, kChunkKeys);
+      constexpr uint32_t idesc_o = umma_idesc_f16(Num<T>::is_bf16, 128, D) | (1u << 16);  // B: columns contiguous
+      int slot = 0, ring_phase = 0;
+      int n_s[2] = {0, 0};                        // key tiles begun on each row tile
+      int item = 0, items1 = 0;
+      bool held = false, held_first = false;      // tile 1's product, half a period behind
+      int held_slot = 0;
+      auto wait = [&](uint64_t* bar, int parity) { ok = __all_sync(0xffffffffu, ok && mbar_wait(bar, parity & 1, p.status)); };
+      auto scores = [&](int q, int kslot) {
+        if (n_s[q] > 0) wait(&pv_done[q], n_s[q] - 1);  // P of the tile before has been read
+        tc_fence_after();
+        if (lane == 0) {
+          const unsigned char* qs = smem + q * C::kQ;
+          const unsigned char* ks = ring + kslot * C::kSlot;
+#pragma unroll 1
+          for (int k = 0; k < D / 16; ++k)
+            umma_f16(tmem + S_COL + q * 128, umma_desc_sw128(qs + (k >> 2) * HALF) + 2 * (k & 3),
+                     umma_desc_sw128(ks + (k >> 2) * HALF) + 2 * (k & 3), idesc_s, k != 0);
+          umma_commit(&s_full[q]);
+        }
+        __syncwarp();
+        ++n_s[q];
+      };
+      auto values = [&](int q, int vslot, bool first) {
+        wait(&p_ready[q], n_s[q] - 1);
+        tc_fence_after();
+        if (lane == 0) {
+          const unsigned char* vs = ring + vslot * C::kSlot;
+          const uint32_t a = tmem + S_COL + q * 128, o = tmem + O_COL + q * D;
+          const uint64_t b = umma_desc_rows(vs, HALF);
+#pragma unroll 1
+          for (int k = 0; k < kChunkKeys / 16; ++k) umma_f16_ts(o, a + k * 8, b + k * 128, idesc_o, !first || k != 0);
+          if constexpr (kTwoTerms) {
+#pragma unroll 1
+            for (int k = 0; k < kChunkKeys / 16; ++k) umma_f16_ts(o, a + 64 + k * 8, b + k * 128, idesc_o, 1);
+          }
+          umma_commit(&pv_done[q]);
+        }
+        __syncwarp();
+      };
+      auto release = [&](int s) {
+        if (lane == 0) umma_commit(&empty[s]);
+        __syncwarp();
+      };
+      auto step = [&](int& s) {
+        if (++slot == NS) {
+          slot = 0;
+          ring_phase ^= 1;
+        }
+        s = slot;
+      };
+      while (pos < end) {
+        const int len = (int)min((long long)(it.n - tile), end - pos);
+        const bool two = it.rows - it.rt * kChunkRows > 128;
+        for (int k = 0; k < len; ++k) {
+          const int kslot = slot;
+          wait(&full[kslot], ring_phase);
+          if (k == 0) wait(&q_ready[0], item);
+          scores(0, kslot);
+          if (held) {
+            values(1, held_slot, held_first);
+            release(held_slot);
+          }
+          if (two) {
+            if (k == 0) wait(&q_ready[1], items1);
+            scores(1, kslot);
+          }
+          release(kslot);
+          int vslot;
+          step(vslot);
+          wait(&full[vslot], ring_phase);
+          const int j0 = (it.tile0 + tile + k) * kChunkKeys;
+          if (j0 + kChunkKeys > it.kv || j0 < it.first) {  // rows of V that are nobody's
+            unsigned char* vs = ring + vslot * C::kSlot;
+            for (int j = 0; j < kChunkKeys; ++j)
+              if (j0 + j >= it.kv || j0 + j < it.first)
+                for (int c = lane; c < D / 8; c += 32)
+                  *reinterpret_cast<uint4*>(vs + (c >> 3) * HALF + j * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          values(0, vslot, k == 0);
+          if (!two) release(vslot);
+          held = two;
+          held_first = k == 0;
+          held_slot = vslot;
+          int next;
+          step(next);
+        }
+        ++item;
+        items1 += two ? 1 : 0;
+        pos += len;
+        if (pos < end) next_item();
+      }
+      if (held) {
+        values(1, held_slot, held_first);
+        release(held_slot);
+      }
+    }
+  } else {  // ---- softmax: warpgroup q, thread = row ----
+    regs_up<216>();
+    const int q = (warp >> 2) - 1, row = tid & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + lanes + S_COL + q * 128, o_addr = tmem + lanes + O_COL + q * D;
+    const float sl = p.scale * 1.4426950408889634f;  // scores in powers of two
+    uint32_t* tickets = static_cast<uint32_t*>(p.workspace);
+    float* parts = reinterpret_cast<float*>(tickets + kPagedTickets);
+    // Q of an item into this tile's shared memory: 16-byte pieces, swizzled as TMA would
+    auto load_q = [&](const ChunkItem& x) {
+      const int r0 = x.rt * kChunkRows + q * 128;
+      constexpr int PIECES = D / 8, AT_ONCE = 8;
+      for (int e0 = row; e0 < 128 * PIECES; e0 += 128 * AT_ONCE) {
+        uint4 u[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+          const int e = e0 + i * 128, r = r0 + e / PIECES, c = e % PIECES, t = r / group;
+          u[i] = make_uint4(0, 0, 0, 0);
+          if (r < x.rows)
+            u[i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (int64_t)(x.q0 + t) * p.q_token +
+                                                         (int64_t)(x.head * group + r - t * group) * p.q_head + c * 8));
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+          const int e = e0 + i * 128, r = e / PIECES, c = e % PIECES;
+          *reinterpret_cast<uint4*>(smem + q * C::kQ + (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = u[i];
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_ready[q]);
+    };
+    auto mine = [&](const ChunkItem& x) { return x.rows - x.rt * kChunkRows > q * 128; };
+    int n = 0;  // key tiles done on this row tile
+    bool loaded = false;
+    while (pos < end) {
+      const int len = (int)min((long long)(it.n - tile), end - pos);
+      if (!mine(it)) {  // one tile of rows only
+        pos += len;
+        if (pos < end) next_item();
+        continue;
+      }
+      if (!loaded) load_q(it);
+      const int r = it.rt * kChunkRows + q * 128 + row;
+      const int pq = it.kv - it.qn + r / group;
+      const int limit = r < it.rows ? pq + 1 : 0, floor_ = paged_first_key(p, pq);
+      // key tiles that every row of this tile sees whole need no mask
+      const int r_lo = it.rt * kChunkRows + q * 128, r_hi = min(it.rows, r_lo + 128) - 1;
+      const int all_end = it.kv - it.qn + r_lo / group + 1, all_first = paged_first_key(p, it.kv - it.qn + r_hi / group);
+      float m = -INFINITY, l = 0.f;
+      for (int k = 0; k < len; ++k, ++n) {
+        ok = ok && mbar_wait(&s_full[q], n & 1, p.status);
+        __syncwarp();
+        tc_fence_after();
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32_async(s_addr + c * 32, s[c]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tie32(s[c]);
+        const int j0 = (it.tile0 + tile + k) * kChunkKeys;
+        if (j0 + kChunkKeys > all_end || j0 < all_first) {
+          const int hi = limit - j0, lo = floor_ - j0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c * 32 + i >= hi || c * 32 + i < lo) s[c][i] = 0xff800000u;  // -infinity
+        }
+        float top[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          top[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+          for (int i = 1; i < 32; ++i) top[c] = fmaxf(top[c], __uint_as_float(s[c][i]));
+        }
+        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl;
+        if (k == 0) {
+          m = mx;
+        } else {
+          const bool raise = mx > m + 8.f;
+          if (__any_sync(0xffffffffu, raise)) {
+            const float fix = raise ? exp2_fast(m - mx) : 1.f;
+            if (raise) m = mx;
+            l *= fix;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32_async(o_addr + c * 32, o);
+              tmem_wait_ld();
+              tie32(o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fix);
+              tmem_st32(o_addr + c * 32, o);
+            }
+          }
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float p0 = exp2_fast(fmaf(__uint_as_float(s[c][i]), sl, -ref));
+            const float p1 = exp2_fast(fmaf(__uint_as_float(s[c][i + 1]), sl, -ref));
+            sum[c] += p0 + p1;
+            const uint32_t hi = pack_round2<T>(p0, p1);
+            s[c][i] = hi;
+            if constexpr (kTwoTerms) s[c][i + 1] = pack_round2<T>(p0 - Pack2<T>::lo(hi), p1 - Pack2<T>::hi(hi));
+          }
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) w[i] = s[h * 2 + (i >> 4)][(i & 15) * 2];
+          tmem_st32(s_addr + h * 32, w);
+          if constexpr (kTwoTerms) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) w[i] = s[h * 2 + (i >> 4)][(i & 15) * 2 + 1];
+            tmem_st32(s_addr + 64 + h * 32, w);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[q]);
+      }
+
+      // The next item's Q, while the last products run: this item's scores are all done.
+      const ChunkItem cur = it;
+      const int cur_tile = tile;
+      const long long item0 = pos - tile;
+      pos += len;
+      loaded = false;
+      if (pos < end) {
+        next_item();
+        if (mine(it)) {
+          load_q(it);
+          loaded = true;
+        }
+      }
+
+      ok = ok && mbar_wait(&pv_done[q], (n - 1) & 1, p.status);
+      __syncwarp();
+      tc_fence_after();
+      const bool begins = cur_tile == 0, whole = begins && cur_tile + len == cur.n;
+      const int t = r / group;
+      T* dst = static_cast<T*>(p.out) + (int64_t)(cur.q0 + t) * p.out_token +
+               (int64_t)(cur.head * group + r - t * group) * p.out_head;
+      auto store = [&](int c, const float* v, float inv) {  // 8 columns
+        uint4 u;
+        u.x = pack_round2<T>(v[0] * inv, v[1] * inv);
+        u.y = pack_round2<T>(v[2] * inv, v[3] * inv);
+        u.z = pack_round2<T>(v[4] * inv, v[5] * inv);
+        u.w = pack_round2<T>(v[6] * inv, v[7] * inv);
+        *reinterpret_cast<uint4*>(dst + c) = u;
+      };
+      // pieces: [column / 4][row] of four floats, then maxima, then sums
+      auto piece = [&](int cta, int first_cta) {
+        return parts + (((long long)cta * 2 + (cta == first_cta ? 1 : 0)) * 2 + q) * C::kPart;
+      };
+      const int c0 = whole ? 0 : split.owner(item0);
+      float* part = piece(blockIdx.x, c0);
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32_async(o_addr + c * 32, o);
+        tmem_wait_ld();
+        tie32(o);
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]);
+        if (whole) {
+          if (r < cur.rows) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) store(c * 32 + i, v + i, inv);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            __stcg(reinterpret_cast<float4*>(part) + (c * 8 + i / 4) * 128 + row,
+                   make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+        }
+      }
+      tc_fence_before();
+      if (!whole) {
+        __stcg(part + 128 * D + row, m);
+        __stcg(part + 128 * (D + 1) + row, l);
+        const int c1 = split.owner(item0 + cur.n - 1);
+        __threadfence();
+        named_barrier(1 + q, 128);
+        if (row == 0) {
+          uint32_t* ticket = tickets + c0 * 2 + q;
+          const bool last = atomicAdd(ticket, 1u) == (uint32_t)(c1 - c0);
+          if (last) *ticket = 0u;
+          __threadfence();
+          s_last[q] = last;
+        }
+        named_barrier(1 + q, 128);
+        const bool last = s_last[q];
+        named_barrier(1 + q, 128);
+        if (last && r < cur.rows) {
+          float top = -INFINITY;
+          for (int x = c0; x <= c1; ++x) top = fmaxf(top, __ldcg(piece(x, c0) + 128 * D + row));
+          const float base = top == -INFINITY ? 0.f : top;
+          float total = 0.f;
+          for (int x = c0; x <= c1; ++x)
+            total = fmaf(__ldcg(piece(x, c0) + 128 * (D + 1) + row), exp2_fast(__ldcg(piece(x, c0) + 128 * D + row) - base),
+                         total);
+          const float inv_all = total > 0.f || total != total ? 1.f / total : 0.f;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0.f;
+            for (int x = c0; x <= c1; ++x) {
+              const float* src = piece(x, c0);
+              const float w = exp2_fast(__ldcg(src + 128 * D + row) - base);
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                const float4 u = __ldcg(reinterpret_cast<const float4*>(src) + (c * 8 + i / 4) * 128 + row);
+                v[i] = fmaf(u.x, w, v[i]);
+                v[i + 1] = fmaf(u.y, w, v[i + 1]);
+                v[i + 2] = fmaf(u.z, w, v[i + 2]);
+                v[i + 3] = fmaf(u.w, w, v[i + 3]);
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) store(c * 32 + i, v + i, inv_all);
+          }
+        }
+        __syncwarp();
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_free(tmem, 512);
+}
+
+namespace {
+
+template <typename T, int D>
+cudaError_t launch_chunk(const ChunkArgs& a, cudaStream_t st, bool pdl) {
+  using C = ChunkCfg<D>;
+  static_assert(C::kSmem <= 227 * 1024, "shared memory");
+  auto kern = paged_attention_chunk_kernel<T, D>;
+  static const cudaError_t attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  if (attr != cudaSuccess) return attr;
+  const int ctas = paged_sm_count();
+  if (ctas * 2 > kPagedTickets || (size_t)ctas * 4 * C::kPart * 4 + kPagedTickets * 4 > kPagedWorkspaceBytes)
+    return cudaErrorNotSupported;
+  return launch_kernel(kern, dim3(ctas), dim3(kChunkThreads), C::kSmem, st, pdl, a);
+}
+
+}  // namespace
+
+cudaError_t launch_paged_attention_chunk(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl) {
+  if ((dtype != kBF16 && dtype != kF16) || (a.dim != 64 && a.dim != 128) || !(a.scale > 0.f))
+    return cudaErrorNotSupported;  // a maximum of scores is one of scaled scores for a positive scale only
+  ChunkArgs c{};
+  c.a = a;
+  c.box = paged_box(a.block_size, kChunkKeys);
+  if (c.box < 8 || !paged_maps(a, dtype, c.box, &c.k_map, &c.v_map)) return cudaErrorNotSupported;
+  if (dtype == kBF16)
+    return a.dim == 64 ? launch_chunk<__nv_bfloat16, 64>(c, st, pdl) : launch_chunk<__nv_bfloat16, 128>(c, st, pdl);
+  return a.dim == 64 ? launch_chunk<__half, 64>(c, st, pdl) : launch_chunk<__half, 128>(c, st, pdl);
+}
+
+}  // namespace mlora

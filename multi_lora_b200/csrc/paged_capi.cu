@@ -205,8 +205,10 @@ int mlora_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
                    pieces(c.v, es, c.v_block_stride, c.v_slot_stride, c.v_head_stride);
   const bool pdl = mlora_get_pdl() != 0;
   const cudaStream_t st = (cudaStream_t)stream;
-  if (vec && es == 2 && max_q_len * (q_heads / c.kv_heads) <= mlora::kDecodeMaxRows) {
-    const cudaError_t e = mlora::launch_paged_attention_decode(a, c.dtype, st, pdl);
+  if (vec && es == 2) {
+    const bool few = (int64_t)a.max_q_len * (q_heads / c.kv_heads) <= mlora::kDecodeMaxRows;
+    const cudaError_t e = few ? mlora::launch_paged_attention_decode(a, c.dtype, st, pdl)
+                              : mlora::launch_paged_attention_chunk(a, c.dtype, st, pdl);
     if (e != cudaErrorNotSupported) return launched(e, "paged attention launch");
   }
   return launched(mlora::launch_paged_attention_general(a, c.dtype, vec, st, pdl), "paged attention launch");
