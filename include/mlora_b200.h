@@ -389,6 +389,7 @@ size_t mlora_paged_attention_workspace_bytes(void);
  *   tokens        int64 [requests, max_drafts + 1]: kept drafts, the drawn
  *                 token, then -1
  *   num_emitted   [requests]: kept drafts + 1; 0 for a request without rows
+ * requests <= 65535, vocab <= 4194304.
  */
 int mlora_verify_draft(const void* target, int64_t rows, int64_t vocab, int64_t target_row_stride, const void* draft,
                        int64_t draft_request_stride, int64_t draft_row_stride, const int64_t* draft_tokens,

@@ -8,6 +8,7 @@ There is deliberately no fallback: if ``libmlora_b200.so`` or the
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 from pathlib import Path
 
@@ -155,6 +156,12 @@ def ops():
             torch.ops.load_library(str(TORCH_LIB_PATH))
             _ops_loaded = True
     return torch.ops.mlora
+
+
+@functools.lru_cache(maxsize=None)
+def op(name: str):
+    """One operator of ``torch.ops.mlora`` (its only overload, so that a call skips the lookup)."""
+    return getattr(ops(), name).default
 
 
 def check(rc: int) -> None:

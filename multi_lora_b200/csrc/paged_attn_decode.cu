@@ -145,7 +145,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
           if (e >= 0 && e < p.num_blocks) block = e;
           else flag_error(p.status, kErrKvRange);
         }
-        if (round > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait(&empty[stage], (round - 1) & 1, p.status));
+        if (round > 0) ok = __all_sync(0xffffffffu, ok && mbar_poll(&empty[stage], (round - 1) & 1, p.status));
         if (ok) {
           if (lane == 0) mbar_arrive_expect_tx(&full[stage], 2 * SIDE);
           __syncwarp();
@@ -198,7 +198,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
     for (int k = 0; k < len; ++k) {
-      ok = ok && mbar_wait(&full[stage], phase, p.status);
+      ok = ok && mbar_poll(&full[stage], phase, p.status);
       __syncwarp();
 #pragma unroll
       for (int sub = 0; sub < C::kSub; ++sub) {

@@ -253,7 +253,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
           }
 #pragma unroll
           for (int side = 0; side < 2; ++side) {
-            if (round > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait(&empty[slot], (round - 1) & 1, p.status));
+            if (round > 0) ok = __all_sync(0xffffffffu, ok && mbar_poll(&empty[slot], (round - 1) & 1, p.status));
             if (ok) {
               if (lane == 0) mbar_arrive_expect_tx(&full[slot], C::kSlot);
               __syncwarp();
@@ -278,7 +278,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       int item = 0, items1 = 0;
       bool held = false, held_first = false;      // tile 1's product, half a period behind
       int held_slot = 0;
-      auto wait = [&](uint64_t* bar, int parity) { ok = __all_sync(0xffffffffu, ok && mbar_wait(bar, parity & 1, p.status)); };
+      auto wait = [&](uint64_t* bar, int parity) { ok = __all_sync(0xffffffffu, ok && mbar_poll(bar, parity & 1, p.status)); };
       auto scores = [&](int q, int kslot) {
         if (n_s[q] > 0) wait(&pv_done[q], n_s[q] - 1);  // P of the tile before has been read
         tc_fence_after();
@@ -421,7 +421,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       const int all_end = it.kv - it.qn + r_lo / group + 1, all_first = paged_first_key(p, it.kv - it.qn + r_hi / group);
       float m = -INFINITY, l = 0.f;
       for (int k = 0; k < len; ++k, ++n) {
-        ok = ok && mbar_wait(&s_full[q], n & 1, p.status);
+        ok = ok && mbar_poll(&s_full[q], n & 1, p.status);
         __syncwarp();
         tc_fence_after();
         uint32_t s[4][32];
@@ -514,7 +514,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         }
       }
 
-      ok = ok && mbar_wait(&pv_done[q], (n - 1) & 1, p.status);
+      ok = ok && mbar_poll(&pv_done[q], (n - 1) & 1, p.status);
       __syncwarp();
       tc_fence_after();
       const bool begins = cur_tile == 0, whole = begins && cur_tile + len == cur.n;

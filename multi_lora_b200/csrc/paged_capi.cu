@@ -224,7 +224,7 @@ int mlora_verify_draft(const void* target, int64_t rows, int64_t vocab, int64_t 
   if (es == 0) return refuse(MLORA_ERR_UNSUPPORTED_DTYPE, "unsupported dtype code %d", dtype);
   if (vocab < 1 || vocab > (1 << 22))
     return refuse(MLORA_ERR_INVALID_ARGUMENT, "vocabulary of %lld: 1 to 4194304 are verified", (long long)vocab);
-  if (rows < 0 || rows > INT32_MAX || requests < 0 || requests > INT32_MAX || max_drafts < 0 || max_drafts > 65535)
+  if (rows < 0 || rows > INT32_MAX || requests < 0 || requests > 65535 || max_drafts < 0 || max_drafts > 65535)
     return refuse(MLORA_ERR_INVALID_ARGUMENT, "%lld rows of %lld requests, %d drafts at most each", (long long)rows,
                   (long long)requests, max_drafts);
   if (target_row_stride < vocab || (draft != nullptr && (draft_row_stride < vocab || draft_request_stride < 0)))

@@ -15,6 +15,7 @@
 
 #include "common.cuh"
 #include "paged.h"
+#include "tma.cuh"
 
 namespace mlora {
 
@@ -119,6 +120,23 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Bounded wait like mbar_wait, for barriers on the critical path: the timer (a read of
+// it takes longer than most waits) is asked every 128th poll only.
+__device__ __forceinline__ bool mbar_poll(uint64_t* bar, uint32_t parity, uint32_t* status) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 1; !mbar_try_wait(bar, parity); ++i) {
+    if ((i & 127u) == 0) {
+      const uint64_t t = global_timer_ns();
+      if (t0 == 0) t0 = t;
+      if (t - t0 > kWaitLimitNs) {
+        flag_error(status, kErrTimeout);
+        return false;
+      }
+    }
+  }
+  return true;
 }
 
 constexpr int kPagedTickets = 1024;  // words at the start of the workspace, zero between calls
