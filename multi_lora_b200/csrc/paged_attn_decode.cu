@@ -27,6 +27,7 @@
 namespace mlora {
 
 constexpr int kDecTile = 64;  // keys a stage
+constexpr int kDecJoin = 3;   // joining a piece costs about three tiles
 
 struct DecodeArgs {
   CUtensorMap k_map, v_map;
@@ -95,7 +96,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
   pdl_wait();
   pdl_trigger();
 
-  PagedSplit split;
+  PagedSplit<kDecJoin> split;
   DecodeItem it;
   long long before;
   int req;
@@ -127,14 +128,21 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       }
     }
   };
+  {
+    const int at = split.snap(tile, it.n);
+    pos += at - tile;
+    tile = at;
+    if (tile == it.n && pos < split.total) next_item();
+  }
+  // Tiles of the current item that are this CTA's; 0: there is nothing left for it.
+  auto take = [&]() { return pos < end ? split.take(end - (pos - tile), it.n, tile) : 0; };
   bool ok = true;
 
   if (warp == C::kWarps) {  // ---- producer ----
     const int boxes = kDecTile / args.box, jobs = boxes * (D / 64) * 2;
     const int b = lane % boxes, half = (lane / boxes) % (D / 64), side = lane / (boxes * (D / 64));
     int stage = 0, round = 0;
-    while (pos < end) {
-      const int len = (int)min((long long)(it.n - tile), end - pos);
+    for (int len; (len = take()) > 0;) {
       const int32_t* table = p.tables + it.req * p.table_stride;
       for (int k = 0; k < len; ++k) {
         const int j = (it.tile0 + tile + k) * kDecTile + b * args.box;
@@ -171,8 +179,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
   uint32_t* tickets = static_cast<uint32_t*>(p.workspace);
   float* parts = reinterpret_cast<float*>(tickets + kPagedTickets);
   constexpr int PART = MT * 16 * (D + 2);  // floats of a piece: sums, maxima, totals
-  while (pos < end) {
-    const int len = (int)min((long long)(it.n - tile), end - pos);
+  for (int len; (len = take()) > 0;) {
     const int rows = it.qn * group;
     // Q fragments: rows lane / 4 and + 8, columns (lane % 4) * 2 (+ 8) of each 16
     uint32_t qf[D / 16][4];
@@ -376,7 +383,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     }
     if (!whole) {
       const long long item0 = pos - tile;
-      const int c0 = split.owner(item0), c1 = split.owner(item0 + it.n - 1);
+      const int c0 = split.first_cta(item0, it.n), c1 = split.last_cta(item0, it.n);
       __threadfence();
       named_barrier(1, C::kWarps * 32);
       if (tid == 0) {

@@ -6,20 +6,21 @@
 // V serves the whole group. A CTA takes 256 of them, as two tiles of 128, over
 // a run of 128-key tiles (the even split of paged_sched.cuh):
 //   S = Q K^T   (tcgen05.mma, both operands from shared memory, S in TMEM)
-//   P = exp2(scale' S - m)  by one warpgroup a tile, a thread a row: a row's
-//               128 scores in registers, P written over S in TMEM
+//   P = exp2(scale' S - m)  by one warpgroup a tile of rows, a thread a row: a
+//               row's 64 scores in registers, P written over S in TMEM
 //   O += P V    (tcgen05.mma, P from TMEM, V from shared memory as it lies, with
 //               the columns as the contiguous dimension; O in TMEM, 2 x 128 fp32 columns)
-// The two tiles run half a period apart: while one warpgroup works on its
-// scores, the tensor cores do the other tile's products. S and P share their TMEM
-// columns (2 x 128 for S/P and 2 x D for O fill the 512), so the scores of the
-// next key tile wait for the product that reads P.
+// A key tile is worked on in two halves of 64 keys, and each tile of rows has two
+// buffers of 64 TMEM columns that hold a half's S and then its P (2 x 2 x 64 of
+// them and 2 x D for O fill the 512). So the tensor cores are a half ahead: they
+// compute S of the next half while the warpgroups work on this one, and neither
+// waits for the other's latency.
 //
 // The running maximum that P is taken against is raised only when a row's
 // scores exceed it by 2^8 (O is rescaled in TMEM then, rarely after the first
 // tiles); P stays below 2^8 and everything is normalised at the end by the sum of P
 // in fp32. An f16 P is rounded once (11 bits). A bf16 P goes in as two terms,
-// its rounding and the rounding's remainder (16 bits): one term of 8 bits would add as much
+// its upper 8 bits and the rest (16 bits): one term of 8 bits would add as much
 // error as the result's own rounding. The second term is one more product of the same size.
 //
 // What bounds it: the exponentials (16 a cycle and SM: 2048 cycles for two
@@ -36,8 +37,10 @@
 namespace mlora {
 
 constexpr int kChunkKeys = 128;   // keys a tile
+constexpr int kHalfKeys = 64;     // keys a step of the tensor cores and the softmax
 constexpr int kChunkRows = 256;   // query rows an item: two tiles of 128
 constexpr int kChunkThreads = 384;
+constexpr int kChunkJoin = 3;     // joining a piece costs about three key tiles
 
 struct ChunkArgs {
   CUtensorMap k_map, v_map;
@@ -80,6 +83,16 @@ __device__ __forceinline__ bool chunk_request(const PagedAttnArgs& p, ChunkItem&
   return r.qn > 0;
 }
 
+// The same for callers that are a converged warp: what it loads is known to be uniform then.
+__device__ __forceinline__ bool chunk_load(const PagedAttnArgs& p, ChunkItem& it, int req, int group) {
+  chunk_request(p, it, req, group, false);
+  it.q0 = same_in_warp(it.q0);
+  it.qn = same_in_warp(it.qn);
+  it.kv = same_in_warp(it.kv);
+  it.rows = it.qn * group;
+  return it.qn > 0;
+}
+
 __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -111,21 +124,45 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
-// D[tmem] (+)= A[tmem] * B[smem]: A's row in its lane, two 16-bit elements a column.
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                            uint32_t accumulate) {
+// Shared-memory descriptors by their halves: the upper one is a constant, the lower
+// one an address in 16-byte units (plus the leading offset), so that stepping
+// through a tile is one 32-bit addition and the tensor cores are not kept waiting
+// for 64-bit address arithmetic.
+constexpr uint32_t kDescHi = (1024u >> 4)       // 8 rows of 128 bytes to the next 8 (stride offset)
+                             | (1u << 14)       // descriptor version of sm_100
+                             | (2u << 29);      // 128-byte swizzle
+// D[tmem] (+)= A[smem] * B[smem]^T, rows of 64 columns (128 bytes) in both.
+__device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"((uint32_t)accumulate), "n"(kDescHi)
       : "memory");
 }
-// Descriptor of V as it lies: rows of 64 columns (128 bytes, 128B swizzle), the
-// next 64 columns `col_bytes` on (leading offset), the next 8 rows 1024 bytes on.
-__device__ __forceinline__ uint64_t umma_desc_rows(const void* tile, uint32_t col_bytes) {
-  return (uint64_t)((smem_addr(tile) >> 4) & 0x3FFFu) | ((uint64_t)(col_bytes >> 4) << 16) | (64ull << 32) |
-         (1ull << 46) | (2ull << 61);
+// D[tmem] (+)= A[tmem] * B[smem]: A's row in its lane, two 16-bit elements a
+// column; B as V lies: rows of 64 columns, the next 64 columns the leading offset on.
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"((uint32_t)accumulate), "n"(kDescHi)
+      : "memory");
+}
+
+// One lane of the (converged) warp, always the same; unlike a comparison of the lane
+// number it lets the compiler keep descriptors in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(is));
+  return is != 0;
 }
 
 template <int N>
@@ -145,11 +182,12 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
   constexpr bool kTwoTerms = Num<T>::is_bf16;
   constexpr uint32_t S_COL = 0, O_COL = 256;
   extern __shared__ __align__(1024) unsigned char s_raw[];
-  __shared__ __align__(8) uint64_t full[NS], empty[NS], q_ready[2], s_full[2], p_ready[2], pv_done[2];
+  __shared__ __align__(8) uint64_t full[NS], empty[NS], q_ready[2], s_full[2][2], p_ready[2][2], pv_done[2][2];
   __shared__ uint32_t s_tmem;
   __shared__ int s_last[2];
   const PagedAttnArgs& p = args.a;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = same_in_warp(tid >> 5);
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* ring = smem + 2 * C::kQ;
   const int group = p.q_heads / p.kv_heads;
@@ -157,13 +195,15 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty[s], 2);  // both warps of the tensor cores
     }
     for (int q = 0; q < 2; ++q) {
       mbar_init(&q_ready[q], 4);
-      mbar_init(&s_full[q], 1);
-      mbar_init(&p_ready[q], 4);
-      mbar_init(&pv_done[q], 1);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&s_full[q][b], 1);
+        mbar_init(&p_ready[q][b], 4);
+        mbar_init(&pv_done[q][b], 1);
+      }
     }
     fence_barrier_init();
     tma_prefetch_map(&args.k_map);
@@ -174,7 +214,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
   pdl_wait();
   pdl_trigger();
 
-  PagedSplit split;
+  PagedSplit<kChunkJoin> split;
   ChunkItem it;
   long long before;
   int req;
@@ -219,15 +259,21 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       if (++it.head == p.kv_heads) {
         it.head = 0;
         for (int i = it.req + 1; i < p.requests; ++i)
-          if (chunk_request(p, it, i, group, false)) break;
+          if (chunk_load(p, it, i, group)) break;
       }
     }
     chunk_span(p, it, group);
   };
   if (pos < end) {
-    chunk_request(p, it, req, group, false);
+    chunk_load(p, it, req, group);
     item_of_request(pos - before);
+    const int at = split.snap(tile, it.n);
+    pos += at - tile;
+    tile = at;
+    if (tile == it.n && pos < split.total) next_item();
   }
+  // Tiles of the current item that are this CTA's; 0: there is nothing left for it.
+  auto take = [&]() { return pos < end ? split.take(end - (pos - tile), it.n, tile) : 0; };
   bool ok = true;
 
   // Registers: 384 threads are launched with 168 each (64512); the four warps of
@@ -239,8 +285,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       const int boxes = kChunkKeys / args.box, jobs = boxes * (D / 64);
       const int b = lane % boxes, half = lane / boxes;
       int slot = 0, round = 0;
-      while (pos < end) {
-        const int len = (int)min((long long)(it.n - tile), end - pos);
+      for (int len; (len = take()) > 0;) {
         const int32_t* table = p.tables + it.req * p.table_stride;
         for (int k = 0; k < len; ++k) {
           const int j = (it.tile0 + tile + k) * kChunkKeys + b * args.box;
@@ -270,105 +315,108 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         pos += len;
         if (pos < end) next_item();
       }
-    } else if (warp == 1) {  // ---- tensor cores ----
-      constexpr uint32_t idesc_s = umma_idesc_f16(Num<T>::is_bf16, 128, kChunkKeys);
+    } else if (warp < 3) {  // ---- tensor cores, a warp a tile of rows: S of a half, then O of the half before ----
+      // A wait costs its warp over 100 cycles even when it need not wait, and the tensor
+      // cores hold no more than two instructions: with one issuing warp they
+      // idled for half the time. While one of these two waits the other one issues.
+      const int q = warp - 1;
+      constexpr uint32_t idesc_s = umma_idesc_f16(Num<T>::is_bf16, 128, kHalfKeys);
       constexpr uint32_t idesc_o = umma_idesc_f16(Num<T>::is_bf16, 128, D) | (1u << 16);  // B: columns contiguous
-      int slot = 0, ring_phase = 0;
-      int n_s[2] = {0, 0};                        // key tiles begun on each row tile
-      int item = 0, items1 = 0;
-      bool held = false, held_first = false;      // tile 1's product, half a period behind
+      constexpr uint32_t kStep = kHalfKeys * 128 >> 4;  // a half of a K or V tile
+      const uint32_t q_lo = smem_addr(smem + q * C::kQ) >> 4, ring_lo = smem_addr(ring) >> 4;
+      const uint32_t s_col = tmem + S_COL + q * 128, o_col = tmem + O_COL + q * D;
+      int kslot = 0, k_phase = 0, vslot = 1, v_phase = 0;
+      int n = 0, items = 0;     // halves and items begun
+      auto wait = [&](uint64_t* bar, int parity) { ok = ok && mbar_poll(bar, parity & 1, p.status); };
+      bool held = false, held_first = false, held_last = false;  // the half whose product with V is to come
+      uint32_t held_lo = 0;
       int held_slot = 0;
-      auto wait = [&](uint64_t* bar, int parity) { ok = __all_sync(0xffffffffu, ok && mbar_poll(bar, parity & 1, p.status)); };
-      auto scores = [&](int q, int kslot) {
-        if (n_s[q] > 0) wait(&pv_done[q], n_s[q] - 1);  // P of the tile before has been read
+      auto values = [&]() {  // half n - 1 of this tile of rows is the newest, half `number` the held one
+        const int number = n - 1, b = number & 1;
+        wait(&p_ready[q][b], number >> 1);
         tc_fence_after();
-        if (lane == 0) {
-          const unsigned char* qs = smem + q * C::kQ;
-          const unsigned char* ks = ring + kslot * C::kSlot;
-#pragma unroll 1
-          for (int k = 0; k < D / 16; ++k)
-            umma_f16(tmem + S_COL + q * 128, umma_desc_sw128(qs + (k >> 2) * HALF) + 2 * (k & 3),
-                     umma_desc_sw128(ks + (k >> 2) * HALF) + 2 * (k & 3), idesc_s, k != 0);
-          umma_commit(&s_full[q]);
-        }
-        __syncwarp();
-        ++n_s[q];
-      };
-      auto values = [&](int q, int vslot, bool first) {
-        wait(&p_ready[q], n_s[q] - 1);
-        tc_fence_after();
-        if (lane == 0) {
-          const unsigned char* vs = ring + vslot * C::kSlot;
-          const uint32_t a = tmem + S_COL + q * 128, o = tmem + O_COL + q * D;
-          const uint64_t b = umma_desc_rows(vs, HALF);
-#pragma unroll 1
-          for (int k = 0; k < kChunkKeys / 16; ++k) umma_f16_ts(o, a + k * 8, b + k * 128, idesc_o, !first || k != 0);
+        if (elect_one()) {
+          const uint32_t a = s_col + b * 64;
+#pragma unroll
+          for (int i = 0; i < kHalfKeys / 16; ++i) umma_ts(o_col, a + i * 8, held_lo + i * 128, idesc_o, !held_first || i > 0);
           if constexpr (kTwoTerms) {
+#pragma unroll
+            for (int i = 0; i < kHalfKeys / 16; ++i) umma_ts(o_col, a + 32 + i * 8, held_lo + i * 128, idesc_o, true);
+          }
+          umma_commit(&pv_done[q][b]);
+          if (held_last) umma_commit(&empty[held_slot]);
+        }
+        held = false;
+      };
+      for (int len; (len = take()) > 0;) {
+        const bool mine = it.rows - it.rt * kChunkRows > q * 128;
+        const bool both = it.rows - it.rt * kChunkRows > 128;
+        if (held) values();  // nothing of the item before waits for this one's Q, or keeps its V from the ring
 #pragma unroll 1
-            for (int k = 0; k < kChunkKeys / 16; ++k) umma_f16_ts(o, a + 64 + k * 8, b + k * 128, idesc_o, 1);
-          }
-          umma_commit(&pv_done[q]);
-        }
-        __syncwarp();
-      };
-      auto release = [&](int s) {
-        if (lane == 0) umma_commit(&empty[s]);
-        __syncwarp();
-      };
-      auto step = [&](int& s) {
-        if (++slot == NS) {
-          slot = 0;
-          ring_phase ^= 1;
-        }
-        s = slot;
-      };
-      while (pos < end) {
-        const int len = (int)min((long long)(it.n - tile), end - pos);
-        const bool two = it.rows - it.rt * kChunkRows > 128;
         for (int k = 0; k < len; ++k) {
-          const int kslot = slot;
-          wait(&full[kslot], ring_phase);
-          if (k == 0) wait(&q_ready[0], item);
-          scores(0, kslot);
-          if (held) {
-            values(1, held_slot, held_first);
-            release(held_slot);
+          wait(&full[kslot], k_phase);
+          if (mine) {
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+              const bool first = k == 0 && h == 0;
+              if (first) wait(&q_ready[q], items++);
+              const int b = n & 1;
+              if (n > 1) wait(&pv_done[q][b], (n >> 1) - 1);  // P in this buffer has been read
+              tc_fence_after();
+              if (elect_one()) {
+                const uint32_t kl = ring_lo + kslot * (C::kSlot >> 4) + h * kStep;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+                  umma_ss(s_col + b * 64, q_lo + (i >> 2) * (HALF >> 4) + 2 * (i & 3), kl + (i >> 2) * (HALF >> 4) + 2 * (i & 3),
+                          idesc_s, i > 0);
+                umma_commit(&s_full[q][b]);
+                if (h == 1) umma_commit(&empty[kslot]);
+              }
+              if (held) values();
+              ++n;
+              if (h == 0) {
+                wait(&full[vslot], v_phase);
+                const int j0 = (it.tile0 + tile + k) * kChunkKeys;
+                if (j0 + kChunkKeys > it.kv || j0 < it.first) {  // rows of V that are nobody's
+                  if (q == 0) {
+                    unsigned char* vs = ring + vslot * C::kSlot;
+#pragma unroll 1
+                    for (int j = 0; j < kChunkKeys; ++j)
+                      if (j0 + j >= it.kv || j0 + j < it.first)
+                        for (int c = lane; c < D / 8; c += 32)
+                          *reinterpret_cast<uint4*>(vs + (c >> 3) * HALF + j * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async_smem();
+                  }
+                  if (both) named_barrier(3, 64);
+                  else __syncwarp();
+                }
+              }
+              held = true;
+              held_first = first;
+              held_last = h == 1;
+              held_lo = ring_lo + vslot * (C::kSlot >> 4) + h * kStep + ((HALF >> 4) << 16);
+              held_slot = vslot;
+            }
+          } else {  // the other warp's alone
+            if (lane == 0) mbar_arrive(&empty[kslot]);
+            wait(&full[vslot], v_phase);
+            if (lane == 0) mbar_arrive(&empty[vslot]);
           }
-          if (two) {
-            if (k == 0) wait(&q_ready[1], items1);
-            scores(1, kslot);
+          kslot += 2;
+          if (kslot >= NS) {
+            kslot -= NS;
+            k_phase ^= 1;
           }
-          release(kslot);
-          int vslot;
-          step(vslot);
-          wait(&full[vslot], ring_phase);
-          const int j0 = (it.tile0 + tile + k) * kChunkKeys;
-          if (j0 + kChunkKeys > it.kv || j0 < it.first) {  // rows of V that are nobody's
-            unsigned char* vs = ring + vslot * C::kSlot;
-            for (int j = 0; j < kChunkKeys; ++j)
-              if (j0 + j >= it.kv || j0 + j < it.first)
-                for (int c = lane; c < D / 8; c += 32)
-                  *reinterpret_cast<uint4*>(vs + (c >> 3) * HALF + j * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();
-            __syncwarp();
+          vslot += 2;
+          if (vslot >= NS) {
+            vslot -= NS;
+            v_phase ^= 1;
           }
-          values(0, vslot, k == 0);
-          if (!two) release(vslot);
-          held = two;
-          held_first = k == 0;
-          held_slot = vslot;
-          int next;
-          step(next);
         }
-        ++item;
-        items1 += two ? 1 : 0;
         pos += len;
         if (pos < end) next_item();
       }
-      if (held) {
-        values(1, held_slot, held_first);
-        release(held_slot);
-      }
+      if (held) values();
     }
   } else {  // ---- softmax: warpgroup q, thread = row ----
     regs_up<216>();
@@ -403,10 +451,9 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       if (lane == 0) mbar_arrive(&q_ready[q]);
     };
     auto mine = [&](const ChunkItem& x) { return x.rows - x.rt * kChunkRows > q * 128; };
-    int n = 0;  // key tiles done on this row tile
+    int n = 0;  // halves done on this tile of rows
     bool loaded = false;
-    while (pos < end) {
-      const int len = (int)min((long long)(it.n - tile), end - pos);
+    for (int len; (len = take()) > 0;) {
       if (!mine(it)) {  // one tile of rows only
         pos += len;
         if (pos < end) next_item();
@@ -420,21 +467,23 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       const int r_lo = it.rt * kChunkRows + q * 128, r_hi = min(it.rows, r_lo + 128) - 1;
       const int all_end = it.kv - it.qn + r_lo / group + 1, all_first = paged_first_key(p, it.kv - it.qn + r_hi / group);
       float m = -INFINITY, l = 0.f;
-      for (int k = 0; k < len; ++k, ++n) {
-        ok = ok && mbar_poll(&s_full[q], n & 1, p.status);
+      const int halves = 2 * len;
+      for (int k = 0; k < halves; ++k, ++n) {
+        const int b = n & 1;
+        ok = ok && mbar_poll(&s_full[q][b], (n >> 1) & 1, p.status);
         __syncwarp();
         tc_fence_after();
-        uint32_t s[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32_async(s_addr + c * 32, s[c]);
+        uint32_t s[2][32];
+        tmem_ld32_async(s_addr + b * 64, s[0]);
+        tmem_ld32_async(s_addr + b * 64 + 32, s[1]);
         tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tie32(s[c]);
-        const int j0 = (it.tile0 + tile + k) * kChunkKeys;
-        if (j0 + kChunkKeys > all_end || j0 < all_first) {
+        tie32(s[0]);
+        tie32(s[1]);
+        const int j0 = (it.tile0 + tile) * kChunkKeys + k * kHalfKeys;
+        if (j0 + kHalfKeys > all_end || j0 < all_first) {
           const int hi = limit - j0, lo = floor_ - j0;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (c * 32 + i >= hi || c * 32 + i < lo) s[c][i] = 0xff800000u;  // -infinity
@@ -442,9 +491,9 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         float top[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          top[c] = __uint_as_float(s[c][0]);
+          top[c] = __uint_as_float(s[c >> 1][(c & 1) * 16]);
 #pragma unroll
-          for (int i = 1; i < 32; ++i) top[c] = fmaxf(top[c], __uint_as_float(s[c][i]));
+          for (int i = 1; i < 16; ++i) top[c] = fmaxf(top[c], __uint_as_float(s[c >> 1][(c & 1) * 16 + i]));
         }
         const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl;
         if (k == 0) {
@@ -452,6 +501,10 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         } else {
           const bool raise = mx > m + 8.f;
           if (__any_sync(0xffffffffu, raise)) {
+            // O holds the halves before this one once the last product is done
+            ok = ok && mbar_poll(&pv_done[q][b ^ 1], ((n - 1) >> 1) & 1, p.status);
+            __syncwarp();
+            tc_fence_after();
             const float fix = raise ? exp2_fast(m - mx) : 1.f;
             if (raise) m = mx;
             l *= fix;
@@ -469,35 +522,28 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         }
         const float ref = m == -INFINITY ? 0.f : m;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t w[32], rest[32];  // P, two keys a column
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float p0 = exp2_fast(fmaf(__uint_as_float(s[c][i]), sl, -ref));
-            const float p1 = exp2_fast(fmaf(__uint_as_float(s[c][i + 1]), sl, -ref));
-            sum[c] += p0 + p1;
-            const uint32_t hi = pack_round2<T>(p0, p1);
-            s[c][i] = hi;
-            if constexpr (kTwoTerms) s[c][i + 1] = pack_round2<T>(p0 - Pack2<T>::lo(hi), p1 - Pack2<T>::hi(hi));
+        for (int i = 0; i < 64; i += 2) {
+          uint32_t &s0 = s[i >> 5][i & 31], &s1 = s[i >> 5][(i & 31) + 1];
+          const float p0 = exp2_fast(fmaf(__uint_as_float(s0), sl, -ref));
+          const float p1 = exp2_fast(fmaf(__uint_as_float(s1), sl, -ref));
+          sum[i >> 4] += p0 + p1;
+          if constexpr (kTwoTerms) {  // the upper 16 bits as they are, and what is left rounded
+            w[i >> 1] = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);
+            rest[i >> 1] = pack_round2<T>(p0 - __uint_as_float(__float_as_uint(p0) & 0xffff0000u),
+                                          p1 - __uint_as_float(__float_as_uint(p1) & 0xffff0000u));
+          } else {
+            w[i >> 1] = pack_round2<T>(p0, p1);
           }
         }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t w[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) w[i] = s[h * 2 + (i >> 4)][(i & 15) * 2];
-          tmem_st32(s_addr + h * 32, w);
-          if constexpr (kTwoTerms) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) w[i] = s[h * 2 + (i >> 4)][(i & 15) * 2 + 1];
-            tmem_st32(s_addr + 64 + h * 32, w);
-          }
-        }
+        tmem_st32(s_addr + b * 64, w);
+        if constexpr (kTwoTerms) tmem_st32(s_addr + b * 64 + 32, rest);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[q]);
+        if (lane == 0) mbar_arrive(&p_ready[q][b]);
       }
 
       // The next item's Q, while the last products run: this item's scores are all done.
@@ -508,13 +554,13 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       loaded = false;
       if (pos < end) {
         next_item();
-        if (mine(it)) {
+        if (take() > 0 && mine(it)) {
           load_q(it);
           loaded = true;
         }
       }
 
-      ok = ok && mbar_poll(&pv_done[q], (n - 1) & 1, p.status);
+      ok = ok && mbar_poll(&pv_done[q][(n - 1) & 1], ((n - 1) >> 1) & 1, p.status);
       __syncwarp();
       tc_fence_after();
       const bool begins = cur_tile == 0, whole = begins && cur_tile + len == cur.n;
@@ -533,7 +579,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       auto piece = [&](int cta, int first_cta) {
         return parts + (((long long)cta * 2 + (cta == first_cta ? 1 : 0)) * 2 + q) * C::kPart;
       };
-      const int c0 = whole ? 0 : split.owner(item0);
+      const int c0 = whole ? 0 : split.first_cta(item0, cur.n);
       float* part = piece(blockIdx.x, c0);
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll 1
@@ -561,7 +607,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       if (!whole) {
         __stcg(part + 128 * D + row, m);
         __stcg(part + 128 * (D + 1) + row, l);
-        const int c1 = split.owner(item0 + cur.n - 1);
+        const int c1 = split.last_cta(item0, cur.n);
         __threadfence();
         named_barrier(1 + q, 128);
         if (row == 0) {
@@ -575,33 +621,37 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         const bool last = s_last[q];
         named_barrier(1 + q, 128);
         if (last && r < cur.rows) {
-          float top = -INFINITY;
+          float top = -INFINITY, total = 0.f;
+#pragma unroll 4
           for (int x = c0; x <= c1; ++x) top = fmaxf(top, __ldcg(piece(x, c0) + 128 * D + row));
           const float base = top == -INFINITY ? 0.f : top;
-          float total = 0.f;
+#pragma unroll 4
           for (int x = c0; x <= c1; ++x)
             total = fmaf(__ldcg(piece(x, c0) + 128 * (D + 1) + row), exp2_fast(__ldcg(piece(x, c0) + 128 * D + row) - base),
                          total);
           const float inv_all = total > 0.f || total != total ? 1.f / total : 0.f;
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            float v[32];
+          for (int c = 0; c < D; c += 64) {  // 16 loads of 16 bytes in flight
+            float v[64];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 0.f;
+            for (int i = 0; i < 64; ++i) v[i] = 0.f;
+#pragma unroll 1
             for (int x = c0; x <= c1; ++x) {
               const float* src = piece(x, c0);
+              float4 u[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) u[i] = __ldcg(reinterpret_cast<const float4*>(src) + (c / 4 + i) * 128 + row);
               const float w = exp2_fast(__ldcg(src + 128 * D + row) - base);
 #pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                const float4 u = __ldcg(reinterpret_cast<const float4*>(src) + (c * 8 + i / 4) * 128 + row);
-                v[i] = fmaf(u.x, w, v[i]);
-                v[i + 1] = fmaf(u.y, w, v[i + 1]);
-                v[i + 2] = fmaf(u.z, w, v[i + 2]);
-                v[i + 3] = fmaf(u.w, w, v[i + 3]);
+              for (int i = 0; i < 16; ++i) {
+                v[4 * i] = fmaf(u[i].x, w, v[4 * i]);
+                v[4 * i + 1] = fmaf(u[i].y, w, v[4 * i + 1]);
+                v[4 * i + 2] = fmaf(u[i].z, w, v[4 * i + 2]);
+                v[4 * i + 3] = fmaf(u[i].w, w, v[4 * i + 3]);
               }
             }
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) store(c * 32 + i, v + i, inv_all);
+            for (int i = 0; i < 64; i += 8) store(c + i, v + i, inv_all);
           }
         }
         __syncwarp();

@@ -19,6 +19,12 @@
 
 namespace mlora {
 
+// A value that every lane has, as one that the compiler knows to be uniform.
+template <typename V>
+__device__ __forceinline__ V same_in_warp(V v) {
+  return __shfl_sync(0xffffffffu, v, 0);
+}
+
 struct PagedRequest {
   int q0, qn, kv;  // first row, rows, keys
 };
@@ -46,6 +52,10 @@ __device__ __forceinline__ int paged_first_key(const PagedAttnArgs& p, int pos) 
   return p.window > 0 ? max(0, pos - p.window + 1) : 0;
 }
 
+// The even split of `total` tiles over the CTAs, with boundaries that fall within T
+// tiles of an item's edge moved to that edge: joining a piece costs about as much as T tiles,
+// so no piece is shorter than that, and short items stay whole.
+template <int T>
 struct PagedSplit {
   long long total, base, rem;  // CTA c has base tiles, the first `rem` CTAs one more
   __device__ void set(long long tiles, int ctas) {
@@ -58,12 +68,21 @@ struct PagedSplit {
     const long long wide = rem * (base + 1);
     return (int)(tile < wide ? tile / (base + 1) : rem + (tile - wide) / base);
   }
+  // Where a boundary x tiles into an item of n goes.
+  static __device__ int snap(long long x, int n) {
+    return x >= n ? n : x <= min(T, n / 2) ? 0 : n - x <= T ? n : (int)x;
+  }
+  // Tiles from `tile` on that a CTA whose range ends `raw` tiles into the item takes.
+  static __device__ int take(long long raw, int n, int tile) { return snap(raw, n) - tile; }
+  // The CTAs that share an item of n tiles beginning at tile `item`; more than one of them.
+  __device__ int first_cta(long long item, int n) const { return owner(item + min(T, n / 2)); }
+  __device__ int last_cta(long long item, int n) const { return owner(item + n - T - 1); }
 };
 
 // Whole block of NT threads: the split over the grid, the request that this CTA's first
 // tile lies in, and the tiles before that request. `tiles(i)`: tiles of request i.
-template <int NT, typename F>
-__device__ __forceinline__ void paged_find(int requests, F tiles, PagedSplit& split, int& req, long long& before) {
+template <int NT, typename F, typename S>
+__device__ __forceinline__ void paged_find(int requests, F tiles, S& split, int& req, long long& before) {
   __shared__ long long s_warp[NT / 32];
   __shared__ long long s_before;
   __shared__ int s_req;
@@ -88,7 +107,7 @@ __device__ __forceinline__ void paged_find(int requests, F tiles, PagedSplit& sp
     upto += w < warp ? u : 0;
     total += u;
   }
-  split.set(total, gridDim.x);
+  split.set(same_in_warp(total), gridDim.x);
   const long long a = split.start(blockIdx.x);
   if (a >= upto && a < upto + mine) {
     int i = r0;
@@ -97,8 +116,8 @@ __device__ __forceinline__ void paged_find(int requests, F tiles, PagedSplit& sp
     s_before = upto;
   }
   __syncthreads();
-  req = s_req;
-  before = s_before;
+  req = same_in_warp(s_req);
+  before = same_in_warp(s_before);
 }
 
 // Rows behind the last request's give zeros; all CTAs share them.

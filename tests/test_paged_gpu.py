@@ -280,6 +280,22 @@ def test_attention_matches_the_oracle(cuda_dev, workspace, shape, dtype):
     assert status.item() == 0
 
 
+@pytest.mark.parametrize("q_lens, kv_lens, heads, dim, dtype", [
+    ([300, 130, 700], [3000, 140, 2500], (16, 16), 64, "bf16"),  # items of two tiles of rows and of one, in turn
+    ([200, 37, 100], [2600, 1900, 3100], (24, 8), 128, "f16"),
+    ([3] * 40, [40 * i + 3 for i in range(40)], (16, 8), 128, "bf16"),
+    ([1] * 90, [31 * i for i in range(90)], (8, 8), 64, "f16"),
+])
+def test_attention_with_many_items_and_tiles_a_cta(cuda_dev, workspace, q_lens, kv_lens, heads, dim, dtype):
+    """Enough work that every CTA runs through its ring of key tiles many times and over item boundaries."""
+    pr = attention_problem(cuda_dev, 10, q_lens, kv_lens, *heads, dim, dtype, 16)
+    status = status_word(cuda_dev)
+    got = attend(pr, workspace, status=status)
+    assert status.item() == 0
+    assert_attention(got, pr, dtype)
+    assert torch.equal(attend(pr, workspace), got)
+
+
 @pytest.mark.parametrize("dim, block, dtype, layout", [
     (128, 16, "f32", "head"), (64, 5, "f32", "token"), (128, 1, "bf16", "token"), (96, 16, "bf16", "head"),
     (256, 12, "f16", "token"), (8, 3, "f16", "head"), (128, 16, "bf16", "odd"), (64, 16, "f32", "odd"),
