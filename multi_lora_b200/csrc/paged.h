@@ -59,6 +59,8 @@ struct PagedAttnArgs {
   void* out;
   int64_t out_token, out_head;
   int tokens, requests, q_heads, kv_heads, dim, block_size, width, max_q_len;
+  int group;                  // q_heads / kv_heads
+  uint32_t group_magic;       // ceil(2^32 / group), 0 for 1: row / group by a multiplication
   int64_t num_blocks;
   int window;                 // keys a query sees at most, its own among them; 0: no limit
   float scale;

@@ -55,15 +55,14 @@ struct DecodeItem {
 };
 
 template <int MT>
-__device__ __forceinline__ void decode_load(const PagedAttnArgs& p, DecodeItem& it, int req, int group) {
-  const PagedRequest r = paged_request(p, req, false);
+__device__ __forceinline__ void decode_request(const PagedAttnArgs& p, DecodeItem& it, int req, const PagedRequest& r) {
   it.req = req;
   it.q0 = r.q0;
   it.qn = r.qn;
   it.kv = r.kv;
   it.first = paged_first_key(p, r.kv - r.qn);
   it.tile0 = it.first / kDecTile;
-  it.n = r.qn > 0 && r.qn <= 16 * MT / group ? max(1, (r.kv + kDecTile - 1) / kDecTile - it.tile0) : 0;
+  it.n = r.qn > 0 && r.qn * p.group <= 16 * MT ? max(1, (r.kv + kDecTile - 1) / kDecTile - it.tile0) : 0;
 }
 
 template <typename T, int D, int MT>
@@ -80,7 +79,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~uintptr_t(1023));
   float* merge = reinterpret_cast<float*>(smem + NS * 2 * SIDE);
-  const int group = p.q_heads / p.kv_heads;
+  const int group = p.group;
 
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
@@ -98,32 +97,35 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
 
   PagedSplit<kDecJoin> split;
   DecodeItem it;
-  long long before;
+  long long before, in_req;
   int req;
-  paged_find<C::kThreads>(
+  PagedRequest found;
+  paged_find<C::kThreads, 1>(
       p.requests,
-      [&](int i) {
-        const PagedRequest r = paged_request(p, i, blockIdx.x == 0);
+      [&](int i, int, int, PagedRequest& r) {
+        r = paged_request(p, i, blockIdx.x == 0);
         // rows beyond what the caller said: reported, and not computed
         if (blockIdx.x == 0 && r.qn > p.max_q_len) flag_error(p.status, kErrLength);
-        if (r.qn == 0 || r.qn > 16 * MT / group) return 0ll;
-        const int t0 = paged_first_key(p, r.kv - r.qn) / kDecTile;
-        return (long long)max(1, (r.kv + kDecTile - 1) / kDecTile - t0) * p.kv_heads;
+        DecodeItem x;
+        decode_request<MT>(p, x, i, r);
+        return (long long)x.n * p.kv_heads;
       },
-      split, req, before);
-  paged_zero_rest<T>(p);
+      split, req, found, before, in_req);
   long long pos = split.start(blockIdx.x);
   const long long end = split.start(blockIdx.x + 1);
-  if (pos >= end) return;
-  decode_load<MT>(p, it, req, group);
-  int tile = (int)((pos - before) % it.n);
-  it.head = (int)((pos - before) / it.n);
+  if (pos >= end) {
+    if (warp == C::kWarps) paged_zero_rest<T>(p);
+    return;
+  }
+  decode_request<MT>(p, it, req, found);
+  it.head = (int)(pos - before) / it.n;
+  int tile = (int)(pos - before) - it.head * it.n;
   auto next_item = [&]() {
     tile = 0;
     if (++it.head == p.kv_heads) {
       it.head = 0;
       for (int i = it.req + 1; i < p.requests; ++i) {
-        decode_load<MT>(p, it, i, group);
+        decode_request<MT>(p, it, i, paged_request(p, i, false));
         if (it.n > 0) break;
       }
     }
@@ -169,6 +171,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       pos += len;
       if (pos < end) next_item();
     }
+    paged_zero_rest<T>(p);
     return;
   }
 
@@ -187,7 +190,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int r = mt * 16 + (lane >> 2) + e * 8;
-      const int t = r / group;
+      const int t = paged_token(p, r);
       const int pq = it.kv - it.qn + t;
       limit[e] = r < rows ? pq + 1 : 0;
       floor_[e] = paged_first_key(p, pq);
@@ -353,7 +356,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       for (int g = 0; g < C::KG; ++g) sum += top == -INFINITY ? 0.f : s_l[w + g][i] * exp2_fast(s_m[w + g][i] - top);
     };
     auto store = [&](int r, int c, const float* v, float inv) {  // 8 columns of row r
-      const int t = r / group;
+      const int t = paged_token(p, r);
       T* dst = static_cast<T*>(p.out) + (it.q0 + t) * p.out_token + (it.head * group + r - t * group) * p.out_head + c;
       uint4 u;
       u.x = pack_round2<T>(v[0] * inv, v[1] * inv);

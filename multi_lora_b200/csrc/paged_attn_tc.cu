@@ -43,9 +43,11 @@ constexpr int kChunkThreads = 384;
 constexpr int kChunkJoin = 3;     // joining a piece costs about three key tiles
 
 struct ChunkArgs {
-  CUtensorMap k_map, v_map;
+  CUtensorMap k_map, v_map, q_map;
   PagedAttnArgs a;
   int box;
+  int q_tma;   // Q tiles are boxes of q_map (group divides 128)
+  int out32;   // rows of the output allow 32-byte stores
 };
 
 template <int D>
@@ -63,34 +65,21 @@ struct ChunkItem {
   int tile0, n;
 };
 
-__device__ __forceinline__ void chunk_span(const PagedAttnArgs& p, ChunkItem& it, int group) {
+__device__ __forceinline__ void chunk_span(const PagedAttnArgs& p, ChunkItem& it) {
   const int r0 = it.rt * kChunkRows, r1 = min(it.rows, r0 + kChunkRows);
   const int base = it.kv - it.qn;
-  it.first = paged_first_key(p, base + r0 / group);
-  it.end = max(0, base + (r1 - 1) / group + 1);
+  it.first = paged_first_key(p, base + paged_token(p, r0));
+  it.end = max(0, base + paged_token(p, r1 - 1) + 1);
   it.tile0 = it.first / kChunkKeys;
   it.n = max(1, (it.end + kChunkKeys - 1) / kChunkKeys - it.tile0);
 }
 
-// False for a request without rows.
-__device__ __forceinline__ bool chunk_request(const PagedAttnArgs& p, ChunkItem& it, int req, int group, bool report) {
-  const PagedRequest r = paged_request(p, req, report);
+__device__ __forceinline__ void chunk_request(const PagedAttnArgs& p, ChunkItem& it, int req, const PagedRequest& r) {
   it.req = req;
   it.q0 = r.q0;
   it.qn = r.qn;
   it.kv = r.kv;
-  it.rows = r.qn * group;
-  return r.qn > 0;
-}
-
-// The same for callers that are a converged warp: what it loads is known to be uniform then.
-__device__ __forceinline__ bool chunk_load(const PagedAttnArgs& p, ChunkItem& it, int req, int group) {
-  chunk_request(p, it, req, group, false);
-  it.q0 = same_in_warp(it.q0);
-  it.qn = same_in_warp(it.qn);
-  it.kv = same_in_warp(it.kv);
-  it.rows = it.qn * group;
-  return it.qn > 0;
+  it.rows = r.qn * p.group;
 }
 
 __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t (&r)[32]) {
@@ -165,6 +154,31 @@ __device__ __forceinline__ bool elect_one() {
   return is != 0;
 }
 
+// Two fp32 values in one register pair, and arithmetic on both at once.
+__device__ __forceinline__ uint64_t pack2u(uint32_t lo, uint32_t hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+  return v;
+}
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) { return pack2u(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ float lo_of(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 template <int N>
 __device__ __forceinline__ void regs_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
@@ -182,7 +196,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
   constexpr bool kTwoTerms = Num<T>::is_bf16;
   constexpr uint32_t S_COL = 0, O_COL = 256;
   extern __shared__ __align__(1024) unsigned char s_raw[];
-  __shared__ __align__(8) uint64_t full[NS], empty[NS], q_ready[2], s_full[2][2], p_ready[2][2], pv_done[2][2];
+  __shared__ __align__(8) uint64_t full[NS], empty[NS], q_ready[2], q_free[2], s_full[2][2], p_ready[2][2], pv_done[2][2];
   __shared__ uint32_t s_tmem;
   __shared__ int s_last[2];
   const PagedAttnArgs& p = args.a;
@@ -190,7 +204,6 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
   const int warp = same_in_warp(tid >> 5);
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* ring = smem + 2 * C::kQ;
-  const int group = p.q_heads / p.kv_heads;
 
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
@@ -198,7 +211,8 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       mbar_init(&empty[s], 2);  // both warps of the tensor cores
     }
     for (int q = 0; q < 2; ++q) {
-      mbar_init(&q_ready[q], 4);
+      mbar_init(&q_ready[q], 1);
+      mbar_init(&q_free[q], 1);
       for (int b = 0; b < 2; ++b) {
         mbar_init(&s_full[q][b], 1);
         mbar_init(&p_ready[q][b], 4);
@@ -208,6 +222,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
     fence_barrier_init();
     tma_prefetch_map(&args.k_map);
     tma_prefetch_map(&args.v_map);
+    if (args.q_tma) tma_prefetch_map(&args.q_map);
   }
   if (warp == 1) tmem_alloc(&s_tmem, 512);
   tc_fence_before();
@@ -216,41 +231,54 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
 
   PagedSplit<kChunkJoin> split;
   ChunkItem it;
-  long long before;
+  long long before, in_req;
   int req;
-  paged_find<kChunkThreads>(
+  PagedRequest found;
+  paged_find<kChunkThreads, 32>(
       p.requests,
-      [&](int i) {
+      [&](int i, int part, int parts, PagedRequest& r) {
+        r = paged_request(p, i, part == 0 && blockIdx.x == 0);
         ChunkItem x;
-        if (!chunk_request(p, x, i, group, blockIdx.x == 0)) return 0ll;
+        chunk_request(p, x, i, r);
         long long n = 0;
-        for (x.rt = 0; x.rt * kChunkRows < x.rows; ++x.rt) {
-          chunk_span(p, x, group);
+        for (x.rt = part; x.rt * kChunkRows < x.rows; x.rt += parts) {
+          chunk_span(p, x);
           n += x.n;
         }
         return n * p.kv_heads;
       },
-      split, req, before);
-  paged_zero_rest<T>(p);
+      split, req, found, before, in_req);
   tc_fence_after();  // the barriers inside paged_find have made s_tmem visible
   const uint32_t tmem = s_tmem;
   long long pos = split.start(blockIdx.x);
   const long long end = split.start(blockIdx.x + 1);
   int tile = 0;
-  auto item_of_request = [&](long long rel) {  // the item that holds tile `rel` of request it.req
-    long long per_head = 0;
-    for (it.rt = 0; it.rt * kChunkRows < it.rows; ++it.rt) {
-      chunk_span(p, it, group);
-      per_head += it.n;
-    }
+  auto item_of_request = [&](long long rel) {  // the item that holds tile `rel` of request it.req: a lane a tile of rows
+    const long long per_head = in_req / p.kv_heads;
     it.head = (int)(rel / per_head);
     rel -= it.head * per_head;
-    for (it.rt = 0;; ++it.rt) {
-      chunk_span(p, it, group);
-      if (rel < it.n) break;
-      rel -= it.n;
+    it.rt = 0;
+    for (int rt0 = 0; rt0 * kChunkRows < it.rows; rt0 += 32) {
+      ChunkItem x = it;
+      x.rt = rt0 + lane;
+      x.n = 0;
+      if (x.rt * kChunkRows < x.rows) chunk_span(p, x);
+      int upto = x.n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += u;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, rel < upto);
+      if (hit != 0u) {
+        const int src = __ffs(hit) - 1;
+        it.rt = rt0 + src;
+        tile = (int)rel - __shfl_sync(0xffffffffu, upto - x.n, src);
+        break;
+      }
+      rel -= __shfl_sync(0xffffffffu, upto, 31);
     }
-    tile = (int)rel;
+    chunk_span(p, it);
   };
   auto next_item = [&]() {
     tile = 0;
@@ -258,14 +286,20 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       it.rt = 0;
       if (++it.head == p.kv_heads) {
         it.head = 0;
-        for (int i = it.req + 1; i < p.requests; ++i)
-          if (chunk_load(p, it, i, group)) break;
+        for (int i = it.req + 1; i < p.requests; ++i) {
+          PagedRequest r = paged_request(p, i, false);
+          r.q0 = same_in_warp(r.q0);
+          r.qn = same_in_warp(r.qn);
+          r.kv = same_in_warp(r.kv);
+          chunk_request(p, it, i, r);
+          if (r.qn > 0) break;
+        }
       }
     }
-    chunk_span(p, it, group);
+    chunk_span(p, it);
   };
   if (pos < end) {
-    chunk_load(p, it, req, group);
+    chunk_request(p, it, req, found);
     item_of_request(pos - before);
     const int at = split.snap(tile, it.n);
     pos += at - tile;
@@ -371,6 +405,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
                           idesc_s, i > 0);
                 umma_commit(&s_full[q][b]);
                 if (h == 1) umma_commit(&empty[kslot]);
+                if (h == 1 && k == len - 1) umma_commit(&q_free[q]);
               }
               if (held) values();
               ++n;
@@ -379,12 +414,15 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
                 const int j0 = (it.tile0 + tile + k) * kChunkKeys;
                 if (j0 + kChunkKeys > it.kv || j0 < it.first) {  // rows of V that are nobody's
                   if (q == 0) {
+                    // whole boxes without a key are zeros already: clear what shares a box with one
+                    const int lo = max(0, it.first - j0), lo0 = lo / args.box * args.box;
+                    const int hi = min(kChunkKeys, max(0, it.kv - j0)), hi1 = min(kChunkKeys, (hi + args.box - 1) / args.box * args.box);
                     unsigned char* vs = ring + vslot * C::kSlot;
 #pragma unroll 1
-                    for (int j = 0; j < kChunkKeys; ++j)
-                      if (j0 + j >= it.kv || j0 + j < it.first)
-                        for (int c = lane; c < D / 8; c += 32)
-                          *reinterpret_cast<uint4*>(vs + (c >> 3) * HALF + j * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    for (int e = lane; e < (lo - lo0 + hi1 - hi) * (D / 8); e += 32) {
+                      const int i = e / (D / 8), c = e % (D / 8), j = i < lo - lo0 ? lo0 + i : hi + i - (lo - lo0);
+                      *reinterpret_cast<uint4*>(vs + (c >> 3) * HALF + j * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
                     fence_proxy_async_smem();
                   }
                   if (both) named_barrier(3, 64);
@@ -417,6 +455,51 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         if (pos < end) next_item();
       }
       if (held) values();
+    } else {  // ---- Q of each item, as soon as the scores of the item before are done ----
+      int items[2] = {0, 0};
+      for (int len; (len = take()) > 0;) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int r0 = it.rt * kChunkRows + q * 128;
+          if (r0 >= it.rows) continue;
+          if (items[q] > 0) ok = __all_sync(0xffffffffu, ok && mbar_poll(&q_free[q], (items[q] - 1) & 1, p.status));
+          ++items[q];
+          if (args.q_tma) {  // rows behind the request's are others', or zeros: no score of theirs is used
+            if (ok && lane == 0) {
+              mbar_arrive_expect_tx(&q_ready[q], C::kQ);
+              for (int c = 0; c < D / 64; ++c)
+                tma_load_3d(smem + q * C::kQ + c * HALF, &args.q_map, c * 64, it.head * p.group, it.q0 + paged_token(p, r0),
+                            &q_ready[q]);
+            }
+            __syncwarp();
+          } else {
+            constexpr int PIECES = D / 8, AT_ONCE = 8;  // 16-byte pieces, swizzled as TMA would
+#pragma unroll 1
+            for (int e0 = lane; e0 < 128 * PIECES; e0 += 32 * AT_ONCE) {
+              uint4 u[AT_ONCE];
+#pragma unroll
+              for (int i = 0; i < AT_ONCE; ++i) {
+                const int e = e0 + i * 32, r = r0 + e / PIECES, c = e % PIECES, t = paged_token(p, r);
+                u[i] = make_uint4(0, 0, 0, 0);
+                if (r < it.rows)
+                  u[i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (int64_t)(it.q0 + t) * p.q_token +
+                                                               (int64_t)(it.head * p.group + r - t * p.group) * p.q_head + c * 8));
+              }
+#pragma unroll
+              for (int i = 0; i < AT_ONCE; ++i) {
+                const int e = e0 + i * 32, r = e / PIECES, c = e % PIECES;
+                *reinterpret_cast<uint4*>(smem + q * C::kQ + (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = u[i];
+              }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_ready[q]);
+          }
+        }
+        pos += len;
+        if (pos < end) next_item();
+      }
+      paged_zero_rest<T>(p);
     }
   } else {  // ---- softmax: warpgroup q, thread = row ----
     regs_up<216>();
@@ -426,46 +509,21 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
     const float sl = p.scale * 1.4426950408889634f;  // scores in powers of two
     uint32_t* tickets = static_cast<uint32_t*>(p.workspace);
     float* parts = reinterpret_cast<float*>(tickets + kPagedTickets);
-    // Q of an item into this tile's shared memory: 16-byte pieces, swizzled as TMA would
-    auto load_q = [&](const ChunkItem& x) {
-      const int r0 = x.rt * kChunkRows + q * 128;
-      constexpr int PIECES = D / 8, AT_ONCE = 8;
-      for (int e0 = row; e0 < 128 * PIECES; e0 += 128 * AT_ONCE) {
-        uint4 u[AT_ONCE];
-#pragma unroll
-        for (int i = 0; i < AT_ONCE; ++i) {
-          const int e = e0 + i * 128, r = r0 + e / PIECES, c = e % PIECES, t = r / group;
-          u[i] = make_uint4(0, 0, 0, 0);
-          if (r < x.rows)
-            u[i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (int64_t)(x.q0 + t) * p.q_token +
-                                                         (int64_t)(x.head * group + r - t * group) * p.q_head + c * 8));
-        }
-#pragma unroll
-        for (int i = 0; i < AT_ONCE; ++i) {
-          const int e = e0 + i * 128, r = e / PIECES, c = e % PIECES;
-          *reinterpret_cast<uint4*>(smem + q * C::kQ + (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = u[i];
-        }
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_ready[q]);
-    };
     auto mine = [&](const ChunkItem& x) { return x.rows - x.rt * kChunkRows > q * 128; };
     int n = 0;  // halves done on this tile of rows
-    bool loaded = false;
     for (int len; (len = take()) > 0;) {
       if (!mine(it)) {  // one tile of rows only
         pos += len;
         if (pos < end) next_item();
         continue;
       }
-      if (!loaded) load_q(it);
       const int r = it.rt * kChunkRows + q * 128 + row;
-      const int pq = it.kv - it.qn + r / group;
+      const int pq = it.kv - it.qn + paged_token(p, r);
       const int limit = r < it.rows ? pq + 1 : 0, floor_ = paged_first_key(p, pq);
       // key tiles that every row of this tile sees whole need no mask
       const int r_lo = it.rt * kChunkRows + q * 128, r_hi = min(it.rows, r_lo + 128) - 1;
-      const int all_end = it.kv - it.qn + r_lo / group + 1, all_first = paged_first_key(p, it.kv - it.qn + r_hi / group);
+      const int all_end = it.kv - it.qn + paged_token(p, r_lo) + 1,
+                all_first = paged_first_key(p, it.kv - it.qn + paged_token(p, r_hi));
       float m = -INFINITY, l = 0.f;
       const int halves = 2 * len;
       for (int k = 0; k < halves; ++k, ++n) {
@@ -491,11 +549,13 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         float top[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          top[c] = __uint_as_float(s[c >> 1][(c & 1) * 16]);
+          const uint32_t* x = &s[c >> 1][(c & 1) * 16];
+          top[c] = __uint_as_float(x[0]);
 #pragma unroll
-          for (int i = 1; i < 16; ++i) top[c] = fmaxf(top[c], __uint_as_float(s[c >> 1][(c & 1) * 16 + i]));
+          for (int i = 1; i < 15; i += 2) top[c] = max3(top[c], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+          top[c] = fmaxf(top[c], __uint_as_float(x[15]));
         }
-        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl;
+        const float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]) * sl;
         if (k == 0) {
           m = mx;
         } else {
@@ -521,23 +581,26 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
           }
         }
         const float ref = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t sl2 = pack2(sl, sl), ref2 = pack2(-ref, -ref);
+        uint64_t sum[4] = {0, 0, 0, 0};
         uint32_t w[32], rest[32];  // P, two keys a column
 #pragma unroll
         for (int i = 0; i < 64; i += 2) {
-          uint32_t &s0 = s[i >> 5][i & 31], &s1 = s[i >> 5][(i & 31) + 1];
-          const float p0 = exp2_fast(fmaf(__uint_as_float(s0), sl, -ref));
-          const float p1 = exp2_fast(fmaf(__uint_as_float(s1), sl, -ref));
-          sum[i >> 4] += p0 + p1;
+          const uint64_t x = fma2(pack2u(s[i >> 5][i & 31], s[i >> 5][(i & 31) + 1]), sl2, ref2);
+          const float p0 = exp2_fast(lo_of(x)), p1 = exp2_fast(hi_of(x));
+          const uint64_t pp = pack2(p0, p1);
+          sum[(i >> 1) & 3] = add2(sum[(i >> 1) & 3], pp);
           if constexpr (kTwoTerms) {  // the upper 16 bits as they are, and what is left rounded
             w[i >> 1] = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);
-            rest[i >> 1] = pack_round2<T>(p0 - __uint_as_float(__float_as_uint(p0) & 0xffff0000u),
-                                          p1 - __uint_as_float(__float_as_uint(p1) & 0xffff0000u));
+            const uint64_t left = fma2(pack2u(__float_as_uint(p0) & 0xffff0000u, __float_as_uint(p1) & 0xffff0000u),
+                                       pack2(-1.f, -1.f), pp);
+            rest[i >> 1] = pack_round2<T>(lo_of(left), hi_of(left));
           } else {
             w[i >> 1] = pack_round2<T>(p0, p1);
           }
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        const uint64_t both = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+        l += lo_of(both) + hi_of(both);
         tmem_st32(s_addr + b * 64, w);
         if constexpr (kTwoTerms) tmem_st32(s_addr + b * 64 + 32, rest);
         tmem_wait_st();
@@ -546,34 +609,29 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         if (lane == 0) mbar_arrive(&p_ready[q][b]);
       }
 
-      // The next item's Q, while the last products run: this item's scores are all done.
       const ChunkItem cur = it;
       const int cur_tile = tile;
       const long long item0 = pos - tile;
       pos += len;
-      loaded = false;
-      if (pos < end) {
-        next_item();
-        if (take() > 0 && mine(it)) {
-          load_q(it);
-          loaded = true;
-        }
-      }
+      if (pos < end) next_item();
 
       ok = ok && mbar_poll(&pv_done[q][(n - 1) & 1], ((n - 1) >> 1) & 1, p.status);
       __syncwarp();
       tc_fence_after();
       const bool begins = cur_tile == 0, whole = begins && cur_tile + len == cur.n;
-      const int t = r / group;
+      const int t = paged_token(p, r);
       T* dst = static_cast<T*>(p.out) + (int64_t)(cur.q0 + t) * p.out_token +
-               (int64_t)(cur.head * group + r - t * group) * p.out_head;
-      auto store = [&](int c, const float* v, float inv) {  // 8 columns
-        uint4 u;
-        u.x = pack_round2<T>(v[0] * inv, v[1] * inv);
-        u.y = pack_round2<T>(v[2] * inv, v[3] * inv);
-        u.z = pack_round2<T>(v[4] * inv, v[5] * inv);
-        u.w = pack_round2<T>(v[6] * inv, v[7] * inv);
-        *reinterpret_cast<uint4*>(dst + c) = u;
+               (int64_t)(cur.head * p.group + r - t * p.group) * p.out_head;
+      auto store = [&](int c, const float* v, float inv) {  // 16 columns: a thread a row, so whole sectors
+        uint32_t u[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] = pack_round2<T>(v[2 * i] * inv, v[2 * i + 1] * inv);
+        if (args.out32) {
+          store32(dst + c, u);
+        } else {
+          *reinterpret_cast<uint4*>(dst + c) = make_uint4(u[0], u[1], u[2], u[3]);
+          *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(u[4], u[5], u[6], u[7]);
+        }
       };
       // pieces: [column / 4][row] of four floats, then maxima, then sums
       auto piece = [&](int cta, int first_cta) {
@@ -594,7 +652,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         if (whole) {
           if (r < cur.rows) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) store(c * 32 + i, v + i, inv);
+            for (int i = 0; i < 32; i += 16) store(c * 32 + i, v + i, inv);
           }
         } else {
 #pragma unroll
@@ -651,7 +709,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
               }
             }
 #pragma unroll
-            for (int i = 0; i < 64; i += 8) store(c + i, v + i, inv_all);
+            for (int i = 0; i < 64; i += 16) store(c + i, v + i, inv_all);
           }
         }
         __syncwarp();
@@ -687,6 +745,8 @@ cudaError_t launch_paged_attention_chunk(const PagedAttnArgs& a, int dtype, cuda
   c.a = a;
   c.box = paged_box(a.block_size, kChunkKeys);
   if (c.box < 8 || !paged_maps(a, dtype, c.box, &c.k_map, &c.v_map)) return cudaErrorNotSupported;
+  c.q_tma = paged_q_map(a, dtype, 128, &c.q_map);
+  c.out32 = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_token % 16 == 0 && a.out_head % 16 == 0;
   if (dtype == kBF16)
     return a.dim == 64 ? launch_chunk<__nv_bfloat16, 64>(c, st, pdl) : launch_chunk<__nv_bfloat16, 128>(c, st, pdl);
   return a.dim == 64 ? launch_chunk<__half, 64>(c, st, pdl) : launch_chunk<__half, 128>(c, st, pdl);

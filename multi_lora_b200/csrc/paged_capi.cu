@@ -190,6 +190,8 @@ int mlora_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
   a.requests = (int)requests;
   a.q_heads = q_heads;
   a.kv_heads = c.kv_heads;
+  a.group = q_heads / c.kv_heads;
+  a.group_magic = a.group > 1 ? (uint32_t)((0x100000000ull + a.group - 1) / a.group) : 0u;
   a.dim = c.head_dim;
   a.block_size = c.block_size;
   a.width = (int)max_blocks;
@@ -205,7 +207,9 @@ int mlora_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
                    pieces(c.v, es, c.v_block_stride, c.v_slot_stride, c.v_head_stride);
   const bool pdl = mlora_get_pdl() != 0;
   const cudaStream_t st = (cudaStream_t)stream;
-  if (vec && es == 2) {
+  // rows (tokens x group) times group below 2^32: where division by multiplication is exact
+  const bool rows_ok = (int64_t)a.tokens * a.group * a.group < (1ll << 32);
+  if (vec && es == 2 && rows_ok) {
     const bool few = (int64_t)a.max_q_len * (q_heads / c.kv_heads) <= mlora::kDecodeMaxRows;
     const cudaError_t e = few ? mlora::launch_paged_attention_decode(a, c.dtype, st, pdl)
                               : mlora::launch_paged_attention_chunk(a, c.dtype, st, pdl);

@@ -47,6 +47,11 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedAttnArgs& p, in
   return r;
 }
 
+// Token of a row (row / group).
+__device__ __forceinline__ int paged_token(const PagedAttnArgs& p, int row) {
+  return p.group_magic != 0 ? (int)__umulhi((uint32_t)row, p.group_magic) : row;
+}
+
 // First key that query row `pos` of a request sees.
 __device__ __forceinline__ int paged_first_key(const PagedAttnArgs& p, int pos) {
   return p.window > 0 ? max(0, pos - p.window + 1) : 0;
@@ -80,22 +85,33 @@ struct PagedSplit {
 };
 
 // Whole block of NT threads: the split over the grid, the request that this CTA's first
-// tile lies in, and the tiles before that request. `tiles(i)`: tiles of request i.
-template <int NT, typename F, typename S>
-__device__ __forceinline__ void paged_find(int requests, F tiles, S& split, int& req, long long& before) {
+// tile lies in with its lengths, the tiles before that request and in it.
+// `tiles(i, part, parts, r)`: the tiles of request i (its lengths go to r), or one of
+// `parts` parts of them (a request's items dealt out; up to MAX_PARTS threads
+// count for one request when there are few).
+template <int NT, int MAX_PARTS, typename F, typename S>
+__device__ __forceinline__ void paged_find(int requests, F tiles, S& split, int& req, PagedRequest& found,
+                                           long long& before, long long& in_req) {
   __shared__ long long s_warp[NT / 32];
-  __shared__ long long s_before;
+  __shared__ long long s_before, s_sum;
   __shared__ int s_req;
+  __shared__ PagedRequest s_found;
+  PagedRequest last = {0, 0, 0};
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = (requests + NT - 1) / NT;
-  const int r0 = min(requests, tid * per), r1 = min(requests, r0 + per);
+  int parts = 1;
+  while (parts < MAX_PARTS && 2 * parts * requests <= NT) parts *= 2;
+  const int per = (requests * parts + NT - 1) / NT;  // 1 when parts > 1
+  const int r0 = min(requests, parts > 1 ? tid / parts : tid * per), r1 = min(requests, r0 + per);
+  const int part = tid & (parts - 1);
   long long mine = 0;
-  for (int i = r0; i < r1; ++i) mine += tiles(i);
-  long long incl = mine;
+  for (int i = r0; i < r1; ++i) mine += tiles(i, part, parts, last);
+  long long incl = mine, all_parts = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const long long u = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += u;
+    const long long w = __shfl_xor_sync(0xffffffffu, all_parts, o);
+    if (o < parts) all_parts += w;
   }
   if (lane == 31) s_warp[warp] = incl;
   if (tid == 0) s_req = requests;
@@ -109,24 +125,32 @@ __device__ __forceinline__ void paged_find(int requests, F tiles, S& split, int&
   }
   split.set(same_in_warp(total), gridDim.x);
   const long long a = split.start(blockIdx.x);
-  if (a >= upto && a < upto + mine) {
+  if (part == 0 && a >= upto && a < upto + all_parts) {
     int i = r0;
-    for (long long n = tiles(i); a >= upto + n; n = tiles(++i)) upto += n;
+    if (per > 1) {
+      for (all_parts = tiles(i, 0, 1, last); a >= upto + all_parts; all_parts = tiles(++i, 0, 1, last)) upto += all_parts;
+    }
     s_req = i;
     s_before = upto;
+    s_sum = all_parts;
+    s_found = last;
   }
   __syncthreads();
   req = same_in_warp(s_req);
   before = same_in_warp(s_before);
+  in_req = same_in_warp(s_sum);
+  found.q0 = same_in_warp(s_found.q0);
+  found.qn = same_in_warp(s_found.qn);
+  found.kv = same_in_warp(s_found.kv);
 }
 
-// Rows behind the last request's give zeros; all CTAs share them.
+// Rows behind the last request's give zeros; one warp of every CTA takes a share.
 template <typename T>
 __device__ __forceinline__ void paged_zero_rest(const PagedAttnArgs& p) {
   const int last = p.requests > 0 ? __ldcg(p.q_indptr + p.requests) : 0;
   if (last < 0 || last >= p.tokens) return;
   const int64_t pieces = p.dim / 8, n = (int64_t)(p.tokens - last) * p.q_heads * pieces;
-  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < n; e += (int64_t)gridDim.x * blockDim.x) {
+  for (int64_t e = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31); e < n; e += (int64_t)gridDim.x * 32) {
     const int64_t row = e / pieces;
     T* o = static_cast<T*>(p.out) + (last + row / p.q_heads) * p.out_token + (row % p.q_heads) * p.out_head +
            (e % pieces) * 8;
@@ -156,6 +180,13 @@ __device__ __forceinline__ bool mbar_poll(uint64_t* bar, uint32_t parity, uint32
     }
   }
   return true;
+}
+
+// 32 bytes at once (one sector).
+__device__ __forceinline__ void store32(void* p, const uint32_t (&r)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 
 constexpr int kPagedTickets = 1024;  // words at the start of the workspace, zero between calls

@@ -49,6 +49,21 @@ bool paged_maps(const PagedAttnArgs& a, int dtype, int box, CUtensorMap* k, CUte
          one_map(v, a.v, dtype, a, a.v_slot, a.v_head, a.v_block, box);
 }
 
+bool paged_q_map(const PagedAttnArgs& a, int dtype, int rows, CUtensorMap* q) {
+  const EncodeTiled enc = encode_tiled();
+  if (enc == nullptr || rows % a.group != 0 || a.tokens < 1) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)a.dim, (cuuint64_t)a.q_heads, (cuuint64_t)a.tokens};
+  const cuuint64_t strides[2] = {a.q_heads > 1 ? (cuuint64_t)a.q_head * 2 : (cuuint64_t)a.dim * 2,
+                                 a.tokens > 1 ? (cuuint64_t)a.q_token * 2 : (cuuint64_t)a.dim * 2};
+  for (const cuuint64_t s : strides)
+    if (s == 0 || s % 16 != 0 || s >= (1ull << 40)) return false;
+  const cuuint32_t box[3] = {64, (cuuint32_t)a.group, (cuuint32_t)(rows / a.group)}, ones[3] = {1, 1, 1};
+  return enc(q, dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+             const_cast<void*>(a.q), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int paged_sm_count() {
   static const int n = [] {
     int dev = 0, c = 0;

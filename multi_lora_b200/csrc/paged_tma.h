@@ -18,6 +18,10 @@ inline int paged_box(int block_size, int tile) {
 // 128-byte swizzle, zeros out of range. False where a map cannot describe the cache.
 bool paged_maps(const PagedAttnArgs& a, int dtype, int box, CUtensorMap* k, CUtensorMap* v);
 
+// Map {dim, head, token} over Q, box 64 columns x group heads x rows / group tokens: a
+// tile of `rows` packed rows (token major, then head). False where group does not divide it.
+bool paged_q_map(const PagedAttnArgs& a, int dtype, int rows, CUtensorMap* q);
+
 int paged_sm_count();
 
 }  // namespace mlora
