@@ -28,6 +28,8 @@ namespace mlora {
 
 constexpr int kDecTile = 64;  // keys a stage
 constexpr int kDecJoin = 3;   // joining a piece costs about three tiles
+constexpr int kDecItem = 3;   // and so does an item besides its tiles
+using DecodeSplit = PagedSplit<kDecJoin, kDecItem>;
 
 struct DecodeArgs {
   CUtensorMap k_map, v_map;
@@ -95,7 +97,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
   pdl_wait();
   pdl_trigger();
 
-  PagedSplit<kDecJoin> split;
+  DecodeSplit split;
   DecodeItem it;
   long long before, in_req;
   int req;
@@ -108,20 +110,20 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
         if (blockIdx.x == 0 && r.qn > p.max_q_len) flag_error(p.status, kErrLength);
         DecodeItem x;
         decode_request<MT>(p, x, i, r);
-        return (long long)x.n * p.kv_heads;
+        return x.n > 0 ? (long long)(x.n + kDecItem) * p.kv_heads : 0ll;
       },
       split, req, found, before, in_req);
-  long long pos = split.start(blockIdx.x);
-  const long long end = split.start(blockIdx.x + 1);
-  if (pos >= end) {
+  PagedCursor<DecodeSplit> cur;
+  cur.pos = split.start(blockIdx.x);
+  cur.end = split.start(blockIdx.x + 1);
+  if (cur.pos >= cur.end) {
     if (warp == C::kWarps) paged_zero_rest<T>(p);
     return;
   }
   decode_request<MT>(p, it, req, found);
-  it.head = (int)(pos - before) / it.n;
-  int tile = (int)(pos - before) - it.head * it.n;
+  it.head = (int)(cur.pos - before) / (it.n + kDecItem);
+  cur.unit = (int)(cur.pos - before) - it.head * (it.n + kDecItem);
   auto next_item = [&]() {
-    tile = 0;
     if (++it.head == p.kv_heads) {
       it.head = 0;
       for (int i = it.req + 1; i < p.requests; ++i) {
@@ -130,24 +132,17 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       }
     }
   };
-  {
-    const int at = split.snap(tile, it.n);
-    pos += at - tile;
-    tile = at;
-    if (tile == it.n && pos < split.total) next_item();
-  }
-  // Tiles of the current item that are this CTA's; 0: there is nothing left for it.
-  auto take = [&]() { return pos < end ? split.take(end - (pos - tile), it.n, tile) : 0; };
+  if (cur.begin(it.n, split.total)) next_item();
   bool ok = true;
 
   if (warp == C::kWarps) {  // ---- producer ----
     const int boxes = kDecTile / args.box, jobs = boxes * (D / 64) * 2;
     const int b = lane % boxes, half = (lane / boxes) % (D / 64), side = lane / (boxes * (D / 64));
     int stage = 0, round = 0;
-    for (int len; (len = take()) > 0;) {
+    while (cur.take(it.n)) {
       const int32_t* table = p.tables + it.req * p.table_stride;
-      for (int k = 0; k < len; ++k) {
-        const int j = (it.tile0 + tile + k) * kDecTile + b * args.box;
+      for (int k = 0; k < cur.len; ++k) {
+        const int j = (it.tile0 + cur.tile + k) * kDecTile + b * args.box;
         int block = (int)p.num_blocks, off = 0;  // out of range: zeros
         if (lane < jobs && j < it.kv && j + args.box > it.first) {
           const int e = __ldcg(table + j / p.block_size);
@@ -168,73 +163,103 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
           ++round;
         }
       }
-      pos += len;
-      if (pos < end) next_item();
+      if (cur.advance()) next_item();
     }
     paged_zero_rest<T>(p);
     return;
   }
 
-  // ---- consumers: warp = (16 rows mt, 16 keys of each tile kg) ----
+  // ---- consumers: warp = (16 rows mt, 16 or 32 keys of each tile kg) ----
   const int mt = warp / C::KG, kg = warp % C::KG;
   const float sl = p.scale * 1.4426950408889634f;  // scores in powers of two
   int stage = 0, phase = 0;
+  bool ready = false;  // the next stage is known to be there
   uint32_t* tickets = static_cast<uint32_t*>(p.workspace);
   float* parts = reinterpret_cast<float*>(tickets + kPagedTickets);
   constexpr int PART = MT * 16 * (D + 2);  // floats of a piece: sums, maxima, totals
-  for (int len; (len = take()) > 0;) {
+  // Q fragments: rows lane / 4 and + 8, columns (lane % 4) * 2 (+ 8) of each 16
+  uint32_t qf[D / 16][4];
+  auto load_q = [&](const DecodeItem& x) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = mt * 16 + (lane >> 2) + e * 8, t = paged_token(p, r);
+      const T* src = static_cast<const T*>(p.q) + (int64_t)(x.q0 + t) * p.q_token +
+                     (int64_t)(x.head * group + r - t * group) * p.q_head + (lane & 3) * 2;
+      const bool real = r < x.qn * group;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        qf[k][e] = real ? __ldcg(reinterpret_cast<const unsigned int*>(src + k * 16)) : 0u;
+        qf[k][2 + e] = real ? __ldcg(reinterpret_cast<const unsigned int*>(src + k * 16 + 8)) : 0u;
+      }
+    }
+  };
+  bool more = cur.take(it.n);
+  if (more) load_q(it);
+  while (more) {
     const int rows = it.qn * group;
-    // Q fragments: rows lane / 4 and + 8, columns (lane % 4) * 2 (+ 8) of each 16
-    uint32_t qf[D / 16][4];
     int limit[2], floor_[2];  // keys below `limit` and at or above `floor_` are seen
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int r = mt * 16 + (lane >> 2) + e * 8;
-      const int t = paged_token(p, r);
-      const int pq = it.kv - it.qn + t;
+      const int pq = it.kv - it.qn + paged_token(p, r);
       limit[e] = r < rows ? pq + 1 : 0;
       floor_[e] = paged_first_key(p, pq);
-      const T* src = static_cast<const T*>(p.q) + (it.q0 + t) * p.q_token +
-                     (it.head * group + r - t * group) * p.q_head + (lane & 3) * 2;
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        qf[k][e] = r < rows ? __ldcg(reinterpret_cast<const unsigned int*>(src + k * 16)) : 0u;
-        qf[k][2 + e] = r < rows ? __ldcg(reinterpret_cast<const unsigned int*>(src + k * 16 + 8)) : 0u;
-      }
     }
     float o[D / 8][4];
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    const int all_end = it.kv - it.qn + 1, all_first = paged_first_key(p, it.kv - 1);  // keys that every row sees
 
-    for (int k = 0; k < len; ++k) {
-      ok = ok && mbar_poll(&full[stage], phase, p.status);
+    for (int k = 0; k < cur.len; ++k) {
+      if (!ready) ok = ok && mbar_poll(&full[stage], phase, p.status);
+      const int next = stage + 1 < NS ? stage + 1 : 0;
+      ready = mbar_try_wait(&full[next], next == 0 ? phase ^ 1 : phase);  // answered while this tile is worked on
       __syncwarp();
 #pragma unroll
       for (int sub = 0; sub < C::kSub; ++sub) {
-        const int k0 = (kg * C::kSub + sub) * 16, j0 = (it.tile0 + tile + k) * kDecTile + k0;  // 16 keys
+        const int k0 = (kg * C::kSub + sub) * 16, j0 = (it.tile0 + cur.tile + k) * kDecTile + k0;  // 16 keys
         if (mt * 16 < rows && j0 < it.kv && j0 + 16 > it.first) {
           const uint32_t ks = smem_addr(smem + stage * 2 * SIDE), vs = ks + SIDE;
-          float s[2][4];
+          // All of K's fragments, then the products as four independent chains.
+          uint32_t kf[2][D / 32][4];
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-            const int key = k0 + n * 8 + (lane & 7);
+          for (int c = 0; c < D / 32; ++c)  // 32 columns: two k steps
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) {  // 32 columns: two k steps
-              const int chunk = c * 4 + (lane >> 3);
-              uint32_t b0, b1, b2, b3;
-              ldsm_x4(ks + (chunk >> 3) * HALF + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), b0, b1, b2, b3);
-              mma_16816<T>(s[n], qf[2 * c][0], qf[2 * c][1], qf[2 * c][2], qf[2 * c][3], b0, b1);
-              mma_16816<T>(s[n], qf[2 * c + 1][0], qf[2 * c + 1][1], qf[2 * c + 1][2], qf[2 * c + 1][3], b2, b3);
+            for (int n = 0; n < 2; ++n) {
+              const int key = k0 + n * 8 + (lane & 7), chunk = c * 4 + (lane >> 3);
+              ldsm_x4(ks + (chunk >> 3) * HALF + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), kf[n][c][0], kf[n][c][1],
+                      kf[n][c][2], kf[n][c][3]);
             }
+          float s4[2][2][4];
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s4[n][0][e] = s4[n][1][e] = 0.f;
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int n = 0; n < 2; ++n)
+                mma_16816<T>(s4[n][h], qf[2 * c + h][0], qf[2 * c + h][1], qf[2 * c + h][2], qf[2 * c + h][3],
+                             kf[n][c][2 * h], kf[n][c][2 * h + 1]);
+          // V's fragments, in flight during the softmax: keys (lane % 4) * 2 + {0, 1} and + 8
+          uint32_t vf[D / 16][4];
+          const int key = k0 + (lane & 15);
+#pragma unroll
+          for (int n = 0; n < D / 16; ++n) {  // 16 columns of V
+            const int chunk = n * 2 + (lane >> 4);
+            ldsm_x4_trans(vs + (chunk >> 3) * HALF + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), vf[n][0], vf[n][1],
+                          vf[n][2], vf[n][3]);
           }
-          const bool edge = j0 + 16 > it.kv - it.qn + 1 || j0 < paged_first_key(p, it.kv - 1);  // not all seen by all rows
+          float s[2][4];
+          const bool edge = j0 + 16 > all_end || j0 < all_first;  // not all seen by all rows
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              s[n][e] *= sl;
+              s[n][e] = (s4[n][0][e] + s4[n][1][e]) * sl;
               if (edge) {
                 const int j = j0 + n * 8 + (lane & 3) * 2 + (e & 1);
                 if (j >= limit[e >> 1] || j < floor_[e >> 1]) s[n][e] = -INFINITY;
@@ -269,42 +294,48 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
               o[n][3] *= fix[1];
             }
           }
-          // V: keys of this thread's fragments are (lane % 4) * 2 + {0, 1} and + 8
-          uint32_t clear0 = 0xffffffffu, clear1 = 0xffffffffu;
-          const bool partial = j0 + 16 > it.kv || j0 < it.first;
-          if (partial) {
+          if (j0 + 16 > it.kv || j0 < it.first) {
             const int j = j0 + (lane & 3) * 2;
             auto keep = [&](int x) { return x < it.kv && x >= it.first; };
-            clear0 = (keep(j) ? 0xffffu : 0u) | (keep(j + 1) ? 0xffff0000u : 0u);
-            clear1 = (keep(j + 8) ? 0xffffu : 0u) | (keep(j + 9) ? 0xffff0000u : 0u);
-          }
-          const int key = k0 + (lane & 15);
+            const uint32_t clear0 = (keep(j) ? 0xffffu : 0u) | (keep(j + 1) ? 0xffff0000u : 0u);
+            const uint32_t clear1 = (keep(j + 8) ? 0xffffu : 0u) | (keep(j + 9) ? 0xffff0000u : 0u);
 #pragma unroll
-          for (int n = 0; n < D / 16; ++n) {  // 16 columns of V
-            const int chunk = n * 2 + (lane >> 4);
-            uint32_t b0, b1, b2, b3;
-            ldsm_x4_trans(vs + (chunk >> 3) * HALF + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), b0, b1, b2, b3);
-            if (partial) {
-              b0 &= clear0;
-              b1 &= clear1;
-              b2 &= clear0;
-              b3 &= clear1;
+            for (int n = 0; n < D / 16; ++n) {
+              vf[n][0] &= clear0;
+              vf[n][1] &= clear1;
+              vf[n][2] &= clear0;
+              vf[n][3] &= clear1;
             }
-            mma_16816<T>(o[2 * n], pf[0], pf[1], pf[2], pf[3], b0, b1);
-            mma_16816<T>(o[2 * n + 1], pf[0], pf[1], pf[2], pf[3], b2, b3);
-            if constexpr (kTwoTerms) {
-              mma_16816<T>(o[2 * n], pr[0], pr[1], pr[2], pr[3], b0, b1);
-              mma_16816<T>(o[2 * n + 1], pr[0], pr[1], pr[2], pr[3], b2, b3);
+          }
+#pragma unroll
+          for (int n = 0; n < D / 16; ++n) {
+            mma_16816<T>(o[2 * n], pf[0], pf[1], pf[2], pf[3], vf[n][0], vf[n][1]);
+            mma_16816<T>(o[2 * n + 1], pf[0], pf[1], pf[2], pf[3], vf[n][2], vf[n][3]);
+          }
+          if constexpr (kTwoTerms) {
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n) {
+              mma_16816<T>(o[2 * n], pr[0], pr[1], pr[2], pr[3], vf[n][0], vf[n][1]);
+              mma_16816<T>(o[2 * n + 1], pr[0], pr[1], pr[2], pr[3], vf[n][2], vf[n][3]);
             }
           }
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[stage]);
-      if (++stage == NS) {
-        stage = 0;
-        phase ^= 1;
-      }
+      stage = next;
+      if (stage == 0) phase ^= 1;
+    }
+
+    // The next item's Q, in flight while this one is joined.
+    const DecodeItem done = it;
+    const bool begins = cur.unit == 0, whole = cur.whole(it.n);
+    const long long item0 = cur.pos - cur.unit;
+    more = cur.advance();
+    if (more) {
+      next_item();
+      more = cur.take(it.n);
+      if (more) load_q(it);
     }
 
     // ---- join the key groups of each 16 rows ----
@@ -318,34 +349,43 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       }
     }
     named_barrier(1, C::kWarps * 32);
-    float scale_own[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int r = (lane >> 2) + e * 8;
       float top = -INFINITY;
 #pragma unroll
       for (int g = 0; g < C::KG; ++g) top = fmaxf(top, s_m[mt * C::KG + g][r]);
-      scale_own[e] = top == -INFINITY ? 0.f : exp2_fast(m[e] - top);
+      const float own = top == -INFINITY ? 0.f : exp2_fast(m[e] - top);
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) {
+        o[n][2 * e] *= own;
+        o[n][2 * e + 1] *= own;
+      }
     }
     for (int g = 0; g < C::KG; ++g) {
       if (kg == g) {
+        float* d = merge + (mt * 16 + (lane >> 2)) * C::kRowF + (lane & 3) * 2;
+        if (g > 0) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float2 u[D / 8];  // all the loads first
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) u[n] = *reinterpret_cast<const float2*>(d + e * 8 * C::kRowF + n * 8);
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) {
+              o[n][2 * e] += u[n].x;
+              o[n][2 * e + 1] += u[n].y;
+            }
+          }
+        }
 #pragma unroll
         for (int n = 0; n < D / 8; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float2* d = reinterpret_cast<float2*>(merge + (mt * 16 + (lane >> 2) + e * 8) * C::kRowF + n * 8 + (lane & 3) * 2);
-            float2 v = make_float2(o[n][2 * e] * scale_own[e], o[n][2 * e + 1] * scale_own[e]);
-            if (g > 0) {
-              const float2 u = *d;
-              v.x += u.x;
-              v.y += u.y;
-            }
-            *d = v;
-          }
+          for (int e = 0; e < 2; ++e)
+            *reinterpret_cast<float2*>(d + e * 8 * C::kRowF + n * 8) = make_float2(o[n][2 * e], o[n][2 * e + 1]);
       }
       named_barrier(1, C::kWarps * 32);
     }
-    const bool begins = tile == 0, ends = tile + len == it.n, whole = begins && ends;
     auto row_stat = [&](int r, float& top, float& sum) {  // over the key groups of row r
       const int w = (r >> 4) * C::KG, i = r & 15;
       top = s_m[w][i];
@@ -357,7 +397,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     };
     auto store = [&](int r, int c, const float* v, float inv) {  // 8 columns of row r
       const int t = paged_token(p, r);
-      T* dst = static_cast<T*>(p.out) + (it.q0 + t) * p.out_token + (it.head * group + r - t * group) * p.out_head + c;
+      T* dst = static_cast<T*>(p.out) + (done.q0 + t) * p.out_token + (done.head * group + r - t * group) * p.out_head + c;
       uint4 u;
       u.x = pack_round2<T>(v[0] * inv, v[1] * inv);
       u.y = pack_round2<T>(v[2] * inv, v[3] * inv);
@@ -385,8 +425,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       }
     }
     if (!whole) {
-      const long long item0 = pos - tile;
-      const int c0 = split.first_cta(item0, it.n), c1 = split.last_cta(item0, it.n);
+      const int c0 = split.first_cta(item0, done.n), c1 = split.last_cta(item0, done.n);
       __threadfence();
       named_barrier(1, C::kWarps * 32);
       if (tid == 0) {
@@ -401,6 +440,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
         for (int e = tid; e < rows * (D / 8); e += C::kWarps * 32) {
           const int r = e / (D / 8), c = (e % (D / 8)) * 8;
           float top = -INFINITY, sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
           for (int x = c0; x <= c1; ++x) top = fmaxf(top, __ldcg(piece(x) + MT * 16 * D + r));
           if (top != -INFINITY) {
 #pragma unroll 4
@@ -425,8 +465,6 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       }
     }
     named_barrier(1, C::kWarps * 32);  // the merge buffer and s_last are free again
-    pos += len;
-    if (pos < end) next_item();
   }
 }
 

@@ -41,6 +41,8 @@ constexpr int kHalfKeys = 64;     // keys a step of the tensor cores and the sof
 constexpr int kChunkRows = 256;   // query rows an item: two tiles of 128
 constexpr int kChunkThreads = 384;
 constexpr int kChunkJoin = 3;     // joining a piece costs about three key tiles
+constexpr int kChunkItem = 3;     // and so does an item besides its tiles
+using ChunkSplit = PagedSplit<kChunkJoin, kChunkItem>;
 
 struct ChunkArgs {
   CUtensorMap k_map, v_map, q_map;
@@ -229,7 +231,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
   pdl_wait();
   pdl_trigger();
 
-  PagedSplit<kChunkJoin> split;
+  ChunkSplit split;
   ChunkItem it;
   long long before, in_req;
   int req;
@@ -243,17 +245,18 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         long long n = 0;
         for (x.rt = part; x.rt * kChunkRows < x.rows; x.rt += parts) {
           chunk_span(p, x);
-          n += x.n;
+          n += x.n + kChunkItem;
         }
         return n * p.kv_heads;
       },
       split, req, found, before, in_req);
   tc_fence_after();  // the barriers inside paged_find have made s_tmem visible
   const uint32_t tmem = s_tmem;
-  long long pos = split.start(blockIdx.x);
-  const long long end = split.start(blockIdx.x + 1);
-  int tile = 0;
-  auto item_of_request = [&](long long rel) {  // the item that holds tile `rel` of request it.req: a lane a tile of rows
+  PagedCursor<ChunkSplit> cur;
+  cur.pos = split.start(blockIdx.x);
+  cur.end = split.start(blockIdx.x + 1);
+  cur.unit = 0;
+  auto item_of_request = [&](long long rel) {  // the item that holds unit `rel` of request it.req: a lane a tile of rows
     const long long per_head = in_req / p.kv_heads;
     it.head = (int)(rel / per_head);
     rel -= it.head * per_head;
@@ -261,9 +264,12 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
     for (int rt0 = 0; rt0 * kChunkRows < it.rows; rt0 += 32) {
       ChunkItem x = it;
       x.rt = rt0 + lane;
-      x.n = 0;
-      if (x.rt * kChunkRows < x.rows) chunk_span(p, x);
-      int upto = x.n;
+      int units = 0;
+      if (x.rt * kChunkRows < x.rows) {
+        chunk_span(p, x);
+        units = x.n + kChunkItem;
+      }
+      int upto = units;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, upto, o);
@@ -273,7 +279,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       if (hit != 0u) {
         const int src = __ffs(hit) - 1;
         it.rt = rt0 + src;
-        tile = (int)rel - __shfl_sync(0xffffffffu, upto - x.n, src);
+        cur.unit = (int)rel - __shfl_sync(0xffffffffu, upto - units, src);
         break;
       }
       rel -= __shfl_sync(0xffffffffu, upto, 31);
@@ -281,7 +287,6 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
     chunk_span(p, it);
   };
   auto next_item = [&]() {
-    tile = 0;
     if (++it.rt * kChunkRows >= it.rows) {
       it.rt = 0;
       if (++it.head == p.kv_heads) {
@@ -298,16 +303,11 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
     }
     chunk_span(p, it);
   };
-  if (pos < end) {
+  if (cur.pos < cur.end) {
     chunk_request(p, it, req, found);
-    item_of_request(pos - before);
-    const int at = split.snap(tile, it.n);
-    pos += at - tile;
-    tile = at;
-    if (tile == it.n && pos < split.total) next_item();
+    item_of_request(cur.pos - before);
+    if (cur.begin(it.n, split.total)) next_item();
   }
-  // Tiles of the current item that are this CTA's; 0: there is nothing left for it.
-  auto take = [&]() { return pos < end ? split.take(end - (pos - tile), it.n, tile) : 0; };
   bool ok = true;
 
   // Registers: 384 threads are launched with 168 each (64512); the four warps of
@@ -319,10 +319,10 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       const int boxes = kChunkKeys / args.box, jobs = boxes * (D / 64);
       const int b = lane % boxes, half = lane / boxes;
       int slot = 0, round = 0;
-      for (int len; (len = take()) > 0;) {
+      while (cur.take(it.n)) {
         const int32_t* table = p.tables + it.req * p.table_stride;
-        for (int k = 0; k < len; ++k) {
-          const int j = (it.tile0 + tile + k) * kChunkKeys + b * args.box;
+        for (int k = 0; k < cur.len; ++k) {
+          const int j = (it.tile0 + cur.tile + k) * kChunkKeys + b * args.box;
           int block = (int)p.num_blocks, off = 0;  // out of range: zeros
           if (lane < jobs && j < it.end && j + args.box > it.first) {
             const int e = __ldcg(table + j / p.block_size);
@@ -346,8 +346,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
             }
           }
         }
-        pos += len;
-        if (pos < end) next_item();
+        if (cur.advance()) next_item();
       }
     } else if (warp < 3) {  // ---- tensor cores, a warp a tile of rows: S of a half, then O of the half before ----
       // A wait costs its warp over 100 cycles even when it need not wait, and the tensor
@@ -382,12 +381,12 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         }
         held = false;
       };
-      for (int len; (len = take()) > 0;) {
+      while (cur.take(it.n)) {
         const bool mine = it.rows - it.rt * kChunkRows > q * 128;
         const bool both = it.rows - it.rt * kChunkRows > 128;
         if (held) values();  // nothing of the item before waits for this one's Q, or keeps its V from the ring
 #pragma unroll 1
-        for (int k = 0; k < len; ++k) {
+        for (int k = 0; k < cur.len; ++k) {
           wait(&full[kslot], k_phase);
           if (mine) {
 #pragma unroll 1
@@ -405,13 +404,13 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
                           idesc_s, i > 0);
                 umma_commit(&s_full[q][b]);
                 if (h == 1) umma_commit(&empty[kslot]);
-                if (h == 1 && k == len - 1) umma_commit(&q_free[q]);
+                if (h == 1 && k == cur.len - 1) umma_commit(&q_free[q]);
               }
               if (held) values();
               ++n;
               if (h == 0) {
                 wait(&full[vslot], v_phase);
-                const int j0 = (it.tile0 + tile + k) * kChunkKeys;
+                const int j0 = (it.tile0 + cur.tile + k) * kChunkKeys;
                 if (j0 + kChunkKeys > it.kv || j0 < it.first) {  // rows of V that are nobody's
                   if (q == 0) {
                     // whole boxes without a key are zeros already: clear what shares a box with one
@@ -451,13 +450,12 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
             v_phase ^= 1;
           }
         }
-        pos += len;
-        if (pos < end) next_item();
+        if (cur.advance()) next_item();
       }
       if (held) values();
     } else {  // ---- Q of each item, as soon as the scores of the item before are done ----
       int items[2] = {0, 0};
-      for (int len; (len = take()) > 0;) {
+      while (cur.take(it.n)) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           const int r0 = it.rt * kChunkRows + q * 128;
@@ -496,8 +494,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
             if (lane == 0) mbar_arrive(&q_ready[q]);
           }
         }
-        pos += len;
-        if (pos < end) next_item();
+        if (cur.advance()) next_item();
       }
       paged_zero_rest<T>(p);
     }
@@ -511,10 +508,9 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
     float* parts = reinterpret_cast<float*>(tickets + kPagedTickets);
     auto mine = [&](const ChunkItem& x) { return x.rows - x.rt * kChunkRows > q * 128; };
     int n = 0;  // halves done on this tile of rows
-    for (int len; (len = take()) > 0;) {
+    while (cur.take(it.n)) {
       if (!mine(it)) {  // one tile of rows only
-        pos += len;
-        if (pos < end) next_item();
+        if (cur.advance()) next_item();
         continue;
       }
       const int r = it.rt * kChunkRows + q * 128 + row;
@@ -525,7 +521,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       const int all_end = it.kv - it.qn + paged_token(p, r_lo) + 1,
                 all_first = paged_first_key(p, it.kv - it.qn + paged_token(p, r_hi));
       float m = -INFINITY, l = 0.f;
-      const int halves = 2 * len;
+      const int halves = 2 * cur.len;
       for (int k = 0; k < halves; ++k, ++n) {
         const int b = n & 1;
         ok = ok && mbar_poll(&s_full[q][b], (n >> 1) & 1, p.status);
@@ -537,7 +533,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         tmem_wait_ld();
         tie32(s[0]);
         tie32(s[1]);
-        const int j0 = (it.tile0 + tile) * kChunkKeys + k * kHalfKeys;
+        const int j0 = (it.tile0 + cur.tile) * kChunkKeys + k * kHalfKeys;
         if (j0 + kHalfKeys > all_end || j0 < all_first) {
           const int hi = limit - j0, lo = floor_ - j0;
 #pragma unroll
@@ -609,19 +605,17 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         if (lane == 0) mbar_arrive(&p_ready[q][b]);
       }
 
-      const ChunkItem cur = it;
-      const int cur_tile = tile;
-      const long long item0 = pos - tile;
-      pos += len;
-      if (pos < end) next_item();
+      const ChunkItem done = it;
+      const bool whole = cur.whole(it.n);
+      const long long item0 = cur.pos - cur.unit;
+      if (cur.advance()) next_item();
 
       ok = ok && mbar_poll(&pv_done[q][(n - 1) & 1], ((n - 1) >> 1) & 1, p.status);
       __syncwarp();
       tc_fence_after();
-      const bool begins = cur_tile == 0, whole = begins && cur_tile + len == cur.n;
       const int t = paged_token(p, r);
-      T* dst = static_cast<T*>(p.out) + (int64_t)(cur.q0 + t) * p.out_token +
-               (int64_t)(cur.head * p.group + r - t * p.group) * p.out_head;
+      T* dst = static_cast<T*>(p.out) + (int64_t)(done.q0 + t) * p.out_token +
+               (int64_t)(done.head * p.group + r - t * p.group) * p.out_head;
       auto store = [&](int c, const float* v, float inv) {  // 16 columns: a thread a row, so whole sectors
         uint32_t u[8];
 #pragma unroll
@@ -637,7 +631,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       auto piece = [&](int cta, int first_cta) {
         return parts + (((long long)cta * 2 + (cta == first_cta ? 1 : 0)) * 2 + q) * C::kPart;
       };
-      const int c0 = whole ? 0 : split.first_cta(item0, cur.n);
+      const int c0 = whole ? 0 : split.first_cta(item0, done.n);
       float* part = piece(blockIdx.x, c0);
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll 1
@@ -650,7 +644,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]);
         if (whole) {
-          if (r < cur.rows) {
+          if (r < done.rows) {
 #pragma unroll
             for (int i = 0; i < 32; i += 16) store(c * 32 + i, v + i, inv);
           }
@@ -665,7 +659,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       if (!whole) {
         __stcg(part + 128 * D + row, m);
         __stcg(part + 128 * (D + 1) + row, l);
-        const int c1 = split.last_cta(item0, cur.n);
+        const int c1 = split.last_cta(item0, done.n);
         __threadfence();
         named_barrier(1 + q, 128);
         if (row == 0) {
@@ -678,7 +672,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         named_barrier(1 + q, 128);
         const bool last = s_last[q];
         named_barrier(1 + q, 128);
-        if (last && r < cur.rows) {
+        if (last && r < done.rows) {
           float top = -INFINITY, total = 0.f;
 #pragma unroll 4
           for (int x = c0; x <= c1; ++x) top = fmaxf(top, __ldcg(piece(x, c0) + 128 * D + row));

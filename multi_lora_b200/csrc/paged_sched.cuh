@@ -57,40 +57,74 @@ __device__ __forceinline__ int paged_first_key(const PagedAttnArgs& p, int pos) 
   return p.window > 0 ? max(0, pos - p.window + 1) : 0;
 }
 
-// The even split of `total` tiles over the CTAs, with boundaries that fall within T
-// tiles of an item's edge moved to that edge: joining a piece costs about as much as T tiles,
-// so no piece is shorter than that, and short items stay whole.
-template <int T>
+// The even split over the CTAs, in units of a key tile's time. An item of n tiles
+// counts n + C units: C for what it costs besides its tiles (its Q, its join or
+// its output), so that many short items weigh what they take. Boundaries that fall
+// within T units of an item's edge move to that edge: joining a piece costs about as much as T
+// tiles, so no piece is shorter than that, and short items stay whole.
+template <int T, int C>
 struct PagedSplit {
-  long long total, base, rem;  // CTA c has base tiles, the first `rem` CTAs one more
-  __device__ void set(long long tiles, int ctas) {
-    total = tiles;
-    base = tiles / ctas;
-    rem = tiles - base * ctas;
+  static constexpr int kItem = C;
+  long long total, base, rem;  // CTA c has base units, the first `rem` CTAs one more
+  __device__ void set(long long units, int ctas) {
+    total = units;
+    base = units / ctas;
+    rem = units - base * ctas;
   }
   __device__ long long start(long long c) const { return c * base + min(c, rem); }
-  __device__ int owner(long long tile) const {
+  __device__ int owner(long long unit) const {
     const long long wide = rem * (base + 1);
-    return (int)(tile < wide ? tile / (base + 1) : rem + (tile - wide) / base);
+    return (int)(unit < wide ? unit / (base + 1) : rem + (unit - wide) / base);
   }
-  // Where a boundary x tiles into an item of n goes.
+  // Where a boundary x units into an item of n tiles goes.
   static __device__ int snap(long long x, int n) {
-    return x >= n ? n : x <= min(T, n / 2) ? 0 : n - x <= T ? n : (int)x;
+    return x >= n + C ? n + C : x <= min(T + C, (n + C) / 2) ? 0 : n + C - x <= T ? n + C : (int)x;
   }
-  // Tiles from `tile` on that a CTA whose range ends `raw` tiles into the item takes.
-  static __device__ int take(long long raw, int n, int tile) { return snap(raw, n) - tile; }
-  // The CTAs that share an item of n tiles beginning at tile `item`; more than one of them.
-  __device__ int first_cta(long long item, int n) const { return owner(item + min(T, n / 2)); }
-  __device__ int last_cta(long long item, int n) const { return owner(item + n - T - 1); }
+  // The CTAs that share an item of n tiles beginning at unit `item`; more than one of them.
+  __device__ int first_cta(long long item, int n) const { return owner(item + min(T + C, (n + C) / 2)); }
+  __device__ int last_cta(long long item, int n) const { return owner(item + n + C - T - 1); }
+};
+
+// A CTA's way through its units: the current item begins at `pos - unit`, and the
+// CTA's part of it is the tiles [tile, tile + len).
+template <typename S>
+struct PagedCursor {
+  long long pos, end;
+  int unit, tile, len, step;
+  // The CTA's part of an item of n tiles; false: nothing is left for it.
+  __device__ __forceinline__ bool take(int n) {
+    if (pos >= end) return false;
+    const int stop = S::snap(end - (pos - unit), n);
+    step = stop - unit;
+    tile = unit == 0 ? 0 : unit - S::kItem;
+    len = stop - S::kItem - tile;
+    return step > 0;
+  }
+  __device__ __forceinline__ bool whole(int n) const { return unit == 0 && step == n + S::kItem; }
+  // Past that part; true when the next item has to be looked up.
+  __device__ __forceinline__ bool advance() {
+    pos += step;
+    unit = 0;
+    return pos < end;
+  }
+  // The first boundary, `unit` units into an item of n tiles; true as for advance.
+  __device__ __forceinline__ bool begin(int n, long long total) {
+    const int at = S::snap(unit, n);
+    pos += at - unit;
+    unit = at;
+    if (at < n + S::kItem) return false;
+    unit = 0;
+    return pos < total;
+  }
 };
 
 // Whole block of NT threads: the split over the grid, the request that this CTA's first
-// tile lies in with its lengths, the tiles before that request and in it.
-// `tiles(i, part, parts, r)`: the tiles of request i (its lengths go to r), or one of
+// unit lies in with its lengths, the units before that request and in it.
+// `units(i, part, parts, r)`: the units of request i (its lengths go to r), or one of
 // `parts` parts of them (a request's items dealt out; up to MAX_PARTS threads
 // count for one request when there are few).
 template <int NT, int MAX_PARTS, typename F, typename S>
-__device__ __forceinline__ void paged_find(int requests, F tiles, S& split, int& req, PagedRequest& found,
+__device__ __forceinline__ void paged_find(int requests, F units, S& split, int& req, PagedRequest& found,
                                            long long& before, long long& in_req) {
   __shared__ long long s_warp[NT / 32];
   __shared__ long long s_before, s_sum;
@@ -104,7 +138,7 @@ __device__ __forceinline__ void paged_find(int requests, F tiles, S& split, int&
   const int r0 = min(requests, parts > 1 ? tid / parts : tid * per), r1 = min(requests, r0 + per);
   const int part = tid & (parts - 1);
   long long mine = 0;
-  for (int i = r0; i < r1; ++i) mine += tiles(i, part, parts, last);
+  for (int i = r0; i < r1; ++i) mine += units(i, part, parts, last);
   long long incl = mine, all_parts = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -128,7 +162,7 @@ __device__ __forceinline__ void paged_find(int requests, F tiles, S& split, int&
   if (part == 0 && a >= upto && a < upto + all_parts) {
     int i = r0;
     if (per > 1) {
-      for (all_parts = tiles(i, 0, 1, last); a >= upto + all_parts; all_parts = tiles(++i, 0, 1, last)) upto += all_parts;
+      for (all_parts = units(i, 0, 1, last); a >= upto + all_parts; all_parts = units(++i, 0, 1, last)) upto += all_parts;
     }
     s_req = i;
     s_before = upto;
