@@ -16,7 +16,7 @@
 //   * key tiles are dealt evenly over the CTAs (paged_sched.cuh).
 // Keys outside [first, kv) may hold anything: scores are replaced, not added
 // to, and their V fragments are cleared before the product, since 0 * NaN is NaN.
-#include <mutex>
+#include <climits>
 
 #include "kernels.h"
 #include "mma.cuh"
@@ -99,7 +99,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
 
   DecodeSplit split;
   DecodeItem it;
-  long long before, in_req;
+  int before, in_req;
   int req;
   PagedRequest found;
   paged_find<C::kThreads, 1>(
@@ -110,19 +110,18 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
         if (blockIdx.x == 0 && r.qn > p.max_q_len) flag_error(p.status, kErrLength);
         DecodeItem x;
         decode_request<MT>(p, x, i, r);
-        return x.n > 0 ? (long long)(x.n + kDecItem) * p.kv_heads : 0ll;
+        return x.n > 0 ? (x.n + kDecItem) * p.kv_heads : 0;
       },
       split, req, found, before, in_req);
-  PagedCursor<DecodeSplit> cur;
-  cur.pos = split.start(blockIdx.x);
-  cur.end = split.start(blockIdx.x + 1);
+  __syncthreads();  // the barriers are initialised
+  PagedCursor<DecodeSplit> cur(split);
   if (cur.pos >= cur.end) {
     if (warp == C::kWarps) paged_zero_rest<T>(p);
     return;
   }
   decode_request<MT>(p, it, req, found);
-  it.head = (int)(cur.pos - before) / (it.n + kDecItem);
-  cur.unit = (int)(cur.pos - before) - it.head * (it.n + kDecItem);
+  it.head = (cur.pos - before) / (it.n + kDecItem);
+  cur.unit = cur.pos - before - it.head * (it.n + kDecItem);
   auto next_item = [&]() {
     if (++it.head == p.kv_heads) {
       it.head = 0;
@@ -132,7 +131,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       }
     }
   };
-  if (cur.begin(it.n, split.total)) next_item();
+  if (cur.begin(it.n)) next_item();
   bool ok = true;
 
   if (warp == C::kWarps) {  // ---- producer ----
@@ -214,7 +213,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     for (int k = 0; k < cur.len; ++k) {
       if (!ready) ok = ok && mbar_poll(&full[stage], phase, p.status);
       const int next = stage + 1 < NS ? stage + 1 : 0;
-      ready = mbar_try_wait(&full[next], next == 0 ? phase ^ 1 : phase);  // answered while this tile is worked on
+      ready = mbar_test(&full[next], next == 0 ? phase ^ 1 : phase);  // answered while this tile is worked on
       __syncwarp();
 #pragma unroll
       for (int sub = 0; sub < C::kSub; ++sub) {
@@ -330,7 +329,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     // The next item's Q, in flight while this one is joined.
     const DecodeItem done = it;
     const bool begins = cur.unit == 0, whole = cur.whole(it.n);
-    const long long item0 = cur.pos - cur.unit;
+    const int item0 = cur.pos - cur.unit;
     more = cur.advance();
     if (more) {
       next_item();
@@ -338,7 +337,8 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       if (more) load_q(it);
     }
 
-    // ---- join the key groups of each 16 rows ----
+    // ---- join the key groups of each 16 rows: `slots` of them lie side by side in the
+    // merge buffer where the rows are few, further ones are added in turn ----
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
@@ -348,6 +348,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
         s_l[warp][(lane >> 2) + e * 8] = l[e];
       }
     }
+    const int slots = rows <= 4 ? min(4, C::KG) : rows <= 8 ? 2 : 1, apart = 16 / (rows <= 4 ? 4 : slots);
     named_barrier(1, C::kWarps * 32);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -362,27 +363,27 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
         o[n][2 * e + 1] *= own;
       }
     }
-    for (int g = 0; g < C::KG; ++g) {
-      if (kg == g) {
-        float* d = merge + (mt * 16 + (lane >> 2)) * C::kRowF + (lane & 3) * 2;
-        if (g > 0) {
+    for (int g = 0; g < C::KG; g += slots) {
+      if (kg >= g && kg < g + slots) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
+        for (int e = 0; e < 2; ++e) {
+          const int r = (lane >> 2) + e * 8;
+          if (mt * 16 + r >= rows) continue;
+          float* d = merge + (mt * 16 + (kg - g) * apart + r) * C::kRowF + (lane & 3) * 2;
+          if (g > 0) {
             float2 u[D / 8];  // all the loads first
 #pragma unroll
-            for (int n = 0; n < D / 8; ++n) u[n] = *reinterpret_cast<const float2*>(d + e * 8 * C::kRowF + n * 8);
+            for (int n = 0; n < D / 8; ++n) u[n] = *reinterpret_cast<const float2*>(d + n * 8);
 #pragma unroll
             for (int n = 0; n < D / 8; ++n) {
               o[n][2 * e] += u[n].x;
               o[n][2 * e + 1] += u[n].y;
             }
           }
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n)
+            *reinterpret_cast<float2*>(d + n * 8) = make_float2(o[n][2 * e], o[n][2 * e + 1]);
         }
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            *reinterpret_cast<float2*>(d + e * 8 * C::kRowF + n * 8) = make_float2(o[n][2 * e], o[n][2 * e + 1]);
       }
       named_barrier(1, C::kWarps * 32);
     }
@@ -410,25 +411,34 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       const int r = e / (D / 8), c = (e % (D / 8)) * 8;
       float top, sum;
       row_stat(r, top, sum);
-      const float4 v0 = *reinterpret_cast<const float4*>(merge + r * C::kRowF + c);
-      const float4 v1 = *reinterpret_cast<const float4*>(merge + r * C::kRowF + c + 4);
+      float4 v0 = *reinterpret_cast<const float4*>(merge + r * C::kRowF + c);
+      float4 v1 = *reinterpret_cast<const float4*>(merge + r * C::kRowF + c + 4);
+      for (int g = 1; g < slots; ++g) {
+        const float4 u0 = *reinterpret_cast<const float4*>(merge + (r + g * apart) * C::kRowF + c);
+        const float4 u1 = *reinterpret_cast<const float4*>(merge + (r + g * apart) * C::kRowF + c + 4);
+        v0.x += u0.x;
+        v0.y += u0.y;
+        v0.z += u0.z;
+        v0.w += u0.w;
+        v1.x += u1.x;
+        v1.y += u1.y;
+        v1.z += u1.z;
+        v1.w += u1.w;
+      }
       if (whole) {
         const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
         store(r, c, v, sum > 0.f || sum != sum ? 1.f / sum : 0.f);
       } else {
         __stcg(reinterpret_cast<float4*>(part + r * D + c), v0);
         __stcg(reinterpret_cast<float4*>(part + r * D + c + 4), v1);
-        if (c == 0) {
-          __stcg(part + MT * 16 * D + r, top);
-          __stcg(part + MT * 16 * (D + 1) + r, sum);
-        }
+        if (c == 0) __stcg(reinterpret_cast<float2*>(part + MT * 16 * D) + r, make_float2(top, sum));
       }
     }
     if (!whole) {
       const int c0 = split.first_cta(item0, done.n), c1 = split.last_cta(item0, done.n);
-      __threadfence();
       named_barrier(1, C::kWarps * 32);
       if (tid == 0) {
+        __threadfence();
         const bool last = atomicAdd(tickets + c0, 1u) == (uint32_t)(c1 - c0);
         if (last) tickets[c0] = 0u;
         __threadfence();
@@ -440,25 +450,24 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
         for (int e = tid; e < rows * (D / 8); e += C::kWarps * 32) {
           const int r = e / (D / 8), c = (e % (D / 8)) * 8;
           float top = -INFINITY, sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-          for (int x = c0; x <= c1; ++x) top = fmaxf(top, __ldcg(piece(x) + MT * 16 * D + r));
-          if (top != -INFINITY) {
-#pragma unroll 4
-            for (int x = c0; x <= c1; ++x) {
-              const float* src = piece(x);
-              const float w = exp2_fast(__ldcg(src + MT * 16 * D + r) - top);
-              sum = fmaf(__ldcg(src + MT * 16 * (D + 1) + r), w, sum);
-              const float4 v0 = __ldcg(reinterpret_cast<const float4*>(src + r * D + c));
-              const float4 v1 = __ldcg(reinterpret_cast<const float4*>(src + r * D + c + 4));
-              v[0] = fmaf(v0.x, w, v[0]);
-              v[1] = fmaf(v0.y, w, v[1]);
-              v[2] = fmaf(v0.z, w, v[2]);
-              v[3] = fmaf(v0.w, w, v[3]);
-              v[4] = fmaf(v1.x, w, v[4]);
-              v[5] = fmaf(v1.y, w, v[5]);
-              v[6] = fmaf(v1.z, w, v[6]);
-              v[7] = fmaf(v1.w, w, v[7]);
-            }
+#pragma unroll 8
+          for (int x = c0; x <= c1; ++x) {
+            const float* src = piece(x);
+            const float2 stat = __ldcg(reinterpret_cast<const float2*>(src + MT * 16 * D) + r);
+            const float4 v0 = __ldcg(reinterpret_cast<const float4*>(src + r * D + c));
+            const float4 v1 = __ldcg(reinterpret_cast<const float4*>(src + r * D + c + 4));
+            const float m_new = fmaxf(top, stat.x), ref = m_new == -INFINITY ? 0.f : m_new;
+            const float fix = exp2_fast(top - ref), w = exp2_fast(stat.x - ref);
+            top = m_new;
+            sum = fmaf(sum, fix, stat.y * w);
+            v[0] = fmaf(v[0], fix, v0.x * w);
+            v[1] = fmaf(v[1], fix, v0.y * w);
+            v[2] = fmaf(v[2], fix, v0.z * w);
+            v[3] = fmaf(v[3], fix, v0.w * w);
+            v[4] = fmaf(v[4], fix, v1.x * w);
+            v[5] = fmaf(v[5], fix, v1.y * w);
+            v[6] = fmaf(v[6], fix, v1.z * w);
+            v[7] = fmaf(v[7], fix, v1.w * w);
           }
           store(r, c, v, sum > 0.f || sum != sum ? 1.f / sum : 0.f);
         }
@@ -496,6 +505,9 @@ cudaError_t launch_decode_m(const DecodeArgs& a, int rows, cudaStream_t st, bool
 
 cudaError_t launch_paged_attention_decode(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl) {
   if ((dtype != kBF16 && dtype != kF16) || (a.dim != 64 && a.dim != 128)) return cudaErrorNotSupported;
+  // units of work (paged_sched.cuh) in 32 bits
+  if ((long long)a.requests * a.kv_heads * ((long long)a.width * a.block_size / kDecTile + 2 + kDecItem) > INT_MAX)
+    return cudaErrorNotSupported;
   DecodeArgs d{};
   d.a = a;
   d.box = paged_box(a.block_size, kDecTile);

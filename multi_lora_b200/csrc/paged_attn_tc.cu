@@ -29,6 +29,8 @@
 //
 // Keys behind the cache's end may hold anything: their scores are replaced,
 // and their rows of V are cleared in shared memory, since 0 * NaN is NaN.
+#include <climits>
+
 #include "kernels.h"
 #include "paged_sched.cuh"
 #include "paged_tma.h"
@@ -233,7 +235,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
 
   ChunkSplit split;
   ChunkItem it;
-  long long before, in_req;
+  int before, in_req;
   int req;
   PagedRequest found;
   paged_find<kChunkThreads, 32>(
@@ -242,7 +244,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         r = paged_request(p, i, part == 0 && blockIdx.x == 0);
         ChunkItem x;
         chunk_request(p, x, i, r);
-        long long n = 0;
+        int n = 0;
         for (x.rt = part; x.rt * kChunkRows < x.rows; x.rt += parts) {
           chunk_span(p, x);
           n += x.n + kChunkItem;
@@ -250,15 +252,13 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         return n * p.kv_heads;
       },
       split, req, found, before, in_req);
-  tc_fence_after();  // the barriers inside paged_find have made s_tmem visible
+  __syncthreads();  // the barriers are initialised and s_tmem is there
+  tc_fence_after();
   const uint32_t tmem = s_tmem;
-  PagedCursor<ChunkSplit> cur;
-  cur.pos = split.start(blockIdx.x);
-  cur.end = split.start(blockIdx.x + 1);
-  cur.unit = 0;
-  auto item_of_request = [&](long long rel) {  // the item that holds unit `rel` of request it.req: a lane a tile of rows
-    const long long per_head = in_req / p.kv_heads;
-    it.head = (int)(rel / per_head);
+  PagedCursor<ChunkSplit> cur(split);
+  auto item_of_request = [&](int rel) {  // the item that holds unit `rel` of request it.req: a lane a tile of rows
+    const int per_head = in_req / p.kv_heads;
+    it.head = rel / per_head;
     rel -= it.head * per_head;
     it.rt = 0;
     for (int rt0 = 0; rt0 * kChunkRows < it.rows; rt0 += 32) {
@@ -279,7 +279,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       if (hit != 0u) {
         const int src = __ffs(hit) - 1;
         it.rt = rt0 + src;
-        cur.unit = (int)rel - __shfl_sync(0xffffffffu, upto - units, src);
+        cur.unit = rel - __shfl_sync(0xffffffffu, upto - units, src);
         break;
       }
       rel -= __shfl_sync(0xffffffffu, upto, 31);
@@ -306,7 +306,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
   if (cur.pos < cur.end) {
     chunk_request(p, it, req, found);
     item_of_request(cur.pos - before);
-    if (cur.begin(it.n, split.total)) next_item();
+    if (cur.begin(it.n)) next_item();
   }
   bool ok = true;
 
@@ -607,7 +607,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
 
       const ChunkItem done = it;
       const bool whole = cur.whole(it.n);
-      const long long item0 = cur.pos - cur.unit;
+      const int item0 = cur.pos - cur.unit;
       if (cur.advance()) next_item();
 
       ok = ok && mbar_poll(&pv_done[q][(n - 1) & 1], ((n - 1) >> 1) & 1, p.status);
@@ -660,9 +660,9 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         __stcg(part + 128 * D + row, m);
         __stcg(part + 128 * (D + 1) + row, l);
         const int c1 = split.last_cta(item0, done.n);
-        __threadfence();
         named_barrier(1 + q, 128);
         if (row == 0) {
+          __threadfence();
           uint32_t* ticket = tickets + c0 * 2 + q;
           const bool last = atomicAdd(ticket, 1u) == (uint32_t)(c1 - c0);
           if (last) *ticket = 0u;
@@ -735,6 +735,9 @@ cudaError_t launch_chunk(const ChunkArgs& a, cudaStream_t st, bool pdl) {
 cudaError_t launch_paged_attention_chunk(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl) {
   if ((dtype != kBF16 && dtype != kF16) || (a.dim != 64 && a.dim != 128) || !(a.scale > 0.f))
     return cudaErrorNotSupported;  // a maximum of scores is one of scaled scores for a positive scale only
+  // units of work (paged_sched.cuh) in 32 bits
+  const long long items = (long long)a.tokens * a.group / kChunkRows + a.requests;
+  if (items * a.kv_heads * ((long long)a.width * a.block_size / kChunkKeys + 2 + kChunkItem) > INT_MAX) return cudaErrorNotSupported;
   ChunkArgs c{};
   c.a = a;
   c.box = paged_box(a.block_size, kChunkKeys);

@@ -57,44 +57,50 @@ __device__ __forceinline__ int paged_first_key(const PagedAttnArgs& p, int pos) 
   return p.window > 0 ? max(0, pos - p.window + 1) : 0;
 }
 
-// The even split over the CTAs, in units of a key tile's time. An item of n tiles
+// The even split over the CTAs, in units of a key tile's time (the caller sees to
+// it that their sum stays below 2^31). An item of n tiles
 // counts n + C units: C for what it costs besides its tiles (its Q, its join or
 // its output), so that many short items weigh what they take. Boundaries that fall
 // within T units of an item's edge move to that edge: joining a piece costs about as much as T
 // tiles, so no piece is shorter than that, and short items stay whole.
-template <int T, int C>
+template <int T_MOST, int C>
 struct PagedSplit {
   static constexpr int kItem = C;
-  long long total, base, rem;  // CTA c has base units, the first `rem` CTAs one more
-  __device__ void set(long long units, int ctas) {
+  int total, base, rem;        // CTA c has base units, the first `rem` CTAs one more
+  int T;                       // T_MOST, or less where the CTAs have less to do than that
+  __device__ void set(int units, int ctas) {
     total = units;
     base = units / ctas;
     rem = units - base * ctas;
+    T = min(T_MOST, base);
   }
-  __device__ long long start(long long c) const { return c * base + min(c, rem); }
-  __device__ int owner(long long unit) const {
-    const long long wide = rem * (base + 1);
-    return (int)(unit < wide ? unit / (base + 1) : rem + (unit - wide) / base);
+  __device__ int start(int c) const { return c * base + min(c, rem); }
+  __device__ int owner(int unit) const {
+    const int wide = rem * (base + 1);
+    return unit < wide ? unit / (base + 1) : rem + (unit - wide) / base;
   }
   // Where a boundary x units into an item of n tiles goes.
-  static __device__ int snap(long long x, int n) {
-    return x >= n + C ? n + C : x <= min(T + C, (n + C) / 2) ? 0 : n + C - x <= T ? n + C : (int)x;
+  __device__ int snap(int x, int n) const {
+    return x >= n + C ? n + C : x <= min(T + C, (n + C) / 2) ? 0 : n + C - x <= T ? n + C : x;
   }
   // The CTAs that share an item of n tiles beginning at unit `item`; more than one of them.
-  __device__ int first_cta(long long item, int n) const { return owner(item + min(T + C, (n + C) / 2)); }
-  __device__ int last_cta(long long item, int n) const { return owner(item + n + C - T - 1); }
+  __device__ int first_cta(int item, int n) const { return owner(item + min(T + C, (n + C) / 2)); }
+  __device__ int last_cta(int item, int n) const { return owner(item + n + C - T - 1); }
 };
 
 // A CTA's way through its units: the current item begins at `pos - unit`, and the
 // CTA's part of it is the tiles [tile, tile + len).
 template <typename S>
 struct PagedCursor {
-  long long pos, end;
+  const S& split;
+  int pos, end;
   int unit, tile, len, step;
+  __device__ explicit PagedCursor(const S& s)
+      : split(s), pos(s.start(blockIdx.x)), end(s.start(blockIdx.x + 1)), unit(0), tile(0), len(0), step(0) {}
   // The CTA's part of an item of n tiles; false: nothing is left for it.
   __device__ __forceinline__ bool take(int n) {
     if (pos >= end) return false;
-    const int stop = S::snap(end - (pos - unit), n);
+    const int stop = split.snap(end - (pos - unit), n);
     step = stop - unit;
     tile = unit == 0 ? 0 : unit - S::kItem;
     len = stop - S::kItem - tile;
@@ -108,13 +114,13 @@ struct PagedCursor {
     return pos < end;
   }
   // The first boundary, `unit` units into an item of n tiles; true as for advance.
-  __device__ __forceinline__ bool begin(int n, long long total) {
-    const int at = S::snap(unit, n);
+  __device__ __forceinline__ bool begin(int n) {
+    const int at = split.snap(unit, n);
     pos += at - unit;
     unit = at;
     if (at < n + S::kItem) return false;
     unit = 0;
-    return pos < total;
+    return pos < split.total;
   }
 };
 
@@ -123,11 +129,44 @@ struct PagedCursor {
 // `units(i, part, parts, r)`: the units of request i (its lengths go to r), or one of
 // `parts` parts of them (a request's items dealt out; up to MAX_PARTS threads
 // count for one request when there are few).
+template <int MAX_PARTS, typename F, typename S>
+__device__ __forceinline__ void paged_find_warp(int requests, F units, S& split, int& req, PagedRequest& found,
+                                                int& before, int& in_req) {
+  const int lane = threadIdx.x & 31;
+  int parts = 1;
+  while (parts < MAX_PARTS && 2 * parts * requests <= 32) parts *= 2;
+  const int i = lane / parts, part = lane & (parts - 1);
+  PagedRequest last = {0, 0, 0};
+  const int mine = i < requests ? units(i, part, parts, last) : 0;
+  int incl = mine, all_parts = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += u;
+    const int w = __shfl_xor_sync(0xffffffffu, all_parts, o);
+    if (o < parts) all_parts += w;
+  }
+  split.set(__shfl_sync(0xffffffffu, incl, 31), gridDim.x);
+  const int a = split.start(blockIdx.x), upto = incl - mine;
+  const unsigned hit = __ballot_sync(0xffffffffu, part == 0 && a >= upto && a < upto + all_parts);
+  const int src = hit != 0u ? __ffs(hit) - 1 : 0;
+  req = __shfl_sync(0xffffffffu, i, src);
+  before = __shfl_sync(0xffffffffu, upto, src);
+  in_req = __shfl_sync(0xffffffffu, all_parts, src);
+  found.q0 = __shfl_sync(0xffffffffu, last.q0, src);
+  found.qn = __shfl_sync(0xffffffffu, last.qn, src);
+  found.kv = __shfl_sync(0xffffffffu, last.kv, src);
+}
+
 template <int NT, int MAX_PARTS, typename F, typename S>
 __device__ __forceinline__ void paged_find(int requests, F units, S& split, int& req, PagedRequest& found,
-                                           long long& before, long long& in_req) {
-  __shared__ long long s_warp[NT / 32];
-  __shared__ long long s_before, s_sum;
+                                           int& before, int& in_req) {
+  if (requests <= 32) {  // every warp for itself, without a barrier
+    paged_find_warp<MAX_PARTS>(requests, units, split, req, found, before, in_req);
+    return;
+  }
+  __shared__ int s_warp[NT / 32];
+  __shared__ int s_before, s_sum;
   __shared__ int s_req;
   __shared__ PagedRequest s_found;
   PagedRequest last = {0, 0, 0};
@@ -137,28 +176,28 @@ __device__ __forceinline__ void paged_find(int requests, F units, S& split, int&
   const int per = (requests * parts + NT - 1) / NT;  // 1 when parts > 1
   const int r0 = min(requests, parts > 1 ? tid / parts : tid * per), r1 = min(requests, r0 + per);
   const int part = tid & (parts - 1);
-  long long mine = 0;
+  int mine = 0;
   for (int i = r0; i < r1; ++i) mine += units(i, part, parts, last);
-  long long incl = mine, all_parts = mine;
+  int incl = mine, all_parts = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, incl, o);
+    const int u = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += u;
-    const long long w = __shfl_xor_sync(0xffffffffu, all_parts, o);
+    const int w = __shfl_xor_sync(0xffffffffu, all_parts, o);
     if (o < parts) all_parts += w;
   }
   if (lane == 31) s_warp[warp] = incl;
   if (tid == 0) s_req = requests;
   __syncthreads();
-  long long total = 0, upto = incl - mine;
+  int total = 0, upto = incl - mine;
 #pragma unroll
   for (int w = 0; w < NT / 32; ++w) {
-    const long long u = s_warp[w];
+    const int u = s_warp[w];
     upto += w < warp ? u : 0;
     total += u;
   }
   split.set(same_in_warp(total), gridDim.x);
-  const long long a = split.start(blockIdx.x);
+  const int a = split.start(blockIdx.x);
   if (part == 0 && a >= upto && a < upto + all_parts) {
     int i = r0;
     if (per > 1) {
@@ -197,6 +236,19 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Whether phase `parity` of `bar` has completed, without waiting (try_wait may suspend the thread).
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
 }
 
 // Bounded wait like mbar_wait, for barriers on the critical path: the timer (a read of
