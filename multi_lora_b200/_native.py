@@ -9,6 +9,9 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import importlib.machinery
+import importlib.util
+import sys
 import threading
 from pathlib import Path
 
@@ -159,9 +162,18 @@ def ops():
 
 
 @functools.lru_cache(maxsize=None)
-def op(name: str):
-    """One operator of ``torch.ops.mlora`` (its only overload, so that a call skips the lookup)."""
-    return getattr(ops(), name).default
+def direct(name: str):
+    """An operator of the paged serving step as a plain function of the binding: the
+    same C++ function as ``torch.ops.mlora.<name>`` without the dispatcher's argument handling."""
+    ops()
+    loader = importlib.machinery.ExtensionFileLoader("_mlora_torch", str(TORCH_LIB_PATH))
+    spec = importlib.util.spec_from_file_location("_mlora_torch", str(TORCH_LIB_PATH), loader=loader)
+    module = sys.modules.get("_mlora_torch")
+    if module is None:
+        module = importlib.util.module_from_spec(spec)
+        loader.exec_module(module)
+        sys.modules["_mlora_torch"] = module
+    return getattr(module, name)
 
 
 def check(rc: int) -> None:

@@ -20,6 +20,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -102,7 +103,7 @@ def build_torch_lib(force: bool = False, verbose: bool = False) -> Path:
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     OBJ.mkdir(exist_ok=True)
     cxx = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-           "-DTORCH_API_INCLUDE_EXTENSION_H", *[f"-I{p}" for p in incs]]
+           "-DTORCH_API_INCLUDE_EXTENSION_H", *[f"-I{p}" for p in incs], f"-I{sysconfig.get_path('include')}"]
     objs = [OBJ / (src.stem + ".o") for src in srcs]
     jobs = [[*cxx, "-c", str(src), "-o", str(obj)] for src, obj in zip(srcs, objs)
             if force or _stale(obj, [src, ROOT / "include" / "mlora_b200.h"])]
@@ -112,7 +113,7 @@ def build_torch_lib(force: bool = False, verbose: bool = False) -> Path:
     cmd = [
         os.environ.get("CXX", "g++"), "-shared", *map(str, objs), "-o", str(TORCH_LIB.with_suffix(".so.tmp")),
         *[f"-L{p}" for p in libs], f"-L{PKG}",
-        "-lmlora_b200", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
+        "-lmlora_b200", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
         "-Wl,-rpath,$ORIGIN",
     ]
     if verbose:

@@ -4,7 +4,9 @@
 // stream. paged_attention, verify_draft allocate only their outputs.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/utils/pybind.h>
 #include <torch/library.h>
 
 #include <tuple>
@@ -146,7 +148,7 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
     TORCH_CHECK(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.stride(2) == 1,
                 "mlora: out must be like q with unit stride in head_dim");
   } else {
-    out = at::empty(q.sizes(), q.options());
+    out = at::detail::empty_cuda(q.sizes(), q.scalar_type(), dev, c10::nullopt);
   }
   done(mlora_paged_attention(q.data_ptr(), q.stride(0), q.stride(1), q.size(0), (int32_t)q.size(1), &c,
                              block_tables.numel() > 0 ? block_tables.data_ptr<int32_t>() : nullptr, rows,
@@ -182,8 +184,8 @@ std::tuple<at::Tensor, at::Tensor> verify_draft(const at::Tensor& target, const 
                 "mlora: draft_probs must be [", r, ", ", k, ", ", vocab, "] of target_probs' dtype with unit stride in vocab");
   }
   const c10::cuda::CUDAGuard guard(dev);
-  at::Tensor tokens = at::empty({r, k + 1}, draft_tokens.options());
-  at::Tensor emitted = at::empty({r}, draft_tokens.options().dtype(at::kInt));
+  at::Tensor tokens = at::detail::empty_cuda({r, k + 1}, at::kLong, dev, c10::nullopt);
+  at::Tensor emitted = at::detail::empty_cuda({r}, at::kInt, dev, c10::nullopt);
   done(mlora_verify_draft(target.data_ptr(), target.size(0), vocab, target.stride(0),
                           draft.has_value() ? draft->data_ptr() : nullptr, draft.has_value() ? draft->stride(0) : 0,
                           draft.has_value() ? draft->stride(1) : 0, draft_tokens.data_ptr<int64_t>(),
@@ -219,4 +221,11 @@ TORCH_LIBRARY_IMPL(mlora, CUDA, m) {
   m.impl("write_paged_kv", &write_paged_kv);
   m.impl("paged_attention", &paged_attention);
   m.impl("verify_draft", &verify_draft);
+}
+
+PYBIND11_MODULE(_mlora_torch, m) {
+  m.def("plan_paged_step", &plan_paged_step);
+  m.def("write_paged_kv", &write_paged_kv);
+  m.def("paged_attention", &paged_attention);
+  m.def("verify_draft", &verify_draft);
 }

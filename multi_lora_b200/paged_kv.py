@@ -91,7 +91,7 @@ def plan_paged_step(ctx_lens: torch.Tensor, new_lens: torch.Tensor, held_blocks:
     zero before its first use, not shared by calls that overlap on the GPU.
     """
     _need_cuda(ctx_lens, "plan_paged_step")
-    _native.op("plan_paged_step")(ctx_lens, new_lens, held_blocks, free_blocks, free_head, block_tables, block_size,
+    _native.direct("plan_paged_step")(ctx_lens, new_lens, held_blocks, free_blocks, free_head, block_tables, block_size,
                                   plan.q_indptr, plan.kv_lens, plan.held_blocks, plan.free_head, plan.positions,
                                   plan.slot_map, workspace, status)
     return plan
@@ -106,7 +106,7 @@ def write_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
     strides with head_dim innermost, slot_map int32 [tokens] without repeats.
     """
     _need_cuda(k, "write_paged_kv")
-    _native.op("write_paged_kv")(k, v, k_cache, v_cache, slot_map, status)
+    _native.direct("write_paged_kv")(k, v, k_cache, v_cache, slot_map, status)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -127,7 +127,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     _need_cuda(q, "paged_attention")
     if scale is None:
         scale = q.shape[-1] ** -0.5
-    return _native.op("paged_attention")(q, k_cache, v_cache, block_tables, kv_lens, q_indptr, max_q_len, scale, window,
+    return _native.direct("paged_attention")(q, k_cache, v_cache, block_tables, kv_lens, q_indptr, max_q_len, scale, window,
                                          out, workspace, status)
 
 

@@ -35,4 +35,4 @@ def verify_draft(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor]
     """
     if not target_probs.is_cuda:
         raise RuntimeError("mlora: verify_draft needs CUDA tensors (no CPU path)")
-    return _native.op("verify_draft")(target_probs, draft_probs, draft_tokens, row_indptr, accept_u, sample_u, status)
+    return _native.direct("verify_draft")(target_probs, draft_probs, draft_tokens, row_indptr, accept_u, sample_u, status)
