@@ -43,8 +43,8 @@ struct PagedWriteArgs {
   int64_t num_blocks;
   uint32_t* status;
 };
-// es: bytes per element; vec: rows and strides allow 16-byte accesses.
-cudaError_t launch_paged_write(const PagedWriteArgs& a, int es, bool vec, cudaStream_t st, bool pdl);
+// es: bytes per element; piece: bytes at once that rows and strides allow (32, 16, or es).
+cudaError_t launch_paged_write(const PagedWriteArgs& a, int es, int piece, cudaStream_t st, bool pdl);
 
 struct PagedAttnArgs {
   const void* q;

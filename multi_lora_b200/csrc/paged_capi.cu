@@ -29,10 +29,10 @@ int launched(cudaError_t e, const char* what) {
 
 int bytes_of(int32_t dtype) { return dtype == MLORA_BF16 || dtype == MLORA_F16 ? 2 : dtype == MLORA_F32 ? 4 : 0; }
 
-// 16-byte pieces: base aligned, strides whole pieces
-bool pieces(const void* p, int es, int64_t a, int64_t b, int64_t c = 0) {
-  const int v = 16 / es;
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a % v == 0 && b % v == 0 && c % v == 0;
+// Pieces of `bytes`: base aligned, strides whole pieces.
+bool pieces(const void* p, int es, int64_t a, int64_t b, int64_t c = 0, int bytes = 16) {
+  const int v = bytes / es;
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0 && a % v == 0 && b % v == 0 && c % v == 0;
 }
 
 int check_cache(const mlora_paged_cache_t* c) {
@@ -127,11 +127,17 @@ int mlora_write_paged_kv(const void* k, int64_t k_token_stride, int64_t k_head_s
   a.num_blocks = c.num_blocks;
   a.status = status;
   const int es = bytes_of(c.dtype);
-  const bool vec = c.head_dim % (16 / es) == 0 && pieces(k, es, k_token_stride, k_head_stride) &&
-                   pieces(v, es, v_token_stride, v_head_stride) &&
-                   pieces(c.k, es, c.k_block_stride, c.k_slot_stride, c.k_head_stride) &&
-                   pieces(c.v, es, c.v_block_stride, c.v_slot_stride, c.v_head_stride);
-  return launched(mlora::launch_paged_write(a, es, vec, (cudaStream_t)stream, mlora_get_pdl() != 0),
+  int piece = 32;
+  for (; piece > es; piece = piece == 32 ? 16 : es)
+    if (c.head_dim % (piece / es) == 0 && pieces(k, es, k_token_stride, k_head_stride, 0, piece) &&
+        pieces(v, es, v_token_stride, v_head_stride, 0, piece) &&
+        pieces(c.k, es, c.k_block_stride, c.k_slot_stride, c.k_head_stride, piece) &&
+        pieces(c.v, es, c.v_block_stride, c.v_slot_stride, c.v_head_stride, piece))
+      break;
+  if (tokens * c.kv_heads * (int64_t)(c.head_dim * es / piece) > INT32_MAX)
+    return refuse(MLORA_ERR_INVALID_ARGUMENT, "%lld tokens of %d x %d: too many for one call", (long long)tokens,
+                  c.kv_heads, c.head_dim);
+  return launched(mlora::launch_paged_write(a, es, piece, (cudaStream_t)stream, mlora_get_pdl() != 0),
                   "cache write launch");
 }
 

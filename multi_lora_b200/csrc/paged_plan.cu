@@ -183,10 +183,10 @@ cudaError_t launch_paged_plan(const PlanArgs& a, cudaStream_t st, bool pdl) {
   static const cudaError_t attr = cudaFuncSetAttribute(
       paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kPlanMaxRequests + 1) * (int)sizeof(PlanRow));
   if (attr != cudaSuccess) return attr;
-  // one CTA where the tokens fit it (no count of CTAs needed), at most 64 else
+  // one CTA where the tokens fit it (no count of CTAs needed), at most one an SM else
   const long long work = a.max_tokens > a.requests ? a.max_tokens : a.requests;
-  long long grid = (work + 4 * kPlanNT - 1) / (4 * kPlanNT);
-  grid = grid < 1 ? 1 : grid > 64 ? 64 : grid;
+  long long grid = (work + 2 * kPlanNT - 1) / (2 * kPlanNT);
+  grid = grid < 1 ? 1 : grid > 148 ? 148 : grid;
   return launch_kernel(paged_plan_kernel, dim3((unsigned)grid), dim3(kPlanNT), (size_t)smem, st, pdl, a);
 }
 
