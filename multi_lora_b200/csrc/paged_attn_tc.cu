@@ -78,6 +78,9 @@ __device__ __forceinline__ void chunk_span(const PagedAttnArgs& p, ChunkItem& it
   it.n = max(1, (it.end + kChunkKeys - 1) / kChunkKeys - it.tile0);
 }
 
+// One tile of rows only: the warps of both tiles work on it, each on every other half of the keys.
+__device__ __forceinline__ bool chunk_solo(const ChunkItem& it) { return it.rows - it.rt * kChunkRows <= 128; }
+
 __device__ __forceinline__ void chunk_request(const PagedAttnArgs& p, ChunkItem& it, int req, const PagedRequest& r) {
   it.req = req;
   it.q0 = r.q0;
@@ -203,6 +206,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
   __shared__ __align__(8) uint64_t full[NS], empty[NS], q_ready[2], q_free[2], s_full[2][2], p_ready[2][2], pv_done[2][2];
   __shared__ uint32_t s_tmem;
   __shared__ int s_last[2];
+  __shared__ float2 s_mate[128];
   const PagedAttnArgs& p = args.a;
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = same_in_warp(tid >> 5);
@@ -216,7 +220,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
     }
     for (int q = 0; q < 2; ++q) {
       mbar_init(&q_ready[q], 1);
-      mbar_init(&q_free[q], 1);
+      mbar_init(&q_free[q], 2);
       for (int b = 0; b < 2; ++b) {
         mbar_init(&s_full[q][b], 1);
         mbar_init(&p_ready[q][b], 4);
@@ -356,10 +360,11 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       constexpr uint32_t idesc_s = umma_idesc_f16(Num<T>::is_bf16, 128, kHalfKeys);
       constexpr uint32_t idesc_o = umma_idesc_f16(Num<T>::is_bf16, 128, D) | (1u << 16);  // B: columns contiguous
       constexpr uint32_t kStep = kHalfKeys * 128 >> 4;  // a half of a K or V tile
-      const uint32_t q_lo = smem_addr(smem + q * C::kQ) >> 4, ring_lo = smem_addr(ring) >> 4;
+      const uint32_t ring_lo = smem_addr(ring) >> 4;
       const uint32_t s_col = tmem + S_COL + q * 128, o_col = tmem + O_COL + q * D;
       int kslot = 0, k_phase = 0, vslot = 1, v_phase = 0;
-      int n = 0, items = 0;     // halves and items begun
+      int n = 0;                 // halves begun
+      int items = 0, pairs = 0;  // items, and those of two tiles of rows
       auto wait = [&](uint64_t* bar, int parity) { ok = ok && mbar_poll(bar, parity & 1, p.status); };
       bool held = false, held_first = false, held_last = false;  // the half whose product with V is to come
       uint32_t held_lo = 0;
@@ -382,62 +387,59 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         held = false;
       };
       while (cur.take(it.n)) {
-        const bool mine = it.rows - it.rt * kChunkRows > q * 128;
-        const bool both = it.rows - it.rt * kChunkRows > 128;
+        const bool solo = chunk_solo(it);  // this warp then has every other half of the one tile
+        const int qs = solo ? 0 : q, h0 = solo ? q : 0, h1 = solo ? q + 1 : 2;
+        const uint32_t q_lo = smem_addr(smem + qs * C::kQ) >> 4;
         if (held) values();  // nothing of the item before waits for this one's Q, or keeps its V from the ring
 #pragma unroll 1
         for (int k = 0; k < cur.len; ++k) {
           wait(&full[kslot], k_phase);
-          if (mine) {
 #pragma unroll 1
-            for (int h = 0; h < 2; ++h) {
-              const bool first = k == 0 && h == 0;
-              if (first) wait(&q_ready[q], items++);
-              const int b = n & 1;
-              if (n > 1) wait(&pv_done[q][b], (n >> 1) - 1);  // P in this buffer has been read
-              tc_fence_after();
-              if (elect_one()) {
-                const uint32_t kl = ring_lo + kslot * (C::kSlot >> 4) + h * kStep;
+          for (int h = h0; h < h1; ++h) {
+            const bool first = k == 0 && h == h0, last = h == h1 - 1;
+            if (first) wait(&q_ready[qs], qs == 0 ? items : pairs);
+            const int b = n & 1;
+            if (n > 1) wait(&pv_done[q][b], (n >> 1) - 1);  // P in this buffer has been read
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t kl = ring_lo + kslot * (C::kSlot >> 4) + h * kStep;
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-                  umma_ss(s_col + b * 64, q_lo + (i >> 2) * (HALF >> 4) + 2 * (i & 3), kl + (i >> 2) * (HALF >> 4) + 2 * (i & 3),
-                          idesc_s, i > 0);
-                umma_commit(&s_full[q][b]);
-                if (h == 1) umma_commit(&empty[kslot]);
-                if (h == 1 && k == cur.len - 1) umma_commit(&q_free[q]);
+              for (int i = 0; i < D / 16; ++i)
+                umma_ss(s_col + b * 64, q_lo + (i >> 2) * (HALF >> 4) + 2 * (i & 3), kl + (i >> 2) * (HALF >> 4) + 2 * (i & 3),
+                        idesc_s, i > 0);
+              umma_commit(&s_full[q][b]);
+              if (last) umma_commit(&empty[kslot]);
+              if (last && k == cur.len - 1) {  // two arrivals free a tile of Q
+                umma_commit(&q_free[qs]);
+                if (!solo) umma_commit(&q_free[qs]);
               }
-              if (held) values();
-              ++n;
-              if (h == 0) {
-                wait(&full[vslot], v_phase);
-                const int j0 = (it.tile0 + cur.tile + k) * kChunkKeys;
-                if (j0 + kChunkKeys > it.kv || j0 < it.first) {  // rows of V that are nobody's
-                  if (q == 0) {
-                    // whole boxes without a key are zeros already: clear what shares a box with one
-                    const int lo = max(0, it.first - j0), lo0 = lo / args.box * args.box;
-                    const int hi = min(kChunkKeys, max(0, it.kv - j0)), hi1 = min(kChunkKeys, (hi + args.box - 1) / args.box * args.box);
-                    unsigned char* vs = ring + vslot * C::kSlot;
-#pragma unroll 1
-                    for (int e = lane; e < (lo - lo0 + hi1 - hi) * (D / 8); e += 32) {
-                      const int i = e / (D / 8), c = e % (D / 8), j = i < lo - lo0 ? lo0 + i : hi + i - (lo - lo0);
-                      *reinterpret_cast<uint4*>(vs + (c >> 3) * HALF + j * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_proxy_async_smem();
-                  }
-                  if (both) named_barrier(3, 64);
-                  else __syncwarp();
-                }
-              }
-              held = true;
-              held_first = first;
-              held_last = h == 1;
-              held_lo = ring_lo + vslot * (C::kSlot >> 4) + h * kStep + ((HALF >> 4) << 16);
-              held_slot = vslot;
             }
-          } else {  // the other warp's alone
-            if (lane == 0) mbar_arrive(&empty[kslot]);
-            wait(&full[vslot], v_phase);
-            if (lane == 0) mbar_arrive(&empty[vslot]);
+            if (held) values();
+            ++n;
+            if (h == h0) {
+              wait(&full[vslot], v_phase);
+              const int j0 = (it.tile0 + cur.tile + k) * kChunkKeys;
+              if (j0 + kChunkKeys > it.kv || j0 < it.first) {  // rows of V that are nobody's
+                if (q == 0) {
+                  // whole boxes without a key are zeros already: clear what shares a box with one
+                  const int lo = max(0, it.first - j0), lo0 = lo / args.box * args.box;
+                  const int hi = min(kChunkKeys, max(0, it.kv - j0)), hi1 = min(kChunkKeys, (hi + args.box - 1) / args.box * args.box);
+                  unsigned char* vs = ring + vslot * C::kSlot;
+#pragma unroll 1
+                  for (int e = lane; e < (lo - lo0 + hi1 - hi) * (D / 8); e += 32) {
+                    const int i = e / (D / 8), c = e % (D / 8), j = i < lo - lo0 ? lo0 + i : hi + i - (lo - lo0);
+                    *reinterpret_cast<uint4*>(vs + (c >> 3) * HALF + j * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                  }
+                  fence_proxy_async_smem();
+                }
+                named_barrier(3, 64);
+              }
+            }
+            held = true;
+            held_first = first;
+            held_last = last;
+            held_lo = ring_lo + vslot * (C::kSlot >> 4) + h * kStep + ((HALF >> 4) << 16);
+            held_slot = vslot;
           }
           kslot += 2;
           if (kslot >= NS) {
@@ -450,6 +452,8 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
             v_phase ^= 1;
           }
         }
+        ++items;
+        pairs += solo ? 0 : 1;
         if (cur.advance()) next_item();
       }
       if (held) values();
@@ -506,22 +510,19 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
     const float sl = p.scale * 1.4426950408889634f;  // scores in powers of two
     uint32_t* tickets = static_cast<uint32_t*>(p.workspace);
     float* parts = reinterpret_cast<float*>(tickets + kPagedTickets);
-    auto mine = [&](const ChunkItem& x) { return x.rows - x.rt * kChunkRows > q * 128; };
-    int n = 0;  // halves done on this tile of rows
+    int n = 0;             // halves done
+    bool lent = false;     // the other warpgroup still reads this one's O
     while (cur.take(it.n)) {
-      if (!mine(it)) {  // one tile of rows only
-        if (cur.advance()) next_item();
-        continue;
-      }
-      const int r = it.rt * kChunkRows + q * 128 + row;
+      const bool solo = chunk_solo(it);  // the warpgroups share its keys, half by half
+      const int r_lo = it.rt * kChunkRows + (solo ? 0 : q * 128), r = r_lo + row;
       const int pq = it.kv - it.qn + paged_token(p, r);
       const int limit = r < it.rows ? pq + 1 : 0, floor_ = paged_first_key(p, pq);
       // key tiles that every row of this tile sees whole need no mask
-      const int r_lo = it.rt * kChunkRows + q * 128, r_hi = min(it.rows, r_lo + 128) - 1;
+      const int r_hi = min(it.rows, r_lo + 128) - 1;
       const int all_end = it.kv - it.qn + paged_token(p, r_lo) + 1,
                 all_first = paged_first_key(p, it.kv - it.qn + paged_token(p, r_hi));
       float m = -INFINITY, l = 0.f;
-      const int halves = 2 * cur.len;
+      const int halves = solo ? cur.len : 2 * cur.len;
       for (int k = 0; k < halves; ++k, ++n) {
         const int b = n & 1;
         ok = ok && mbar_poll(&s_full[q][b], (n >> 1) & 1, p.status);
@@ -533,7 +534,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         tmem_wait_ld();
         tie32(s[0]);
         tie32(s[1]);
-        const int j0 = (it.tile0 + cur.tile) * kChunkKeys + k * kHalfKeys;
+        const int j0 = (it.tile0 + cur.tile) * kChunkKeys + (solo ? 2 * k + q : k) * kHalfKeys;
         if (j0 + kHalfKeys > all_end || j0 < all_first) {
           const int hi = limit - j0, lo = floor_ - j0;
 #pragma unroll
@@ -602,6 +603,10 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
+        if (lent) {  // this half's product overwrites O
+          named_barrier(5, 256);
+          lent = false;
+        }
         if (lane == 0) mbar_arrive(&p_ready[q][b]);
       }
 
@@ -613,6 +618,26 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       ok = ok && mbar_poll(&pv_done[q][(n - 1) & 1], ((n - 1) >> 1) & 1, p.status);
       __syncwarp();
       tc_fence_after();
+      // An item that both warpgroups worked on: the first one reads the other's O too
+      // (their threads of a row have the same TMEM lane).
+      float own = 1.f, others = 0.f;  // what the two warpgroups' sums are multiplied by
+      if (solo) {
+        if (q == 1) {
+          s_mate[row] = make_float2(m, l);
+          tc_fence_before();
+          named_arrive(4, 256);
+          lent = true;
+          continue;
+        }
+        named_barrier(4, 256);
+        tc_fence_after();
+        const float2 mate = s_mate[row];
+        const float top = fmaxf(m, mate.x), base = top == -INFINITY ? 0.f : top;
+        own = exp2_fast(m - base);
+        others = exp2_fast(mate.x - base);
+        l = l * own + mate.y * others;
+        m = top;
+      }
       const int t = paged_token(p, r);
       T* dst = static_cast<T*>(p.out) + (int64_t)(done.q0 + t) * p.out_token +
                (int64_t)(done.head * p.group + r - t * p.group) * p.out_head;
@@ -643,6 +668,13 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]);
+        if (solo) {
+          tmem_ld32_async(o_addr + D + c * 32, o);
+          tmem_wait_ld();
+          tie32(o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = fmaf(__uint_as_float(o[i]), others, v[i] * own);
+        }
         if (whole) {
           if (r < done.rows) {
 #pragma unroll
@@ -656,6 +688,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         }
       }
       tc_fence_before();
+      if (solo) named_arrive(5, 256);
       if (!whole) {
         __stcg(part + 128 * D + row, m);
         __stcg(part + 128 * (D + 1) + row, l);
@@ -709,6 +742,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         __syncwarp();
       }
     }
+    if (lent) named_barrier(5, 256);
   }
   tc_fence_before();
   __syncthreads();
