@@ -79,12 +79,12 @@ struct PagedSplit {
     const int wide = rem * (base + 1);
     return unit < wide ? unit / (base + 1) : rem + (unit - wide) / base;
   }
-  // Where a boundary x units into an item of n tiles goes.
-  __device__ int snap(int x, int n) const {
-    return x >= n + C ? n + C : x <= min(T + C, (n + C) / 2) ? 0 : n + C - x <= T ? n + C : x;
-  }
+  // Boundaries up to here into an item of n tiles go to its beginning (all those
+  // within the C units among them: no piece is without tiles), others to its end or stay.
+  __device__ int low(int n) const { return max(C, min(T + C, (n + C) / 2)); }
+  __device__ int snap(int x, int n) const { return x >= n + C ? n + C : x <= low(n) ? 0 : n + C - x <= T ? n + C : x; }
   // The CTAs that share an item of n tiles beginning at unit `item`; more than one of them.
-  __device__ int first_cta(int item, int n) const { return owner(item + min(T + C, (n + C) / 2)); }
+  __device__ int first_cta(int item, int n) const { return owner(item + low(n)); }
   __device__ int last_cta(int item, int n) const { return owner(item + n + C - T - 1); }
 };
 
