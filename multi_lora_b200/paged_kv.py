@@ -181,17 +181,19 @@ class PagedKVCache:
                                self.block_tables, plan, block_size=self.block_size, workspace=self._ticket,
                                status=self.status)
 
-    def _current(self) -> PagedStepPlan:
+    @property
+    def plan_now(self) -> PagedStepPlan:
+        """The plan of the current step."""
         if self._plan is None:
             raise RuntimeError("PagedKVCache: plan a step first")
         return self._plan
 
     def write(self, index: int, k: torch.Tensor, v: torch.Tensor) -> None:
-        write_paged_kv(k, v, *self.layer(index), self._current().slot_map, status=self.status)
+        write_paged_kv(k, v, *self.layer(index), self.plan_now.slot_map, status=self.status)
 
     def attend(self, index: int, q: torch.Tensor, max_q_len: int, *, scale: Optional[float] = None, window: int = 0,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        plan = self._current()
+        plan = self.plan_now
         return paged_attention(q, *self.layer(index), self.block_tables, plan.kv_lens, plan.q_indptr,
                                max_q_len=max_q_len, workspace=self._workspace, scale=scale, window=window, out=out,
                                status=self.status)
