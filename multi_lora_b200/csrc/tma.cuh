@@ -137,6 +137,12 @@ __device__ __forceinline__ float4 ld_dsmem_v4(uint32_t cluster_addr) {
   return v;
 }
 
+__device__ __forceinline__ float2 ld_dsmem_v2(uint32_t cluster_addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_addr) : "memory");
+  return v;
+}
+
 // Split cluster barrier: arrive (release) early, wait (acquire) late.
 __device__ __forceinline__ void cluster_arrive_release() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");

@@ -119,7 +119,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     q_indptr[i+1] - 1, the last of them at position kv_lens[i] - 1. Query head h
     reads key head h // (q_heads // kv_heads). ``window`` > 0 limits a query to
     that many keys, its own among them. ``max_q_len``: the longest request's
-    new tokens, or more, on the host. ``workspace``: :func:`attention_workspace`.
+    new tokens, or more, on the host. The width of ``block_tables`` bounds the keys: a
+    view of its first columns lets a few short requests take a launch of lower
+    latency. ``workspace``: :func:`attention_workspace`.
     Queries that see no key and rows past q_indptr[-1] give zeros. bfloat16,
     float16 or float32; head_dim a multiple of 8, at most 256; the tensor-core
     kernels take 16-bit caches with head_dim 64 or 128.
