@@ -74,7 +74,7 @@ cudaError_t launch_paged_attention_general(const PagedAttnArgs& a, int dtype, bo
 // everywhere. Decode: up to kDecodeMaxRows rows (max_q_len * q_heads / kv_heads);
 // chunk: any number. cudaErrorNotSupported: the shape is not one of these.
 cudaError_t launch_paged_attention_decode(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl);
-constexpr int kDecodeMaxRows = 32;
+constexpr int kDecodeMaxRows = 16;
 
 cudaError_t launch_paged_attention_chunk(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl);
 

@@ -1,21 +1,33 @@
-// Attention over the paged cache for few query rows: decode steps and drafts.
+// Attention over the paged cache for few query rows: decode steps and short drafts.
 //
 // The G = q_heads / kv_heads query heads of a key head and the request's new
-// tokens form one block of rows (row r: token r / G, head r % G; at most 64),
-// so K and V are read once for all of them. What bounds it is that read: with
-// R rows there are R operations a byte, far under what the tensor cores
-// need to be the limit. Everything else serves keeping loads in flight:
-//   * a producer warp fetches tiles of 64 keys by TMA, one box of a page
-//     (gcd(block size, 64) rows of 64 columns) a lane, through a ring of
-//     stages of K and V; a box behind the keys is a coordinate out of range,
-//     which reads zeros and no memory;
-//   * consumer warps take 16 rows and 16 or 32 of the 64 keys each on mma.sync
-//     tiles and keep their own running maximum, sum and 16 x D output sums over
-//     the whole item, with no exchange between warps until its end; scores and sums are fp32, the probabilities are rounded to
-//     the cache's type for the second product (their fp32 values make the sum);
-//   * key tiles are dealt evenly over the CTAs (paged_sched.cuh).
+// tokens form one block of rows (row r: token r / G, head r % G; at most 16: a
+// tile of the warp-level tensor-core instruction, which more rows would pay for
+// again, while csrc/paged_attn_tc.cu's do not: 64 requests x 2000 keys took 182 us
+// here and 132 there with 32 and 36 rows). So K and V are read once for all of
+// them. What bounds it is that read: R rows are R operations a byte. Everything
+// else serves keeping loads in flight:
+//   * a producer warp fetches tiles of 64 keys by TMA, one box of a page (the
+//     largest power of two of slots that divides the block size, at most 64, by 64
+//     columns) a lane, through a ring of stages of K and V; a box behind the keys
+//     is a coordinate out of range, which reads zeros and no memory;
+//   * four consumer warps take 16 of the 64 keys each and keep their own running
+//     maximum, sum and 16 x D output sums over the whole item, with no exchange
+//     between warps until its end. K's fragments are all loaded before the
+//     products, which run as four chains, and V's are in flight during the
+//     softmax: a warp that waited for each in turn took twice as long a tile.
+//     Scores, sums and statistics are fp32. For the second product an f16
+//     probability is rounded once (11 bits); a bf16 one goes in as two terms, its
+//     rounding and the rounding's remainder (16 bits), since the 8 bits of one
+//     term would add as much error as the result's own rounding;
+//   * key tiles are dealt evenly over two CTAs an SM (paged_sched.cuh), or, for few
+//     short requests, an item to a cluster.
 // Keys outside [first, kv) may hold anything: scores are replaced, not added
 // to, and their V fragments are cleared before the product, since 0 * NaN is NaN.
+//
+// Measured: 64 requests of 33 to 2048 keys, 32 heads of 128: 189 us, 5.6 TB/s (85 % of
+// the measured copy bandwidth); 4 requests of 20000 to 65536 keys, 8 key heads:
+// 110 us, 5.6 TB/s; one request of 777 keys: 6.3 us.
 #include <climits>
 
 #include "kernels.h"
@@ -37,17 +49,16 @@ struct DecodeArgs {
   int box;     // rows of a TMA box
 };
 
-template <int D, int MT>
+template <int D>
 struct DecodeCfg {
   static constexpr int KG = 4;                    // key groups: warps that share 16 rows
-  static constexpr int kSub = kDecTile / 16 / KG; // groups of 16 keys that a warp takes of a tile
-  static constexpr int kWarps = KG * MT;
+  static constexpr int kWarps = KG;
   static constexpr int kThreads = kWarps * 32 + 32;
-  static constexpr int kPerSm = MT == 1 ? 2 : 1;
+  static constexpr int kPerSm = 2;
   static constexpr int kSide = kDecTile * D * 2;  // bytes of K (or V) in a stage
-  static constexpr int kStages = (MT == 1 ? 96 : 160) * 1024 / (2 * kSide);
+  static constexpr int kStages = 96 * 1024 / (2 * kSide);
   static constexpr int kRowF = D + 4;             // floats of a row in the merge buffer
-  static constexpr int kMerge = MT * 16 * kRowF * 4;
+  static constexpr int kMerge = 16 * kRowF * 4;
   static constexpr int kSmem = kStages * 2 * kSide + kMerge + 1024;
 };
 
@@ -56,7 +67,6 @@ struct DecodeItem {
   int req, head, q0, qn, kv, first, tile0, n;
 };
 
-template <int MT>
 __device__ __forceinline__ void decode_request(const PagedAttnArgs& p, DecodeItem& it, int req, const PagedRequest& r) {
   it.req = req;
   it.q0 = r.q0;
@@ -64,17 +74,17 @@ __device__ __forceinline__ void decode_request(const PagedAttnArgs& p, DecodeIte
   it.kv = r.kv;
   it.first = paged_first_key(p, r.kv - r.qn);
   it.tile0 = it.first / kDecTile;
-  it.n = r.qn > 0 && r.qn * p.group <= 16 * MT ? max(1, (r.kv + kDecTile - 1) / kDecTile - it.tile0) : 0;
+  it.n = r.qn > 0 && r.qn * p.group <= kDecodeMaxRows ? max(1, (r.kv + kDecTile - 1) / kDecTile - it.tile0) : 0;
 }
 
 constexpr int kFewCtas = 8;    // CTAs of a cluster
 constexpr int kFewItems = 16;  // (request, key head)s that clusters are launched for, at most
 constexpr int kFewKeys = 4096; // keys that the block tables have room for, at most
 
-template <typename T, int D, int MT, bool CLUSTER>
-__global__ void __launch_bounds__(DecodeCfg<D, MT>::kThreads, DecodeCfg<D, MT>::kPerSm)
+template <typename T, int D, bool CLUSTER>
+__global__ void __launch_bounds__(DecodeCfg<D>::kThreads, DecodeCfg<D>::kPerSm)
 paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
-  using C = DecodeCfg<D, MT>;
+  using C = DecodeCfg<D>;
   constexpr bool kTwoTerms = Num<T>::is_bf16;
   constexpr int NS = C::kStages, SIDE = C::kSide, HALF = kDecTile * 128;
   extern __shared__ __align__(1024) unsigned char s_raw[];
@@ -112,7 +122,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     // rows beyond what the caller said: reported, and not computed
     if (report && r.qn > p.max_q_len) flag_error(p.status, kErrLength);
     DecodeItem x;
-    decode_request<MT>(p, x, i, r);
+    decode_request(p, x, i, r);
     return x.n > 0 ? (x.n + kDecItem) * p.kv_heads : 0;
   };
   // CLUSTER: a cluster takes one item, each CTA an eighth of its tiles, and the sums
@@ -122,7 +132,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     const int item = blockIdx.x / kFewCtas;
     req = item / p.kv_heads;
     units(req, 0, 1, found);
-    decode_request<MT>(p, it, req, found);
+    decode_request(p, it, req, found);
     if (it.n == 0) {  // the same in the whole cluster
       if (warp == C::kWarps) paged_zero_rest<T>(p);
       return;
@@ -139,7 +149,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       if (warp == C::kWarps) paged_zero_rest<T>(p);
       return;
     }
-    decode_request<MT>(p, it, req, found);
+    decode_request(p, it, req, found);
     it.head = (cur.pos - before) / (it.n + kDecItem);
     cur.unit = cur.pos - before - it.head * (it.n + kDecItem);
   }
@@ -147,7 +157,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     if (++it.head == p.kv_heads) {
       it.head = 0;
       for (int i = it.req + 1; i < p.requests; ++i) {
-        decode_request<MT>(p, it, i, paged_request(p, i, false));
+        decode_request(p, it, i, paged_request(p, i, false));
         if (it.n > 0) break;
       }
     }
@@ -205,20 +215,20 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     return;
   }
 
-  // ---- consumers: warp = (16 rows mt, 16 or 32 keys of each tile kg) ----
-  const int mt = warp / C::KG, kg = warp % C::KG;
+  // ---- consumers: 16 rows, 16 keys of each tile a warp ----
+  const int kg = warp;
   const float sl = p.scale * 1.4426950408889634f;  // scores in powers of two
   int stage = 0, phase = 0;
   bool ready = false;  // the next stage is known to be there
   uint32_t* tickets = static_cast<uint32_t*>(p.workspace);
   float* parts = reinterpret_cast<float*>(tickets + kPagedTickets);
-  constexpr int PART = MT * 16 * (D + 2);  // floats of a piece: sums, maxima, totals
+  constexpr int PART = 16 * (D + 2);  // floats of a piece: sums, maxima, totals
   // Q fragments: rows lane / 4 and + 8, columns (lane % 4) * 2 (+ 8) of each 16
   uint32_t qf[D / 16][4];
   auto load_q = [&](const DecodeItem& x) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int r = mt * 16 + (lane >> 2) + e * 8, t = paged_token(p, r);
+      const int r = (lane >> 2) + e * 8, t = paged_token(p, r);
       const T* src = static_cast<const T*>(p.q) + (int64_t)(x.q0 + t) * p.q_token +
                      (int64_t)(x.head * group + r - t * group) * p.q_head + (lane & 3) * 2;
       const bool real = r < x.qn * group;
@@ -236,7 +246,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     int limit[2], floor_[2];  // keys below `limit` and at or above `floor_` are seen
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int r = mt * 16 + (lane >> 2) + e * 8;
+      const int r = (lane >> 2) + e * 8;
       const int pq = it.kv - it.qn + paged_token(p, r);
       limit[e] = r < rows ? pq + 1 : 0;
       floor_[e] = paged_first_key(p, pq);
@@ -252,108 +262,105 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       const int next = stage + 1 < NS ? stage + 1 : 0;
       ready = mbar_test(&full[next], next == 0 ? phase ^ 1 : phase);  // answered while this tile is worked on
       __syncwarp();
+      const int k0 = kg * 16, j0 = (it.tile0 + cur.tile + k) * kDecTile + k0;  // 16 keys
+      if (j0 < it.kv && j0 + 16 > it.first) {
+        const uint32_t ks = smem_addr(smem + stage * 2 * SIDE), vs = ks + SIDE;
+        // All of K's fragments, then the products as four independent chains.
+        uint32_t kf[2][D / 32][4];
 #pragma unroll
-      for (int sub = 0; sub < C::kSub; ++sub) {
-        const int k0 = (kg * C::kSub + sub) * 16, j0 = (it.tile0 + cur.tile + k) * kDecTile + k0;  // 16 keys
-        if (mt * 16 < rows && j0 < it.kv && j0 + 16 > it.first) {
-          const uint32_t ks = smem_addr(smem + stage * 2 * SIDE), vs = ks + SIDE;
-          // All of K's fragments, then the products as four independent chains.
-          uint32_t kf[2][D / 32][4];
+        for (int c = 0; c < D / 32; ++c)  // 32 columns: two k steps
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c)  // 32 columns: two k steps
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              const int key = k0 + n * 8 + (lane & 7), chunk = c * 4 + (lane >> 3);
-              ldsm_x4(ks + (chunk >> 3) * HALF + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), kf[n][c][0], kf[n][c][1],
-                      kf[n][c][2], kf[n][c][3]);
-            }
-          float s4[2][2][4];
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s4[n][0][e] = s4[n][1][e] = 0.f;
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int n = 0; n < 2; ++n)
-                mma_16816<T>(s4[n][h], qf[2 * c + h][0], qf[2 * c + h][1], qf[2 * c + h][2], qf[2 * c + h][3],
-                             kf[n][c][2 * h], kf[n][c][2 * h + 1]);
-          // V's fragments, in flight during the softmax: keys (lane % 4) * 2 + {0, 1} and + 8
-          uint32_t vf[D / 16][4];
-          const int key = k0 + (lane & 15);
-#pragma unroll
-          for (int n = 0; n < D / 16; ++n) {  // 16 columns of V
-            const int chunk = n * 2 + (lane >> 4);
-            ldsm_x4_trans(vs + (chunk >> 3) * HALF + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), vf[n][0], vf[n][1],
-                          vf[n][2], vf[n][3]);
+          for (int n = 0; n < 2; ++n) {
+            const int key = k0 + n * 8 + (lane & 7), chunk = c * 4 + (lane >> 3);
+            ldsm_x4(ks + (chunk >> 3) * HALF + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), kf[n][c][0], kf[n][c][1],
+                    kf[n][c][2], kf[n][c][3]);
           }
-          float s[2][4];
-          const bool edge = j0 + 16 > all_end || j0 < all_first;  // not all seen by all rows
+        float s4[2][2][4];
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              s[n][e] = (s4[n][0][e] + s4[n][1][e]) * sl;
-              if (edge) {
-                const int j = j0 + n * 8 + (lane & 3) * 2 + (e & 1);
-                if (j >= limit[e >> 1] || j < floor_[e >> 1]) s[n][e] = -INFINITY;
-              }
-            }
-          uint32_t pf[4], pr[4];
-          float fix[2];
+          for (int e = 0; e < 4; ++e) s4[n][0][e] = s4[n][1][e] = 0.f;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float m_new = fmaxf(m[e], top), ref = m_new == -INFINITY ? 0.f : m_new;
-            fix[e] = exp2_fast(m[e] - ref);
-            m[e] = m_new;
-            const float p0 = exp2_fast(s[0][2 * e] - ref), p1 = exp2_fast(s[0][2 * e + 1] - ref);
-            const float p2 = exp2_fast(s[1][2 * e] - ref), p3 = exp2_fast(s[1][2 * e + 1] - ref);
-            l[e] = l[e] * fix[e] + ((p0 + p1) + (p2 + p3));
-            pf[e] = pack_round2<T>(p0, p1);
-            pf[2 + e] = pack_round2<T>(p2, p3);
-            if constexpr (kTwoTerms) {
-              pr[e] = pack_round2<T>(p0 - Pack2<T>::lo(pf[e]), p1 - Pack2<T>::hi(pf[e]));
-              pr[2 + e] = pack_round2<T>(p2 - Pack2<T>::lo(pf[2 + e]), p3 - Pack2<T>::hi(pf[2 + e]));
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+              mma_16816<T>(s4[n][h], qf[2 * c + h][0], qf[2 * c + h][1], qf[2 * c + h][2], qf[2 * c + h][3],
+                           kf[n][c][2 * h], kf[n][c][2 * h + 1]);
+        // V's fragments, in flight during the softmax: keys (lane % 4) * 2 + {0, 1} and + 8
+        uint32_t vf[D / 16][4];
+        const int key = k0 + (lane & 15);
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {  // 16 columns of V
+          const int chunk = n * 2 + (lane >> 4);
+          ldsm_x4_trans(vs + (chunk >> 3) * HALF + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), vf[n][0], vf[n][1],
+                        vf[n][2], vf[n][3]);
+        }
+        float s[2][4];
+        const bool edge = j0 + 16 > all_end || j0 < all_first;  // not all seen by all rows
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[n][e] = (s4[n][0][e] + s4[n][1][e]) * sl;
+            if (edge) {
+              const int j = j0 + n * 8 + (lane & 3) * 2 + (e & 1);
+              if (j >= limit[e >> 1] || j < floor_[e >> 1]) s[n][e] = -INFINITY;
             }
           }
-          if (__any_sync(0xffffffffu, fix[0] != 1.f || fix[1] != 1.f)) {
+        uint32_t pf[4], pr[4];
+        float fix[2];
 #pragma unroll
-            for (int n = 0; n < D / 8; ++n) {
-              o[n][0] *= fix[0];
-              o[n][1] *= fix[0];
-              o[n][2] *= fix[1];
-              o[n][3] *= fix[1];
-            }
+        for (int e = 0; e < 2; ++e) {
+          float top = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const float m_new = fmaxf(m[e], top), ref = m_new == -INFINITY ? 0.f : m_new;
+          fix[e] = exp2_fast(m[e] - ref);
+          m[e] = m_new;
+          const float p0 = exp2_fast(s[0][2 * e] - ref), p1 = exp2_fast(s[0][2 * e + 1] - ref);
+          const float p2 = exp2_fast(s[1][2 * e] - ref), p3 = exp2_fast(s[1][2 * e + 1] - ref);
+          l[e] = l[e] * fix[e] + ((p0 + p1) + (p2 + p3));
+          pf[e] = pack_round2<T>(p0, p1);
+          pf[2 + e] = pack_round2<T>(p2, p3);
+          if constexpr (kTwoTerms) {
+            pr[e] = pack_round2<T>(p0 - Pack2<T>::lo(pf[e]), p1 - Pack2<T>::hi(pf[e]));
+            pr[2 + e] = pack_round2<T>(p2 - Pack2<T>::lo(pf[2 + e]), p3 - Pack2<T>::hi(pf[2 + e]));
           }
-          if (j0 + 16 > it.kv || j0 < it.first) {
-            const int j = j0 + (lane & 3) * 2;
-            auto keep = [&](int x) { return x < it.kv && x >= it.first; };
-            const uint32_t clear0 = (keep(j) ? 0xffffu : 0u) | (keep(j + 1) ? 0xffff0000u : 0u);
-            const uint32_t clear1 = (keep(j + 8) ? 0xffffu : 0u) | (keep(j + 9) ? 0xffff0000u : 0u);
+        }
+        if (__any_sync(0xffffffffu, fix[0] != 1.f || fix[1] != 1.f)) {
 #pragma unroll
-            for (int n = 0; n < D / 16; ++n) {
-              vf[n][0] &= clear0;
-              vf[n][1] &= clear1;
-              vf[n][2] &= clear0;
-              vf[n][3] &= clear1;
-            }
+          for (int n = 0; n < D / 8; ++n) {
+            o[n][0] *= fix[0];
+            o[n][1] *= fix[0];
+            o[n][2] *= fix[1];
+            o[n][3] *= fix[1];
           }
+        }
+        if (j0 + 16 > it.kv || j0 < it.first) {
+          const int j = j0 + (lane & 3) * 2;
+          auto keep = [&](int x) { return x < it.kv && x >= it.first; };
+          const uint32_t clear0 = (keep(j) ? 0xffffu : 0u) | (keep(j + 1) ? 0xffff0000u : 0u);
+          const uint32_t clear1 = (keep(j + 8) ? 0xffffu : 0u) | (keep(j + 9) ? 0xffff0000u : 0u);
 #pragma unroll
           for (int n = 0; n < D / 16; ++n) {
-            mma_16816<T>(o[2 * n], pf[0], pf[1], pf[2], pf[3], vf[n][0], vf[n][1]);
-            mma_16816<T>(o[2 * n + 1], pf[0], pf[1], pf[2], pf[3], vf[n][2], vf[n][3]);
+            vf[n][0] &= clear0;
+            vf[n][1] &= clear1;
+            vf[n][2] &= clear0;
+            vf[n][3] &= clear1;
           }
-          if constexpr (kTwoTerms) {
+        }
 #pragma unroll
-            for (int n = 0; n < D / 16; ++n) {
-              mma_16816<T>(o[2 * n], pr[0], pr[1], pr[2], pr[3], vf[n][0], vf[n][1]);
-              mma_16816<T>(o[2 * n + 1], pr[0], pr[1], pr[2], pr[3], vf[n][2], vf[n][3]);
-            }
+        for (int n = 0; n < D / 16; ++n) {
+          mma_16816<T>(o[2 * n], pf[0], pf[1], pf[2], pf[3], vf[n][0], vf[n][1]);
+          mma_16816<T>(o[2 * n + 1], pf[0], pf[1], pf[2], pf[3], vf[n][2], vf[n][3]);
+        }
+        if constexpr (kTwoTerms) {
+#pragma unroll
+          for (int n = 0; n < D / 16; ++n) {
+            mma_16816<T>(o[2 * n], pr[0], pr[1], pr[2], pr[3], vf[n][0], vf[n][1]);
+            mma_16816<T>(o[2 * n + 1], pr[0], pr[1], pr[2], pr[3], vf[n][2], vf[n][3]);
           }
         }
       }
@@ -385,14 +392,14 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
         s_l[warp][(lane >> 2) + e * 8] = l[e];
       }
     }
-    const int slots = rows <= 4 ? min(4, C::KG) : rows <= 8 ? 2 : 1, apart = 16 / (rows <= 4 ? 4 : slots);
+    const int slots = rows <= 4 ? C::KG : rows <= 8 ? 2 : 1, apart = 16 / (rows <= 4 ? 4 : slots);
     named_barrier(1, C::kWarps * 32);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int r = (lane >> 2) + e * 8;
       float top = -INFINITY;
 #pragma unroll
-      for (int g = 0; g < C::KG; ++g) top = fmaxf(top, s_m[mt * C::KG + g][r]);
+      for (int g = 0; g < C::KG; ++g) top = fmaxf(top, s_m[g][r]);
       const float own = top == -INFINITY ? 0.f : exp2_fast(m[e] - top);
 #pragma unroll
       for (int n = 0; n < D / 8; ++n) {
@@ -405,8 +412,8 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int r = (lane >> 2) + e * 8;
-          if (mt * 16 + r >= rows) continue;
-          float* d = merge + (mt * 16 + (kg - g) * apart + r) * C::kRowF + (lane & 3) * 2;
+          if (r >= rows) continue;
+          float* d = merge + ((kg - g) * apart + r) * C::kRowF + (lane & 3) * 2;
           if (g > 0) {
             float2 u[D / 8];  // all the loads first
 #pragma unroll
@@ -425,13 +432,12 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       named_barrier(1, C::kWarps * 32);
     }
     auto row_stat = [&](int r, float& top, float& sum) {  // over the key groups of row r
-      const int w = (r >> 4) * C::KG, i = r & 15;
-      top = s_m[w][i];
+      top = s_m[0][r];
 #pragma unroll
-      for (int g = 1; g < C::KG; ++g) top = fmaxf(top, s_m[w + g][i]);
+      for (int g = 1; g < C::KG; ++g) top = fmaxf(top, s_m[g][r]);
       sum = 0.f;
 #pragma unroll
-      for (int g = 0; g < C::KG; ++g) sum += top == -INFINITY ? 0.f : s_l[w + g][i] * exp2_fast(s_m[w + g][i] - top);
+      for (int g = 0; g < C::KG; ++g) sum += top == -INFINITY ? 0.f : s_l[g][r] * exp2_fast(s_m[g][r] - top);
     };
     auto store = [&](int r, int c, const float* v, float inv) {  // 8 columns of row r
       const int t = paged_token(p, r);
@@ -467,14 +473,14 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       if (CLUSTER) {
         *reinterpret_cast<float4*>(part + r * D + c) = v0;
         *reinterpret_cast<float4*>(part + r * D + c + 4) = v1;
-        if (c == 0) reinterpret_cast<float2*>(part + MT * 16 * D)[r] = make_float2(top, sum);
+        if (c == 0) reinterpret_cast<float2*>(part + 16 * D)[r] = make_float2(top, sum);
       } else if (whole) {
         const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
         store(r, c, v, sum > 0.f || sum != sum ? 1.f / sum : 0.f);
       } else {
         __stcg(reinterpret_cast<float4*>(part + r * D + c), v0);
         __stcg(reinterpret_cast<float4*>(part + r * D + c + 4), v1);
-        if (c == 0) __stcg(reinterpret_cast<float2*>(part + MT * 16 * D) + r, make_float2(top, sum));
+        if (c == 0) __stcg(reinterpret_cast<float2*>(part + 16 * D) + r, make_float2(top, sum));
       }
     }
     if constexpr (CLUSTER) {
@@ -488,7 +494,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
 #pragma unroll
         for (int x = 0; x < kFewCtas; ++x) {
           u[x] = ld_dsmem_v4(cluster_map(base + (row * D + c) * 4, x));
-          stat[x] = ld_dsmem_v2(cluster_map(base + (MT * 16 * D + row * 2) * 4, x));
+          stat[x] = ld_dsmem_v2(cluster_map(base + (16 * D + row * 2) * 4, x));
         }
         float top = stat[0].x, sum = 0.f;
 #pragma unroll
@@ -532,7 +538,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
 #pragma unroll 8
           for (int x = c0; x <= c1; ++x) {
             const float* src = piece(x);
-            const float2 stat = __ldcg(reinterpret_cast<const float2*>(src + MT * 16 * D) + r);
+            const float2 stat = __ldcg(reinterpret_cast<const float2*>(src + 16 * D) + r);
             const float4 v0 = __ldcg(reinterpret_cast<const float4*>(src + r * D + c));
             const float4 v1 = __ldcg(reinterpret_cast<const float4*>(src + r * D + c + 4));
             const float m_new = fmaxf(top, stat.x), ref = m_new == -INFINITY ? 0.f : m_new;
@@ -558,17 +564,17 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
 
 namespace {
 
-template <typename T, int D, int MT, bool CLUSTER>
+template <typename T, int D, bool CLUSTER>
 cudaError_t launch_decode(const DecodeArgs& a, cudaStream_t st, bool pdl) {
-  using C = DecodeCfg<D, MT>;
-  auto kern = paged_attention_decode_kernel<T, D, MT, CLUSTER>;
+  using C = DecodeCfg<D>;
+  auto kern = paged_attention_decode_kernel<T, D, CLUSTER>;
   static const cudaError_t attr =
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (attr != cudaSuccess) return attr;
   const int ctas = paged_sm_count() * C::kPerSm;
   static_assert(C::kSmem <= 227 * 1024, "shared memory");
   if (ctas > kPagedTickets ||
-      (size_t)ctas * 2 * MT * 16 * (D + 2) * 4 + kPagedTickets * 4 > kPagedWorkspaceBytes)
+      (size_t)ctas * 2 * 16 * (D + 2) * 4 + kPagedTickets * 4 > kPagedWorkspaceBytes)
     return cudaErrorNotSupported;
   if constexpr (!CLUSTER) {
     return launch_kernel(kern, dim3(ctas), dim3(C::kThreads), C::kSmem, st, pdl, a);
@@ -592,13 +598,12 @@ cudaError_t launch_decode(const DecodeArgs& a, cudaStream_t st, bool pdl) {
 }
 
 template <typename T, int D>
-cudaError_t launch_decode_m(const DecodeArgs& a, int rows, cudaStream_t st, bool pdl) {
-  if (rows > 16) return launch_decode<T, D, 2, false>(a, st, pdl);
+cudaError_t launch_decode_any(const DecodeArgs& a, cudaStream_t st, bool pdl) {
   // One request of 777 keys, 8 key heads: 6.3 us with clusters, 11.3 without; 4000 keys 12.9 and 18.5. From
   // twice that on an item needs more CTAs than a cluster has. The host knows the lengths' bound only.
   if ((long long)a.a.requests * a.a.kv_heads <= kFewItems && (long long)a.a.width * a.a.block_size <= kFewKeys)
-    return launch_decode<T, D, 1, true>(a, st, pdl);
-  return launch_decode<T, D, 1, false>(a, st, pdl);
+    return launch_decode<T, D, true>(a, st, pdl);
+  return launch_decode<T, D, false>(a, st, pdl);
 }
 
 }  // namespace
@@ -612,12 +617,9 @@ cudaError_t launch_paged_attention_decode(const PagedAttnArgs& a, int dtype, cud
   d.a = a;
   d.box = paged_box(a.block_size, kDecTile);
   if (d.box < 8 || !paged_maps(a, dtype, d.box, &d.k_map, &d.v_map)) return cudaErrorNotSupported;
-  const long long all = (long long)a.max_q_len * (a.q_heads / a.kv_heads);
-  const int rows = all > kDecodeMaxRows ? kDecodeMaxRows : (int)all;
   if (dtype == kBF16)
-    return a.dim == 64 ? launch_decode_m<__nv_bfloat16, 64>(d, rows, st, pdl)
-                       : launch_decode_m<__nv_bfloat16, 128>(d, rows, st, pdl);
-  return a.dim == 64 ? launch_decode_m<__half, 64>(d, rows, st, pdl) : launch_decode_m<__half, 128>(d, rows, st, pdl);
+    return a.dim == 64 ? launch_decode_any<__nv_bfloat16, 64>(d, st, pdl) : launch_decode_any<__nv_bfloat16, 128>(d, st, pdl);
+  return a.dim == 64 ? launch_decode_any<__half, 64>(d, st, pdl) : launch_decode_any<__half, 128>(d, st, pdl);
 }
 
 }  // namespace mlora
