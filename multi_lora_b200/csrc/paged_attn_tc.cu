@@ -89,6 +89,12 @@ __device__ __forceinline__ void chunk_request(const PagedAttnArgs& p, ChunkItem&
   it.rows = r.qn * p.group;
 }
 
+// Whether the second half of the CTA's last tile of the item lies behind every row's keys.
+template <typename Cursor>
+__device__ __forceinline__ bool chunk_odd(const ChunkItem& it, const Cursor& cur) {
+  return (it.tile0 + cur.tile + cur.len - 1) * kChunkKeys + kHalfKeys >= it.end;
+}
+
 __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -388,12 +394,14 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       };
       while (cur.take(it.n)) {
         const bool solo = chunk_solo(it);  // this warp then has every other half of the one tile
-        const int qs = solo ? 0 : q, h0 = solo ? q : 0, h1 = solo ? q + 1 : 2;
+        const int qs = solo ? 0 : q, h0 = solo ? q : 0;
+        const bool odd = !solo && chunk_odd(it, cur);
         const uint32_t q_lo = smem_addr(smem + qs * C::kQ) >> 4;
         if (held) values();  // nothing of the item before waits for this one's Q, or keeps its V from the ring
 #pragma unroll 1
         for (int k = 0; k < cur.len; ++k) {
           wait(&full[kslot], k_phase);
+          const int h1 = solo ? q + 1 : odd && k == cur.len - 1 ? 1 : 2;
 #pragma unroll 1
           for (int h = h0; h < h1; ++h) {
             const bool first = k == 0 && h == h0, last = h == h1 - 1;
@@ -523,7 +531,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
                 all_first = paged_first_key(p, it.kv - it.qn + paged_token(p, r_hi));
       const bool none = r - lane >= it.rows;  // no row in this warp: its lanes of P and O are never looked at
       float m = -INFINITY, l = 0.f;
-      const int halves = solo ? cur.len : 2 * cur.len;
+      const int halves = solo ? cur.len : 2 * cur.len - chunk_odd(it, cur);
       for (int k = 0; k < halves; ++k, ++n) {
         const int b = n & 1;
         ok = ok && mbar_poll(&s_full[q][b], (n >> 1) & 1, p.status);
