@@ -15,8 +15,8 @@
 //
 // What bounds it is reading one or two rows of the vocabulary a request, behind
 // three dependent loads (offsets, drafts, their probabilities). A cluster of up to 8
-// CTAs takes one request: 128 warps with a contiguous stretch of the vocabulary
-// each sum their weights in one pass, the CTAs tell one another their sums over
+// CTAs takes one request: its warps, with a contiguous stretch of the vocabulary
+// each, sum their weights in one pass, the CTAs tell one another their sums over
 // distributed shared memory, and the CTA that has the place reads the one warp's
 // stretch again (from L2), an element a thread, to find the token. The weights are exact, so no order of these
 // sums has to be kept.
@@ -29,7 +29,7 @@
 
 namespace mlora {
 
-constexpr int kVerifyNT = 512;
+constexpr int kVerifyNT = 256;
 constexpr int kVerifyMaxCtas = 8;  // of a cluster
 
 // floor(2^40 x) as 2^23 hi + lo, x clamped to [0, 1] (NaN gives 0), by exact steps in
@@ -54,9 +54,9 @@ __device__ __forceinline__ void verify_tell(long long* p, uint32_t rank, long lo
   asm volatile("st.shared::cluster.s64 [%0], %1;" ::"r"(cluster_map(smem_addr(p), rank)), "l"(v) : "memory");
 }
 
-// CTAs an SM: four where the registers allow it (256 x 128256 in fp32: 54 us, 58 with three)
+// CTAs an SM: eight where the registers allow it (256 x 128256 in fp32: 51 us; 54 with six, or with four of 512 threads)
 template <typename T, int V>  // V elements a load: 16 bytes, or one
-__global__ void __launch_bounds__(kVerifyNT, sizeof(T) == 4 ? 4 : 3) verify_draft_kernel(const VerifyArgs p, int segment) {
+__global__ void __launch_bounds__(kVerifyNT, sizeof(T) == 4 ? 8 : 6) verify_draft_kernel(const VerifyArgs p, int segment) {
   constexpr int kWarps = kVerifyNT / 32;
   __shared__ long long s_warp[kWarps], s_find[kWarps], s_cta[2][kVerifyMaxCtas];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -228,12 +228,9 @@ namespace {
 template <typename T>
 cudaError_t launch_verify_t(const VerifyArgs& a, bool vec, cudaStream_t st, bool pdl) {
   constexpr int V = 16 / (int)sizeof(T);
-  // 4096 elements a CTA or more: below that the clusters only wait for one another
+  // 4096 elements a CTA or more: below that the CTAs of a cluster only wait for one another
   int ctas = 1;
-  // Large batches fill the GPU with smaller clusters, whose CTAs wait less for one
-  // another: 256 x 128256 took 54 us with 4 CTAs, 56 with 2 and 63 with 8.
-  const int most = a.requests > 64 ? 4 : kVerifyMaxCtas;
-  while (ctas < most && a.vocab > 4096 * ctas) ctas *= 2;
+  while (ctas < kVerifyMaxCtas && a.vocab > 4096 * ctas) ctas *= 2;
   const int unit = 32 * V, warps = ctas * (kVerifyNT / 32);
   const int segment = ((a.vocab + warps - 1) / warps + unit - 1) / unit * unit;
   cudaLaunchConfig_t cfg = {};
