@@ -22,12 +22,14 @@
 //     term would add as much error as the result's own rounding;
 //   * key tiles are dealt evenly over two CTAs an SM (paged_sched.cuh), or, for few
 //     short requests, an item to a cluster.
-// Keys outside [first, kv) may hold anything: scores are replaced, not added
-// to, and their V fragments are cleared before the product, since 0 * NaN is NaN.
+// Keys that a row does not see may hold anything: scores are replaced, not added
+// to, and since 0 * NaN is NaN the V fragments of keys outside [first, kv) are cleared
+// before the product, and infinities and NaN of keys that only some rows see are
+// taken out and added to these rows alone.
 //
 // Measured: 64 requests of 33 to 2048 keys, 32 heads of 128: 189 us, 5.6 TB/s (85 % of
 // the measured copy bandwidth); 4 requests of 20000 to 65536 keys, 8 key heads:
-// 110 us, 5.6 TB/s; one request of 777 keys: 6.3 us.
+// 114 us, 5.4 TB/s; one request of 777 keys: 6.5 us.
 #include <climits>
 
 #include "kernels.h"
@@ -290,13 +292,16 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
                            kf[n][c][2 * h], kf[n][c][2 * h + 1]);
         // V's fragments, in flight during the softmax: keys (lane % 4) * 2 + {0, 1} and + 8
         uint32_t vf[D / 16][4];
-        const int key = k0 + (lane & 15);
+        auto load_v = [&]() {
+          const int key = k0 + (lane & 15);
 #pragma unroll
-        for (int n = 0; n < D / 16; ++n) {  // 16 columns of V
-          const int chunk = n * 2 + (lane >> 4);
-          ldsm_x4_trans(vs + (chunk >> 3) * HALF + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), vf[n][0], vf[n][1],
-                        vf[n][2], vf[n][3]);
-        }
+          for (int n = 0; n < D / 16; ++n) {  // 16 columns of V
+            const int chunk = n * 2 + (lane >> 4);
+            ldsm_x4_trans(vs + (chunk >> 3) * HALF + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), vf[n][0], vf[n][1],
+                          vf[n][2], vf[n][3]);
+          }
+        };
+        load_v();
         float s[2][4];
         const bool edge = j0 + 16 > all_end || j0 < all_first;  // not all seen by all rows
 #pragma unroll
@@ -349,6 +354,43 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
             vf[n][1] &= clear1;
             vf[n][2] &= clear0;
             vf[n][3] &= clear1;
+          }
+        }
+        if (edge && it.qn > 1) {
+          uint32_t any = 0u;
+#pragma unroll
+          for (int n = 0; n < D / 16; ++n) 
+#pragma unroll
+            for (int e = 0; e < 4; ++e) any = paged_taint<T>(vf[n][e], any);
+          if (__builtin_expect(__any_sync(0xffffffffu, any != 0u), 0)) {
+#pragma unroll 1
+            for (int i = 0; i < 16; ++i) {
+              const int j = j0 + i, row = k0 + i;
+#pragma unroll
+              for (int n = 0; n < D / 8; ++n) {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(smem + stage * 2 * SIDE + SIDE + (n >> 3) * HALF + row * 128 +
+                                                                      (((n & 7) ^ (row & 7)) << 4) + (lane & 3) * 4);
+                const float a = Pack2<T>::lo(w), b = Pack2<T>::hi(w);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  if (j >= limit[e] || j < floor_[e]) continue;
+                  if (!isfinite(a)) o[n][2 * e] += a;
+                  if (!isfinite(b)) o[n][2 * e + 1] += b;
+                }
+              }
+            }
+            __syncwarp();
+#pragma unroll 1
+            for (int i = lane; i < 16 * (D / 2); i += 32) {  // out of the stage, whose fragments are loaded again
+              const int row = k0 + i / (D / 2), c = i % (D / 2);
+              uint32_t* at = reinterpret_cast<uint32_t*>(smem + stage * 2 * SIDE + SIDE + (c >> 5) * HALF + row * 128 +
+                                                         ((((c >> 2) & 7) ^ (row & 7)) << 4) + (c & 3) * 4);
+              const int j = j0 + row - k0;
+              *at = j < it.kv && j >= it.first ? paged_finite<T>(*at) : 0u;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            load_v();
           }
         }
 #pragma unroll
@@ -599,7 +641,7 @@ cudaError_t launch_decode(const DecodeArgs& a, cudaStream_t st, bool pdl) {
 
 template <typename T, int D>
 cudaError_t launch_decode_any(const DecodeArgs& a, cudaStream_t st, bool pdl) {
-  // One request of 777 keys, 8 key heads: 6.3 us with clusters, 11.3 without; 4000 keys 12.9 and 18.5. From
+  // One request of 777 keys, 8 key heads: 6.5 us with clusters, 11.3 without; 4000 keys 12.9 and 18.5. From
   // twice that on an item needs more CTAs than a cluster has. The host knows the lengths' bound only.
   if ((long long)a.a.requests * a.a.kv_heads <= kFewItems && (long long)a.a.width * a.a.block_size <= kFewKeys)
     return launch_decode<T, D, true>(a, st, pdl);

@@ -25,10 +25,18 @@
 //
 // What bounds it: the exponentials (16 a cycle and SM: 2048 cycles for two
 // 128 x 128 tiles) and the tensor cores (4096 multiply-adds a cycle: 2048
-// cycles for f16, 3072 for bf16 with its second term, at D = 128).
+// cycles for f16, 3072 for bf16 with its second term, at D = 128), and over a
+// long launch the power that these draw. Measured: 2048 tokens x 32 heads over 16384 keys in 630 to 710 us,
+// the tensor pipe 68 % busy at 1.6 GHz (f16: 593 us, 985 TFLOP/s); 8 prompts of 128 to
+// 1024 tokens 69 us, where an item's beginning and end (8000 cycles) weigh as
+// much as its tiles (4300 each); 32 requests of 1 to 6 drafts over up to 8192 keys 97 us,
+// 67 % of the measured copy bandwidth.
 //
-// Keys behind the cache's end may hold anything: their scores are replaced,
-// and their rows of V are cleared in shared memory, since 0 * NaN is NaN.
+// Keys that a row does not see may hold anything: their scores are replaced, and
+// since 0 * NaN is NaN their V is not multiplied by them. Rows of V that no row of
+// the item sees are cleared in shared memory; infinities and NaN in those that some
+// rows see are taken out there and added to these rows' outputs at the end. Both are done by
+// the warp that fetches Q, while the softmax works.
 #include <climits>
 
 #include "kernels.h"
@@ -76,6 +84,14 @@ __device__ __forceinline__ void chunk_span(const PagedAttnArgs& p, ChunkItem& it
   it.end = max(0, base + paged_token(p, r1 - 1) + 1);
   it.tile0 = it.first / kChunkKeys;
   it.n = max(1, (it.end + kChunkKeys - 1) / kChunkKeys - it.tile0);
+}
+
+// Keys [lo, hi) that every row of the item sees (none when lo >= hi).
+__device__ __forceinline__ void chunk_seen(const PagedAttnArgs& p, const ChunkItem& it, int& lo, int& hi) {
+  const int r0 = it.rt * kChunkRows, r1 = min(it.rows, r0 + kChunkRows);
+  const int base = it.kv - it.qn;
+  lo = paged_first_key(p, base + paged_token(p, r1 - 1));
+  hi = max(0, base + paged_token(p, r0) + 1);
 }
 
 // One tile of rows only: the warps of both tiles work on it, each on every other half of the keys.
@@ -192,6 +208,53 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+// What was taken out of V, added in TMEM to the outputs of row r, if it sees it: the
+// item's keys of [from, to) that not every row sees, those of every
+// tile's half `half` if that is not negative. Seldom run, so kept out of the kernel's registers.
+template <typename T, int D>
+__device__ __noinline__ void chunk_give_back(const PagedAttnArgs& p, uint32_t o_addr, int req, int head, int rt, int qn, int kv,
+                                             int r, int from, int to, int half) {
+  ChunkItem it;
+  it.qn = qn;
+  it.kv = kv;
+  it.rt = rt;
+  it.rows = qn * p.group;
+  int seen_lo, seen_hi;
+  chunk_seen(p, it, seen_lo, seen_hi);
+  const int pos = kv - qn + paged_token(p, r);
+  if (r < it.rows) {
+    from = max(from, paged_first_key(p, pos));
+    to = min(to, pos + 1);
+  } else {
+    to = from;
+  }
+#pragma unroll 1
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t o[32];
+    tmem_ld32_async(o_addr + c * 32, o);
+    tmem_wait_ld();
+    tie32(o);
+#pragma unroll 1
+    for (int j = from; j < to; ++j) {
+      if ((j >= seen_lo && j < seen_hi) || (half >= 0 && ((j / kHalfKeys) & 1) != half)) continue;
+      const int block = __ldcg(p.tables + req * p.table_stride + j / p.block_size);
+      if (block < 0 || block >= p.num_blocks) continue;
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.v) + block * p.v_block +
+                                                              (j % p.block_size) * p.v_slot + head * p.v_head + c * 32);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t w = __ldcg(src + i);
+        const float a = Pack2<T>::lo(w), b = Pack2<T>::hi(w);
+        if (!isfinite(a)) o[2 * i] = __float_as_uint(__uint_as_float(o[2 * i]) + a);
+        if (!isfinite(b)) o[2 * i + 1] = __float_as_uint(__uint_as_float(o[2 * i + 1]) + b);
+      }
+    }
+    __syncwarp();
+    tmem_st32(o_addr + c * 32, o);
+  }
+  tmem_wait_st();
+}
+
 template <int N>
 __device__ __forceinline__ void regs_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
@@ -213,6 +276,8 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
   __shared__ uint32_t s_tmem;
   __shared__ int s_last[2];
   __shared__ float2 s_mate[128];
+  __shared__ uint32_t s_clean;  // V tiles that have been cleaned
+  __shared__ uint32_t s_taken;           // a value that is not finite was taken out of one of them
   const PagedAttnArgs& p = args.a;
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = same_in_warp(tid >> 5);
@@ -222,7 +287,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 2);  // both warps of the tensor cores
+      mbar_init(&empty[s], 3);  // both warps of the tensor cores, and the one that cleans V
     }
     for (int q = 0; q < 2; ++q) {
       mbar_init(&q_ready[q], 1);
@@ -234,6 +299,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       }
     }
     fence_barrier_init();
+    s_clean = s_taken = 0u;
     tma_prefetch_map(&args.k_map);
     tma_prefetch_map(&args.v_map);
     if (args.q_tma) tma_prefetch_map(&args.q_map);
@@ -375,8 +441,10 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       bool held = false, held_first = false, held_last = false;  // the half whose product with V is to come
       uint32_t held_lo = 0;
       int held_slot = 0;
+      uint32_t dirty = 0, held_dirty = 0;  // V tiles to be cleaned so far; those that the held half waits for
       auto values = [&]() {  // half n - 1 of this tile of rows is the newest, half `number` the held one
         const int number = n - 1, b = number & 1;
+        if (held_dirty != 0u) ok = ok && count_poll(&s_clean, held_dirty, p.status);
         wait(&p_ready[q][b], number >> 1);
         tc_fence_after();
         if (elect_one()) {
@@ -397,6 +465,9 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         const int qs = solo ? 0 : q, h0 = solo ? q : 0;
         const bool odd = !solo && chunk_odd(it, cur);
         const uint32_t q_lo = smem_addr(smem + qs * C::kQ) >> 4;
+        int seen_lo, seen_hi;
+        chunk_seen(p, it, seen_lo, seen_hi);
+        bool tile_dirty = false;
         if (held) values();  // nothing of the item before waits for this one's Q, or keeps its V from the ring
 #pragma unroll 1
         for (int k = 0; k < cur.len; ++k) {
@@ -427,22 +498,10 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
             if (h == h0) {
               wait(&full[vslot], v_phase);
               const int j0 = (it.tile0 + cur.tile + k) * kChunkKeys;
-              if (j0 + kChunkKeys > it.kv || j0 < it.first) {  // rows of V that are nobody's
-                if (q == 0) {
-                  // whole boxes without a key are zeros already: clear what shares a box with one
-                  const int lo = max(0, it.first - j0), lo0 = lo / args.box * args.box;
-                  const int hi = min(kChunkKeys, max(0, it.kv - j0)), hi1 = min(kChunkKeys, (hi + args.box - 1) / args.box * args.box);
-                  unsigned char* vs = ring + vslot * C::kSlot;
-#pragma unroll 1
-                  for (int e = lane; e < (lo - lo0 + hi1 - hi) * (D / 8); e += 32) {
-                    const int i = e / (D / 8), c = e % (D / 8), j = i < lo - lo0 ? lo0 + i : hi + i - (lo - lo0);
-                    *reinterpret_cast<uint4*>(vs + (c >> 3) * HALF + j * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-                  }
-                  fence_proxy_async_smem();
-                }
-                named_barrier(3, 64);
-              }
+              tile_dirty = j0 + kChunkKeys > seen_hi || j0 < seen_lo;
+              if (tile_dirty) ++dirty;
             }
+            held_dirty = tile_dirty ? dirty : 0u;
             held = true;
             held_first = first;
             held_last = last;
@@ -465,8 +524,10 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         if (cur.advance()) next_item();
       }
       if (held) values();
-    } else {  // ---- Q of each item, as soon as the scores of the item before are done ----
+    } else {  // ---- Q of each item, as soon as the scores of the item before are done; V's tiles cleaned ----
       int items[2] = {0, 0};
+      int slot = 0, phase = 0;
+      uint32_t dirty = 0;
       while (cur.take(it.n)) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
@@ -504,6 +565,61 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_ready[q]);
+          }
+        }
+        int seen_lo, seen_hi;
+        chunk_seen(p, it, seen_lo, seen_hi);
+        for (int k = 0; k < 2 * cur.len; ++k) {  // K, V, K, V: every slot is let go by this warp too, so it never misses a phase
+          const int j0 = (it.tile0 + cur.tile + (k >> 1)) * kChunkKeys;
+          ok = __all_sync(0xffffffffu, ok && mbar_poll(&full[slot], phase, p.status));
+          if ((k & 1) != 0 && (j0 + kChunkKeys > seen_hi || j0 < seen_lo)) {
+            ++dirty;
+            unsigned char* vs = ring + slot * C::kSlot;
+            // whole boxes without a key are zeros already: clear what shares a box with one
+            const int lo = min(kChunkKeys, max(0, it.first - j0)), lo0 = lo / args.box * args.box;
+            const int hi = min(kChunkKeys, max(0, it.end - j0)), hi1 = min(kChunkKeys, (hi + args.box - 1) / args.box * args.box);
+            if (ok) {
+#pragma unroll 1
+              for (int e = lane; e < (lo - lo0 + hi1 - hi) * (D / 8); e += 32) {
+                const int i = e / (D / 8), c = e % (D / 8), j = i < lo - lo0 ? lo0 + i : hi + i - (lo - lo0);
+                *reinterpret_cast<uint4*>(vs + (c >> 3) * HALF + j * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+              }
+              // keys that only some rows see: [lo, some) by the window, [rest, hi) by the causal mask
+              const int some = max(lo, min(hi, seen_lo - j0)), rest = max(some, min(hi, seen_hi - j0));
+              uint32_t taken = 0u;
+              constexpr int PER = D / 8, STEP = 32 / PER, AT_ONCE = 8;  // 16-byte pieces a row, rows at once, and in flight
+              const int c = lane % PER;
+              unsigned char* col = vs + (c >> 3) * HALF + (c & 7) * 16;
+#pragma unroll 1
+              for (int part = 0; part < 2; ++part) {
+                const int end = part == 0 ? some : hi;
+#pragma unroll 1
+                for (int j = (part == 0 ? lo : rest) + lane / PER; j < end; j += STEP * AT_ONCE) {
+                  uint32_t seen = 0u;
+#pragma unroll
+                  for (int i = 0; i < AT_ONCE; ++i) {  // a row twice rather than one behind the end
+                    const uint4 u = *reinterpret_cast<const uint4*>(col + min(j + i * STEP, end - 1) * 128);
+                    seen = paged_taint<T>(u.w, paged_taint<T>(u.z, paged_taint<T>(u.y, paged_taint<T>(u.x, seen))));
+                  }
+                  if (seen == 0u) continue;
+                  taken = 1u;
+#pragma unroll 1
+                  for (int i = j; i < min(end, j + STEP * AT_ONCE); i += STEP) {
+                    uint4* at = reinterpret_cast<uint4*>(col + i * 128);
+                    *at = make_uint4(paged_finite<T>(at->x), paged_finite<T>(at->y), paged_finite<T>(at->z), paged_finite<T>(at->w));
+                  }
+                }
+              }
+              if (taken != 0u) count_store(&s_taken, 1u);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) count_store(&s_clean, dirty);
+          }
+          if (lane == 0) mbar_arrive(&empty[slot]);
+          if (++slot == NS) {
+            slot = 0;
+            phase ^= 1;
           }
         }
         if (cur.advance()) next_item();
@@ -630,11 +746,16 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       const ChunkItem done = it;
       const bool whole = cur.whole(it.n);
       const int item0 = cur.pos - cur.unit;
+      const int tile0 = it.tile0 + cur.tile, tiles = cur.len;
       if (cur.advance()) next_item();
 
       ok = ok && mbar_poll(&pv_done[q][(n - 1) & 1], ((n - 1) >> 1) & 1, p.status);
       __syncwarp();
       tc_fence_after();
+      if (__any_sync(0xffffffffu, *const_cast<volatile uint32_t*>(&s_taken) != 0u)) {
+        chunk_give_back<T, D>(p, o_addr, done.req, done.head, done.rt, done.qn, done.kv, r, tile0 * kChunkKeys,
+                              (tile0 + tiles) * kChunkKeys, solo ? q : -1);
+      }
       // An item that both warpgroups worked on: the first one reads the other's O too
       // (their threads of a row have the same TMEM lane).
       float own = 1.f, others = 0.f;  // what the two warpgroups' sums are multiplied by

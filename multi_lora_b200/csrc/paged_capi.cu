@@ -159,7 +159,7 @@ int mlora_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
   if (tokens < 0 || tokens * q_heads > INT32_MAX || requests < 0 || requests > INT32_MAX || max_q_len < 0)
     return refuse(MLORA_ERR_INVALID_ARGUMENT, "%lld tokens of %lld requests, %lld at most each", (long long)tokens,
                   (long long)requests, (long long)max_q_len);
-  if (max_blocks < 0 || max_blocks > INT32_MAX / c.block_size || table_row_stride < max_blocks)
+  if (max_blocks < 0 || max_blocks > (INT32_MAX - 256) / c.block_size || table_row_stride < max_blocks)
     return refuse(MLORA_ERR_INVALID_ARGUMENT, "block tables %lld wide, rows %lld apart", (long long)max_blocks,
                   (long long)table_row_stride);
   if (window < 0) return refuse(MLORA_ERR_INVALID_ARGUMENT, "window %d < 0", window);

@@ -231,6 +231,20 @@ __device__ __forceinline__ void paged_zero_rest(const PagedAttnArgs& p) {
   }
 }
 
+// Infinities and NaN in pairs of 16-bit values: fma(w, 0, seen) stays zero while everything is finite.
+template <typename T>
+__device__ __forceinline__ uint32_t paged_taint(uint32_t w, uint32_t seen) {
+  if constexpr (Num<T>::is_bf16) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(seen) : "r"(w), "r"(0u));
+  else asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(seen) : "r"(w), "r"(0u));
+  return seen;
+}
+// The pair with zeros in their place.
+template <typename T>
+__device__ __forceinline__ uint32_t paged_finite(uint32_t w) {
+  constexpr uint32_t kExp = Num<T>::is_bf16 ? 0x7f807f80u : 0x7c007c00u, kOne = Num<T>::is_bf16 ? 0x00800080u : 0x04000400u;
+  return w & ~(((((w & kExp) + kOne) & 0x80008000u) >> 15) * 0xffffu);  // a carry where all exponent bits are set
+}
+
 // 2^x on the special function unit; 0 for -infinity.
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -266,6 +280,27 @@ __device__ __forceinline__ bool mbar_poll(uint64_t* bar, uint32_t parity, uint32
     }
   }
   return true;
+}
+
+// A count in shared memory that one warp raises and others wait for.
+__device__ __forceinline__ void count_store(uint32_t* at, uint32_t n) {
+  asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(smem_addr(at)), "r"(n) : "memory");
+}
+__device__ __forceinline__ bool count_poll(uint32_t* at, uint32_t n, uint32_t* status) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 1;; ++i) {
+    uint32_t now;
+    asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(now) : "r"(smem_addr(at)) : "memory");
+    if (now >= n) return true;
+    if ((i & 127u) == 0) {
+      const uint64_t t = global_timer_ns();
+      if (t0 == 0) t0 = t;
+      if (t - t0 > kWaitLimitNs) {
+        flag_error(status, kErrTimeout);
+        return false;
+      }
+    }
+  }
 }
 
 // 32 bytes at once (one sector).
