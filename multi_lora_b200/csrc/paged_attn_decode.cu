@@ -20,6 +20,8 @@
 //     probability is rounded once (11 bits); a bf16 one goes in as two terms, its
 //     rounding and the rounding's remainder (16 bits), since the 8 bits of one
 //     term would add as much error as the result's own rounding;
+//   * head_dims below 64 and between 64 and 128 run as these: the boxes' columns behind
+//     them are zeros, and no memory;
 //   * key tiles are dealt evenly over two CTAs an SM (paged_sched.cuh), or, for few
 //     short requests, an item to a cluster.
 // Keys that a row does not see may hold anything: scores are replaced, not added
@@ -236,8 +238,8 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       const bool real = r < x.qn * group;
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
-        qf[k][e] = real ? __ldcg(reinterpret_cast<const unsigned int*>(src + k * 16)) : 0u;
-        qf[k][2 + e] = real ? __ldcg(reinterpret_cast<const unsigned int*>(src + k * 16 + 8)) : 0u;
+        qf[k][e] = real && k * 16 < p.dim ? __ldcg(reinterpret_cast<const unsigned int*>(src + k * 16)) : 0u;
+        qf[k][2 + e] = real && k * 16 + 8 < p.dim ? __ldcg(reinterpret_cast<const unsigned int*>(src + k * 16 + 8)) : 0u;
       }
     }
   };
@@ -482,6 +484,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       for (int g = 0; g < C::KG; ++g) sum += top == -INFINITY ? 0.f : s_l[g][r] * exp2_fast(s_m[g][r] - top);
     };
     auto store = [&](int r, int c, const float* v, float inv) {  // 8 columns of row r
+      if (c >= p.dim) return;
       const int t = paged_token(p, r);
       T* dst = static_cast<T*>(p.out) + (done.q0 + t) * p.out_token + (done.head * group + r - t * group) * p.out_head + c;
       uint4 u;
@@ -551,6 +554,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
           v.z = fmaf(u[x].z, w, v.z);
           v.w = fmaf(u[x].w, w, v.w);
         }
+        if (c >= p.dim) continue;
         const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
         const int t = paged_token(p, row);
         T* dst = static_cast<T*>(p.out) + (int64_t)(done.q0 + t) * p.out_token +
@@ -651,7 +655,7 @@ cudaError_t launch_decode_any(const DecodeArgs& a, cudaStream_t st, bool pdl) {
 }  // namespace
 
 cudaError_t launch_paged_attention_decode(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl) {
-  if ((dtype != kBF16 && dtype != kF16) || (a.dim != 64 && a.dim != 128)) return cudaErrorNotSupported;
+  if ((dtype != kBF16 && dtype != kF16) || a.dim > 128) return cudaErrorNotSupported;
   // units of work (paged_sched.cuh) in 32 bits
   if ((long long)a.requests * a.kv_heads * ((long long)a.width * a.block_size / kDecTile + 2 + kDecItem) > INT_MAX)
     return cudaErrorNotSupported;
@@ -660,8 +664,8 @@ cudaError_t launch_paged_attention_decode(const PagedAttnArgs& a, int dtype, cud
   d.box = paged_box(a.block_size, kDecTile);
   if (d.box < 8 || !paged_maps(a, dtype, d.box, &d.k_map, &d.v_map)) return cudaErrorNotSupported;
   if (dtype == kBF16)
-    return a.dim == 64 ? launch_decode_any<__nv_bfloat16, 64>(d, st, pdl) : launch_decode_any<__nv_bfloat16, 128>(d, st, pdl);
-  return a.dim == 64 ? launch_decode_any<__half, 64>(d, st, pdl) : launch_decode_any<__half, 128>(d, st, pdl);
+    return a.dim <= 64 ? launch_decode_any<__nv_bfloat16, 64>(d, st, pdl) : launch_decode_any<__nv_bfloat16, 128>(d, st, pdl);
+  return a.dim <= 64 ? launch_decode_any<__half, 64>(d, st, pdl) : launch_decode_any<__half, 128>(d, st, pdl);
 }
 
 }  // namespace mlora

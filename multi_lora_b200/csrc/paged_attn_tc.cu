@@ -23,6 +23,9 @@
 // its upper 8 bits and the rest (16 bits): one term of 8 bits would add as much
 // error as the result's own rounding. The second term is one more product of the same size.
 //
+// Head_dims below 64 and between 64 and 128 run as these, with columns of zeros that
+// TMA fills in.
+//
 // What bounds it: the exponentials (16 a cycle and SM: 2048 cycles for two
 // 128 x 128 tiles) and the tensor cores (4096 multiply-adds a cycle: 2048
 // cycles for f16, 3072 for bf16 with its second term, at D = 128), and over a
@@ -243,7 +246,7 @@ __device__ __noinline__ void chunk_give_back(const PagedAttnArgs& p, uint32_t o_
                                                               (j % p.block_size) * p.v_slot + head * p.v_head + c * 32);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const uint32_t w = __ldcg(src + i);
+        const uint32_t w = c * 32 + 2 * i < p.dim ? __ldcg(src + i) : 0u;
         const float a = Pack2<T>::lo(w), b = Pack2<T>::hi(w);
         if (!isfinite(a)) o[2 * i] = __float_as_uint(__uint_as_float(o[2 * i]) + a);
         if (!isfinite(b)) o[2 * i + 1] = __float_as_uint(__uint_as_float(o[2 * i + 1]) + b);
@@ -552,7 +555,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
               for (int i = 0; i < AT_ONCE; ++i) {
                 const int e = e0 + i * 32, r = r0 + e / PIECES, c = e % PIECES, t = paged_token(p, r);
                 u[i] = make_uint4(0, 0, 0, 0);
-                if (r < it.rows)
+                if (r < it.rows && c * 8 < p.dim)
                   u[i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (int64_t)(it.q0 + t) * p.q_token +
                                                                (int64_t)(it.head * p.group + r - t * p.group) * p.q_head + c * 8));
               }
@@ -784,10 +787,10 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) u[i] = pack_round2<T>(v[2 * i] * inv, v[2 * i + 1] * inv);
         if (args.out32) {
-          store32(dst + c, u);
+          if (c < p.dim) store32(dst + c, u);
         } else {
-          *reinterpret_cast<uint4*>(dst + c) = make_uint4(u[0], u[1], u[2], u[3]);
-          *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(u[4], u[5], u[6], u[7]);
+          if (c < p.dim) *reinterpret_cast<uint4*>(dst + c) = make_uint4(u[0], u[1], u[2], u[3]);
+          if (c + 8 < p.dim) *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(u[4], u[5], u[6], u[7]);
         }
       };
       // pieces: [column / 4][row] of four floats, then maxima, then sums
@@ -905,7 +908,7 @@ cudaError_t launch_chunk(const ChunkArgs& a, cudaStream_t st, bool pdl) {
 }  // namespace
 
 cudaError_t launch_paged_attention_chunk(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl) {
-  if ((dtype != kBF16 && dtype != kF16) || (a.dim != 64 && a.dim != 128) || !(a.scale > 0.f))
+  if ((dtype != kBF16 && dtype != kF16) || a.dim > 128 || !(a.scale > 0.f))
     return cudaErrorNotSupported;  // a maximum of scores is one of scaled scores for a positive scale only
   // units of work (paged_sched.cuh) in 32 bits
   const long long items = (long long)a.tokens * a.group / kChunkRows + a.requests;
@@ -915,10 +918,10 @@ cudaError_t launch_paged_attention_chunk(const PagedAttnArgs& a, int dtype, cuda
   c.box = paged_box(a.block_size, kChunkKeys);
   if (c.box < 8 || !paged_maps(a, dtype, c.box, &c.k_map, &c.v_map)) return cudaErrorNotSupported;
   c.q_tma = paged_q_map(a, dtype, 128, &c.q_map);
-  c.out32 = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_token % 16 == 0 && a.out_head % 16 == 0;
+  c.out32 = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_token % 16 == 0 && a.out_head % 16 == 0 && a.dim % 16 == 0;
   if (dtype == kBF16)
-    return a.dim == 64 ? launch_chunk<__nv_bfloat16, 64>(c, st, pdl) : launch_chunk<__nv_bfloat16, 128>(c, st, pdl);
-  return a.dim == 64 ? launch_chunk<__half, 64>(c, st, pdl) : launch_chunk<__half, 128>(c, st, pdl);
+    return a.dim <= 64 ? launch_chunk<__nv_bfloat16, 64>(c, st, pdl) : launch_chunk<__nv_bfloat16, 128>(c, st, pdl);
+  return a.dim <= 64 ? launch_chunk<__half, 64>(c, st, pdl) : launch_chunk<__half, 128>(c, st, pdl);
 }
 
 }  // namespace mlora

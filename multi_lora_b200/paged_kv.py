@@ -125,7 +125,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     Queries that see no key and rows past q_indptr[-1] give zeros. What a query
     does not see does not reach it, infinities and NaN included. bfloat16,
     float16 or float32; head_dim a multiple of 8, at most 256; the tensor-core
-    kernels take 16-bit caches with head_dim 64 or 128.
+    kernels take 16-bit caches with head_dim up to 128 and blocks of a multiple of 8 slots.
     """
     _need_cuda(q, "paged_attention")
     if scale is None:
