@@ -32,3 +32,21 @@ def test_attention_of_head_dims_between(cuda_dev, workspace, case, dim, layout, 
     assert (out[:, :, dim:] == 7).all()
     assert (got[sum(q_lens):] == 0).all()
     assert_attention(got, pr, dtype)
+
+
+@pytest.mark.parametrize("dim, dtype, block", [(256, "bf16", 16), (136, "f16", 8), (128, "f32", 16), (40, "f32", 5)])
+@pytest.mark.parametrize("q_lens, kv_lens, heads, window", [
+    ([1], [5000], (8, 8), 0),            # a cluster an item
+    ([1, 2], [2100, 700], (14, 2), 0),   # seven heads a key head: four and three
+    ([2], [3000], (4, 2), 900),
+    ([1, 0, 1], [1, 5, 300], (6, 1), 0),
+    ([90, 1] * 3, [90, 1500] * 3, (4, 2), 64),
+    ([3], [1], (2, 2), 0),               # rows without a key
+])
+def test_attention_of_large_heads_and_fp32(cuda_dev, workspace, q_lens, kv_lens, heads, window, dim, dtype, block):  # noqa: F811
+    pr = attention_problem(cuda_dev, 32, q_lens, kv_lens, *heads, dim, dtype, block)
+    status = status_word(cuda_dev)
+    got = attend(pr, workspace, window=window, status=status)
+    assert status.item() == 0
+    assert_attention(got, pr, dtype, window)
+    assert torch.equal(attend(pr, workspace, window=window), got)
