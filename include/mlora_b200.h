@@ -315,7 +315,7 @@ int mlora_row_parallel_apply_p2p(const void* x, int64_t rows, int64_t in_shard, 
  *              Past the last token: 0 and -1.
  *   ticket     one device word, zero before the first call; calls that share
  *              it must not overlap on the GPU.
- * requests <= 8192. The launch does not overlap the kernels that follow it.
+ * requests <= 8192, requests * (max_tokens + 1) < 2^32. The launch does not overlap the kernels that follow it.
  */
 int mlora_plan_paged_step(const int32_t* ctx_lens, const int32_t* new_lens, const int32_t* held_blocks,
                           int64_t requests, const int32_t* free_blocks, int64_t num_free, const int32_t* free_head,

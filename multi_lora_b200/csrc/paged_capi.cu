@@ -73,6 +73,9 @@ int mlora_plan_paged_step(const int32_t* ctx_lens, const int32_t* new_lens, cons
   if (num_free < 0 || num_free > INT32_MAX || max_tokens < 0 || max_tokens >= INT32_MAX)
     return refuse(MLORA_ERR_INVALID_ARGUMENT, "%lld free blocks, %lld tokens", (long long)num_free,
                   (long long)max_tokens);
+  if ((max_tokens + 1) * (requests > 0 ? requests : 1) > (int64_t)UINT32_MAX)  // sums of clamped lengths in 32 bits
+    return refuse(MLORA_ERR_INVALID_ARGUMENT, "%lld requests of %lld tokens: the product passes 32 bits",
+                  (long long)requests, (long long)max_tokens);
   if (q_indptr == nullptr || free_head == nullptr || free_head_out == nullptr || ticket == nullptr)
     return refuse(MLORA_ERR_INVALID_ARGUMENT, "q_indptr / free_head / free_head_out / ticket is NULL");
   if (requests > 0 && (ctx_lens == nullptr || new_lens == nullptr || held_blocks == nullptr || kv_lens == nullptr ||
@@ -165,6 +168,8 @@ int mlora_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
   if (window < 0) return refuse(MLORA_ERR_INVALID_ARGUMENT, "window %d < 0", window);
   if (q_token_stride < 0 || q_head_stride < 0 || out_token_stride < 0 || out_head_stride < c.head_dim)
     return refuse(MLORA_ERR_INVALID_ARGUMENT, "q / out stride");
+  if (tokens > 1 && out_token_stride < c.head_dim)
+    return refuse(MLORA_ERR_INVALID_ARGUMENT, "rows of out %lld apart overlap", (long long)out_token_stride);
   if (workspace == nullptr || workspace_bytes < mlora_paged_attention_workspace_bytes() ||
       reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
     return refuse(MLORA_ERR_INVALID_ARGUMENT, "workspace of %zu bytes: %zu, 256-byte aligned, are wanted",

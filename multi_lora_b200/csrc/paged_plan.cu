@@ -18,6 +18,9 @@
 // own memory: the CTA that counts itself last (every other one has read its
 // inputs by then) writes them.
 //
+// Measured: 64 requests of one token 3.5 us, 256 requests with 131000 tokens 5.2 us
+// (1.0 MB written), of which an empty launch is about 2.5.
+//
 // The kernel never triggers dependent launches: kernels that follow may read
 // q_indptr as segment routing before their own wait.
 #include <climits>

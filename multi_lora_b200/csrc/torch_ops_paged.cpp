@@ -47,6 +47,9 @@ uint32_t* status_word(const c10::optional<at::Tensor>& status, const at::Device&
 
 void done(int rc) { TORCH_CHECK(rc == MLORA_OK, "mlora: ", mlora_last_error()); }
 
+// Stride of dimension d: `dense` where there is one entry, whose stride may be anything.
+int64_t stride_of(const at::Tensor& t, int64_t d, int64_t dense) { return t.size(d) > 1 ? t.stride(d) : dense; }
+
 int64_t table_rows(const at::Tensor& t, int64_t requests, const at::Device& dev) {
   on_device(t, "block_tables", dev);
   TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == 2 && t.size(0) == requests &&
@@ -150,11 +153,11 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
   } else {
     out = at::detail::empty_cuda(q.sizes(), q.scalar_type(), dev, c10::nullopt);
   }
-  done(mlora_paged_attention(q.data_ptr(), q.stride(0), q.stride(1), q.size(0), (int32_t)q.size(1), &c,
+  done(mlora_paged_attention(q.data_ptr(), stride_of(q, 0, c.head_dim), stride_of(q, 1, c.head_dim), q.size(0), (int32_t)q.size(1), &c,
                              block_tables.numel() > 0 ? block_tables.data_ptr<int32_t>() : nullptr, rows,
                              block_tables.size(1), i32(kv_lens, "kv_lens", r, dev),
                              i32(q_indptr, "q_indptr", r + 1, dev), r, max_q_len, (float)scale, (int32_t)window,
-                             out.data_ptr(), out.stride(0), out.stride(1), workspace.data_ptr(),
+                             out.data_ptr(), stride_of(out, 0, c.head_dim), stride_of(out, 1, c.head_dim), workspace.data_ptr(),
                              (size_t)workspace.nbytes(), status_word(status, dev),
                              at::cuda::getCurrentCUDAStream().stream()));
   return out;
@@ -186,9 +189,10 @@ std::tuple<at::Tensor, at::Tensor> verify_draft(const at::Tensor& target, const 
   const c10::cuda::CUDAGuard guard(dev);
   at::Tensor tokens = at::detail::empty_cuda({r, k + 1}, at::kLong, dev, c10::nullopt);
   at::Tensor emitted = at::detail::empty_cuda({r}, at::kInt, dev, c10::nullopt);
-  done(mlora_verify_draft(target.data_ptr(), target.size(0), vocab, target.stride(0),
-                          draft.has_value() ? draft->data_ptr() : nullptr, draft.has_value() ? draft->stride(0) : 0,
-                          draft.has_value() ? draft->stride(1) : 0, draft_tokens.data_ptr<int64_t>(),
+  done(mlora_verify_draft(target.data_ptr(), target.size(0), vocab, stride_of(target, 0, vocab),
+                          draft.has_value() ? draft->data_ptr() : nullptr,
+                          draft.has_value() ? stride_of(*draft, 0, k * vocab) : 0,
+                          draft.has_value() ? stride_of(*draft, 1, vocab) : 0, draft_tokens.data_ptr<int64_t>(),
                           i32(row_indptr, "row_indptr", r + 1, dev), r, (int32_t)k, accept_u.data_ptr<float>(),
                           sample_u.data_ptr<float>(), tokens.data_ptr<int64_t>(), emitted.data_ptr<int32_t>(),
                           code(target.scalar_type()), status_word(status, dev),

@@ -18,8 +18,10 @@
 // CTAs takes one request: its warps, with a contiguous stretch of the vocabulary
 // each, sum their weights in one pass, the CTAs tell one another their sums over
 // distributed shared memory, and the CTA that has the place reads the one warp's
-// stretch again (from L2), an element a thread, to find the token. The weights are exact, so no order of these
-// sums has to be kept.
+// stretch again (from L2), an element a thread, to find the token. The weights are
+// exact, so no order of these sums has to be kept. Measured: 256 requests of 0 to 4
+// drafts over 128256 words in fp32 51 us, 3.9 TB/s (59 % of the measured copy): the loads pause while
+// drafts are accepted and sums exchanged; one request of 32000 words 5.1 us.
 #include <type_traits>
 
 #include "common.cuh"

@@ -79,6 +79,15 @@ def test_write_plan_and_verify_argument_validation():
         assert verify(**bad) == code, bad
 
 
+def test_more_refusals():
+    assert attend(ot=32) == -1  # rows of the output that overlap
+    assert attend(tokens=1, ot=0, r=0, most=0, oh=8) == -1
+    lib = _native.capi()
+    plan = lambda r, most: lib.mlora_plan_paged_step(16, 16, 16, r, 16, 4, 16, 16, 4, 4, 16, 16, 16, 16, 16, 16, 16,  # noqa: E731
+                                                     most, 16, None, None)
+    assert plan(8192, 2 ** 19) == -1 and b"32 bits" in lib.mlora_last_error()
+
+
 def test_cpu_tensors_are_refused():
     z = torch.zeros(1)
     with pytest.raises(RuntimeError, match="CUDA"):
