@@ -18,10 +18,10 @@
 // CTAs takes one request: its warps, with a contiguous stretch of the vocabulary
 // each, sum their weights in one pass, the CTAs tell one another their sums over
 // distributed shared memory, and the CTA that has the place reads the one warp's
-// stretch again (from L2), an element a thread, to find the token. The weights are
+// stretch again (from L2), 16 bytes a thread, to find the token. The weights are
 // exact, so no order of these sums has to be kept. Measured: 256 requests of 0 to 4
-// drafts over 128256 words in fp32 51 us, 3.9 TB/s (59 % of the measured copy): the loads pause while
-// drafts are accepted and sums exchanged; one request of 32000 words 5.1 us.
+// drafts over 128256 words in fp32 47.5 us, 4.1 TB/s (63 % of the measured copy): the loads pause while
+// drafts are accepted and sums exchanged; one request of 32000 words 5.2 us.
 #include <type_traits>
 
 #include "common.cuh"
@@ -56,7 +56,7 @@ __device__ __forceinline__ void verify_tell(long long* p, uint32_t rank, long lo
   asm volatile("st.shared::cluster.s64 [%0], %1;" ::"r"(cluster_map(smem_addr(p), rank)), "l"(v) : "memory");
 }
 
-// CTAs an SM: eight where the registers allow it (256 x 128256 in fp32: 51 us; 54 with six, or with four of 512 threads)
+// CTAs an SM: eight where the registers allow it (256 x 128256 in fp32, before the search below took 16 bytes a thread: 51 us; 54 with six, or with four of 512 threads)
 template <typename T, int V>  // V elements a load: 16 bytes, or one
 __global__ void __launch_bounds__(kVerifyNT, sizeof(T) == 4 ? 8 : 6) verify_draft_kernel(const VerifyArgs p, int segment) {
   constexpr int kWarps = kVerifyNT / 32;
@@ -118,6 +118,7 @@ __global__ void __launch_bounds__(kVerifyNT, sizeof(T) == 4 ? 8 : 6) verify_draf
     }
   }
 
+  auto weight_of = [](uint32_t hi, uint32_t lo) { return ((long long)(hi - kVerifyBias) << 23) + (lo - kVerifyBias); };
   // hi and lo of elements v .. v + W - 1 below `end`
   auto weights = [&](auto width, int v, int end, uint32_t* hi, uint32_t* lo) {
     constexpr int W = decltype(width)::value;
@@ -186,14 +187,20 @@ __global__ void __launch_bounds__(kVerifyNT, sizeof(T) == 4 ? 8 : 6) verify_draf
       if (place >= 0 && place < own) {
         int w = 0;
         while (place >= s_warp[w]) place -= s_warp[w++];
-        // the stretch that holds it, by the whole CTA, an element a thread
+        // the stretch that holds it, by the whole CTA: PER elements side by side a thread (one element each: 256 x 128256 51 us, 47.5 so)
+        constexpr int PIECES = V == 1 ? 4 : 1, PER = PIECES * V;
         const int b0 = (int)(first + (int64_t)w * segment), b1 = min(p.vocab, b0 + segment);
         long long at = 0;
-        for (int b = b0; b < b1 && at <= place; b += kVerifyNT) {
-          const int v = b + tid;
-          uint32_t hi = kVerifyBias, lo = kVerifyBias;
-          if (v < b1) weights(std::integral_constant<int, 1>(), v, b1, &hi, &lo);
-          const long long mine = ((long long)(hi - kVerifyBias) << 23) + (lo - kVerifyBias);
+        for (int b = b0; b < b1 && at <= place; b += kVerifyNT * PER) {
+          const int v = b + tid * PER;
+          uint32_t hi[PIECES][V], lo[PIECES][V];
+          long long mine = 0;
+#pragma unroll
+          for (int k = 0; k < PIECES; ++k) {
+            weights(std::integral_constant<int, V>(), v + k * V, b1, hi[k], lo[k]);
+#pragma unroll
+            for (int e = 0; e < V; ++e) mine += weight_of(hi[k][e], lo[k][e]);
+          }
           long long incl = mine;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
@@ -208,7 +215,18 @@ __global__ void __launch_bounds__(kVerifyNT, sizeof(T) == 4 ? 8 : 6) verify_draf
             incl += k < warp ? s_find[k] : 0;
             all += s_find[k];
           }
-          if (place < incl && place >= incl - mine) out[kept] = v;
+          if (place < incl && place >= incl - mine) {
+            long long left = place - (incl - mine);
+            int found = -1;
+#pragma unroll
+            for (int k = 0; k < PIECES; ++k)
+#pragma unroll
+              for (int e = 0; e < V; ++e) {
+                left -= weight_of(hi[k][e], lo[k][e]);
+                if (left < 0 && found < 0) found = v + k * V + e;
+              }
+            out[kept] = found;
+          }
           at += all;
           __syncthreads();
         }
