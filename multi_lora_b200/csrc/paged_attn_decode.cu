@@ -567,41 +567,65 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     }
     if (!whole) {
       const int c0 = split.first_cta(item0, done.n), c1 = split.last_cta(item0, done.n);
-      named_barrier(1, C::kWarps * 32);
-      if (tid == 0) {
-        __threadfence();
-        const bool last = atomicAdd(tickets + c0, 1u) == (uint32_t)(c1 - c0);
-        if (last) tickets[c0] = 0u;
-        __threadfence();
-        s_last = last;
-      }
-      named_barrier(1, C::kWarps * 32);
-      if (s_last) {
-        auto piece = [&](int c) { return parts + ((long long)c * 2 + (c == c0 ? 1 : 0)) * PART; };
-        for (int e = tid; e < rows * (D / 8); e += C::kWarps * 32) {
-          const int r = e / (D / 8), c = (e % (D / 8)) * 8;
-          float top = -INFINITY, sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-          for (int x = c0; x <= c1; ++x) {
-            const float* src = piece(x);
-            const float2 stat = __ldcg(reinterpret_cast<const float2*>(src + 16 * D) + r);
-            const float4 v0 = __ldcg(reinterpret_cast<const float4*>(src + r * D + c));
-            const float4 v1 = __ldcg(reinterpret_cast<const float4*>(src + r * D + c + 4));
-            const float m_new = fmaxf(top, stat.x), ref = m_new == -INFINITY ? 0.f : m_new;
-            const float fix = exp2_fast(top - ref), w = exp2_fast(stat.x - ref);
-            top = m_new;
-            sum = fmaf(sum, fix, stat.y * w);
-            v[0] = fmaf(v[0], fix, v0.x * w);
-            v[1] = fmaf(v[1], fix, v0.y * w);
-            v[2] = fmaf(v[2], fix, v0.z * w);
-            v[3] = fmaf(v[3], fix, v0.w * w);
-            v[4] = fmaf(v[4], fix, v1.x * w);
-            v[5] = fmaf(v[5], fix, v1.y * w);
-            v[6] = fmaf(v[6], fix, v1.z * w);
-            v[7] = fmaf(v[7], fix, v1.w * w);
-          }
-          store(r, c, v, sum > 0.f || sum != sum ? 1.f / sum : 0.f);
+      const PagedJoin run(c0, c1, blockIdx.x);
+      auto piece = [&](int c) { return parts + ((long long)c * 2 + (c == c0 ? 1 : 0)) * PART; };
+      auto last_of = [&](uint32_t* ticket, int n) {  // whether this CTA is the last of n to get here
+        named_barrier(1, C::kWarps * 32);
+        if (tid == 0) {
+          __threadfence();
+          const bool last = atomicAdd(ticket, 1u) == (uint32_t)(n - 1);
+          if (last) *ticket = 0u;
+          __threadfence();
+          s_last = last;
         }
+        named_barrier(1, C::kWarps * 32);
+        return s_last != 0;
+      };
+      // Pieces x0, x0 + by, .. x1, to the output or as one piece to x0's place.
+      auto join = [&](int x0, int x1, int by, bool final) {
+        for (int e0 = 0; e0 < rows * (D / 8); e0 += C::kWarps * 32) {
+          const int e = e0 + tid, r = e / (D / 8), c = (e % (D / 8)) * 8;
+          const bool real = e < rows * (D / 8);
+          float top = -INFINITY, sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          if (real) {
+#pragma unroll 8
+            for (int x = x0; x <= x1; x += by) {
+              const float* src = piece(x);
+              const float2 stat = __ldcg(reinterpret_cast<const float2*>(src + 16 * D) + r);
+              const float4 v0 = __ldcg(reinterpret_cast<const float4*>(src + r * D + c));
+              const float4 v1 = __ldcg(reinterpret_cast<const float4*>(src + r * D + c + 4));
+              const float m_new = fmaxf(top, stat.x), ref = m_new == -INFINITY ? 0.f : m_new;
+              const float fix = exp2_fast(top - ref), w = exp2_fast(stat.x - ref);
+              top = m_new;
+              sum = fmaf(sum, fix, stat.y * w);
+              v[0] = fmaf(v[0], fix, v0.x * w);
+              v[1] = fmaf(v[1], fix, v0.y * w);
+              v[2] = fmaf(v[2], fix, v0.z * w);
+              v[3] = fmaf(v[3], fix, v0.w * w);
+              v[4] = fmaf(v[4], fix, v1.x * w);
+              v[5] = fmaf(v[5], fix, v1.y * w);
+              v[6] = fmaf(v[6], fix, v1.z * w);
+              v[7] = fmaf(v[7], fix, v1.w * w);
+            }
+            if (final) {
+              store(r, c, v, sum > 0.f || sum != sum ? 1.f / sum : 0.f);
+            } else {
+              __stcg(reinterpret_cast<float4*>(piece(x0) + r * D + c), make_float4(v[0], v[1], v[2], v[3]));
+              __stcg(reinterpret_cast<float4*>(piece(x0) + r * D + c + 4), make_float4(v[4], v[5], v[6], v[7]));
+            }
+          }
+          if (!final) {  // a row's threads are in one turn: 128 is a multiple of D / 8
+            named_barrier(1, C::kWarps * 32);
+            if (real && c == 0) __stcg(reinterpret_cast<float2*>(piece(x0) + 16 * D) + r, make_float2(top, sum));
+          }
+        }
+      };
+      uint32_t* run_ticket = tickets + gridDim.x + run.x0 * 2 + (run.x0 == c0 ? 1 : 0);
+      if (run.runs == 1) {
+        if (last_of(tickets + c0, c1 - c0 + 1)) join(c0, c1, 1, true);
+      } else if (last_of(run_ticket, run.x1 - run.x0 + 1)) {
+        join(run.x0, run.x1, 1, false);
+        if (last_of(tickets + c0, run.runs)) join(c0, c1, run.by, true);
       }
     }
     named_barrier(1, C::kWarps * 32);  // the merge buffer and s_last are free again
@@ -619,7 +643,7 @@ cudaError_t launch_decode(const DecodeArgs& a, cudaStream_t st, bool pdl) {
   if (attr != cudaSuccess) return attr;
   const int ctas = paged_sm_count() * C::kPerSm;
   static_assert(C::kSmem <= 227 * 1024, "shared memory");
-  if (ctas > kPagedTickets ||
+  if (ctas * 3 > kPagedTickets ||
       (size_t)ctas * 2 * 16 * (D + 2) * 4 + kPagedTickets * 4 > kPagedWorkspaceBytes)
     return cudaErrorNotSupported;
   if constexpr (!CLUSTER) {

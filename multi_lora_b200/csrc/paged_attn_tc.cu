@@ -782,7 +782,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       const int t = paged_token(p, r);
       T* dst = static_cast<T*>(p.out) + (int64_t)(done.q0 + t) * p.out_token +
                (int64_t)(done.head * p.group + r - t * p.group) * p.out_head;
-      auto store = [&](int c, const float* v, float inv) {  // 16 columns: a thread a row, so whole sectors
+      auto store = [&](T* dst, int c, const float* v, float inv) {  // 16 columns: a thread a row, so whole sectors
         uint32_t u[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) u[i] = pack_round2<T>(v[2 * i] * inv, v[2 * i + 1] * inv);
@@ -819,7 +819,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         if (whole) {
           if (r < done.rows) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 16) store(c * 32 + i, v + i, inv);
+            for (int i = 0; i < 32; i += 16) store(dst, c * 32 + i, v + i, inv);
           }
         } else {
 #pragma unroll
@@ -834,51 +834,93 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         __stcg(part + 128 * D + row, m);
         __stcg(part + 128 * (D + 1) + row, l);
         const int c1 = split.last_cta(item0, done.n);
-        named_barrier(1 + q, 128);
-        if (row == 0) {
-          __threadfence();
-          uint32_t* ticket = tickets + c0 * 2 + q;
-          const bool last = atomicAdd(ticket, 1u) == (uint32_t)(c1 - c0);
-          if (last) *ticket = 0u;
-          __threadfence();
-          s_last[q] = last;
-        }
-        named_barrier(1 + q, 128);
-        const bool last = s_last[q];
-        named_barrier(1 + q, 128);
-        if (last && r < done.rows) {
+        const PagedJoin run(c0, c1, blockIdx.x);
+        auto last_of = [&](uint32_t* ticket, int n) {  // whether this warpgroup is the last of n to get here
+          named_barrier(1 + q, 128);
+          if (row == 0) {
+            __threadfence();
+            const bool last = atomicAdd(ticket, 1u) == (uint32_t)(n - 1);
+            if (last) *ticket = 0u;
+            __threadfence();
+            s_last[q] = last;
+          }
+          named_barrier(1 + q, 128);
+          const bool last = s_last[q];
+          named_barrier(1 + q, 128);
+          return last;
+        };
+        // Pieces x0, x0 + by, .. x1 of this tile of rows, to the output or as one piece to x0's
+        // place; one, two or four threads a row, 32 columns of four pieces at once.
+        auto join = [&](int x0, int x1, int by, bool final) {
+          const int live = min(128, done.rows - r_lo), share = live <= 32 ? 4 : live <= 64 ? 2 : 1;
+          const int jr = row & (128 / share - 1), c_from = row / (128 / share) * 32;
           float top = -INFINITY, total = 0.f;
+          if (jr < live) {
 #pragma unroll 4
-          for (int x = c0; x <= c1; ++x) top = fmaxf(top, __ldcg(piece(x, c0) + 128 * D + row));
-          const float base = top == -INFINITY ? 0.f : top;
+            for (int x = x0; x <= x1; x += by) top = fmaxf(top, __ldcg(piece(x, c0) + 128 * D + jr));
+            const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll 4
-          for (int x = c0; x <= c1; ++x)
-            total = fmaf(__ldcg(piece(x, c0) + 128 * (D + 1) + row), exp2_fast(__ldcg(piece(x, c0) + 128 * D + row) - base),
-                         total);
-          const float inv_all = total > 0.f || total != total ? 1.f / total : 0.f;
+            for (int x = x0; x <= x1; x += by)
+              total = fmaf(__ldcg(piece(x, c0) + 128 * (D + 1) + jr), exp2_fast(__ldcg(piece(x, c0) + 128 * D + jr) - base), total);
+            const float inv_all = total > 0.f || total != total ? 1.f / total : 0.f;
+            const int jt = paged_token(p, r_lo + jr);
+            T* jdst = static_cast<T*>(p.out) + (int64_t)(done.q0 + jt) * p.out_token +
+                      (int64_t)(done.head * p.group + r_lo + jr - jt * p.group) * p.out_head;
 #pragma unroll 1
-          for (int c = 0; c < D; c += 64) {  // 16 loads of 16 bytes in flight
-            float v[64];
+            for (int c = c_from; c < D; c += share * 32) {
+              float v[32];
 #pragma unroll
-            for (int i = 0; i < 64; ++i) v[i] = 0.f;
+              for (int i = 0; i < 32; ++i) v[i] = 0.f;
 #pragma unroll 1
-            for (int x = c0; x <= c1; ++x) {
-              const float* src = piece(x, c0);
-              float4 u[16];
+              for (int x = x0; x <= x1; x += 4 * by) {
+                float4 u[4][8];
+                float w[4];
 #pragma unroll
-              for (int i = 0; i < 16; ++i) u[i] = __ldcg(reinterpret_cast<const float4*>(src) + (c / 4 + i) * 128 + row);
-              const float w = exp2_fast(__ldcg(src + 128 * D + row) - base);
+                for (int k = 0; k < 4; ++k) {
+                  const int xk = x + k * by;
+                  const float* src = piece(xk, c0);
+                  w[k] = xk <= x1 ? exp2_fast(__ldcg(src + 128 * D + jr) - base) : 0.f;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                v[4 * i] = fmaf(u[i].x, w, v[4 * i]);
-                v[4 * i + 1] = fmaf(u[i].y, w, v[4 * i + 1]);
-                v[4 * i + 2] = fmaf(u[i].z, w, v[4 * i + 2]);
-                v[4 * i + 3] = fmaf(u[i].w, w, v[4 * i + 3]);
+                  for (int i = 0; i < 8; ++i)
+                    u[k][i] = xk <= x1 ? __ldcg(reinterpret_cast<const float4*>(src) + (c / 4 + i) * 128 + jr)
+                                       : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) {
+                    v[4 * i] = fmaf(u[k][i].x, w[k], v[4 * i]);
+                    v[4 * i + 1] = fmaf(u[k][i].y, w[k], v[4 * i + 1]);
+                    v[4 * i + 2] = fmaf(u[k][i].z, w[k], v[4 * i + 2]);
+                    v[4 * i + 3] = fmaf(u[k][i].w, w[k], v[4 * i + 3]);
+                  }
+              }
+              if (final) {
+                store(jdst, c, v, inv_all);
+                store(jdst, c + 16, v + 16, inv_all);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; i += 4)
+                  __stcg(reinterpret_cast<float4*>(piece(x0, c0)) + (c / 4 + i / 4) * 128 + jr,
+                         make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
               }
             }
-#pragma unroll
-            for (int i = 0; i < 64; i += 16) store(c + i, v + i, inv_all);
           }
+          if (!final) {
+            named_barrier(1 + q, 128);  // all threads of a row have read its statistics
+            if (jr < live && c_from == 0) {
+              __stcg(piece(x0, c0) + 128 * D + jr, top);
+              __stcg(piece(x0, c0) + 128 * (D + 1) + jr, total);
+            }
+          }
+        };
+        uint32_t* ticket = tickets + c0 * 2 + q;
+        uint32_t* run_ticket = tickets + gridDim.x * 2 + (run.x0 * 2 + (run.x0 == c0 ? 1 : 0)) * 2 + q;
+        if (run.runs == 1) {
+          if (last_of(ticket, c1 - c0 + 1)) join(c0, c1, 1, true);
+        } else if (last_of(run_ticket, run.x1 - run.x0 + 1)) {
+          join(run.x0, run.x1, 1, false);
+          if (last_of(ticket, run.runs)) join(c0, c1, run.by, true);
         }
         __syncwarp();
       }
@@ -900,7 +942,7 @@ cudaError_t launch_chunk(const ChunkArgs& a, cudaStream_t st, bool pdl) {
   static const cudaError_t attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (attr != cudaSuccess) return attr;
   const int ctas = paged_sm_count();
-  if (ctas * 2 > kPagedTickets || (size_t)ctas * 4 * C::kPart * 4 + kPagedTickets * 4 > kPagedWorkspaceBytes)
+  if (ctas * 6 > kPagedTickets || (size_t)ctas * 4 * C::kPart * 4 + kPagedTickets * 4 > kPagedWorkspaceBytes)
     return cudaErrorNotSupported;
   return launch_kernel(kern, dim3(ctas), dim3(kChunkThreads), C::kSmem, st, pdl, a);
 }

@@ -7,8 +7,8 @@
 // same number of keys whatever the lengths are, and a single long request spreads over the
 // whole GPU. An item inside one CTA is finished there; of an item that
 // several CTAs share each writes its unnormalised sums, maximum and total to
-// the workspace, and the CTA that counts itself last joins them in CTA order
-// (the same order, so the same bits, every time). A CTA has at most two such
+// the workspace, and the CTA that counts itself last (of a run of CTAs, then of the
+// runs, where they are many) joins them in CTA order, the same every time, so the bits are too. A CTA has at most two such
 // pieces: the rest of an item that an earlier CTA began (slot 0), and the
 // beginning of one that a later CTA ends (slot 1).
 #pragma once
@@ -309,6 +309,26 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&r)[8]) {
                "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
+
+// The pieces of an item that CTAs c0 .. c1 share are joined in two stages where they are many: runs of
+// `by` CTAs first, by the last of each run to arrive, and then their results, by the last of those.
+// One CTA that reads all of them is most of the launch otherwise: 70 rows over 32000 keys
+// of one head, 95 pieces of 36 KB, 105 us and 48 in two stages; one row over 60000 keys
+// of one head, 296 pieces of 0.5 KB, 49 us and 25.
+struct PagedJoin {
+  int by, x0, x1, runs;  // this CTA's run, and how many there are
+  __device__ PagedJoin(int c0, int c1, int cta) {
+    const int n = c1 - c0 + 1;
+    by = n;
+    if (n > 6) {
+      by = 3;
+      while (by * by < n) ++by;
+    }
+    x0 = c0 + (cta - c0) / by * by;
+    x1 = min(x0 + by - 1, c1);
+    runs = (n + by - 1) / by;
+  }
+};
 
 constexpr int kPagedTickets = 1024;  // words at the start of the workspace, zero between calls
 constexpr size_t kPagedWorkspaceBytes = (size_t)64 << 20;
