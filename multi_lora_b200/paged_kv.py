@@ -18,7 +18,7 @@ segment a request, so the LoRA projections of the step can be routed by it.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import List, Optional, Sequence
+from typing import Dict, List, Optional, Sequence
 
 import torch
 
@@ -167,6 +167,8 @@ class PagedKVCache:
         self.status = i32(1)
         self._ticket = i32(1)
         self._workspace = attention_workspace(self.device)
+        # one for each max_tokens, for as long as the cache lives: captured graphs hold their addresses
+        self._plans: Dict[int, PagedStepPlan] = {}
         self._plan: Optional[PagedStepPlan] = None
 
     def layer(self, index: int):
@@ -176,19 +178,22 @@ class PagedKVCache:
 
     def plan(self, new_lens: torch.Tensor, max_tokens: int) -> PagedStepPlan:
         """Plan a step of ``new_lens`` (int32 [max_requests]) tokens, ``max_tokens`` rows in all; blocks are taken
-        for good. The plan's tensors are reused while ``max_tokens`` stays the same."""
-        plan = self._plan
-        if plan is None or plan.slot_map.numel() != max_tokens:
+        for good. Every step of the same ``max_tokens`` writes the same plan, whose tensors live as long as the
+        cache does: a CUDA graph that captured them may be replayed between steps of other sizes. A size costs
+        8 bytes a token and a request, so a server rounds its sizes up to a few."""
+        plan = self._plans.get(max_tokens)
+        if plan is None:
             plan = PagedStepPlan.new(self.ctx_lens.numel(), max_tokens, self.device)
             plan.held_blocks, plan.free_head = self.held_blocks, self.free_head
-            self._plan = plan
+            self._plans[max_tokens] = plan
+        self._plan = plan
         return plan_paged_step(self.ctx_lens, new_lens, self.held_blocks, self.free_blocks, self.free_head,
                                self.block_tables, plan, block_size=self.block_size, workspace=self._ticket,
                                status=self.status)
 
     @property
     def plan_now(self) -> PagedStepPlan:
-        """The plan of the current step."""
+        """The plan of the step that :meth:`plan` was last called for (a replayed graph has the one it captured)."""
         if self._plan is None:
             raise RuntimeError("PagedKVCache: plan a step first")
         return self._plan
