@@ -671,7 +671,9 @@ template <typename T, int D>
 cudaError_t launch_decode_any(const DecodeArgs& a, cudaStream_t st, bool pdl) {
   // One request of 777 keys, 8 key heads: 6.5 us with clusters, 11.3 without; 4000 keys 12.9 and 18.5. From
   // twice that on an item needs more CTAs than a cluster has. The host knows the lengths' bound only.
-  if ((long long)a.a.requests * a.a.kv_heads <= kFewItems && (long long)a.a.width * a.a.block_size <= kFewKeys)
+  // Without requests there is no item to launch a cluster for: the other kernel's CTAs write the zeros.
+  if (a.a.requests > 0 && (long long)a.a.requests * a.a.kv_heads <= kFewItems &&
+      (long long)a.a.width * a.a.block_size <= kFewKeys)
     return launch_decode<T, D, true>(a, st, pdl);
   return launch_decode<T, D, false>(a, st, pdl);
 }
