@@ -23,9 +23,9 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "device.h"
 #include "kernels.h"
 #include "paged.h"
-#include "paged_tma.h"
 #include "tma.cuh"
 
 namespace mlora {
@@ -306,7 +306,7 @@ cudaError_t general_h(const PagedAttnArgs& a, cudaStream_t st, bool pdl) {
   // start of more clusters costs as much as more keys do. fp32, 32 query heads over 8 of 128, us with and without: 1
   // request (8 items) of 777 keys 15 and 35, 200 keys 12 and 10; 16 requests (128 items) of 2000 keys 101 and 135, 800
   // keys 95 and 68; 64 requests of 2000 keys 395 and 298.
-  const bool few = items <= paged_sm_count() && (int64_t)a.width * a.block_size > std::max<int64_t>(256, 8 * items);
+  const bool few = items <= device_sm_count() && (int64_t)a.width * a.block_size > std::max<int64_t>(256, 8 * items);
   const int ctas = few ? kAttnCtas : 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(items * ctas));

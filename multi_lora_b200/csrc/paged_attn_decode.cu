@@ -34,6 +34,7 @@
 // 114 us, 5.4 TB/s; one request of 777 keys: 6.5 us.
 #include <climits>
 
+#include "device.h"
 #include "kernels.h"
 #include "mma.cuh"
 #include "paged_sched.cuh"
@@ -638,10 +639,9 @@ template <typename T, int D, bool CLUSTER>
 cudaError_t launch_decode(const DecodeArgs& a, cudaStream_t st, bool pdl) {
   using C = DecodeCfg<D>;
   auto kern = paged_attention_decode_kernel<T, D, CLUSTER>;
-  static const cudaError_t attr =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
-  if (attr != cudaSuccess) return attr;
-  const int ctas = paged_sm_count() * C::kPerSm;
+  static SmemLimit limit;
+  if (const cudaError_t e = limit.raise(kern, C::kSmem); e != cudaSuccess) return e;
+  const int ctas = device_sm_count() * C::kPerSm;
   static_assert(C::kSmem <= 227 * 1024, "shared memory");
   if (ctas * 3 > kPagedTickets ||
       (size_t)ctas * 2 * 16 * (D + 2) * 4 + kPagedTickets * 4 > kPagedWorkspaceBytes)

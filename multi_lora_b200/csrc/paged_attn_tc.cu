@@ -42,6 +42,7 @@
 // the warp that fetches Q, while the softmax works.
 #include <climits>
 
+#include "device.h"
 #include "kernels.h"
 #include "paged_sched.cuh"
 #include "paged_tma.h"
@@ -939,9 +940,9 @@ cudaError_t launch_chunk(const ChunkArgs& a, cudaStream_t st, bool pdl) {
   using C = ChunkCfg<D>;
   static_assert(C::kSmem <= 227 * 1024, "shared memory");
   auto kern = paged_attention_chunk_kernel<T, D>;
-  static const cudaError_t attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
-  if (attr != cudaSuccess) return attr;
-  const int ctas = paged_sm_count();
+  static SmemLimit limit;
+  if (const cudaError_t e = limit.raise(kern, C::kSmem); e != cudaSuccess) return e;
+  const int ctas = device_sm_count();
   if (ctas * 6 > kPagedTickets || (size_t)ctas * 4 * C::kPart * 4 + kPagedTickets * 4 > kPagedWorkspaceBytes)
     return cudaErrorNotSupported;
   return launch_kernel(kern, dim3(ctas), dim3(kChunkThreads), C::kSmem, st, pdl, a);

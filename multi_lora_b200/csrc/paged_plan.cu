@@ -26,6 +26,7 @@
 #include <climits>
 
 #include "common.cuh"
+#include "device.h"
 #include "kernels.h"
 #include "paged.h"
 
@@ -183,9 +184,9 @@ __global__ void __launch_bounds__(kPlanNT) paged_plan_kernel(const PlanArgs p) {
 
 cudaError_t launch_paged_plan(const PlanArgs& a, cudaStream_t st, bool pdl) {
   const int smem = (a.requests + 1) * (int)sizeof(PlanRow);
-  static const cudaError_t attr = cudaFuncSetAttribute(
-      paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kPlanMaxRequests + 1) * (int)sizeof(PlanRow));
-  if (attr != cudaSuccess) return attr;
+  static SmemLimit limit;
+  const cudaError_t e = limit.raise(paged_plan_kernel, (kPlanMaxRequests + 1) * (int)sizeof(PlanRow));
+  if (e != cudaSuccess) return e;
   // one CTA where the tokens fit it (no count of CTAs needed), at most one an SM else
   const long long work = a.max_tokens > a.requests ? a.max_tokens : a.requests;
   long long grid = (work + 2 * kPlanNT - 1) / (2 * kPlanNT);

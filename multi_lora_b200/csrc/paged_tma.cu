@@ -64,17 +64,4 @@ bool paged_q_map(const PagedAttnArgs& a, int dtype, int rows, CUtensorMap* q) {
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int paged_sm_count() {
-  static const int n = [] {
-    int dev = 0, c = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-      (void)cudaGetLastError();
-      return 148;
-    }
-    return c;
-  }();
-  return n;
-}
-
 }  // namespace mlora

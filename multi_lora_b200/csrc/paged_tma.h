@@ -22,6 +22,4 @@ bool paged_maps(const PagedAttnArgs& a, int dtype, int box, CUtensorMap* k, CUte
 // tile of `rows` packed rows (token major, then head). False where group does not divide it.
 bool paged_q_map(const PagedAttnArgs& a, int dtype, int rows, CUtensorMap* q);
 
-int paged_sm_count();
-
 }  // namespace mlora

@@ -1,5 +1,5 @@
 """The launches of the paged step on the library's host side, with a runtime that has no GPU (tests/fake_cudart.cpp):
-grids that are not empty."""
+grids that are not empty, and what each kernel needs on each device of a process."""
 
 from __future__ import annotations
 
@@ -36,3 +36,41 @@ def test_every_attention_launch_has_blocks(fake, requests, rows, most, width, dt
     assert attend(fake, requests=requests, rows=rows, most=most, width=width, dtype=dtype) == 0, fake.error()
     launches = fake.launches()
     assert len(launches) == 1 and launches[0].result == 0 and min(launches[0].grid) > 0
+
+
+def plan(fake, requests):
+    return fake.c.mlora_plan_paged_step(16, 16, 16, requests, 16, 4, 16, 16, 4, 4, 16, 16, 16, 16, 16, 16, 16, 8, 16, None,
+                                        None)
+
+
+@pytest.mark.parametrize("call", [
+    lambda f: attend(f), lambda f: attend(f, width=4000), lambda f: attend(f, rows=300, most=90),
+    lambda f: attend(f, rows=300, most=90, dim=128, dtype=1), lambda f: attend(f, dtype=2), lambda f: plan(f, 8192),
+], ids=["cluster", "dealt", "chunk", "chunk-f16-128", "general", "plan"])
+def test_every_device_of_a_process(fake, call):
+    """Shared memory above the 48 KB that a launch has by itself is granted for a kernel on one device."""
+    for dev in (3, 1, 0, 3, 2, 1):
+        fake.reset()
+        fake.device(dev)
+        assert call(fake) == 0, (dev, fake.error())
+        assert [x.device for x in fake.launches()] == [dev]
+        fake.reset()
+        fake.device(dev)
+        assert call(fake) == 0 and fake.c.fake_attribute_calls() == 0  # granted by now: nothing is asked again
+
+
+def test_a_device_that_refused_once_is_asked_again(fake):
+    fake.reset()
+    fake.device(7)
+    fake.c.fake_fail(2)
+    assert attend(fake, width=4000) != 0 and attend(fake, width=4000) != 0 and not fake.launches()
+    assert attend(fake, width=4000) == 0 and fake.launches()[0].result == 0
+
+
+def test_a_grid_has_the_device_s_own_sms(fake):
+    fake.reset()
+    for dev, sms in ((8, 148), (9, 132), (8, 148), (9, 132)):
+        fake.c.fake_sms(dev, sms)
+        fake.device(dev)
+        assert attend(fake, width=4000) == 0 and attend(fake, rows=300, most=90) == 0
+        assert [x.grid[0] for x in fake.launches()[-2:]] == [2 * sms, sms]
