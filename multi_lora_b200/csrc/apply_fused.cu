@@ -46,9 +46,11 @@
 #include <map>
 #include <mutex>
 #include <cstdlib>
-#include <utility>
+#include <set>
+#include <tuple>
 
 #include "common.cuh"
+#include "device.h"
 #include "kernels.h"
 #include "mma.cuh"
 #include "tma.cuh"
@@ -680,33 +682,28 @@ namespace {
 template <typename T, int RM, bool XCHG>
 struct FusedLauncher {
   std::mutex mu;
-  int smem_set = 0;
-  bool nonportable_set = false;
-  std::map<std::pair<int, int>, int> occ;  // (cs, smem KiB) -> resident CTAs per SM (0: cannot place)
+  SmemLimit limit;
+  std::set<int> nonportable;                     // devices on which clusters above 8 are allowed
+  std::map<std::tuple<int, int, int>, int> occ;  // (device, cs, smem KiB) -> resident CTAs per SM (0: cannot place)
 
   // Resident CTAs per SM for this shape (0 when a cluster of cs cannot be placed).
   int occupancy(int cs, size_t smem) {
     std::lock_guard<std::mutex> lock(mu);
     auto kern = apply_fused_kernel<T, RM, XCHG>;
     const int kib = (int)((smem + 1023) / 1024);
-    auto key = std::make_pair(cs, kib);
+    const int dev = current_device();
+    const auto key = std::make_tuple(dev, cs, kib);
     auto it = occ.find(key);
     if (it != occ.end()) return it->second;
     int result = 0;
-    if (cs > 8 && !nonportable_set) {
+    if (cs > 8 && nonportable.count(dev) == 0) {
       if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
         (void)cudaGetLastError();
-        return occ[key] = 0;
+        return 0;
       }
-      nonportable_set = true;
+      nonportable.insert(dev);
     }
-    if (kib * 1024 > smem_set) {
-      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kib * 1024) != cudaSuccess) {
-        (void)cudaGetLastError();
-        return occ[key] = 0;
-      }
-      smem_set = kib * 1024;
-    }
+    if (limit.raise(kern, kib * 1024) != cudaSuccess) return 0;
     cudaLaunchConfig_t q = {};
     q.gridDim = dim3(cs, 1, 1);
     q.blockDim = dim3(kFusedNT);
@@ -765,18 +762,6 @@ size_t fused_smem(const FusedArgs& a, int rm, int ks, int ob_max, int cs) {
          (size_t)4 * ((size_t)(kFusedNT / 32) * kFusedTT * rm + (size_t)cs * kFusedTT * rm);
 }
 
-int sm_count() {
-  static int n = [] {
-    int dev = 0, c = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-      (void)cudaGetLastError();
-      return 148;
-    }
-    return c;
-  }();
-  return n;
-}
-
 template <typename T, int RM, bool XCHG>
 cudaError_t launch_rmx(FusedArgs a, cudaStream_t st, bool pdl) {
   auto& l = launcher<T, RM, XCHG>();
@@ -808,7 +793,7 @@ cudaError_t launch_rmx(FusedArgs a, cudaStream_t st, bool pdl) {
     const int per_sm = l.occupancy(cs, smem);
     if (per_sm <= 0) continue;
     const long long ctas = (long long)c.n_mod * c.num_slots * cs;
-    const int waves = (int)((ctas + (long long)sm_count() * per_sm - 1) / ((long long)sm_count() * per_sm));
+    const int waves = (int)((ctas + (long long)device_sm_count() * per_sm - 1) / ((long long)device_sm_count() * per_sm));
     if (XCHG && waves > 1) continue;  // its CTAs wait on peers' CTAs: the whole grid must be resident
     auto pref = [](int c) { return c == 8 ? 0 : c == 16 ? 1 : c == 4 ? 2 : 3; };
     if (waves < best_waves || (waves == best_waves && pref(cs) < pref(best_cs))) {

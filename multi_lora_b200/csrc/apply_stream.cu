@@ -33,9 +33,9 @@
 // Each CTA needs ~100 KB of shared memory, so a shrink CTA and an expand CTA
 // share an SM. Every mbarrier wait is bounded (status bit on timeout).
 #include <cstdlib>
-#include <mutex>
 
 #include "common.cuh"
+#include "device.h"
 #include "kernels.h"
 #include "mma.cuh"
 #include "tma.cuh"
@@ -763,45 +763,20 @@ __global__ void __launch_bounds__(kStreamThreads) lora_expand_stream_kernel(cons
 // ---------------------------------------------------------------------------
 namespace {
 
-int stream_sm_count() {
-  static int n = [] {
-    int dev = 0, c = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-      (void)cudaGetLastError();
-      return 148;
-    }
-    return c;
-  }();
-  return n;
-}
-
-template <typename K>
-bool ensure_smem(K kern, int bytes, int& set, std::mutex& mu) {
-  std::lock_guard<std::mutex> lock(mu);
-  if (bytes <= set) return true;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return false;
-  }
-  set = bytes;
-  return true;
-}
-
 template <typename T, int RM, bool XCHG>
 cudaError_t launch_stream_rmx(const StreamArgs& a, cudaStream_t st, bool pdl) {
-  static std::mutex mu;
-  static int set_s = 0, set_e = 0;
+  static SmemLimit limit_s, limit_e;
   const int route = align128(stream_routing_bytes(a.num_slots, a.S));
   const int smem_s = kStreamShrinkStages * ShrinkStage<RM>::BYTES + route;
   const int smem_e = kStreamStages * ExpandStage<RM>::BYTES + route;
   auto ks = lora_shrink_stream_kernel<T, RM, XCHG>;
   auto ke = lora_expand_stream_kernel<T, RM, XCHG>;
-  if (!ensure_smem(ks, smem_s, set_s, mu) || !ensure_smem(ke, smem_e, set_e, mu)) return cudaErrorNotSupported;
-  const dim3 grid(stream_sm_count());
+  if (limit_s.raise(ks, smem_s) != cudaSuccess || limit_e.raise(ke, smem_e) != cudaSuccess) return cudaErrorNotSupported;
+  const dim3 grid(device_sm_count());
   if (a.phase == 2)  // expand only: mid comes from the caller (e.g. all-reduced shrink partials)
     return launch_kernel(ke, grid, dim3(kStreamThreads), smem_e, st, pdl, a);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(stream_sm_count() / kStreamShrinkSplit * kStreamShrinkSplit));
+  cfg.gridDim = dim3((unsigned)(device_sm_count() / kStreamShrinkSplit * kStreamShrinkSplit));
   cfg.blockDim = dim3(kStreamThreads);
   cfg.dynamicSmemBytes = smem_s;
   cfg.stream = st;

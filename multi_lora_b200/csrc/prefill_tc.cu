@@ -27,9 +27,8 @@
 // Shapes: bf16/f16, max_rank 16, 32 or 64, in % 64 == 0, out % 8 == 0. Adapter weights
 // are requested before griddepcontrol.wait; x, mid and y after it. Waits are
 // bounded; TMEM is always freed.
-#include <mutex>
-
 #include "common.cuh"
+#include "device.h"
 #include "kernels.h"
 #include "tc.cuh"
 
@@ -462,29 +461,6 @@ bool encode_2d(CUtensorMap* map, const void* base, int dtype, uint64_t inner, ui
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-long long tc_sm_count() {
-  static const int n = [] {
-    int dev = 0, c = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-      (void)cudaGetLastError();
-      return 148;
-    }
-    return c;
-  }();
-  return n;
-}
-
-template <typename K>
-bool ensure_smem_tc(K kern, int bytes) {
-  static std::mutex mu;
-  std::lock_guard<std::mutex> lock(mu);
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return false;
-  }
-  return true;
-}
-
 template <typename T, int RT>
 cudaError_t launch_prefill_t(PrefillArgs& a, cudaStream_t st, bool pdl) {
   const int nm = a.n_mod;
@@ -501,16 +477,16 @@ cudaError_t launch_prefill_t(PrefillArgs& a, cudaStream_t st, bool pdl) {
   auto ke = lora_expand_tc_kernel<T, RT>;
   // at least the largest shrink launched at this RT (four projections: the larger of
   // the 2-stage ring and the K-split partial tile)
-  static const bool smem_ok =
-      ensure_smem_tc(ks, (4 * RT <= 128 ? 4 : 3) * (kTcTileM * kTcBK * 2 + 4 * RT * kTcBK * 2) + 1024) &&
-      ensure_smem_tc(ke, expand_smem);
-  if (!smem_ok) return cudaErrorNotSupported;
+  static SmemLimit limit_s, limit_e;
+  if (limit_s.raise(ks, (4 * RT <= 128 ? 4 : 3) * (kTcTileM * kTcBK * 2 + 4 * RT * kTcBK * 2) + 1024) != cudaSuccess ||
+      limit_e.raise(ke, expand_smem) != cudaSuccess)
+    return cudaErrorNotSupported;
   const long long tiles = (a.S + kTcTileM - 1) / kTcTileM + (long long)a.bs;
   if (tiles > 65535) return cudaErrorNotSupported;
   int blocks = 0;
   for (int m = 0; m < nm; ++m) blocks += (a.mod[m].out_dim + kTcBN - 1) / kTcBN;
   // K splits: enough shrink CTAs for two per SM, at least 4 K blocks each, a cluster of <= 8
-  int splits = (int)(2 * tc_sm_count() / tiles);
+  int splits = (int)(2ll * device_sm_count() / tiles);
   splits = splits < 1 ? 1 : splits > 8 ? 8 : splits;
   while (splits > 1 && a.in_dim / kTcBK < 4 * splits) --splits;
   cudaLaunchConfig_t cfg = {};
