@@ -27,7 +27,8 @@
 // Keys that a row does not see may hold anything: scores are replaced, not added
 // to, and since 0 * NaN is NaN the V fragments of keys outside [first, kv) are cleared
 // before the product, and infinities and NaN of keys that only some rows see are
-// taken out and added to these rows alone.
+// taken out and added to these rows alone. Where the products made NaN of an infinity that
+// a row does see, its output is settled after it was stored (paged_settle).
 //
 // Measured: 64 requests of 33 to 2048 keys, 32 heads of 128: 189 us, 5.6 TB/s (85 % of
 // the measured copy bandwidth); 4 requests of 20000 to 65536 keys, 8 key heads:
@@ -96,6 +97,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
   __shared__ __align__(8) uint64_t full[NS], empty[NS];
   __shared__ float s_m[C::kWarps][16], s_l[C::kWarps][16];
   __shared__ int s_last;
+  __shared__ PagedPlace s_place;  // of the item that is being joined
   const PagedAttnArgs& p = args.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~uintptr_t(1023));
@@ -419,6 +421,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     const DecodeItem done = it;
     const bool begins = cur.unit == 0, whole = cur.whole(it.n);
     const int item0 = cur.pos - cur.unit;
+    if (tid == 0) s_place = {done.req, done.head, done.kv, done.qn};
     more = advance();
     if (more) {
       next_item();
@@ -484,57 +487,73 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
 #pragma unroll
       for (int g = 0; g < C::KG; ++g) sum += top == -INFINITY ? 0.f : s_l[g][r] * exp2_fast(s_m[g][r] - top);
     };
-    auto store = [&](int r, int c, const float* v, float inv) {  // 8 columns of row r
-      if (c >= p.dim) return;
+    auto place = [&](int r, int c) {
       const int t = paged_token(p, r);
-      T* dst = static_cast<T*>(p.out) + (done.q0 + t) * p.out_token + (done.head * group + r - t * group) * p.out_head + c;
+      return static_cast<T*>(p.out) + (int64_t)(done.q0 + t) * p.out_token +
+             (int64_t)(done.head * group + r - t * group) * p.out_head + c;
+    };
+    auto store = [&](int r, int c, const float* v, float inv) {  // 8 columns of row r; whether they may need settle()
+      if (c >= p.dim) return false;
       uint4 u;
       u.x = pack_round2<T>(v[0] * inv, v[1] * inv);
       u.y = pack_round2<T>(v[2] * inv, v[3] * inv);
       u.z = pack_round2<T>(v[4] * inv, v[5] * inv);
       u.w = pack_round2<T>(v[6] * inv, v[7] * inv);
-      *reinterpret_cast<uint4*>(dst) = u;
+      *reinterpret_cast<uint4*>(place(r, c)) = u;
+      return inv == inv && paged_taint<T>(u.w, paged_taint<T>(u.z, paged_taint<T>(u.y, paged_taint<T>(u.x, 0u)))) != 0u;
+    };
+    // What a lane stored in columns from c of row r where it is not finite, though the row's sum is: the whole warp.
+    auto settle = [&](auto words, int r, int c, bool odd) {
+      if (__builtin_expect(__any_sync(0xffffffffu, odd), 0)) {
+        paged_settle<T, decltype(words)::value>(p, &s_place, r, c, place(r, c), odd);
+      }
     };
     // Where the sums go that are not finished here: a piece of the workspace, or for the
     // cluster the ring of stages, which is empty now.
     float* part = CLUSTER ? reinterpret_cast<float*>(smem) : parts + ((long long)blockIdx.x * 2 + (begins ? 1 : 0)) * PART;
-    for (int e = tid; e < rows * (D / 8); e += C::kWarps * 32) {
-      const int r = e / (D / 8), c = (e % (D / 8)) * 8;
-      float top, sum;
-      row_stat(r, top, sum);
-      float4 v0 = *reinterpret_cast<const float4*>(merge + r * C::kRowF + c);
-      float4 v1 = *reinterpret_cast<const float4*>(merge + r * C::kRowF + c + 4);
-      for (int g = 1; g < slots; ++g) {
-        const float4 u0 = *reinterpret_cast<const float4*>(merge + (r + g * apart) * C::kRowF + c);
-        const float4 u1 = *reinterpret_cast<const float4*>(merge + (r + g * apart) * C::kRowF + c + 4);
-        v0.x += u0.x;
-        v0.y += u0.y;
-        v0.z += u0.z;
-        v0.w += u0.w;
-        v1.x += u1.x;
-        v1.y += u1.y;
-        v1.z += u1.z;
-        v1.w += u1.w;
+    for (int e0 = 0; e0 < rows * (D / 8); e0 += C::kWarps * 32) {
+      const int e = e0 + tid, r = e / (D / 8), c = (e % (D / 8)) * 8;
+      bool odd = false;
+      if (e < rows * (D / 8)) {
+        float top, sum;
+        row_stat(r, top, sum);
+        float4 v0 = *reinterpret_cast<const float4*>(merge + r * C::kRowF + c);
+        float4 v1 = *reinterpret_cast<const float4*>(merge + r * C::kRowF + c + 4);
+        for (int g = 1; g < slots; ++g) {
+          const float4 u0 = *reinterpret_cast<const float4*>(merge + (r + g * apart) * C::kRowF + c);
+          const float4 u1 = *reinterpret_cast<const float4*>(merge + (r + g * apart) * C::kRowF + c + 4);
+          v0.x += u0.x;
+          v0.y += u0.y;
+          v0.z += u0.z;
+          v0.w += u0.w;
+          v1.x += u1.x;
+          v1.y += u1.y;
+          v1.z += u1.z;
+          v1.w += u1.w;
+        }
+        if (CLUSTER) {
+          *reinterpret_cast<float4*>(part + r * D + c) = v0;
+          *reinterpret_cast<float4*>(part + r * D + c + 4) = v1;
+          if (c == 0) reinterpret_cast<float2*>(part + 16 * D)[r] = make_float2(top, sum);
+        } else if (whole) {
+          const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+          odd = store(r, c, v, sum > 0.f || sum != sum ? 1.f / sum : 0.f);
+        } else {
+          __stcg(reinterpret_cast<float4*>(part + r * D + c), v0);
+          __stcg(reinterpret_cast<float4*>(part + r * D + c + 4), v1);
+          if (c == 0) __stcg(reinterpret_cast<float2*>(part + 16 * D) + r, make_float2(top, sum));
+        }
       }
-      if (CLUSTER) {
-        *reinterpret_cast<float4*>(part + r * D + c) = v0;
-        *reinterpret_cast<float4*>(part + r * D + c + 4) = v1;
-        if (c == 0) reinterpret_cast<float2*>(part + 16 * D)[r] = make_float2(top, sum);
-      } else if (whole) {
-        const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-        store(r, c, v, sum > 0.f || sum != sum ? 1.f / sum : 0.f);
-      } else {
-        __stcg(reinterpret_cast<float4*>(part + r * D + c), v0);
-        __stcg(reinterpret_cast<float4*>(part + r * D + c + 4), v1);
-        if (c == 0) __stcg(reinterpret_cast<float2*>(part + 16 * D) + r, make_float2(top, sum));
-      }
+      if (!CLUSTER) settle(std::integral_constant<int, 4>(), r, c, odd);
     }
     if constexpr (CLUSTER) {
       cluster_arrive_release();
       cluster_wait_acquire();
       const uint32_t base = smem_addr(part);
-      for (int e = tid * kFewCtas + rank; e < rows * (D / 4); e += C::kWarps * 32 * kFewCtas) {
-        const int row = e / (D / 4), c = (e % (D / 4)) * 4;
+      const int e = tid * kFewCtas + rank, row = e / (D / 4), c = (e % (D / 4)) * 4;
+      static_assert(16 * (D / 4) <= C::kWarps * 32 * kFewCtas, "a thread has one piece of the output");
+      bool odd = false;
+      if (e < rows * (D / 4) && c < p.dim) {
         float4 u[kFewCtas];
         float2 stat[kFewCtas];
 #pragma unroll
@@ -555,13 +574,12 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
           v.z = fmaf(u[x].z, w, v.z);
           v.w = fmaf(u[x].w, w, v.w);
         }
-        if (c >= p.dim) continue;
         const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-        const int t = paged_token(p, row);
-        T* dst = static_cast<T*>(p.out) + (int64_t)(done.q0 + t) * p.out_token +
-                 (int64_t)(done.head * group + row - t * group) * p.out_head + c;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_round2<T>(v.x * inv, v.y * inv), pack_round2<T>(v.z * inv, v.w * inv));
+        const uint2 w = make_uint2(pack_round2<T>(v.x * inv, v.y * inv), pack_round2<T>(v.z * inv, v.w * inv));
+        *reinterpret_cast<uint2*>(place(row, c)) = w;
+        odd = inv == inv && paged_taint<T>(w.y, paged_taint<T>(w.x, 0u)) != 0u;
       }
+      settle(std::integral_constant<int, 2>(), row, c, odd);
       cluster_arrive_release();  // no CTA leaves while another reads its sums
       cluster_wait_acquire();
       return;
@@ -588,6 +606,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
           const int e = e0 + tid, r = e / (D / 8), c = (e % (D / 8)) * 8;
           const bool real = e < rows * (D / 8);
           float top = -INFINITY, sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          bool odd = false;
           if (real) {
 #pragma unroll 8
             for (int x = x0; x <= x1; x += by) {
@@ -609,12 +628,13 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
               v[7] = fmaf(v[7], fix, v1.w * w);
             }
             if (final) {
-              store(r, c, v, sum > 0.f || sum != sum ? 1.f / sum : 0.f);
+              odd = store(r, c, v, sum > 0.f || sum != sum ? 1.f / sum : 0.f);
             } else {
               __stcg(reinterpret_cast<float4*>(piece(x0) + r * D + c), make_float4(v[0], v[1], v[2], v[3]));
               __stcg(reinterpret_cast<float4*>(piece(x0) + r * D + c + 4), make_float4(v[4], v[5], v[6], v[7]));
             }
           }
+          if (final) settle(std::integral_constant<int, 4>(), r, c, odd);
           if (!final) {  // a row's threads are in one turn: 128 is a multiple of D / 8
             named_barrier(1, C::kWarps * 32);
             if (real && c == 0) __stcg(reinterpret_cast<float2*>(piece(x0) + 16 * D) + r, make_float2(top, sum));

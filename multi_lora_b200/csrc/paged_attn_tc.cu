@@ -39,7 +39,8 @@
 // since 0 * NaN is NaN their V is not multiplied by them. Rows of V that no row of
 // the item sees are cleared in shared memory; infinities and NaN in those that some
 // rows see are taken out there and added to these rows' outputs at the end. Both are done by
-// the warp that fetches Q, while the softmax works.
+// the warp that fetches Q, while the softmax works. Where the products made NaN of an infinity that a
+// row does see, its output is settled after it was stored (paged_settle).
 #include <climits>
 
 #include "device.h"
@@ -259,6 +260,28 @@ __device__ __noinline__ void chunk_give_back(const PagedAttnArgs& p, uint32_t o_
   tmem_wait_st();
 }
 
+// What the lanes of a softmax warp wrote of an item: one, two or four threads a row (`share`), 32 columns in turn.
+struct ChunkPlace {
+  PagedPlace item;
+  int q0, row0, share;
+};
+// The outputs of the marked lanes, settled; the marks are taken back.
+template <typename T>
+__device__ __noinline__ void chunk_settle(const PagedAttnArgs& p, const ChunkPlace* at, uint32_t* marks) {
+  const int thread = threadIdx.x & 127, per = 128 / at->share, row = at->row0 + (thread & (per - 1));
+  const bool mine = (*marks >> (thread & 31) & 1u) != 0u;
+  const int t = paged_token(p, row);
+  T* dst = static_cast<T*>(p.out) + (int64_t)(at->q0 + t) * p.out_token +
+           (int64_t)(at->item.head * p.group + row - t * p.group) * p.out_head;
+#pragma unroll 1
+  for (int c0 = thread / per * 32; c0 < p.dim; c0 += at->share * 32)
+#pragma unroll 1
+    for (int c = c0; c < min(c0 + 32, p.dim); c += 8) paged_settle<T, 4>(p, &at->item, row, c, dst + c, mine);
+  __syncwarp();
+  if ((thread & 31) == 0) *marks = 0u;
+  __syncwarp();
+}
+
 template <int N>
 __device__ __forceinline__ void regs_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
@@ -280,6 +303,8 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
   __shared__ uint32_t s_tmem;
   __shared__ int s_last[2];
   __shared__ float2 s_mate[128];
+  __shared__ uint32_t s_odd[8];    // lanes of a softmax warp that stored what is not finite though the row's sum is
+  __shared__ ChunkPlace s_place[8];  // of the item whose output each softmax warp writes
   __shared__ uint32_t s_clean;  // V tiles that have been cleaned
   __shared__ uint32_t s_taken;           // a value that is not finite was taken out of one of them
   const PagedAttnArgs& p = args.a;
@@ -304,6 +329,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
     }
     fence_barrier_init();
     s_clean = s_taken = 0u;
+    for (int w = 0; w < 8; ++w) s_odd[w] = 0u;
     tma_prefetch_map(&args.k_map);
     tma_prefetch_map(&args.v_map);
     if (args.q_tma) tma_prefetch_map(&args.q_map);
@@ -751,6 +777,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       const bool whole = cur.whole(it.n);
       const int item0 = cur.pos - cur.unit;
       const int tile0 = it.tile0 + cur.tile, tiles = cur.len;
+      if (lane == 0) s_place[warp - 4] = {{done.req, done.head, done.kv, done.qn}, done.q0, r_lo, 1};
       if (cur.advance()) next_item();
 
       ok = ok && mbar_poll(&pv_done[q][(n - 1) & 1], ((n - 1) >> 1) & 1, p.status);
@@ -787,6 +814,10 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         uint32_t u[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) u[i] = pack_round2<T>(v[2 * i] * inv, v[2 * i + 1] * inv);
+        uint32_t odd = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) odd = paged_taint<T>(u[i], odd);
+        if (odd != 0u && inv == inv) atomicOr(&s_odd[warp - 4], 1u << lane);
         if (args.out32) {
           if (c < p.dim) store32(dst + c, u);
         } else {
@@ -907,6 +938,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
               }
             }
           }
+          if (final && lane == 0) s_place[warp - 4].share = share;
           if (!final) {
             named_barrier(1 + q, 128);  // all threads of a row have read its statistics
             if (jr < live && c_from == 0) {
@@ -925,6 +957,9 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         }
         __syncwarp();
       }
+      __syncwarp();
+      if (__builtin_expect(*const_cast<volatile uint32_t*>(&s_odd[warp - 4]) != 0u, 0))
+        chunk_settle<T>(p, &s_place[warp - 4], &s_odd[warp - 4]);
     }
     if (lent) named_barrier(5, 256);
   }

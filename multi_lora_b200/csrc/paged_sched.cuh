@@ -13,6 +13,9 @@
 // beginning of one that a later CTA ends (slot 1).
 #pragma once
 
+#include <climits>
+#include <type_traits>
+
 #include "common.cuh"
 #include "paged.h"
 #include "tma.cuh"
@@ -243,6 +246,107 @@ template <typename T>
 __device__ __forceinline__ uint32_t paged_finite(uint32_t w) {
   constexpr uint32_t kExp = Num<T>::is_bf16 ? 0x7f807f80u : 0x7c007c00u, kOne = Num<T>::is_bf16 ? 0x00800080u : 0x04000400u;
   return w & ~(((((w & kExp) + kOne) & 0x80008000u) >> 15) * 0xffffu);  // a carry where all exponent bits are set
+}
+
+// Outputs that are NaN although the sum of their P is a number: V is not finite at a key that they see. P is
+// positive, so what is right there is the sum of V's infinities and NaN in that column; but a P that is zero in the type
+// of its product, or whose second term is zero or negative, makes a NaN of an infinity. Whole warp: the
+// 2 W columns from c of a lane's row lie at dst, and `mine` says that they may
+// be such outputs. The lanes look at 128 keys at once and tell one another what is not finite. Seldom run: the
+// keys are read again, about 1.5 us for 128 of them and 2 W columns.
+// The request and key head wait in shared memory, not in registers that the tiles need.
+struct PagedPlace {
+  int req, head, kv, qn;
+};
+template <typename T, int W>
+__device__ __noinline__ void paged_settle(const PagedAttnArgs& p, const PagedPlace* at, int row, int c, T* dst, bool mine) {
+  const int req = at->req, head = at->head;
+  const int pos = at->kv - at->qn + paged_token(p, row), first = paged_first_key(p, pos), limit = pos + 1;
+  using Words = typename std::conditional<W == 4, uint4, uint2>::type;
+  constexpr int AT_ONCE = 4;
+  union Pieces {
+    Words all;
+    uint32_t w[W];
+  };
+  const int lane = threadIdx.x & 31;
+  Pieces o;
+  uint32_t nans = 0u;  // a bit a column
+#pragma unroll
+  for (int i = 0; i < W; ++i) o.w[i] = 0u;
+  if (mine) {
+    o.all = *reinterpret_cast<const Words*>(dst);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      if (isnan(Pack2<T>::lo(o.w[i]))) nans |= 1u << (2 * i);
+      if (isnan(Pack2<T>::hi(o.w[i]))) nans |= 2u << (2 * i);
+    }
+  }
+  unsigned todo = __ballot_sync(0xffffffffu, nans != 0u);
+  while (todo != 0u) {
+    const int col = __shfl_sync(0xffffffffu, c, __ffs(todo) - 1);
+    const bool with = nans != 0u && c == col;
+    const int from = __reduce_min_sync(0xffffffffu, with ? first : INT_MAX);
+    const int to = __reduce_max_sync(0xffffffffu, with ? limit : 0);
+    const T* base = static_cast<const T*>(p.v) + head * p.v_head + col;
+    const int32_t* table = p.tables + req * p.table_stride;
+    float sum[2 * W];
+#pragma unroll
+    for (int i = 0; i < 2 * W; ++i) sum[i] = 0.f;
+    bool open = true;  // some column may still change: a NaN stays one
+#pragma unroll 1
+    for (int j0 = from; open && j0 < to; j0 += 32 * AT_ONCE) {
+      Pieces v[AT_ONCE];
+      uint32_t odd[AT_ONCE];
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const int j = j0 + k * 32 + lane;
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[k].w[i] = 0u;
+        if (j < to) {
+          const int block = __ldcg(table + j / p.block_size);
+          if (block >= 0 && block < p.num_blocks)
+            v[k].all = __ldcg(reinterpret_cast<const Words*>(base + block * p.v_block + (j % p.block_size) * p.v_slot));
+        }
+      }
+      unsigned any = 0u;
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) {
+        uint32_t seen = 0u;
+#pragma unroll
+        for (int i = 0; i < W; ++i) seen = paged_taint<T>(v[k].w[i], seen);
+        odd[k] = __ballot_sync(0xffffffffu, seen != 0u);
+        any |= odd[k];
+      }
+      if (any == 0u) continue;
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k)
+        for (unsigned left = odd[k]; left != 0u; left &= left - 1u) {
+          const int from_lane = __ffs(left) - 1, j = j0 + k * 32 + from_lane;
+          const bool sees = with && j >= first && j < limit;
+#pragma unroll
+          for (int i = 0; i < W; ++i) {
+            const uint32_t x = __shfl_sync(0xffffffffu, v[k].w[i], from_lane);
+            const float a = Pack2<T>::lo(x), b = Pack2<T>::hi(x);
+            if (sees && !isfinite(a)) sum[2 * i] += a;
+            if (sees && !isfinite(b)) sum[2 * i + 1] += b;
+          }
+        }
+      bool mine_open = false;
+#pragma unroll
+      for (int i = 0; i < 2 * W; ++i) mine_open |= (nans >> i & 1u) != 0u && !isnan(sum[i]);
+      open = __any_sync(0xffffffffu, with && mine_open);
+    }
+    if (with) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {  // a NaN without such a value stays
+        const float a = (nans >> (2 * i) & 1u) != 0u && sum[2 * i] != 0.f ? sum[2 * i] : Pack2<T>::lo(o.w[i]);
+        const float b = (nans >> (2 * i) & 2u) != 0u && sum[2 * i + 1] != 0.f ? sum[2 * i + 1] : Pack2<T>::hi(o.w[i]);
+        o.w[i] = pack_round2<T>(a, b);
+      }
+      *reinterpret_cast<Words*>(dst) = o.all;
+    }
+    todo &= ~__ballot_sync(0xffffffffu, with);
+  }
 }
 
 // 2^x on the special function unit; 0 for -infinity.
