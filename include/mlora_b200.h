@@ -357,7 +357,9 @@ int mlora_write_paged_kv(const void* k, int64_t k_token_stride, int64_t k_head_s
  * q_indptr[i]) + (t - q_indptr[i]), and it sees keys j <= pos, with window > 0
  * only j > pos - window. Query head h reads key head h / (q_heads / kv_heads).
  * fp32 scores, sums and statistics. A query that sees no key, and rows past
- * q_indptr[requests], give zeros.
+ * q_indptr[requests], give zeros; so do rows that are not computed, which are
+ * reported: those of requests whose offsets make no sense, and those of
+ * requests longer than max_q_len that the kernel chosen by it does not hold.
  *   q, out     [tokens, q_heads, head_dim] of the cache's dtype, head_dim
  *              <= 256 and a multiple of 8; token and head strides in elements
  *   block_tables [requests, max_blocks] (rows table_row_stride apart)

@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) paged_attention_general_kerne
       kv = kv < 0 ? 0 : (int)cap;
     }
   } else {
-    if (tid == 0 && t < q1) flag_error(p.status, kErrIndptr);
+    if (tid == 0 && (t < q1 || q1 < q0)) flag_error(p.status, kErrIndptr);
     q1 = q0 = t;
   }
   const int pos = kv - (q1 - q0) + (t - q0);

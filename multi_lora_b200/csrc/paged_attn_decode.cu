@@ -124,24 +124,36 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
   int req;
   PagedRequest found;
   const bool report = CLUSTER ? blockIdx.x % (kFewCtas * p.kv_heads) == 0 : blockIdx.x == 0;
+  bool skipped = false;  // a request that is not computed
   auto units = [&](int i, int, int, PagedRequest& r) {
     r = paged_request(p, i, report);
-    // rows beyond what the caller said: reported, and not computed
+    // rows beyond what the caller said: reported, and where they do not fit the tile not computed
     if (report && r.qn > p.max_q_len) flag_error(p.status, kErrLength);
     DecodeItem x;
     decode_request(p, x, i, r);
+    skipped |= r.odd || (r.qn > 0 && x.n == 0);
     return x.n > 0 ? (x.n + kDecItem) * p.kv_heads : 0;
   };
   // CLUSTER: a cluster takes one item, each CTA an eighth of its tiles, and the sums
   // are joined over distributed shared memory, without a search and without the workspace.
   const int rank = blockIdx.x % kFewCtas;
+  auto zero_others = [&]() {  // one warp: rows that are nobody's
+    if constexpr (CLUSTER) {  // which has asked about its own request only (about all of them before its first tile: 0.2 us later)
+      static_assert(kFewItems <= 32, "a lane a request");
+      PagedRequest r;
+      if (lane < p.requests) units(lane, 0, 1, r);
+      skipped = __any_sync(0xffffffffu, skipped);
+    }
+    if (skipped) paged_zero_uncomputed<T>(p, kDecodeMaxRows);
+    else paged_zero_rest<T>(p);
+  };
   if constexpr (CLUSTER) {
     const int item = blockIdx.x / kFewCtas;
     req = item / p.kv_heads;
     units(req, 0, 1, found);
     decode_request(p, it, req, found);
     if (it.n == 0) {  // the same in the whole cluster
-      if (warp == C::kWarps) paged_zero_rest<T>(p);
+      if (warp == C::kWarps) zero_others();
       return;
     }
     it.head = item - req * p.kv_heads;
@@ -149,11 +161,12 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
   } else {
     paged_find<C::kThreads, 1>(p.requests, units, split, req, found, before, in_req);
   }
-  __syncthreads();  // the barriers are initialised
+  if constexpr (CLUSTER) __syncthreads();     // the barriers are initialised
+  else skipped = __syncthreads_or(skipped);
   PagedCursor<DecodeSplit> cur(split);
   if constexpr (!CLUSTER) {
     if (cur.pos >= cur.end) {
-      if (warp == C::kWarps) paged_zero_rest<T>(p);
+      if (warp == C::kWarps) zero_others();
       return;
     }
     decode_request(p, it, req, found);
@@ -212,7 +225,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       }
       if (advance()) next_item();
     }
-    paged_zero_rest<T>(p);
+    zero_others();
     if constexpr (CLUSTER) {  // with the consumers: sums written, sums read
       for (int i = 0; i < 2; ++i) {
         cluster_arrive_release();

@@ -302,6 +302,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
   __shared__ __align__(8) uint64_t full[NS], empty[NS], q_ready[2], q_free[2], s_full[2][2], p_ready[2][2], pv_done[2][2];
   __shared__ uint32_t s_tmem;
   __shared__ int s_last[2];
+  __shared__ bool s_skipped;
   __shared__ float2 s_mate[128];
   __shared__ uint32_t s_odd[8];    // lanes of a softmax warp that stored what is not finite though the row's sum is
   __shared__ ChunkPlace s_place[8];  // of the item whose output each softmax warp writes
@@ -344,10 +345,12 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
   int before, in_req;
   int req;
   PagedRequest found;
+  bool skipped = false;  // a request that is not computed
   paged_find<kChunkThreads, 32>(
       p.requests,
       [&](int i, int part, int parts, PagedRequest& r) {
         r = paged_request(p, i, part == 0 && blockIdx.x == 0);
+        skipped |= r.odd;
         ChunkItem x;
         chunk_request(p, x, i, r);
         int n = 0;
@@ -358,7 +361,8 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         return n * p.kv_heads;
       },
       split, req, found, before, in_req);
-  __syncthreads();  // the barriers are initialised and s_tmem is there
+  skipped = __syncthreads_or(skipped);  // and the barriers are initialised, and s_tmem is there
+  if (tid == 96) s_skipped = skipped;   // for its own warp, at the end: no register holds it until then
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   PagedCursor<ChunkSplit> cur(split);
@@ -654,7 +658,9 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         }
         if (cur.advance()) next_item();
       }
-      paged_zero_rest<T>(p);
+      __syncwarp();
+      if (s_skipped) paged_zero_uncomputed<T>(p, INT_MAX);
+      else paged_zero_rest<T>(p);
     }
   } else {  // ---- softmax: warpgroup q, thread = row ----
     regs_up<216>();

@@ -30,6 +30,7 @@ __device__ __forceinline__ V same_in_warp(V v) {
 
 struct PagedRequest {
   int q0, qn, kv;  // first row, rows, keys
+  bool odd;        // offsets that make no sense (no rows then)
 };
 
 __device__ __forceinline__ PagedRequest paged_request(const PagedAttnArgs& p, int i, bool report) {
@@ -38,7 +39,8 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedAttnArgs& p, in
   const int q1 = __ldcg(p.q_indptr + i + 1);
   r.kv = __ldcg(p.kv_lens + i);
   r.qn = q1 - r.q0;
-  if (r.q0 < 0 || q1 < r.q0 || q1 > p.tokens) {
+  r.odd = r.q0 < 0 || q1 < r.q0 || q1 > p.tokens;
+  if (r.odd) {
     if (report) flag_error(p.status, kErrIndptr);
     r.q0 = r.qn = 0;
   }
@@ -139,7 +141,7 @@ __device__ __forceinline__ void paged_find_warp(int requests, F units, S& split,
   int parts = 1;
   while (parts < MAX_PARTS && 2 * parts * requests <= 32) parts *= 2;
   const int i = lane / parts, part = lane & (parts - 1);
-  PagedRequest last = {0, 0, 0};
+  PagedRequest last = {0, 0, 0, false};
   const int mine = i < requests ? units(i, part, parts, last) : 0;
   int incl = mine, all_parts = mine;
 #pragma unroll
@@ -172,7 +174,7 @@ __device__ __forceinline__ void paged_find(int requests, F units, S& split, int&
   __shared__ int s_before, s_sum;
   __shared__ int s_req;
   __shared__ PagedRequest s_found;
-  PagedRequest last = {0, 0, 0};
+  PagedRequest last = {0, 0, 0, false};
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int parts = 1;
   while (parts < MAX_PARTS && 2 * parts * requests <= NT) parts *= 2;
@@ -231,6 +233,26 @@ __device__ __forceinline__ void paged_zero_rest(const PagedAttnArgs& p) {
     T* o = static_cast<T*>(p.out) + (last + row / p.q_heads) * p.out_token + (row % p.q_heads) * p.out_head +
            (e % pieces) * 8;
     *reinterpret_cast<uint4*>(o) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// Zeros in every row that no request has, where some requests are not computed: their offsets make no sense, or they have
+// more rows (tokens x group) than `most`. One warp of every CTA takes a share. Only for calls that
+// report an error, so simple: each row asks all requests.
+template <typename T>
+__device__ __noinline__ void paged_zero_uncomputed(const PagedAttnArgs& p, int most) {
+  const int lane = threadIdx.x & 31, pieces = p.q_heads * (p.dim / 8);
+  for (int t = blockIdx.x; t < p.tokens; t += gridDim.x) {
+    bool computed = false;
+    for (int i0 = 0; i0 < p.requests && !computed; i0 += 32) {
+      PagedRequest r = {0, 0, 0, true};
+      if (i0 + lane < p.requests) r = paged_request(p, i0 + lane, false);
+      computed = __any_sync(0xffffffffu, t >= r.q0 && t < r.q0 + r.qn && r.qn * p.group <= most);
+    }
+    if (computed) continue;
+    for (int e = lane; e < pieces; e += 32)
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + t * p.out_token + e / (p.dim / 8) * p.out_head + e % (p.dim / 8) * 8) =
+          make_uint4(0, 0, 0, 0);
   }
 }
 
