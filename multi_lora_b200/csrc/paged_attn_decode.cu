@@ -716,7 +716,7 @@ cudaError_t launch_decode_any(const DecodeArgs& a, cudaStream_t st, bool pdl) {
 cudaError_t launch_paged_attention_decode(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl) {
   if ((dtype != kBF16 && dtype != kF16) || a.dim > 128) return cudaErrorNotSupported;
   // units of work (paged_sched.cuh) in 32 bits
-  if ((long long)a.requests * a.kv_heads * ((long long)a.width * a.block_size / kDecTile + 2 + kDecItem) > INT_MAX)
+  if ((long long)a.requests * a.kv_heads * ((long long)a.width * a.block_size / kDecTile + 2 + kDecItem) >= INT_MAX)
     return cudaErrorNotSupported;
   DecodeArgs d{};
   d.a = a;

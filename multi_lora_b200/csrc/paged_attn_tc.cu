@@ -659,7 +659,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         if (cur.advance()) next_item();
       }
       __syncwarp();
-      if (s_skipped) paged_zero_uncomputed<T>(p, INT_MAX);
+      if (s_skipped) paged_zero_uncomputed<T>(p, split.total > 0 ? INT_MAX : -1);
       else paged_zero_rest<T>(p);
     }
   } else {  // ---- softmax: warpgroup q, thread = row ----
@@ -996,7 +996,7 @@ cudaError_t launch_paged_attention_chunk(const PagedAttnArgs& a, int dtype, cuda
     return cudaErrorNotSupported;  // a maximum of scores is one of scaled scores for a positive scale only
   // units of work (paged_sched.cuh) in 32 bits
   const long long items = (long long)a.tokens * a.group / kChunkRows + a.requests;
-  if (items * a.kv_heads * ((long long)a.width * a.block_size / kChunkKeys + 2 + kChunkItem) > INT_MAX) return cudaErrorNotSupported;
+  if (items * a.kv_heads * ((long long)a.width * a.block_size / kChunkKeys + 2 + kChunkItem) >= INT_MAX) return cudaErrorNotSupported;
   ChunkArgs c{};
   c.a = a;
   c.box = paged_box(a.block_size, kChunkKeys);

@@ -74,6 +74,7 @@ struct PagedSplit {
   int total, base, rem;        // CTA c has base units, the first `rem` CTAs one more
   int T;                       // T_MOST, or less where the CTAs have less to do than that
   __device__ void set(int units, int ctas) {
+    if (units == INT_MAX) units = 0;  // see paged_sum
     total = units;
     base = units / ctas;
     rem = units - base * ctas;
@@ -129,6 +130,10 @@ struct PagedCursor {
   }
 };
 
+// Sums of units stop at INT_MAX. The caller keeps the sum over requests that share no rows below it; offsets that go back
+// and forth may give the same rows to many requests, and their work may pass it: then nothing is computed.
+__device__ __forceinline__ int paged_sum(int a, int b) { return (int)min((unsigned)a + (unsigned)b, (unsigned)INT_MAX); }
+
 // Whole block of NT threads: the split over the grid, the request that this CTA's first
 // unit lies in with its lengths, the units before that request and in it.
 // `units(i, part, parts, r)`: the units of request i (its lengths go to r), or one of
@@ -147,9 +152,9 @@ __device__ __forceinline__ void paged_find_warp(int requests, F units, S& split,
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += u;
+    if (lane >= o) incl = paged_sum(incl, u);
     const int w = __shfl_xor_sync(0xffffffffu, all_parts, o);
-    if (o < parts) all_parts += w;
+    if (o < parts) all_parts = paged_sum(all_parts, w);
   }
   split.set(__shfl_sync(0xffffffffu, incl, 31), gridDim.x);
   const int a = split.start(blockIdx.x), upto = incl - mine;
@@ -182,14 +187,14 @@ __device__ __forceinline__ void paged_find(int requests, F units, S& split, int&
   const int r0 = min(requests, parts > 1 ? tid / parts : tid * per), r1 = min(requests, r0 + per);
   const int part = tid & (parts - 1);
   int mine = 0;
-  for (int i = r0; i < r1; ++i) mine += units(i, part, parts, last);
+  for (int i = r0; i < r1; ++i) mine = paged_sum(mine, units(i, part, parts, last));
   int incl = mine, all_parts = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += u;
+    if (lane >= o) incl = paged_sum(incl, u);
     const int w = __shfl_xor_sync(0xffffffffu, all_parts, o);
-    if (o < parts) all_parts += w;
+    if (o < parts) all_parts = paged_sum(all_parts, w);
   }
   if (lane == 31) s_warp[warp] = incl;
   if (tid == 0) s_req = requests;
@@ -199,14 +204,15 @@ __device__ __forceinline__ void paged_find(int requests, F units, S& split, int&
   for (int w = 0; w < NT / 32; ++w) {
     const int u = s_warp[w];
     upto += w < warp ? u : 0;
-    total += u;
+    total = paged_sum(total, u);
   }
   split.set(same_in_warp(total), gridDim.x);
   const int a = split.start(blockIdx.x);
   if (part == 0 && a >= upto && a < upto + all_parts) {
     int i = r0;
     if (per > 1) {
-      for (all_parts = units(i, 0, 1, last); a >= upto + all_parts; all_parts = units(++i, 0, 1, last)) upto += all_parts;
+      for (all_parts = units(i, 0, 1, last); a >= upto + all_parts && i + 1 < r1; all_parts = units(++i, 0, 1, last))
+        upto += all_parts;
     }
     s_req = i;
     s_before = upto;

@@ -86,3 +86,23 @@ def test_rows_of_invalid_offsets_in_fp32(cuda_dev, workspace, q):  # noqa: F811
             assert ((out == want) | (out == 0)).all()
             with pytest.raises(RuntimeError, match="q_indptr"):
                 P.check_status(status)
+
+
+@pytest.mark.parametrize("requests, tokens, heads, width, block, most", [
+    (10, 600, (4, 2), 20, 16, 1),
+    (1025, 300, (4, 2), 20, 16, 1),
+    (8192, 4096, (64, 8), 1024, 128, 0),  # the key tiles of all requests pass 32 bits: nothing is computed
+])
+def test_offsets_that_go_back_and_forth(cuda_dev, workspace, requests, tokens, heads, width, block, most):  # noqa: F811
+    """Every other request claims all rows: reported, and the rows are anyone's (all values are one) or zeros."""
+    k = torch.ones(4, block, heads[1], 64, dtype=torch.bfloat16, device=cuda_dev)
+    q = torch.ones(tokens, heads[0], 64, dtype=torch.bfloat16, device=cuda_dev)
+    offsets = torch.arange(requests + 1, device=cuda_dev, dtype=torch.int32) % 2 * tokens
+    out = torch.full_like(q, float("nan"))
+    status = status_word(cuda_dev)
+    P.paged_attention(q, k, k, torch.zeros(requests, width, dtype=torch.int32, device=cuda_dev),
+                      torch.full((requests,), width * block, dtype=torch.int32, device=cuda_dev), offsets,
+                      max_q_len=tokens, workspace=workspace, out=out, status=status)
+    assert ((out >= 0) & (out <= most)).all()
+    with pytest.raises(RuntimeError, match="q_indptr"):
+        P.check_status(status)
