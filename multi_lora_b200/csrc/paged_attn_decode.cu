@@ -19,7 +19,9 @@
 //     Scores, sums and statistics are fp32. For the second product an f16
 //     probability is rounded once (11 bits); a bf16 one goes in as two terms, its
 //     rounding and the rounding's remainder (16 bits), since the 8 bits of one
-//     term would add as much error as the result's own rounding;
+//     term would add as much error as the result's own rounding. f16 has few exponents: P
+//     and its sum are taken times 2^15 (the largest P is 2^15), so that what is subnormal lies below
+//     2^-29 of the largest and not 2^-14: tens of thousands of small ones would be lost together;
 //   * head_dims below 64 and between 64 and 128 run as these: the boxes' columns behind
 //     them are zeros, and no memory;
 //   * key tiles are dealt evenly over two CTAs an SM (paged_sched.cuh), or, for few
@@ -92,6 +94,7 @@ __global__ void __launch_bounds__(DecodeCfg<D>::kThreads, DecodeCfg<D>::kPerSm)
 paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
   using C = DecodeCfg<D>;
   constexpr bool kTwoTerms = Num<T>::is_bf16;
+  constexpr float kUp = Num<T>::is_bf16 ? 0.f : 15.f;  // P is taken times 2^kUp
   constexpr int NS = C::kStages, SIDE = C::kSide, HALF = kDecTile * 128;
   extern __shared__ __align__(1024) unsigned char s_raw[];
   __shared__ __align__(8) uint64_t full[NS], empty[NS];
@@ -342,8 +345,9 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
           const float m_new = fmaxf(m[e], top), ref = m_new == -INFINITY ? 0.f : m_new;
           fix[e] = exp2_fast(m[e] - ref);
           m[e] = m_new;
-          const float p0 = exp2_fast(s[0][2 * e] - ref), p1 = exp2_fast(s[0][2 * e + 1] - ref);
-          const float p2 = exp2_fast(s[1][2 * e] - ref), p3 = exp2_fast(s[1][2 * e + 1] - ref);
+          const float base = ref - kUp;
+          const float p0 = exp2_fast(s[0][2 * e] - base), p1 = exp2_fast(s[0][2 * e + 1] - base);
+          const float p2 = exp2_fast(s[1][2 * e] - base), p3 = exp2_fast(s[1][2 * e + 1] - base);
           l[e] = l[e] * fix[e] + ((p0 + p1) + (p2 + p3));
           pf[e] = pack_round2<T>(p0, p1);
           pf[2 + e] = pack_round2<T>(p2, p3);

@@ -19,7 +19,9 @@
 // The running maximum that P is taken against is raised only when a row's
 // scores exceed it by 2^8 (O is rescaled in TMEM then, rarely after the first
 // tiles); P stays below 2^8 and everything is normalised at the end by the sum of P
-// in fp32. An f16 P is rounded once (11 bits). A bf16 P goes in as two terms,
+// in fp32. f16 has few exponents: P and its sum are taken times 2^11 there and the maximum is
+// raised from 2^4 on, so that P stays below 2^15 and what is subnormal lies below 2^-25 of the largest:
+// tens of thousands of small ones would be lost together. An f16 P is rounded once (11 bits). A bf16 P goes in as two terms,
 // its upper 8 bits and the rest (16 bits): one term of 8 bits would add as much
 // error as the result's own rounding. The second term is one more product of the same size.
 //
@@ -297,6 +299,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
   using C = ChunkCfg<D>;
   constexpr int NS = C::kSlots, HALF = kChunkKeys * 128;
   constexpr bool kTwoTerms = Num<T>::is_bf16;
+  constexpr float kRaise = Num<T>::is_bf16 ? 8.f : 4.f, kUp = Num<T>::is_bf16 ? 0.f : 11.f;  // in powers of two
   constexpr uint32_t S_COL = 0, O_COL = 256;
   extern __shared__ __align__(1024) unsigned char s_raw[];
   __shared__ __align__(8) uint64_t full[NS], empty[NS], q_ready[2], q_free[2], s_full[2][2], p_ready[2][2], pv_done[2][2];
@@ -725,7 +728,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
         if (k == 0) {
           m = mx;
         } else {
-          const bool raise = mx > m + 8.f;
+          const bool raise = mx > m + kRaise;
           if (__any_sync(0xffffffffu, raise)) {
             // O holds the halves before this one once the last product is done
             ok = ok && mbar_poll(&pv_done[q][b ^ 1], ((n - 1) >> 1) & 1, p.status);
@@ -746,7 +749,7 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
             }
           }
         }
-        const float ref = m == -INFINITY ? 0.f : m;
+        const float ref = (m == -INFINITY ? 0.f : m) - kUp;
         const uint64_t sl2 = pack2(sl, sl), ref2 = pack2(-ref, -ref);
         uint64_t sum[4] = {0, 0, 0, 0};
         uint32_t w[32], rest[32];  // P, two keys a column
