@@ -16,10 +16,10 @@
 //     between warps until its end. K's fragments are all loaded before the
 //     products, which run as four chains, and V's are in flight during the
 //     softmax: a warp that waited for each in turn took twice as long a tile.
-//     Scores, sums and statistics are fp32. For the second product an f16
-//     probability is rounded once (11 bits); a bf16 one goes in as two terms, its
-//     rounding and the rounding's remainder (16 bits), since the 8 bits of one
-//     term would add as much error as the result's own rounding. f16 has few exponents: P
+//     Scores, sums and statistics are fp32. For the second product a
+//     probability goes in as two terms, its rounding and the rounding's remainder (16 bits of
+//     it in bf16, 21 in f16), since one term's 8 or 11 bits would add as much error as the result's own
+//     rounding (f16: 1.2 times the whole error; 64 requests to 2048 keys 188 us with one term, 190 with two). f16 has few exponents: P
 //     and its sum are taken times 2^15 (the largest P is 2^15), so that what is subnormal lies below
 //     2^-29 of the largest and not 2^-14: tens of thousands of small ones would be lost together;
 //   * head_dims below 64 and between 64 and 128 run as these: the boxes' columns behind
@@ -93,7 +93,6 @@ template <typename T, int D, bool CLUSTER>
 __global__ void __launch_bounds__(DecodeCfg<D>::kThreads, DecodeCfg<D>::kPerSm)
 paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
   using C = DecodeCfg<D>;
-  constexpr bool kTwoTerms = Num<T>::is_bf16;
   constexpr float kUp = Num<T>::is_bf16 ? 0.f : 15.f;  // P is taken times 2^kUp
   constexpr int NS = C::kStages, SIDE = C::kSide, HALF = kDecTile * 128;
   extern __shared__ __align__(1024) unsigned char s_raw[];
@@ -351,10 +350,8 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
           l[e] = l[e] * fix[e] + ((p0 + p1) + (p2 + p3));
           pf[e] = pack_round2<T>(p0, p1);
           pf[2 + e] = pack_round2<T>(p2, p3);
-          if constexpr (kTwoTerms) {
-            pr[e] = pack_round2<T>(p0 - Pack2<T>::lo(pf[e]), p1 - Pack2<T>::hi(pf[e]));
-            pr[2 + e] = pack_round2<T>(p2 - Pack2<T>::lo(pf[2 + e]), p3 - Pack2<T>::hi(pf[2 + e]));
-          }
+          pr[e] = pack_round2<T>(p0 - Pack2<T>::lo(pf[e]), p1 - Pack2<T>::hi(pf[e]));
+          pr[2 + e] = pack_round2<T>(p2 - Pack2<T>::lo(pf[2 + e]), p3 - Pack2<T>::hi(pf[2 + e]));
         }
         if (__any_sync(0xffffffffu, fix[0] != 1.f || fix[1] != 1.f)) {
 #pragma unroll
@@ -420,12 +417,10 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
           mma_16816<T>(o[2 * n], pf[0], pf[1], pf[2], pf[3], vf[n][0], vf[n][1]);
           mma_16816<T>(o[2 * n + 1], pf[0], pf[1], pf[2], pf[3], vf[n][2], vf[n][3]);
         }
-        if constexpr (kTwoTerms) {
 #pragma unroll
-          for (int n = 0; n < D / 16; ++n) {
-            mma_16816<T>(o[2 * n], pr[0], pr[1], pr[2], pr[3], vf[n][0], vf[n][1]);
-            mma_16816<T>(o[2 * n + 1], pr[0], pr[1], pr[2], pr[3], vf[n][2], vf[n][3]);
-          }
+        for (int n = 0; n < D / 16; ++n) {
+          mma_16816<T>(o[2 * n], pr[0], pr[1], pr[2], pr[3], vf[n][0], vf[n][1]);
+          mma_16816<T>(o[2 * n + 1], pr[0], pr[1], pr[2], pr[3], vf[n][2], vf[n][3]);
         }
       }
       __syncwarp();

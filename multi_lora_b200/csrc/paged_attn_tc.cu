@@ -21,16 +21,18 @@
 // tiles); P stays below 2^8 and everything is normalised at the end by the sum of P
 // in fp32. f16 has few exponents: P and its sum are taken times 2^11 there and the maximum is
 // raised from 2^4 on, so that P stays below 2^15 and what is subnormal lies below 2^-25 of the largest:
-// tens of thousands of small ones would be lost together. An f16 P is rounded once (11 bits). A bf16 P goes in as two terms,
-// its upper 8 bits and the rest (16 bits): one term of 8 bits would add as much
-// error as the result's own rounding. The second term is one more product of the same size.
+// tens of thousands of small ones would be lost together. P goes in as two terms,
+// its upper 8 bits (f16: 11) and the rest (16 bits of it; 21): one term would add as much
+// error as the result's own rounding. The second term is one more product of the same size. In f16, one
+// term and two: 2048 tokens over 16384 keys 542 and 662 us, eight prompts 69 and 76, 1 to 6 drafts 98 and
+// 103, at 1.2 times the error (2.5e-4 and 2.1e-4 of the result, which is the rounding of the result alone).
 //
 // Head_dims below 64 and between 64 and 128 run as these, with columns of zeros that
 // TMA fills in.
 //
 // What bounds it: the exponentials (16 a cycle and SM: 2048 cycles for two
-// 128 x 128 tiles) and the tensor cores (4096 multiply-adds a cycle: 2048
-// cycles for f16, 3072 for bf16 with its second term, at D = 128), and over a
+// 128 x 128 tiles) and the tensor cores (4096 multiply-adds a cycle: 3072
+// cycles with the second term, at D = 128), and over a
 // long launch the power that these draw. Measured: 2048 tokens x 32 heads over 16384 keys in 630 to 710 us,
 // the tensor pipe 68 % busy at 1.6 GHz (f16: 593 us, 985 TFLOP/s); 8 prompts of 128 to
 // 1024 tokens 69 us, where an item's beginning and end (8000 cycles) weigh as
@@ -298,7 +300,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
   using C = ChunkCfg<D>;
   constexpr int NS = C::kSlots, HALF = kChunkKeys * 128;
-  constexpr bool kTwoTerms = Num<T>::is_bf16;
+  constexpr uint32_t kKeep = Num<T>::is_bf16 ? 0xffff0000u : 0xffffe000u;  // bits of fp32 that the type holds
   constexpr float kRaise = Num<T>::is_bf16 ? 8.f : 4.f, kUp = Num<T>::is_bf16 ? 0.f : 11.f;  // in powers of two
   constexpr uint32_t S_COL = 0, O_COL = 256;
   extern __shared__ __align__(1024) unsigned char s_raw[];
@@ -488,10 +490,8 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
           const uint32_t a = s_col + b * 64;
 #pragma unroll
           for (int i = 0; i < kHalfKeys / 16; ++i) umma_ts(o_col, a + i * 8, held_lo + i * 128, idesc_o, !held_first || i > 0);
-          if constexpr (kTwoTerms) {
 #pragma unroll
-            for (int i = 0; i < kHalfKeys / 16; ++i) umma_ts(o_col, a + 32 + i * 8, held_lo + i * 128, idesc_o, true);
-          }
+          for (int i = 0; i < kHalfKeys / 16; ++i) umma_ts(o_col, a + 32 + i * 8, held_lo + i * 128, idesc_o, true);
           umma_commit(&pv_done[q][b]);
           if (held_last) umma_commit(&empty[held_slot]);
         }
@@ -759,19 +759,17 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
           const float p0 = exp2_fast(lo_of(x)), p1 = exp2_fast(hi_of(x));
           const uint64_t pp = pack2(p0, p1);
           sum[(i >> 1) & 3] = add2(sum[(i >> 1) & 3], pp);
-          if constexpr (kTwoTerms) {  // the upper 16 bits as they are, and what is left rounded
-            w[i >> 1] = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);
-            const uint64_t left = fma2(pack2u(__float_as_uint(p0) & 0xffff0000u, __float_as_uint(p1) & 0xffff0000u),
-                                       pack2(-1.f, -1.f), pp);
-            rest[i >> 1] = pack_round2<T>(lo_of(left), hi_of(left));
-          } else {
-            w[i >> 1] = pack_round2<T>(p0, p1);
-          }
+          // the upper bits as they are (in f16 rounded where they are subnormal), and what is left rounded
+          const uint32_t u0 = __float_as_uint(p0) & kKeep, u1 = __float_as_uint(p1) & kKeep;
+          if constexpr (Num<T>::is_bf16) w[i >> 1] = __byte_perm(u0, u1, 0x7632);
+          else w[i >> 1] = pack_round2<T>(__uint_as_float(u0), __uint_as_float(u1));
+          const uint64_t left = fma2(pack2u(u0, u1), pack2(-1.f, -1.f), pp);
+          rest[i >> 1] = pack_round2<T>(lo_of(left), hi_of(left));
         }
         const uint64_t both = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
         l += lo_of(both) + hi_of(both);
         tmem_st32(s_addr + b * 64, w);
-        if constexpr (kTwoTerms) tmem_st32(s_addr + b * 64 + 32, rest);
+        tmem_st32(s_addr + b * 64 + 32, rest);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
