@@ -20,6 +20,7 @@ import torch
 PKG = Path(__file__).resolve().parent
 CUDA_LIB_PATH = PKG / "libmlora_b200.so"
 TORCH_LIB_PATH = PKG / "_mlora_torch.so"
+DIRECT_LIB_PATH = PKG / "_mlora_direct.so"
 
 # dtype codes of include/mlora_b200.h
 DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -166,13 +167,16 @@ def direct(name: str):
     """An operator of the paged serving step as a plain function of the binding: the
     same C++ function as ``torch.ops.mlora.<name>`` without the dispatcher's argument handling."""
     ops()
-    loader = importlib.machinery.ExtensionFileLoader("_mlora_torch", str(TORCH_LIB_PATH))
-    spec = importlib.util.spec_from_file_location("_mlora_torch", str(TORCH_LIB_PATH), loader=loader)
-    module = sys.modules.get("_mlora_torch")
+    module = sys.modules.get("_mlora_direct")
     if module is None:
+        if not DIRECT_LIB_PATH.exists():
+            raise NativeLibraryError(
+                f"{DIRECT_LIB_PATH.name} not built; run `python -m multi_lora_b200.build`")
+        loader = importlib.machinery.ExtensionFileLoader("_mlora_direct", str(DIRECT_LIB_PATH))
+        spec = importlib.util.spec_from_file_location("_mlora_direct", str(DIRECT_LIB_PATH), loader=loader)
         module = importlib.util.module_from_spec(spec)
         loader.exec_module(module)
-        sys.modules["_mlora_torch"] = module
+        sys.modules["_mlora_direct"] = module
     return getattr(module, name)
 
 

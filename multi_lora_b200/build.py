@@ -4,9 +4,11 @@
   ``include/mlora_b200.h``; compiled by nvcc for sm_100a only, static cudart,
   no torch dependency.
 * ``_mlora_torch.so`` — the ``torch.ops.mlora`` binding (torch_ops*.cpp),
-  linked against ``libmlora_b200.so`` through an ``$ORIGIN`` rpath.
+  linked against ``libmlora_b200.so`` through an ``$ORIGIN`` rpath; torch's C++ libraries and no Python.
+* ``_mlora_direct.so`` — the paged step's operators as a Python module
+  (torch_direct.cpp), linked against ``_mlora_torch.so``.
 
-Both land next to this file so that they travel with the source tree. A
+They land next to this file so that they travel with the source tree. A
 library is rebuilt only when one of its sources is newer than it.
 
     python -m multi_lora_b200.build [--force]
@@ -29,6 +31,7 @@ CSRC = PKG / "csrc"
 OBJ = ROOT / "_build"
 CUDA_LIB = PKG / "libmlora_b200.so"
 TORCH_LIB = PKG / "_mlora_torch.so"
+DIRECT_LIB = PKG / "_mlora_direct.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
@@ -91,41 +94,50 @@ def build_cuda_lib(force: bool = False, verbose: bool = False) -> Path:
     return CUDA_LIB
 
 
-def build_torch_lib(force: bool = False, verbose: bool = False) -> Path:
-    srcs = sorted(CSRC.glob("torch_ops*.cpp"))
-    if not force and not _stale(TORCH_LIB, [*srcs, CUDA_LIB, ROOT / "include" / "mlora_b200.h"]):
-        return TORCH_LIB
+def _build_torch(target: Path, srcs: list[Path], deps: list[Path], libs: list[str], force: bool, verbose: bool) -> Path:
+    """A library over torch's C++ API from `srcs`, which include `deps`, linked against `libs` of this folder or torch's."""
+    if not force and not _stale(target, [*srcs, *deps]):
+        return target
     import torch
     import torch.utils.cpp_extension as ext
 
-    incs = ext.include_paths("cuda")
-    libs = ext.library_paths("cuda")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     OBJ.mkdir(exist_ok=True)
     cxx = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-           "-DTORCH_API_INCLUDE_EXTENSION_H", *[f"-I{p}" for p in incs], f"-I{sysconfig.get_path('include')}"]
+           "-DTORCH_API_INCLUDE_EXTENSION_H", *[f"-I{p}" for p in ext.include_paths("cuda")],
+           f"-I{sysconfig.get_path('include')}"]
     objs = [OBJ / (src.stem + ".o") for src in srcs]
-    jobs = [[*cxx, "-c", str(src), "-o", str(obj)] for src, obj in zip(srcs, objs)
-            if force or _stale(obj, [src, ROOT / "include" / "mlora_b200.h"])]
+    headers = [d for d in deps if d.suffix == ".h"]
+    jobs = [[*cxx, "-c", str(src), "-o", str(obj)] for src, obj in zip(srcs, objs) if force or _stale(obj, [src, *headers])]
     with cf.ThreadPoolExecutor(max_workers=max(1, len(jobs))) as ex:
         for done in [ex.submit(_run, c) for c in jobs]:
             done.result()
-    cmd = [
-        os.environ.get("CXX", "g++"), "-shared", *map(str, objs), "-o", str(TORCH_LIB.with_suffix(".so.tmp")),
-        *[f"-L{p}" for p in libs], f"-L{PKG}",
-        "-lmlora_b200", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
-        "-Wl,-rpath,$ORIGIN",
-    ]
+    tmp = target.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-shared", *map(str, objs), "-o", str(tmp),
+           *[f"-L{p}" for p in ext.library_paths("cuda")], f"-L{PKG}", *libs,
+           "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-Wl,-rpath,$ORIGIN"]
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     _run(cmd)
-    os.replace(TORCH_LIB.with_suffix(".so.tmp"), TORCH_LIB)
-    return TORCH_LIB
+    os.replace(tmp, target)
+    return target
+
+
+def build_torch_lib(force: bool = False, verbose: bool = False) -> Path:
+    deps = [*sorted(CSRC.glob("torch_ops*.h")), ROOT / "include" / "mlora_b200.h", CUDA_LIB]
+    return _build_torch(TORCH_LIB, sorted(CSRC.glob("torch_ops*.cpp")), deps, ["-lmlora_b200"], force, verbose)
+
+
+def build_direct_lib(force: bool = False, verbose: bool = False) -> Path:
+    deps = [*sorted(CSRC.glob("torch_ops*.h")), TORCH_LIB]
+    return _build_torch(DIRECT_LIB, [CSRC / "torch_direct.cpp"], deps, ["-l:_mlora_torch.so", "-ltorch_python"], force,
+                        verbose)
 
 
 def build_all(force: bool = False, verbose: bool = False) -> None:
     build_cuda_lib(force=force, verbose=verbose)
     build_torch_lib(force=force, verbose=verbose)
+    build_direct_lib(force=force, verbose=verbose)
 
 
 def main() -> None:
@@ -134,7 +146,7 @@ def main() -> None:
     ap.add_argument("-v", "--verbose", action="store_true")
     args = ap.parse_args()
     build_all(force=args.force, verbose=args.verbose)
-    print(f"built {CUDA_LIB.name} and {TORCH_LIB.name}")
+    print(f"built {CUDA_LIB.name}, {TORCH_LIB.name} and {DIRECT_LIB.name}")
 
 
 if __name__ == "__main__":

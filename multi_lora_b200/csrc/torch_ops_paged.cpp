@@ -6,12 +6,10 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
-#include <torch/csrc/utils/pybind.h>
 #include <torch/library.h>
 
-#include <tuple>
-
 #include "../../include/mlora_b200.h"
+#include "torch_ops_paged.h"
 
 namespace {
 
@@ -83,6 +81,10 @@ mlora_paged_cache_t cache_of(const at::Tensor& k, const at::Tensor& v, const at:
   c.v_head_stride = v.stride(2);
   return c;
 }
+
+}  // namespace
+
+namespace mlora_torch {
 
 void plan_paged_step(const at::Tensor& ctx_lens, const at::Tensor& new_lens, const at::Tensor& held_blocks,
                      const at::Tensor& free_blocks, const at::Tensor& free_head, at::Tensor block_tables,
@@ -200,7 +202,7 @@ std::tuple<at::Tensor, at::Tensor> verify_draft(const at::Tensor& target, const 
   return {tokens, emitted};
 }
 
-}  // namespace
+}  // namespace mlora_torch
 
 TORCH_LIBRARY_FRAGMENT(mlora, m) {
   m.def(
@@ -221,15 +223,8 @@ TORCH_LIBRARY_FRAGMENT(mlora, m) {
 }
 
 TORCH_LIBRARY_IMPL(mlora, CUDA, m) {
-  m.impl("plan_paged_step", &plan_paged_step);
-  m.impl("write_paged_kv", &write_paged_kv);
-  m.impl("paged_attention", &paged_attention);
-  m.impl("verify_draft", &verify_draft);
-}
-
-PYBIND11_MODULE(_mlora_torch, m) {
-  m.def("plan_paged_step", &plan_paged_step);
-  m.def("write_paged_kv", &write_paged_kv);
-  m.def("paged_attention", &paged_attention);
-  m.def("verify_draft", &verify_draft);
+  m.impl("plan_paged_step", &mlora_torch::plan_paged_step);
+  m.impl("write_paged_kv", &mlora_torch::write_paged_kv);
+  m.impl("paged_attention", &mlora_torch::paged_attention);
+  m.impl("verify_draft", &mlora_torch::verify_draft);
 }
