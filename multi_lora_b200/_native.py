@@ -164,8 +164,9 @@ def ops():
 
 @functools.lru_cache(maxsize=None)
 def direct(name: str):
-    """An operator of the paged serving step as a plain function of the binding: the
-    same C++ function as ``torch.ops.mlora.<name>`` without the dispatcher's argument handling."""
+    """An operator of the paged serving step as a plain function: the same C++ function as
+    ``torch.ops.mlora.<name>``, without the dispatcher's argument handling where the dispatcher
+    has nothing else to do."""
     ops()
     module = sys.modules.get("_mlora_direct")
     if module is None:
