@@ -3,6 +3,9 @@ find those that are called through ``torch.ops``."""
 
 from __future__ import annotations
 
+import threading
+import time
+
 import pytest
 import torch
 from torch.utils._python_dispatch import TorchDispatchMode
@@ -82,3 +85,31 @@ def test_the_cache_is_no_part_of_a_graph(cuda_dev, workspace):  # noqa: F811
         P.write_paged_kv(kv[:, :2], kv[:, 2:], pr["k"], pr["v"], i32([0, 1, 2], cuda_dev))
     assert not pr["k"].requires_grad and pr["k"].grad_fn is None and not pr["v"].requires_grad
     assert torch.equal(pr["k"][0, :3], kv[:, :2])
+
+
+def test_other_threads_go_on_while_a_launch_waits(cuda_dev, workspace):  # noqa: F811
+    """Behind a busy GPU the queue of launches fills up, and a launch waits for room in it."""
+    _, call = step(cuda_dev, workspace)[1]
+    call()
+    torch.cuda.synchronize()
+    gaps, stop = [], threading.Event()
+
+    def watch():
+        last = time.perf_counter()
+        while not stop.is_set():
+            time.sleep(0.001)
+            now = time.perf_counter()
+            gaps.append(now - last)
+            last = now
+
+    watcher = threading.Thread(target=watch)
+    watcher.start()
+    start = time.perf_counter()
+    torch.cuda._sleep(1_500_000_000)  # most of a second
+    for _ in range(3000):
+        call()
+    took = time.perf_counter() - start
+    torch.cuda.synchronize()
+    stop.set()
+    watcher.join()
+    assert took > 0.4 and max(gaps) < 0.2, (took, max(gaps))
