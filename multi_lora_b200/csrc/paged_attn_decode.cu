@@ -178,10 +178,9 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
   auto next_item = [&]() {
     if (++it.head == p.kv_heads) {
       it.head = 0;
-      for (int i = it.req + 1; i < p.requests; ++i) {
-        decode_request(p, it, i, paged_request(p, i, false));
-        if (it.n > 0) break;
-      }
+      PagedRequest r;
+      const int i = paged_next(p, it.req, kDecodeMaxRows, r);
+      if (i < p.requests) decode_request(p, it, i, r);
     }
   };
   if (!CLUSTER && cur.begin(it.n)) next_item();

@@ -406,13 +406,13 @@ paged_attention_chunk_kernel(const __grid_constant__ ChunkArgs args) {
       it.rt = 0;
       if (++it.head == p.kv_heads) {
         it.head = 0;
-        for (int i = it.req + 1; i < p.requests; ++i) {
-          PagedRequest r = paged_request(p, i, false);
+        PagedRequest r;
+        const int i = paged_next(p, it.req, INT_MAX, r);
+        if (i < p.requests) {
           r.q0 = same_in_warp(r.q0);
           r.qn = same_in_warp(r.qn);
           r.kv = same_in_warp(r.kv);
           chunk_request(p, it, i, r);
-          if (r.qn > 0) break;
         }
       }
     }

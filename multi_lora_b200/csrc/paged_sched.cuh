@@ -228,6 +228,48 @@ __device__ __forceinline__ void paged_find(int requests, F units, S& split, int&
   found.kv = same_in_warp(s_found.kv);
 }
 
+// The first request from i on with rows, at most `most` of them (tokens x group), in the rare case that there
+// is none among the 32 before: 128 at once, which are one round trip to L2.
+__device__ __forceinline__ int paged_skip_idle(const PagedAttnArgs& p, int i, int most) {
+  constexpr int AT_ONCE = 4;
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int i0 = i; i0 < p.requests; i0 += 32 * AT_ONCE) {
+    int q0[AT_ONCE], q1[AT_ONCE];
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+      const int at = min(i0 + k * 32 + lane, p.requests - 1);  // the last one again, rather than one behind it
+      q0[k] = __ldcg(p.q_indptr + at);
+      q1[k] = __ldcg(p.q_indptr + at + 1);
+    }
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+      const bool has = q0[k] >= 0 && q1[k] > q0[k] && q1[k] <= p.tokens && (q1[k] - q0[k]) * p.group <= most;
+      const unsigned hit = __ballot_sync(0xffffffffu, has);
+      if (hit != 0u) return min(i0 + k * 32 + __ffs(hit) - 1, p.requests - 1);
+    }
+  }
+  return p.requests;
+}
+// The next request after i with rows (as above) and its lengths, p.requests if there is none: the whole warp. Idle
+// requests may be many: a cache plans all that it has room for at every step.
+__device__ __forceinline__ int paged_next(const PagedAttnArgs& p, int i, int most, PagedRequest& r) {
+  const int at = i + 1 + (threadIdx.x & 31);
+  r = {0, 0, 0, false};
+  if (at < p.requests) r = paged_request(p, at, false);
+  const unsigned hit = __ballot_sync(0xffffffffu, r.qn > 0 && r.qn * p.group <= most);
+  if (__builtin_expect(hit == 0u, 0)) {
+    i = paged_skip_idle(p, i + 33, most);
+    if (i < p.requests) r = paged_request(p, i, false);
+    return i;
+  }
+  const int src = __ffs(hit) - 1;
+  r.q0 = __shfl_sync(0xffffffffu, r.q0, src);
+  r.qn = __shfl_sync(0xffffffffu, r.qn, src);
+  r.kv = __shfl_sync(0xffffffffu, r.kv, src);
+  return i + 1 + src;
+}
+
 // Rows behind the last request's give zeros; one warp of every CTA takes a share.
 template <typename T>
 __device__ __forceinline__ void paged_zero_rest(const PagedAttnArgs& p) {
