@@ -356,7 +356,8 @@ int mlora_write_paged_kv(const void* k, int64_t k_token_stride, int64_t k_head_s
  * request i sees: its position is pos = kv_lens[i] - (q_indptr[i+1] -
  * q_indptr[i]) + (t - q_indptr[i]), and it sees keys j <= pos, with window > 0
  * only j > pos - window. Query head h reads key head h / (q_heads / kv_heads).
- * fp32 scores, sums and statistics. A query that sees no key, and rows past
+ * fp32 scores, sums and statistics. A query that sees no key (or only keys
+ * whose scores are minus infinity), and rows past
  * q_indptr[requests], give zeros; so do rows that are not computed, which are
  * reported: those of requests whose offsets make no sense, and those of
  * requests longer than max_q_len that the kernel chosen by it does not hold.

@@ -70,7 +70,7 @@ struct PagedAttnArgs {
 // Any dtype, head_dim <= 256, block size and stride.
 cudaError_t launch_paged_attention_general(const PagedAttnArgs& a, int dtype, bool vec, cudaStream_t st, bool pdl);
 
-// 16-bit caches with head_dim 64 or 128, block size a multiple of 8, 16-byte pieces
+// 16-bit caches with head_dim up to 128, block size a multiple of 8, 16-byte pieces
 // everywhere. Decode: up to kDecodeMaxRows rows (max_q_len * q_heads / kv_heads);
 // chunk: any number. cudaErrorNotSupported: the shape is not one of these.
 cudaError_t launch_paged_attention_decode(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl);

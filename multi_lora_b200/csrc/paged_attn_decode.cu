@@ -19,9 +19,10 @@
 //     Scores, sums and statistics are fp32. For the second product a
 //     probability goes in as two terms, its rounding and the rounding's remainder (16 bits of
 //     it in bf16, 21 in f16), since one term's 8 or 11 bits would add as much error as the result's own
-//     rounding (f16: 1.2 times the whole error; 64 requests to 2048 keys 188 us with one term, 190 with two). f16 has few exponents: P
-//     and its sum are taken times 2^15 (the largest P is 2^15), so that what is subnormal lies below
-//     2^-29 of the largest and not 2^-14: tens of thousands of small ones would be lost together;
+//     rounding (f16: 1.2 times the whole error; 64 requests to 2048 keys 188 to 193 us
+//     with one term, 190 to 206 with two). f16 has few exponents: P and its sum are taken times 2^15
+//     (the largest P is 2^15), so that what is subnormal lies below 2^-29 of the largest and
+//     not 2^-14: tens of thousands of small ones would be lost together;
 //   * head_dims below 64 and between 64 and 128 run as these: the boxes' columns behind
 //     them are zeros, and no memory;
 //   * key tiles are dealt evenly over two CTAs an SM (paged_sched.cuh), or, for few
@@ -32,9 +33,10 @@
 // taken out and added to these rows alone. Where the products made NaN of an infinity that
 // a row does see, its output is settled after it was stored (paged_settle).
 //
-// Measured: 64 requests of 33 to 2048 keys, 32 heads of 128: 189 us, 5.6 TB/s (85 % of
-// the measured copy bandwidth); 4 requests of 20000 to 65536 keys, 8 key heads:
-// 114 us, 5.4 TB/s; one request of 777 keys: 6.5 us.
+// Measured: 64 requests of 33 to 2048 keys, 32 heads of 128: 190 to 197 us, 5.4 to 5.6 TB/s (82 to 85 %
+// of the measured copy bandwidth); 4 requests of 20000 to 65536 keys, 8 key heads:
+// 115 us, 5.3 TB/s; one request of 777 keys: 6.5 us; 64 requests of 8192 keys with a window of
+// 1000, 8 key heads: 60 us, 4.4 TB/s.
 #include <climits>
 
 #include "device.h"

@@ -19,13 +19,15 @@
 // The running maximum that P is taken against is raised only when a row's
 // scores exceed it by 2^8 (O is rescaled in TMEM then, rarely after the first
 // tiles); P stays below 2^8 and everything is normalised at the end by the sum of P
-// in fp32. f16 has few exponents: P and its sum are taken times 2^11 there and the maximum is
-// raised from 2^4 on, so that P stays below 2^15 and what is subnormal lies below 2^-25 of the largest:
-// tens of thousands of small ones would be lost together. P goes in as two terms,
-// its upper 8 bits (f16: 11) and the rest (16 bits of it; 21): one term would add as much
-// error as the result's own rounding. The second term is one more product of the same size. In f16, one
-// term and two: 2048 tokens over 16384 keys 542 and 662 us, eight prompts 69 and 76, 1 to 6 drafts 98 and
-// 103, at 1.2 times the error (2.5e-4 and 2.1e-4 of the result, which is the rounding of the result alone).
+// in fp32. f16 has few exponents: P and its sum are taken times 2^11 there and the
+// maximum is raised from 2^4 on, so that P stays below 2^15 and what is subnormal lies
+// below 2^-25 of the largest: tens of thousands of small ones would be lost together.
+//
+// P goes in as two terms, its upper 8 bits (f16: 11) and the rest (16 bits of it; 21):
+// one term would add as much error as the result's own rounding. The second term is one
+// more product of the same size. In f16, one term and two: 2048 tokens over 16384 keys
+// 542 and 662 us, eight prompts 69 and 76, 1 to 6 drafts 98 and 109, the error 2.5e-4 and
+// 2.1e-4 of the result's norm, the latter the rounding of the result alone.
 //
 // Head_dims below 64 and between 64 and 128 run as these, with columns of zeros that
 // TMA fills in.
@@ -33,11 +35,12 @@
 // What bounds it: the exponentials (16 a cycle and SM: 2048 cycles for two
 // 128 x 128 tiles) and the tensor cores (4096 multiply-adds a cycle: 3072
 // cycles with the second term, at D = 128), and over a
-// long launch the power that these draw. Measured: 2048 tokens x 32 heads over 16384 keys in 630 to 710 us,
-// the tensor pipe 68 % busy at 1.6 GHz (f16: 593 us, 985 TFLOP/s); 8 prompts of 128 to
-// 1024 tokens 69 us, where an item's beginning and end (8000 cycles) weigh as
-// much as its tiles (4300 each); 32 requests of 1 to 6 drafts over up to 8192 keys 97 us,
-// 67 % of the measured copy bandwidth.
+// long launch the power that these draw. Measured, bf16 and f16: 2048 tokens x 32 heads over 16384 keys in
+// 720 us back to back (810 TFLOP/s; 640 before the power cap is reached, the tensor pipe 69 % busy at
+// 1.6 GHz); 8 prompts of 128 to 1024 tokens 69 and 76 us: 4.3 items a CTA whose beginnings and ends
+// (8000 cycles each) are a third of the work beside 14.5 tiles of 4300; 32 requests of 1 to 6 drafts
+// over up to 8192 keys 105 and 109 us, 68 % of the measured copy bandwidth, where the second term keeps
+// V's slots longer in a ring of 2.5 tiles; 512 tokens over 8192 keys with a window of 1000 33 us.
 //
 // Keys that a row does not see may hold anything: their scores are replaced, and
 // since 0 * NaN is NaN their V is not multiplied by them. Rows of V that no row of

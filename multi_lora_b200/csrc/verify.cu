@@ -248,7 +248,7 @@ namespace {
 template <typename T>
 cudaError_t launch_verify_t(const VerifyArgs& a, bool vec, cudaStream_t st, bool pdl) {
   constexpr int V = 16 / (int)sizeof(T);
-  // 4096 elements a CTA or more: below that the CTAs of a cluster only wait for one another
+  // more than 2048 elements a CTA: below that the CTAs of a cluster only wait for one another
   int ctas = 1;
   while (ctas < kVerifyMaxCtas && a.vocab > 4096 * ctas) ctas *= 2;
   const int unit = 32 * V, warps = ctas * (kVerifyNT / 32);
