@@ -142,7 +142,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
   // are joined over distributed shared memory, without a search and without the workspace.
   const int rank = blockIdx.x % kFewCtas;
   auto zero_others = [&]() {  // one warp: rows that are nobody's
-    if constexpr (CLUSTER) {  // which has asked about its own request only (about all of them before its first tile: 0.2 us later)
+    if constexpr (CLUSTER) {  // which has asked about its own request only (all of them at the start: 0.2 us more)
       static_assert(kFewItems <= 32, "a lane a request");
       PagedRequest r;
       if (lane < p.requests) units(lane, 0, 1, r);

@@ -1000,7 +1000,8 @@ cudaError_t launch_paged_attention_chunk(const PagedAttnArgs& a, int dtype, cuda
     return cudaErrorNotSupported;  // a maximum of scores is one of scaled scores for a positive scale only
   // units of work (paged_sched.cuh) in 32 bits
   const long long items = (long long)a.tokens * a.group / kChunkRows + a.requests;
-  if (items * a.kv_heads * ((long long)a.width * a.block_size / kChunkKeys + 2 + kChunkItem) >= INT_MAX) return cudaErrorNotSupported;
+  if (items * a.kv_heads * ((long long)a.width * a.block_size / kChunkKeys + 2 + kChunkItem) >= INT_MAX)
+    return cudaErrorNotSupported;
   ChunkArgs c{};
   c.a = a;
   c.box = paged_box(a.block_size, kChunkKeys);

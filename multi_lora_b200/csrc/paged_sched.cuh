@@ -298,9 +298,9 @@ __device__ __noinline__ void paged_zero_uncomputed(const PagedAttnArgs& p, int m
       computed = __any_sync(0xffffffffu, t >= r.q0 && t < r.q0 + r.qn && r.qn * p.group <= most);
     }
     if (computed) continue;
+    T* row = static_cast<T*>(p.out) + t * p.out_token;
     for (int e = lane; e < pieces; e += 32)
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + t * p.out_token + e / (p.dim / 8) * p.out_head + e % (p.dim / 8) * 8) =
-          make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(row + e / (p.dim / 8) * p.out_head + e % (p.dim / 8) * 8) = make_uint4(0, 0, 0, 0);
   }
 }
 

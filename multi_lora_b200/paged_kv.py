@@ -125,8 +125,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     view of its first columns lets a few short requests take a launch of lower
     latency. ``workspace``: :func:`attention_workspace`.
     Queries that see no key and rows past q_indptr[-1] give zeros; rows of a request with more new tokens than
-    ``max_q_len`` or with offsets that make no sense are reported in ``status`` and are zeros where they are not computed. What a query
-    does not see does not reach it, infinities and NaN included. bfloat16,
+    ``max_q_len`` or with offsets that make no sense are reported in ``status`` and are zeros where they are not
+    computed. What a query does not see does not reach it, infinities and NaN included. bfloat16,
     float16 or float32; head_dim a multiple of 8, at most 256; the tensor-core
     kernels take 16-bit caches with head_dim up to 128 and blocks of a multiple of 8 slots.
     """

@@ -21,8 +21,8 @@ class Launch:
 
 class FakeLib:
     def __init__(self, folder):
-        build.build_cuda_lib()
         objects = [build.OBJ / (src.stem + ".o") for src in sorted(build.CSRC.glob("*.cu"))]
+        build.build_cuda_lib(force=not all(o.exists() for o in objects))
         path = folder / "libmlora_fake.so"
         subprocess.run(["g++", "-std=c++17", "-O1", "-fPIC", "-shared", "-Wl,-Bsymbolic", "-I/usr/local/cuda/include",
                         str(build.ROOT / "tests" / "fake_cudart.cpp"), *map(str, objects), "-o", str(path)], check=True)

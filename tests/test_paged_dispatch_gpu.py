@@ -23,8 +23,9 @@ def step(dev, workspace):
     pr = attention_problem(dev, 81, [1, 2], [20, 30], 4, 2, 64, "bf16", 16)
     plan = P.PagedStepPlan.new(2, 3, dev)
     one, free = i32([1, 1], dev), i32([4, 5], dev)
-    probs, drafts, rows = torch.full((2, 8), 0.125, device=dev), torch.zeros(1, 1, dtype=torch.long, device=dev), i32([0, 2], dev)
-    u, head, tables, ticket, slots = torch.zeros(1, 1, device=dev), i32([0], dev), i32([[0, -1], [1, -1]], dev), i32([0], dev), i32([-1] * 3, dev)
+    probs, drafts = torch.full((2, 8), 0.125, device=dev), torch.zeros(1, 1, dtype=torch.long, device=dev)
+    rows, u = i32([0, 2], dev), torch.zeros(1, 1, device=dev)
+    head, tables, ticket, slots = (i32(x, dev) for x in ([0], [[0, -1], [1, -1]], [0], [-1] * 3))
     return [
         ("plan_paged_step", lambda: P.plan_paged_step(one, one, one, free, head, tables, plan, block_size=16,
                                                       workspace=ticket)),
