@@ -25,6 +25,7 @@ extern "C" {
 #define MLORA_BF16 0
 #define MLORA_F16 1
 #define MLORA_F32 2
+#define MLORA_E4M3 3 /* codes of a paged cache held in 8 bits; of nothing else */
 
 /* return codes */
 #define MLORA_OK 0
@@ -352,6 +353,58 @@ int mlora_write_paged_kv(const void* k, int64_t k_token_stride, int64_t k_head_s
                          const mlora_paged_cache_t* cache, const int32_t* slot_map, uint32_t* status, void* stream);
 
 /*
+ * Rotary positions. Pair i of a row at position t is turned by the angle 2 pi turns[i] t / 2^64:
+ *   (a, b) -> factor * (a cos - b sin, b cos + a sin)
+ * in fp32, rounded once. turns are frequencies in 2^-64 turns a position, so an angle modulo one turn is
+ * exact at every position. Pairs are elements (i, i + pairs) or, interleaved, (2i, 2i + 1); elements
+ * from 2 * pairs on are not turned.
+ */
+typedef struct mlora_rotary {
+  const int64_t* turns; /* [pairs], on the device */
+  int32_t pairs;
+  int32_t interleaved;
+  float factor;
+} mlora_rotary_t;
+
+/*
+ * out[t, h] = x[t, h] turned by positions[t] (int32 [tokens]). x, out: [tokens, heads, head_dim] of `dtype`, strides in
+ * elements; out may be x itself (same address and strides), otherwise they do not overlap.
+ * head_dim <= 512, 1 <= pairs <= head_dim / 2.
+ */
+int mlora_rotate(const void* x, int64_t x_token_stride, int64_t x_head_stride, int64_t tokens, int32_t heads,
+                 int32_t head_dim, const int32_t* positions, const mlora_rotary_t* rotary, void* out,
+                 int64_t out_token_stride, int64_t out_head_stride, int32_t dtype, void* stream);
+
+/*
+ * Scales of a cache of MLORA_E4M3 codes: what is held in block b, head h is code * k[b * k_block_stride +
+ * h * k_head_stride], the same for v; finite, not negative.
+ */
+typedef struct mlora_paged_scales {
+  float* k;
+  float* v;
+  int64_t k_block_stride, k_head_stride, v_block_stride, v_head_stride;
+} mlora_paged_scales_t;
+
+/*
+ * A step's new rows in one launch: cache[slot_map[t]] = (k[t] turned by positions[t], v[t]) for every t < tokens with
+ * slot_map[t] >= 0, and q_out = q turned (q_heads 0: no queries; q_out as out of mlora_rotate). rotary may be NULL where
+ * q_heads is 0: nothing is turned. q, k, v are of `dtype`, and so is the cache, or it holds MLORA_E4M3 codes and
+ * `scales` is not NULL. No two tokens may have the same slot. head_dim <= 512.
+ *
+ * Codes: the tokens of a block are consecutive, with consecutive slots (what a plan gives them), and the block has at
+ * most 2048 slots. Its scale becomes f = 2^k with the smallest k >= -100 for which the largest finite magnitude of the new
+ * rows is at most 448 * 2^k; where they begin behind the block's first slot, not less than the
+ * scale it has, and the rows before them are rounded again (to nearest even) if it grows. A code is the value over f
+ * rounded to nearest even, +-448 for infinities. Rows behind the new ones stay as they are.
+ */
+int mlora_append_paged_kv(const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t q_heads, void* q_out,
+                          int64_t q_out_token_stride, int64_t q_out_head_stride, const void* k, int64_t k_token_stride,
+                          int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                          int64_t tokens, int32_t dtype, const mlora_paged_cache_t* cache,
+                          const mlora_paged_scales_t* scales, const mlora_rotary_t* rotary, const int32_t* positions,
+                          const int32_t* slot_map, uint32_t* status, void* stream);
+
+/*
  * out[t, h] = softmax(scale * q[t, h] . K^T) V over the keys that token t of
  * request i sees: its position is pos = kv_lens[i] - (q_indptr[i+1] -
  * q_indptr[i]) + (t - q_indptr[i]), and it sees keys j <= pos, with window > 0
@@ -375,6 +428,18 @@ int mlora_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
                           void* out, int64_t out_token_stride, int64_t out_head_stride, void* workspace,
                           size_t workspace_bytes, uint32_t* status, void* stream);
 size_t mlora_paged_attention_workspace_bytes(void);
+
+/*
+ * The same over a cache of MLORA_E4M3 codes with scales: K and V are the values that the codes stand for, to
+ * fp32's accuracy (codes enter the products as they are, scales in fp32). `dtype` is that of q and out.
+ */
+int mlora_paged_attention_8bit(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,
+                               int32_t q_heads, int32_t dtype, const mlora_paged_cache_t* cache,
+                               const mlora_paged_scales_t* scales, const int32_t* block_tables,
+                               int64_t table_row_stride, int64_t max_blocks, const int32_t* kv_lens,
+                               const int32_t* q_indptr, int64_t requests, int64_t max_q_len, float scale,
+                               int32_t window, void* out, int64_t out_token_stride, int64_t out_head_stride,
+                               void* workspace, size_t workspace_bytes, uint32_t* status, void* stream);
 
 /*
  * Speculative verification. Request i has n + 1 rows row_indptr[i] ..

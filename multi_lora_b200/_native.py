@@ -77,6 +77,20 @@ class PagedCacheT(ctypes.Structure):
     ]
 
 
+class RotaryT(ctypes.Structure):
+    """ctypes mirror of ``mlora_rotary_t``."""
+
+    _fields_ = [("turns", ctypes.c_void_p), ("pairs", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("factor", ctypes.c_float)]
+
+
+class PagedScalesT(ctypes.Structure):
+    """ctypes mirror of ``mlora_paged_scales_t``."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                *[(f"{side}_{name}_stride", ctypes.c_int64) for side in "kv" for name in ("block", "head")]]
+
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
@@ -111,6 +125,13 @@ CAPI_SIGNATURES = {
     "mlora_write_paged_kv": (_I32, [_P, _I64, _I64, _P, _I64, _I64, _I64, ctypes.POINTER(PagedCacheT), _P, _P, _P]),
     "mlora_paged_attention": (_I32, [_P, _I64, _I64, _I64, _I32, ctypes.POINTER(PagedCacheT), _P, _I64, _I64, _P, _P,
                                      _I64, _I64, ctypes.c_float, _I32, _P, _I64, _I64, _P, ctypes.c_size_t, _P, _P]),
+    "mlora_paged_attention_8bit": (_I32, [_P, _I64, _I64, _I64, _I32, _I32, ctypes.POINTER(PagedCacheT),
+                                          ctypes.POINTER(PagedScalesT), _P, _I64, _I64, _P, _P, _I64, _I64, ctypes.c_float,
+                                          _I32, _P, _I64, _I64, _P, ctypes.c_size_t, _P, _P]),
+    "mlora_rotate": (_I32, [_P, _I64, _I64, _I64, _I32, _I32, _P, ctypes.POINTER(RotaryT), _P, _I64, _I64, _I32, _P]),
+    "mlora_append_paged_kv": (_I32, [_P, _I64, _I64, _I32, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I32,
+                                     ctypes.POINTER(PagedCacheT), ctypes.POINTER(PagedScalesT), ctypes.POINTER(RotaryT),
+                                     _P, _P, _P, _P]),
     "mlora_paged_attention_workspace_bytes": (ctypes.c_size_t, []),
     "mlora_verify_draft": (_I32, [_P, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I32, _P, _P, _P, _P, _I32, _P,
                                   _P]),

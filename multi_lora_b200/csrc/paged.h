@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "rotary.cuh"
+
 namespace mlora {
 
 struct PlanArgs {
@@ -46,6 +48,27 @@ struct PagedWriteArgs {
 // es: bytes per element; piece: bytes at once that rows and strides allow (32, 16, or es).
 cudaError_t launch_paged_write(const PagedWriteArgs& a, int es, int piece, cudaStream_t st, bool pdl);
 
+// Rows of q rotated into `out`, new keys rotated into the cache and values beside them (csrc/paged_append.cu).
+struct PagedAppendArgs {
+  RotaryAngles angles;
+  const void* q;
+  int64_t q_token, q_head;
+  void* out;
+  int64_t out_token, out_head;
+  PagedSide side[2];          // K and V; their heads are kv_heads (0: there is no cache, and no slot_map)
+  const int32_t* slot_map;
+  int tokens, q_heads, kv_heads, dim, block_size;
+  int64_t num_blocks;
+  // a cache of e4m3 codes: a scale for each block and head
+  float* scale[2];
+  int64_t scale_block[2], scale_head[2];
+  uint32_t* status;
+};
+constexpr int kAppendMaxBlock = 2048;  // slots of a block of codes, at most
+// vec: elements at once that rows, strides and pairs allow: 16 bytes, 8 or one element.
+cudaError_t launch_paged_append(const PagedAppendArgs& a, int dtype, int vec, cudaStream_t st, bool pdl);
+cudaError_t launch_paged_append_codes(const PagedAppendArgs& a, int dtype, int vec, cudaStream_t st, bool pdl);
+
 struct PagedAttnArgs {
   const void* q;
   int64_t q_token, q_head;
@@ -66,6 +89,10 @@ struct PagedAttnArgs {
   float scale;
   void* workspace;
   uint32_t* status;
+  // K and V are e4m3 codes where these are not null: a scale for each block and head
+  const float* k_scale;
+  const float* v_scale;
+  int64_t ks_block, ks_head, vs_block, vs_head;
 };
 // Any dtype, head_dim <= 256, block size and stride.
 cudaError_t launch_paged_attention_general(const PagedAttnArgs& a, int dtype, bool vec, cudaStream_t st, bool pdl);

@@ -1,5 +1,7 @@
 // Attention of new tokens over the paged cache, for every shape: any of the
-// three dtypes, head_dim up to 256, any block size and stride.
+// three dtypes, head_dim up to 256, any block size and stride; the cache of the queries'
+// dtype or of e4m3 codes with a scale for each block and head (a key's scale multiplies
+// its score, a value's the probability that goes to the product).
 //
 // Query t of request i (q_len_i new tokens, kv_len_i in the cache, its own
 // among them) sits at position pos = kv_len_i - q_len_i + t and sees keys
@@ -20,7 +22,10 @@
 // heads): 64 requests of 2000 keys 298 us, 3.5 TB/s of keys and values; one of 60000
 // keys 475 us; 512 new tokens 256 us. A warp a (token, query head) and a lane a key
 // took 2596, 72700 and 948 us.
+#include <cuda_fp8.h>
+
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "device.h"
@@ -34,7 +39,33 @@ constexpr int kAttnWarps = 8;
 constexpr int kAttnMaxDim = 256;
 constexpr int kAttnCtas = 8;  // of a cluster
 
-template <typename T, int V, int H>  // V elements a load of K and Q: 16 bytes, or one; H query heads
+// V e4m3 codes as they lie in memory.
+template <int V>
+struct CodeChunk {
+  typename RawBytes<V>::type u;
+  __device__ __forceinline__ void zero() { u = {}; }
+  __device__ __forceinline__ void ldcg(const unsigned char* p) { u = __ldcg(reinterpret_cast<const typename RawBytes<V>::type*>(p)); }
+  __device__ __forceinline__ void to_f(float* f) const {
+    unsigned char c[V];
+    memcpy(c, &u, V);
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 x = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((unsigned short)(c[i] | c[i + 1] << 8), __NV_E4M3)));
+      f[i] = x.x;
+      f[i + 1] = x.y;
+    }
+  }
+};
+template <>
+struct CodeChunk<1> {
+  unsigned char u;
+  __device__ __forceinline__ void zero() { u = 0; }
+  __device__ __forceinline__ void ldcg(const unsigned char* p) { u = __ldcg(p); }
+  __device__ __forceinline__ void to_f(float* f) const { f[0] = __half2float(__half(__nv_cvt_fp8_to_halfraw(u, __NV_E4M3))); }
+};
+
+// V elements a load of K and Q: 16 bytes of T, or one; H query heads; CODES: K and V are codes with scales
+template <typename T, int V, int H, bool CODES>
 __global__ void __launch_bounds__(kAttnWarps * 32) paged_attention_general_kernel(const PagedAttnArgs p, int ctas) {
   __shared__ __align__(16) float s_q[H][kAttnMaxDim];
   __shared__ __align__(16) float s_acc[kAttnWarps][H][kAttnMaxDim];
@@ -83,8 +114,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32) paged_attention_general_kerne
   }
   __syncthreads();
   const int32_t* table = p.tables + lo * p.table_stride;
-  const T* kbase = static_cast<const T*>(p.k) + g * p.k_head;
-  const T* vbase = static_cast<const T*>(p.v) + g * p.v_head;
+  using E = typename std::conditional<CODES, unsigned char, T>::type;  // an element of the cache
+  using Piece = typename std::conditional<CODES, CodeChunk<V>, Chunk<T, V>>::type;
+  const E* kbase = static_cast<const E*>(p.k) + g * p.k_head;
+  const E* vbase = static_cast<const E*>(p.v) + g * p.v_head;
   constexpr int kCols = kAttnMaxDim / 128;  // runs of 128 columns, four of each a lane
   float acc[H][kCols][4], m[H], l[H];
 #pragma unroll
@@ -109,13 +142,18 @@ __global__ void __launch_bounds__(kAttnWarps * 32) paged_attention_general_kerne
         block = -1;
       }
     }
+    float k_scale = 0.f, v_scale = 0.f;
+    if (CODES && block >= 0) {
+      k_scale = __ldcg(p.k_scale + block * p.ks_block + g * p.ks_head);
+      v_scale = __ldcg(p.v_scale + block * p.vs_block + g * p.vs_head);
+    }
     float s[H];
 #pragma unroll
     for (int h = 0; h < H; ++h) s[h] = 0.f;
     constexpr int AT_ONCE = 4;
 #pragma unroll
     for (int i0 = 0; i0 < 8; i0 += AT_ONCE) {  // four keys in each of these steps
-      const T* row[AT_ONCE];
+      const E* row[AT_ONCE];
       float d[AT_ONCE][H];
 #pragma unroll
       for (int i = 0; i < AT_ONCE; ++i) {
@@ -126,7 +164,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) paged_attention_general_kerne
         for (int h = 0; h < H; ++h) d[i][h] = 0.f;
       }
       for (int c = (lane & 7) * V; c < p.dim; c += 8 * V) {
-        Chunk<T, V> ch[AT_ONCE];
+        Piece ch[AT_ONCE];
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
           ch[i].zero();
@@ -158,6 +196,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) paged_attention_general_kerne
     float w[H];
 #pragma unroll
     for (int h = 0; h < H; ++h) {
+      if (CODES) s[h] *= k_scale;
       if (!real) s[h] = -INFINITY;
       float top = s[h];
 #pragma unroll
@@ -166,6 +205,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) paged_attention_general_kerne
       const float fix = m_new == -INFINITY ? 1.f : expf(m[h] - m_new);
       w[h] = s[h] == -INFINITY ? 0.f : expf(s[h] - m_new);
       l[h] = fmaf(l[h], fix, w[h]);
+      if (CODES) w[h] *= v_scale;  // of the value that it is multiplied by
       m[h] = m_new;
       if (fix != 1.f) {
 #pragma unroll
@@ -180,12 +220,23 @@ __global__ void __launch_bounds__(kAttnWarps * 32) paged_attention_general_kerne
 #pragma unroll
       for (int i = 0; i < AT_ONCE; ++i) {
         const int from = i * 8 + (i0 >> 2), b = __shfl_sync(0xffffffffu, block, from), o = __shfl_sync(0xffffffffu, off, from);
-        const T* src = vbase + b * p.v_block + o * p.v_slot + lane * 4;
+        const E* src = vbase + b * p.v_block + o * p.v_slot + lane * 4;
 #pragma unroll
         for (int c = 0; c < kCols; ++c) {
           v[i][c][0] = v[i][c][1] = v[i][c][2] = v[i][c][3] = 0.f;
           if (b >= 0 && c * 128 + lane * 4 < p.dim) {
-            if constexpr (V > 1 && sizeof(T) == 4) {
+            if constexpr (CODES && V > 1) {
+              CodeChunk<4> u;
+              u.ldcg(src + c * 128);
+              u.to_f(v[i][c]);
+            } else if constexpr (CODES) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                CodeChunk<1> u;
+                u.ldcg(src + c * 128 + e);
+                u.to_f(&v[i][c][e]);
+              }
+            } else if constexpr (V > 1 && sizeof(T) == 4) {
               const float4 u = __ldcg(reinterpret_cast<const float4*>(src + c * 128));
               v[i][c][0] = u.x;
               v[i][c][1] = u.y;
@@ -199,7 +250,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) paged_attention_general_kerne
               v[i][c][3] = Pack2<T>::hi(u.y);
             } else {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) v[i][c][e] = ldcg_f(src + c * 128 + e);
+              for (int e = 0; e < 4; ++e) v[i][c][e] = ldcg_f(static_cast<const T*>(src) + c * 128 + e);
             }
           }
         }
@@ -299,7 +350,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) paged_attention_general_kerne
 }
 
 namespace {
-template <typename T, int V, int H>
+template <typename T, int V, int H, bool CODES>
 cudaError_t general_h(const PagedAttnArgs& a, cudaStream_t st, bool pdl) {
   const int64_t items = (int64_t)a.tokens * a.kv_heads * ((a.group + H - 1) / H);
   // A cluster an item where there are fewer items than SMs, if the tables have room for enough keys; the
@@ -321,13 +372,17 @@ cudaError_t general_h(const PagedAttnArgs& a, cudaStream_t st, bool pdl) {
   at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, paged_attention_general_kernel<T, V, H>, a, ctas);
+  return cudaLaunchKernelEx(&cfg, paged_attention_general_kernel<T, V, H, CODES>, a, ctas);
+}
+template <typename T, bool CODES>
+cudaError_t general_c(const PagedAttnArgs& a, bool vec, cudaStream_t st, bool pdl) {
+  constexpr int V = 16 / (int)sizeof(T);
+  if (a.group == 1) return vec ? general_h<T, V, 1, CODES>(a, st, pdl) : general_h<T, 1, 1, CODES>(a, st, pdl);
+  return vec ? general_h<T, V, 4, CODES>(a, st, pdl) : general_h<T, 1, 4, CODES>(a, st, pdl);
 }
 template <typename T>
 cudaError_t general_t(const PagedAttnArgs& a, bool vec, cudaStream_t st, bool pdl) {
-  constexpr int V = 16 / (int)sizeof(T);
-  if (a.group == 1) return vec ? general_h<T, V, 1>(a, st, pdl) : general_h<T, 1, 1>(a, st, pdl);
-  return vec ? general_h<T, V, 4>(a, st, pdl) : general_h<T, 1, 4>(a, st, pdl);
+  return a.k_scale != nullptr ? general_c<T, true>(a, vec, st, pdl) : general_c<T, false>(a, vec, st, pdl);
 }
 }  // namespace
 

@@ -35,9 +35,9 @@ bool pieces(const void* p, int es, int64_t a, int64_t b, int64_t c = 0, int byte
   return reinterpret_cast<uintptr_t>(p) % bytes == 0 && a % v == 0 && b % v == 0 && c % v == 0;
 }
 
-int check_cache(const mlora_paged_cache_t* c) {
+int check_cache(const mlora_paged_cache_t* c, bool codes = false) {
   if (c == nullptr) return refuse(MLORA_ERR_INVALID_ARGUMENT, "cache is NULL");
-  if (bytes_of(c->dtype) == 0) return refuse(MLORA_ERR_UNSUPPORTED_DTYPE, "unsupported dtype code %d", c->dtype);
+  if (codes ? c->dtype != MLORA_E4M3 : bytes_of(c->dtype) == 0) return refuse(MLORA_ERR_UNSUPPORTED_DTYPE, "unsupported dtype code %d", c->dtype);
   if (c->block_size < 1 || c->kv_heads < 1 || c->head_dim < 1 || c->num_blocks < 0)
     return refuse(MLORA_ERR_INVALID_ARGUMENT, "cache of %lld blocks of %d slots, %d heads of %d",
                   (long long)c->num_blocks, c->block_size, c->kv_heads, c->head_dim);
@@ -50,6 +50,55 @@ int check_cache(const mlora_paged_cache_t* c) {
       c->v_slot_stride < 0 || c->v_head_stride < 0)
     return refuse(MLORA_ERR_INVALID_ARGUMENT, "negative cache stride");
   return MLORA_OK;
+}
+
+int check_scales(const mlora_paged_scales_t* s) {
+  if (s->k == nullptr || s->v == nullptr) return refuse(MLORA_ERR_INVALID_ARGUMENT, "k / v of the scales are NULL");
+  if (s->k_block_stride < 0 || s->k_head_stride < 0 || s->v_block_stride < 0 || s->v_head_stride < 0)
+    return refuse(MLORA_ERR_INVALID_ARGUMENT, "negative stride of the scales");
+  return MLORA_OK;
+}
+
+int check_rotary(const mlora_rotary_t* r, const int32_t* positions, int32_t head_dim) {
+  if (r->pairs < 1 || r->pairs > head_dim / 2)
+    return refuse(MLORA_ERR_INVALID_ARGUMENT, "%d pairs of a head_dim of %d", r->pairs, head_dim);
+  if (r->turns == nullptr || positions == nullptr) return refuse(MLORA_ERR_INVALID_ARGUMENT, "turns / positions is NULL");
+  return MLORA_OK;
+}
+
+constexpr int32_t kAppendMaxDim = 512;
+
+// Rows that are written: they must not overlap one another.
+bool rows_apart(int64_t tokens, int64_t token_stride, int64_t heads, int64_t head_stride, int64_t dim) {
+  return token_stride >= 0 && head_stride >= 0 && (tokens <= 1 || token_stride >= dim) && (heads <= 1 || head_stride >= dim);
+}
+
+// What is checked and set alike for a rotation and an append.
+int append_common(mlora::PagedAppendArgs& a, const mlora_rotary_t* rotary, const int32_t* positions, int32_t head_dim) {
+  if (head_dim < 1 || head_dim > kAppendMaxDim)
+    return refuse(MLORA_ERR_INVALID_ARGUMENT, "head_dim %d: 1 to %d are rotated", head_dim, kAppendMaxDim);
+  a.dim = head_dim;
+  if (rotary == nullptr) return MLORA_OK;
+  if (int rc = check_rotary(rotary, positions, head_dim)) return rc;
+  a.angles = {rotary->turns, positions, rotary->pairs, rotary->interleaved != 0, rotary->factor};
+  return MLORA_OK;
+}
+
+// Elements at once that the rows of q, out, k and v allow: 16 bytes, 8 or one element.
+int append_vec(const mlora::PagedAppendArgs& a, int es, bool codes) {
+  for (int bytes = 16; bytes >= 8; bytes /= 2) {
+    const int v = bytes / es;
+    if (v < 2 || a.dim % v != 0 || a.angles.pairs % v != 0) continue;
+    if (a.q_heads > 0 && !(pieces(a.q, es, a.q_token, a.q_head, 0, bytes) && pieces(a.out, es, a.out_token, a.out_head, 0, bytes)))
+      continue;
+    bool ok = true;
+    for (const mlora::PagedSide& s : a.side)
+      if (a.kv_heads > 0)
+        ok = ok && pieces(s.src, es, s.src_token, s.src_head, 0, bytes) &&
+             pieces(s.dst, codes ? 1 : es, s.block, s.slot, s.head, codes ? v : bytes);
+    if (ok) return v;
+  }
+  return 1;
 }
 
 }  // namespace
@@ -144,16 +193,113 @@ int mlora_write_paged_kv(const void* k, int64_t k_token_stride, int64_t k_head_s
                   "cache write launch");
 }
 
+int mlora_rotate(const void* x, int64_t x_token_stride, int64_t x_head_stride, int64_t tokens, int32_t heads,
+                 int32_t head_dim, const int32_t* positions, const mlora_rotary_t* rotary, void* out,
+                 int64_t out_token_stride, int64_t out_head_stride, int32_t dtype, void* stream) {
+  report_error(0, "");
+  const int es = bytes_of(dtype);
+  if (es == 0) return refuse(MLORA_ERR_UNSUPPORTED_DTYPE, "unsupported dtype code %d", dtype);
+  if (tokens < 0 || heads < 0 || tokens * (heads > 0 ? heads : 1) > INT32_MAX)
+    return refuse(MLORA_ERR_INVALID_ARGUMENT, "%lld tokens of %d heads", (long long)tokens, heads);
+  if (rotary == nullptr) return refuse(MLORA_ERR_INVALID_ARGUMENT, "rotary is NULL");
+  if (head_dim < 1 || head_dim > kAppendMaxDim || rotary->pairs < 1 || rotary->pairs > head_dim / 2)
+    return refuse(MLORA_ERR_INVALID_ARGUMENT, "%d pairs of a head_dim of %d: head_dim 2 to %d", rotary->pairs, head_dim,
+                  kAppendMaxDim);
+  if (x_token_stride < 0 || x_head_stride < 0 || !rows_apart(tokens, out_token_stride, heads, out_head_stride, head_dim))
+    return refuse(MLORA_ERR_INVALID_ARGUMENT, "x / out stride");
+  if (tokens == 0 || heads == 0) return MLORA_OK;
+  if (x == nullptr || out == nullptr) return refuse(MLORA_ERR_INVALID_ARGUMENT, "x / out is NULL");
+  mlora::PagedAppendArgs a{};
+  if (int rc = append_common(a, rotary, positions, head_dim)) return rc;
+  a.q = x;
+  a.q_token = x_token_stride;
+  a.q_head = x_head_stride;
+  a.out = out;
+  a.out_token = out_token_stride;
+  a.out_head = out_head_stride;
+  a.tokens = (int)tokens;
+  a.q_heads = heads;
+  a.block_size = 1;
+  return launched(mlora::launch_paged_append(a, dtype, append_vec(a, es, false), (cudaStream_t)stream, mlora_get_pdl() != 0),
+                  "rotation launch");
+}
+
+int mlora_append_paged_kv(const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t q_heads, void* q_out,
+                          int64_t q_out_token_stride, int64_t q_out_head_stride, const void* k, int64_t k_token_stride,
+                          int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                          int64_t tokens, int32_t dtype, const mlora_paged_cache_t* cache,
+                          const mlora_paged_scales_t* scales, const mlora_rotary_t* rotary, const int32_t* positions,
+                          const int32_t* slot_map, uint32_t* status, void* stream) {
+  report_error(0, "");
+  const int es = bytes_of(dtype);
+  if (es == 0) return refuse(MLORA_ERR_UNSUPPORTED_DTYPE, "unsupported dtype code %d", dtype);
+  const bool codes = scales != nullptr;
+  if (int rc = check_cache(cache, codes)) return rc;
+  const mlora_paged_cache_t& c = *cache;
+  if (codes) {
+    if (c.num_blocks > 0)
+      if (int rc = check_scales(scales)) return rc;
+    if (c.block_size > mlora::kAppendMaxBlock)
+      return refuse(MLORA_ERR_INVALID_ARGUMENT, "blocks of %d codes: at most %d are appended to", c.block_size, mlora::kAppendMaxBlock);
+  } else if (c.dtype != dtype) {
+    return refuse(MLORA_ERR_INVALID_ARGUMENT, "rows of dtype %d for a cache of %d", dtype, c.dtype);
+  }
+  if (tokens < 0 || q_heads < 0 || q_heads > INT32_MAX / 4 || c.kv_heads > INT32_MAX / 4 ||
+      tokens * ((int64_t)q_heads + 2 * c.kv_heads) > INT32_MAX)
+    return refuse(MLORA_ERR_INVALID_ARGUMENT, "%lld tokens of %d and %d heads", (long long)tokens, q_heads, c.kv_heads);
+  if (q_heads > 0 && rotary == nullptr) return refuse(MLORA_ERR_INVALID_ARGUMENT, "queries without rotary");
+  if (k_token_stride < 0 || k_head_stride < 0 || v_token_stride < 0 || v_head_stride < 0)
+    return refuse(MLORA_ERR_INVALID_ARGUMENT, "negative k / v stride");
+  if (q_heads > 0 && (q_token_stride < 0 || q_head_stride < 0 ||
+                      !rows_apart(tokens, q_out_token_stride, q_heads, q_out_head_stride, c.head_dim)))
+    return refuse(MLORA_ERR_INVALID_ARGUMENT, "q / q_out stride");
+  if (c.head_dim > kAppendMaxDim || (rotary != nullptr && (rotary->pairs < 1 || rotary->pairs > c.head_dim / 2)))
+    return refuse(MLORA_ERR_INVALID_ARGUMENT, "%d pairs of a head_dim of %d: at most %d", rotary != nullptr ? rotary->pairs : 0,
+                  c.head_dim, kAppendMaxDim);
+  if (tokens == 0) return MLORA_OK;
+  if (k == nullptr || v == nullptr || slot_map == nullptr || (q_heads > 0 && (q == nullptr || q_out == nullptr)))
+    return refuse(MLORA_ERR_INVALID_ARGUMENT, "q / q_out / k / v / slot_map is NULL");
+  mlora::PagedAppendArgs a{};
+  if (int rc = append_common(a, rotary, positions, c.head_dim)) return rc;
+  a.q = q;
+  a.q_token = q_token_stride;
+  a.q_head = q_head_stride;
+  a.out = q_out;
+  a.out_token = q_out_token_stride;
+  a.out_head = q_out_head_stride;
+  a.side[0] = {k, k_token_stride, k_head_stride, c.k, c.k_block_stride, c.k_slot_stride, c.k_head_stride};
+  a.side[1] = {v, v_token_stride, v_head_stride, c.v, c.v_block_stride, c.v_slot_stride, c.v_head_stride};
+  a.slot_map = slot_map;
+  a.tokens = (int)tokens;
+  a.q_heads = q_heads;
+  a.kv_heads = c.kv_heads;
+  a.block_size = c.block_size;
+  a.num_blocks = c.num_blocks;
+  a.status = status;
+  const int vec = append_vec(a, es, codes);
+  const cudaStream_t st = (cudaStream_t)stream;
+  const bool pdl = mlora_get_pdl() != 0;
+  if (!codes) return launched(mlora::launch_paged_append(a, dtype, vec, st, pdl), "append launch");
+  a.scale[0] = scales->k;
+  a.scale[1] = scales->v;
+  a.scale_block[0] = scales->k_block_stride;
+  a.scale_block[1] = scales->v_block_stride;
+  a.scale_head[0] = scales->k_head_stride;
+  a.scale_head[1] = scales->v_head_stride;
+  return launched(mlora::launch_paged_append_codes(a, dtype, vec, st, pdl), "append launch");
+}
+
 size_t mlora_paged_attention_workspace_bytes(void) { return (size_t)64 << 20; }
 
-int mlora_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,
-                          int32_t q_heads, const mlora_paged_cache_t* cache, const int32_t* block_tables,
-                          int64_t table_row_stride, int64_t max_blocks, const int32_t* kv_lens,
-                          const int32_t* q_indptr, int64_t requests, int64_t max_q_len, float scale, int32_t window,
-                          void* out, int64_t out_token_stride, int64_t out_head_stride, void* workspace,
-                          size_t workspace_bytes, uint32_t* status, void* stream) {
-  report_error(0, "");
-  if (int rc = check_cache(cache)) return rc;
+}  // extern "C"
+
+namespace {
+
+int attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int32_t q_heads, int32_t dtype,
+              const mlora_paged_cache_t* cache, const mlora_paged_scales_t* scales, const int32_t* block_tables,
+              int64_t table_row_stride, int64_t max_blocks, const int32_t* kv_lens, const int32_t* q_indptr,
+              int64_t requests, int64_t max_q_len, float scale, int32_t window, void* out, int64_t out_token_stride,
+              int64_t out_head_stride, void* workspace, size_t workspace_bytes, uint32_t* status, void* stream) {
   const mlora_paged_cache_t& c = *cache;
   if (c.head_dim > 256 || c.head_dim % 8 != 0)
     return refuse(MLORA_ERR_INVALID_ARGUMENT, "head_dim %d: a multiple of 8, at most 256, is wanted", c.head_dim);
@@ -212,21 +358,64 @@ int mlora_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
   a.scale = scale;
   a.workspace = workspace;
   a.status = status;
-  const int es = bytes_of(c.dtype);
+  const int es = bytes_of(dtype), ces = scales != nullptr ? 1 : es;
+  if (scales != nullptr) {
+    a.k_scale = scales->k;
+    a.v_scale = scales->v;
+    a.ks_block = scales->k_block_stride;
+    a.ks_head = scales->k_head_stride;
+    a.vs_block = scales->v_block_stride;
+    a.vs_head = scales->v_head_stride;
+  }
   const bool vec = pieces(q, es, q_token_stride, q_head_stride) && pieces(out, es, out_token_stride, out_head_stride) &&
-                   pieces(c.k, es, c.k_block_stride, c.k_slot_stride, c.k_head_stride) &&
-                   pieces(c.v, es, c.v_block_stride, c.v_slot_stride, c.v_head_stride);
+                   pieces(c.k, ces, c.k_block_stride, c.k_slot_stride, c.k_head_stride) &&
+                   pieces(c.v, ces, c.v_block_stride, c.v_slot_stride, c.v_head_stride);
   const bool pdl = mlora_get_pdl() != 0;
   const cudaStream_t st = (cudaStream_t)stream;
   // rows (tokens x group) times group below 2^32: where division by multiplication is exact
   const bool rows_ok = (int64_t)a.tokens * a.group * a.group < (1ll << 32);
-  if (vec && es == 2 && rows_ok) {
+  if (vec && es == 2 && rows_ok && scales == nullptr) {
     const bool few = (int64_t)a.max_q_len * (q_heads / c.kv_heads) <= mlora::kDecodeMaxRows;
-    const cudaError_t e = few ? mlora::launch_paged_attention_decode(a, c.dtype, st, pdl)
-                              : mlora::launch_paged_attention_chunk(a, c.dtype, st, pdl);
+    const cudaError_t e = few ? mlora::launch_paged_attention_decode(a, dtype, st, pdl)
+                              : mlora::launch_paged_attention_chunk(a, dtype, st, pdl);
     if (e != cudaErrorNotSupported) return launched(e, "paged attention launch");
   }
-  return launched(mlora::launch_paged_attention_general(a, c.dtype, vec, st, pdl), "paged attention launch");
+  return launched(mlora::launch_paged_attention_general(a, dtype, vec, st, pdl), "paged attention launch");
+}
+
+}  // namespace
+
+extern "C" {
+
+int mlora_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,
+                          int32_t q_heads, const mlora_paged_cache_t* cache, const int32_t* block_tables,
+                          int64_t table_row_stride, int64_t max_blocks, const int32_t* kv_lens,
+                          const int32_t* q_indptr, int64_t requests, int64_t max_q_len, float scale, int32_t window,
+                          void* out, int64_t out_token_stride, int64_t out_head_stride, void* workspace,
+                          size_t workspace_bytes, uint32_t* status, void* stream) {
+  report_error(0, "");
+  if (int rc = check_cache(cache)) return rc;
+  return attention(q, q_token_stride, q_head_stride, tokens, q_heads, cache->dtype, cache, nullptr, block_tables,
+                   table_row_stride, max_blocks, kv_lens, q_indptr, requests, max_q_len, scale, window, out,
+                   out_token_stride, out_head_stride, workspace, workspace_bytes, status, stream);
+}
+
+int mlora_paged_attention_8bit(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,
+                               int32_t q_heads, int32_t dtype, const mlora_paged_cache_t* cache,
+                               const mlora_paged_scales_t* scales, const int32_t* block_tables,
+                               int64_t table_row_stride, int64_t max_blocks, const int32_t* kv_lens,
+                               const int32_t* q_indptr, int64_t requests, int64_t max_q_len, float scale,
+                               int32_t window, void* out, int64_t out_token_stride, int64_t out_head_stride,
+                               void* workspace, size_t workspace_bytes, uint32_t* status, void* stream) {
+  report_error(0, "");
+  if (bytes_of(dtype) == 0) return refuse(MLORA_ERR_UNSUPPORTED_DTYPE, "unsupported dtype code %d", dtype);
+  if (int rc = check_cache(cache, true)) return rc;
+  if (scales == nullptr) return refuse(MLORA_ERR_INVALID_ARGUMENT, "scales is NULL");
+  if (cache->num_blocks > 0)
+    if (int rc = check_scales(scales)) return rc;
+  return attention(q, q_token_stride, q_head_stride, tokens, q_heads, dtype, cache, scales, block_tables,
+                   table_row_stride, max_blocks, kv_lens, q_indptr, requests, max_q_len, scale, window, out,
+                   out_token_stride, out_head_stride, workspace, workspace_bytes, status, stream);
 }
 
 int mlora_verify_draft(const void* target, int64_t rows, int64_t vocab, int64_t target_row_stride, const void* draft,

@@ -1,0 +1,129 @@
+// Rotary positions: what the kernels that rotate share.
+//
+// Pair i of a row at position t is turned by the angle t * f_i. f_i is held as a whole
+// number of 2^-64 turns, so that the product modulo one turn is a 64-bit integer multiplication,
+// exact at every position; its upper 32 bits as a float of half turns go to sincospif
+// (1.5e-9 radians from the truncation, 2^-24 relative from the float).
+#pragma once
+
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace mlora {
+
+struct RotaryAngles {
+  const int64_t* turns;      // [pairs], null: nothing is rotated
+  const int32_t* positions;  // [tokens]
+  int pairs;                 // half of the dimensions that are rotated
+  int interleaved;           // pairs (2i, 2i + 1), or (i, i + pairs)
+  float factor;              // of both outputs
+};
+
+// {cos, sin} * factor
+__device__ __forceinline__ float2 rotary_turn(int64_t turns, int position, float factor) {
+  const uint64_t angle = (uint64_t)turns * (uint64_t)(int64_t)position;
+  const float half_turns = (float)(int32_t)(uint32_t)((angle + 0x80000000ull) >> 32) * 0x1p-31f;
+  float s, c;
+  sincospif(half_turns, &s, &c);
+  return make_float2(c * factor, s * factor);
+}
+
+// V elements of T as they lie in memory.
+template <int BYTES>
+struct RawBytes;
+template <>
+struct RawBytes<16> {
+  using type = uint4;
+};
+template <>
+struct RawBytes<8> {
+  using type = uint2;
+};
+template <>
+struct RawBytes<4> {
+  using type = uint32_t;
+};
+template <>
+struct RawBytes<1> {
+  using type = unsigned char;
+};
+template <>
+struct RawBytes<2> {
+  using type = unsigned short;
+};
+
+template <typename T, int V>
+struct Vec {
+  using Raw = typename RawBytes<V * (int)sizeof(T)>::type;
+  union {
+    Raw raw;
+    T at[V];
+  };
+  __device__ __forceinline__ Vec() : raw() {}
+  __device__ __forceinline__ void load(const T* p) { raw = __ldcg(reinterpret_cast<const Raw*>(p)); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Raw*>(p) = raw; }
+  __device__ __forceinline__ void to_f(float (&f)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = Num<T>::to_f(at[i]);
+  }
+  __device__ __forceinline__ void from_f(const float (&f)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) at[i] = Num<T>::from_f(f[i]);
+  }
+};
+
+// A row of `dim` elements is worked on in units of two vectors of V: those of V pairs (V divides
+// their number), or 2 V elements that are not rotated. Where unit u lies: its vectors' first elements
+// (the second one may lie past the row: dim behind the pairs is a multiple of V only), the first pair.
+struct RotaryUnit {
+  int e0, e1, pair;
+  bool turned, both;
+};
+__device__ __forceinline__ RotaryUnit rotary_unit(const RotaryAngles& a, bool rotated, int dim, int V, int u) {
+  RotaryUnit r;
+  r.pair = u * V;
+  r.turned = rotated && r.pair < a.pairs;
+  if (r.turned && !a.interleaved) {
+    r.e0 = r.pair;
+    r.e1 = r.pair + a.pairs;
+  } else {
+    r.e0 = 2 * r.pair;
+    r.e1 = r.e0 + V;
+  }
+  r.both = r.e1 < dim;
+  return r;
+}
+
+// The two vectors of a rotated unit, `cs` the {cos, sin} of its pairs.
+template <int V>
+__device__ __forceinline__ void rotary_apply(bool interleaved, const float2* cs, float (&a)[V], float (&b)[V]) {
+  float2 t[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) t[i] = cs[i];
+  if (interleaved) {
+    if constexpr (V == 1) {
+      const float x = a[0] * t[0].x - b[0] * t[0].y;
+      b[0] = b[0] * t[0].x + a[0] * t[0].y;
+      a[0] = x;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; i += 2) {
+        const float x = a[i] * t[i / 2].x - a[i + 1] * t[i / 2].y, y = b[i] * t[V / 2 + i / 2].x - b[i + 1] * t[V / 2 + i / 2].y;
+        a[i + 1] = a[i + 1] * t[i / 2].x + a[i] * t[i / 2].y;
+        b[i + 1] = b[i + 1] * t[V / 2 + i / 2].x + b[i] * t[V / 2 + i / 2].y;
+        a[i] = x;
+        b[i] = y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float x = a[i] * t[i].x - b[i] * t[i].y;
+      b[i] = b[i] * t[i].x + a[i] * t[i].y;
+      a[i] = x;
+    }
+  }
+}
+
+}  // namespace mlora

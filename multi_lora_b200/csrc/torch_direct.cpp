@@ -68,5 +68,8 @@ PYBIND11_MODULE(_mlora_direct, m) {
   def("plan_paged_step", either(&mlora_torch::plan_paged_step, "mlora::plan_paged_step", false));
   def("write_paged_kv", either(&mlora_torch::write_paged_kv, "mlora::write_paged_kv", false));
   def("paged_attention", either(&mlora_torch::paged_attention, "mlora::paged_attention", true));
+  def("paged_attention_8bit", either(&mlora_torch::paged_attention_8bit, "mlora::paged_attention_8bit", true));
+  def("rotate", either(&mlora_torch::rotate, "mlora::rotate", true));
+  def("append_paged_kv", either(&mlora_torch::append_paged_kv, "mlora::append_paged_kv", false));
   def("verify_draft", either(&mlora_torch::verify_draft, "mlora::verify_draft", false));
 }

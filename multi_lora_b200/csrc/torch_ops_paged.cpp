@@ -57,7 +57,7 @@ int64_t table_rows(const at::Tensor& t, int64_t requests, const at::Device& dev)
   return requests > 1 ? t.stride(0) : t.size(1);
 }
 
-mlora_paged_cache_t cache_of(const at::Tensor& k, const at::Tensor& v, const at::Device& dev) {
+mlora_paged_cache_t cache_of(const at::Tensor& k, const at::Tensor& v, const at::Device& dev, bool codes = false) {
   on_device(k, "k_cache", dev);
   on_device(v, "v_cache", dev);
   TORCH_CHECK(k.dim() == 4 && v.sizes() == k.sizes(),
@@ -72,7 +72,8 @@ mlora_paged_cache_t cache_of(const at::Tensor& k, const at::Tensor& v, const at:
   c.block_size = (int32_t)k.size(1);
   c.kv_heads = (int32_t)k.size(2);
   c.head_dim = (int32_t)k.size(3);
-  c.dtype = code(k.scalar_type());
+  if (codes) TORCH_CHECK(k.scalar_type() == at::kFloat8_e4m3fn, "mlora: a cache with scales must be float8_e4m3fn (got ", k.scalar_type(), ")");
+  c.dtype = codes ? MLORA_E4M3 : code(k.scalar_type());
   c.k_block_stride = k.stride(0);
   c.k_slot_stride = k.stride(1);
   c.k_head_stride = k.stride(2);
@@ -80,6 +81,85 @@ mlora_paged_cache_t cache_of(const at::Tensor& k, const at::Tensor& v, const at:
   c.v_slot_stride = v.stride(1);
   c.v_head_stride = v.stride(2);
   return c;
+}
+
+mlora_paged_scales_t scales_of(const at::Tensor& k, const at::Tensor& v, const mlora_paged_cache_t& c, const at::Device& dev) {
+  on_device(k, "k_scales", dev);
+  on_device(v, "v_scales", dev);
+  for (const at::Tensor* t : {&k, &v})
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == c.num_blocks && t->size(1) == c.kv_heads,
+                "mlora: k_scales and v_scales must be float32 [", c.num_blocks, ", ", c.kv_heads, "] (got ", t->scalar_type(),
+                " ", t->sizes(), ")");
+  return {k.data_ptr<float>(), v.data_ptr<float>(), k.stride(0), k.stride(1), v.stride(0), v.stride(1)};
+}
+
+// Frequencies for rows of head_dim elements at `positions`.
+mlora_rotary_t rotary_of(const at::Tensor& turns, bool interleaved, double factor, const at::Device& dev) {
+  on_device(turns, "rotary.turns", dev);
+  TORCH_CHECK(turns.scalar_type() == at::kLong && turns.dim() == 1 && turns.is_contiguous() && turns.numel() <= INT32_MAX,
+              "mlora: rotary.turns must be a contiguous int64 [pairs] (got ", turns.scalar_type(), " ", turns.sizes(), ")");
+  return {turns.data_ptr<int64_t>(), (int32_t)turns.numel(), interleaved, (float)factor};
+}
+
+// x [tokens, heads, head_dim] rotated to `out`: that tensor, or a new one.
+at::Tensor rotated_like(const at::Tensor& x, const c10::optional<at::Tensor>& out, const char* name, const at::Device& dev) {
+  if (!out.has_value()) return at::detail::empty_cuda(x.sizes(), x.scalar_type(), dev, c10::nullopt);
+  on_device(*out, name, dev);
+  TORCH_CHECK(out->sizes() == x.sizes() && out->scalar_type() == x.scalar_type() && out->stride(2) == 1, "mlora: ", name,
+              " must be like its input with unit stride in head_dim");
+  if (out->data_ptr() == x.data_ptr())
+    for (int64_t d = 0; d < 2; ++d)
+      TORCH_CHECK(x.size(d) <= 1 || x.stride(d) == out->stride(d), "mlora: ", name, " overlaps its input in another layout");
+  return *out;
+}
+
+at::Tensor attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                     const at::Tensor* k_scales, const at::Tensor* v_scales, const at::Tensor& block_tables,
+                     const at::Tensor& kv_lens, const at::Tensor& q_indptr, int64_t max_q_len, double scale,
+                     int64_t window, const c10::optional<at::Tensor>& out_, const at::Tensor& workspace,
+                     const c10::optional<at::Tensor>& status) {
+  const at::Device dev = q.device();
+  on_device(q, "q", dev);
+  const bool codes = k_scales != nullptr;
+  const mlora_paged_cache_t c = cache_of(k_cache, v_cache, dev, codes);
+  TORCH_CHECK(q.dim() == 3 && q.size(2) == c.head_dim && q.stride(2) == 1,
+              "mlora: q must be [tokens, q_heads, ", c.head_dim, "] with unit stride in head_dim (got ", q.sizes(), ")");
+  const int32_t dtype = code(q.scalar_type());
+  TORCH_CHECK(codes || q.scalar_type() == k_cache.scalar_type(), "mlora: q and the cache must share a dtype");
+  TORCH_CHECK(q.size(1) >= 1 && q.size(1) % c.kv_heads == 0, "mlora: ", q.size(1), " query heads over ", c.kv_heads,
+              " key heads");
+  const int64_t r = kv_lens.numel();
+  const int64_t rows = table_rows(block_tables, r, dev);
+  TORCH_CHECK(window >= 0 && window <= INT32_MAX, "mlora: window ", window, " invalid");
+  on_device(workspace, "workspace", dev);
+  TORCH_CHECK(workspace.is_contiguous(), "mlora: workspace must be contiguous");
+  const c10::cuda::CUDAGuard guard(dev);
+  at::Tensor out;
+  if (out_.has_value()) {
+    out = *out_;
+    on_device(out, "out", dev);
+    TORCH_CHECK(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.stride(2) == 1,
+                "mlora: out must be like q with unit stride in head_dim");
+  } else {
+    out = at::detail::empty_cuda(q.sizes(), q.scalar_type(), dev, c10::nullopt);
+  }
+  const int64_t qt = stride_of(q, 0, c.head_dim), qh = stride_of(q, 1, c.head_dim), ot = stride_of(out, 0, c.head_dim),
+                oh = stride_of(out, 1, c.head_dim);
+  const int32_t* tables = block_tables.numel() > 0 ? block_tables.data_ptr<int32_t>() : nullptr;
+  const int32_t *lens = i32(kv_lens, "kv_lens", r, dev), *indptr = i32(q_indptr, "q_indptr", r + 1, dev);
+  const auto stream = at::cuda::getCurrentCUDAStream().stream();
+  if (codes) {
+    const mlora_paged_scales_t f = scales_of(*k_scales, *v_scales, c, dev);
+    done(mlora_paged_attention_8bit(q.data_ptr(), qt, qh, q.size(0), (int32_t)q.size(1), dtype, &c, &f, tables, rows,
+                                    block_tables.size(1), lens, indptr, r, max_q_len, (float)scale, (int32_t)window,
+                                    out.data_ptr(), ot, oh, workspace.data_ptr(), (size_t)workspace.nbytes(),
+                                    status_word(status, dev), stream));
+  } else {
+    done(mlora_paged_attention(q.data_ptr(), qt, qh, q.size(0), (int32_t)q.size(1), &c, tables, rows, block_tables.size(1),
+                               lens, indptr, r, max_q_len, (float)scale, (int32_t)window, out.data_ptr(), ot, oh,
+                               workspace.data_ptr(), (size_t)workspace.nbytes(), status_word(status, dev), stream));
+  }
+  return out;
 }
 
 }  // namespace
@@ -130,38 +210,90 @@ void write_paged_kv(const at::Tensor& k, const at::Tensor& v, at::Tensor k_cache
 
 at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
                            const at::Tensor& block_tables, const at::Tensor& kv_lens, const at::Tensor& q_indptr,
-                           int64_t max_q_len, double scale, int64_t window, const c10::optional<at::Tensor>& out_,
+                           int64_t max_q_len, double scale, int64_t window, const c10::optional<at::Tensor>& out,
                            const at::Tensor& workspace, const c10::optional<at::Tensor>& status) {
-  const at::Device dev = q.device();
-  on_device(q, "q", dev);
-  const mlora_paged_cache_t c = cache_of(k_cache, v_cache, dev);
-  TORCH_CHECK(q.dim() == 3 && q.size(2) == c.head_dim && q.stride(2) == 1,
-              "mlora: q must be [tokens, q_heads, ", c.head_dim, "] with unit stride in head_dim (got ", q.sizes(), ")");
-  TORCH_CHECK(q.scalar_type() == k_cache.scalar_type(), "mlora: q and the cache must share a dtype");
-  TORCH_CHECK(q.size(1) >= 1 && q.size(1) % c.kv_heads == 0, "mlora: ", q.size(1), " query heads over ", c.kv_heads,
-              " key heads");
-  const int64_t r = kv_lens.numel();
-  const int64_t rows = table_rows(block_tables, r, dev);
-  TORCH_CHECK(window >= 0 && window <= INT32_MAX, "mlora: window ", window, " invalid");
-  on_device(workspace, "workspace", dev);
-  TORCH_CHECK(workspace.is_contiguous(), "mlora: workspace must be contiguous");
+  return attention(q, k_cache, v_cache, nullptr, nullptr, block_tables, kv_lens, q_indptr, max_q_len, scale, window, out,
+                   workspace, status);
+}
+
+at::Tensor paged_attention_8bit(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                const at::Tensor& k_scales, const at::Tensor& v_scales, const at::Tensor& block_tables,
+                                const at::Tensor& kv_lens, const at::Tensor& q_indptr, int64_t max_q_len, double scale,
+                                int64_t window, const c10::optional<at::Tensor>& out, const at::Tensor& workspace,
+                                const c10::optional<at::Tensor>& status) {
+  return attention(q, k_cache, v_cache, &k_scales, &v_scales, block_tables, kv_lens, q_indptr, max_q_len, scale, window,
+                   out, workspace, status);
+}
+
+at::Tensor rotate(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& turns, bool interleaved,
+                  double factor, const c10::optional<at::Tensor>& out_) {
+  const at::Device dev = x.device();
+  on_device(x, "x", dev);
+  TORCH_CHECK(x.dim() == 3 && x.stride(2) == 1, "mlora: x must be [tokens, heads, head_dim] with unit stride in head_dim (got ",
+              x.sizes(), ")");
+  TORCH_CHECK(x.size(1) <= INT32_MAX && x.size(2) <= INT32_MAX, "mlora: x of ", x.sizes(), " is too large");
+  const mlora_rotary_t r = rotary_of(turns, interleaved, factor, dev);
+  const int32_t dtype = code(x.scalar_type());
   const c10::cuda::CUDAGuard guard(dev);
-  at::Tensor out;
-  if (out_.has_value()) {
-    out = *out_;
-    on_device(out, "out", dev);
-    TORCH_CHECK(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.stride(2) == 1,
-                "mlora: out must be like q with unit stride in head_dim");
-  } else {
-    out = at::detail::empty_cuda(q.sizes(), q.scalar_type(), dev, c10::nullopt);
+  at::Tensor out = rotated_like(x, out_, "out", dev);
+  done(mlora_rotate(x.data_ptr(), stride_of(x, 0, x.size(2)), stride_of(x, 1, x.size(2)), x.size(0), (int32_t)x.size(1),
+                    (int32_t)x.size(2), i32(positions, "positions", x.size(0), dev), &r, out.data_ptr(),
+                    stride_of(out, 0, x.size(2)), stride_of(out, 1, x.size(2)), dtype,
+                    at::cuda::getCurrentCUDAStream().stream()));
+  return out;
+}
+
+at::Tensor append_paged_kv(const at::Tensor& k, const at::Tensor& v, at::Tensor k_cache, at::Tensor v_cache,
+                           const at::Tensor& slot_map, const c10::optional<at::Tensor>& positions,
+                           const c10::optional<at::Tensor>& turns, bool interleaved, double factor,
+                           const c10::optional<at::Tensor>& q, const c10::optional<at::Tensor>& q_out,
+                           const c10::optional<at::Tensor>& k_scales, const c10::optional<at::Tensor>& v_scales,
+                           const c10::optional<at::Tensor>& status) {
+  const at::Device dev = k.device();
+  on_device(k, "k", dev);
+  on_device(v, "v", dev);
+  TORCH_CHECK(k_scales.has_value() == v_scales.has_value(), "mlora: k_scales and v_scales come together");
+  const bool codes = k_scales.has_value();
+  const mlora_paged_cache_t c = cache_of(k_cache, v_cache, dev, codes);
+  TORCH_CHECK(k.dim() == 3 && k.size(1) == c.kv_heads && k.size(2) == c.head_dim && v.sizes() == k.sizes(),
+              "mlora: k and v must be [tokens, ", c.kv_heads, ", ", c.head_dim, "] (got ", k.sizes(), " and ", v.sizes(),
+              ")");
+  TORCH_CHECK(v.scalar_type() == k.scalar_type() && (codes || k.scalar_type() == k_cache.scalar_type()),
+              "mlora: k, v and the cache must share a dtype (or the cache have scales)");
+  TORCH_CHECK(k.stride(2) == 1 && v.stride(2) == 1, "mlora: k and v must have unit stride in head_dim");
+  const int32_t dtype = code(k.scalar_type());
+  const int64_t n = k.size(0), dim = c.head_dim;
+  const c10::cuda::CUDAGuard guard(dev);
+  mlora_rotary_t r{};
+  const int32_t* at_positions = nullptr;
+  TORCH_CHECK(positions.has_value() == turns.has_value(), "mlora: rotary and positions come together");
+  if (turns.has_value()) {
+    r = rotary_of(*turns, interleaved, factor, dev);
+    at_positions = i32(*positions, "positions", n, dev);
   }
-  done(mlora_paged_attention(q.data_ptr(), stride_of(q, 0, c.head_dim), stride_of(q, 1, c.head_dim), q.size(0), (int32_t)q.size(1), &c,
-                             block_tables.numel() > 0 ? block_tables.data_ptr<int32_t>() : nullptr, rows,
-                             block_tables.size(1), i32(kv_lens, "kv_lens", r, dev),
-                             i32(q_indptr, "q_indptr", r + 1, dev), r, max_q_len, (float)scale, (int32_t)window,
-                             out.data_ptr(), stride_of(out, 0, c.head_dim), stride_of(out, 1, c.head_dim), workspace.data_ptr(),
-                             (size_t)workspace.nbytes(), status_word(status, dev),
-                             at::cuda::getCurrentCUDAStream().stream()));
+  mlora_paged_scales_t f{};
+  if (codes) f = scales_of(*k_scales, *v_scales, c, dev);
+  at::Tensor out;
+  int64_t qt = 0, qh = 0, ot = 0, oh = 0;
+  if (q.has_value()) {
+    on_device(*q, "q", dev);
+    TORCH_CHECK(turns.has_value(), "mlora: q is there to be rotated: rotary is missing");
+    TORCH_CHECK(q->dim() == 3 && q->size(0) == n && q->size(2) == dim && q->stride(2) == 1 && q->size(1) <= INT32_MAX,
+                "mlora: q must be [", n, ", q_heads, ", dim, "] with unit stride in head_dim (got ", q->sizes(), ")");
+    TORCH_CHECK(q->scalar_type() == k.scalar_type(), "mlora: q and k must share a dtype");
+    out = rotated_like(*q, q_out, "q_out", dev);
+    qt = stride_of(*q, 0, dim);
+    qh = stride_of(*q, 1, dim);
+    ot = stride_of(out, 0, dim);
+    oh = stride_of(out, 1, dim);
+  } else {
+    TORCH_CHECK(!q_out.has_value(), "mlora: q_out without q");
+  }
+  done(mlora_append_paged_kv(q.has_value() ? q->data_ptr() : nullptr, qt, qh, q.has_value() ? (int32_t)q->size(1) : 0,
+                             q.has_value() ? out.data_ptr() : nullptr, ot, oh, k.data_ptr(), k.stride(0), k.stride(1),
+                             v.data_ptr(), v.stride(0), v.stride(1), n, dtype, &c, codes ? &f : nullptr,
+                             turns.has_value() ? &r : nullptr, at_positions, i32(slot_map, "slot_map", n, dev),
+                             status_word(status, dev), at::cuda::getCurrentCUDAStream().stream()));
   return out;
 }
 
@@ -218,6 +350,15 @@ TORCH_LIBRARY_FRAGMENT(mlora, m) {
       "int max_q_len, float scale, int window, Tensor(a!)? out, Tensor(b!) workspace, Tensor(c!)? status=None) "
       "-> Tensor");
   m.def(
+      "paged_attention_8bit(Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scales, Tensor v_scales, Tensor block_tables, "
+      "Tensor kv_lens, Tensor q_indptr, int max_q_len, float scale, int window, Tensor(a!)? out, Tensor(b!) workspace, "
+      "Tensor(c!)? status=None) -> Tensor");
+  m.def("rotate(Tensor x, Tensor positions, Tensor turns, bool interleaved, float factor, Tensor(a!)? out=None) -> Tensor");
+  m.def(
+      "append_paged_kv(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor slot_map, Tensor? positions, "
+      "Tensor? turns, bool interleaved, float factor, Tensor? q, Tensor(c!)? q_out, Tensor(d!)? k_scales, "
+      "Tensor(e!)? v_scales, Tensor(f!)? status=None) -> Tensor");
+  m.def(
       "verify_draft(Tensor target_probs, Tensor? draft_probs, Tensor draft_tokens, Tensor row_indptr, Tensor accept_u, "
       "Tensor sample_u, Tensor(a!)? status=None) -> (Tensor, Tensor)");
 }
@@ -226,5 +367,8 @@ TORCH_LIBRARY_IMPL(mlora, CUDA, m) {
   m.impl("plan_paged_step", &mlora_torch::plan_paged_step);
   m.impl("write_paged_kv", &mlora_torch::write_paged_kv);
   m.impl("paged_attention", &mlora_torch::paged_attention);
+  m.impl("paged_attention_8bit", &mlora_torch::paged_attention_8bit);
+  m.impl("rotate", &mlora_torch::rotate);
+  m.impl("append_paged_kv", &mlora_torch::append_paged_kv);
   m.impl("verify_draft", &mlora_torch::verify_draft);
 }

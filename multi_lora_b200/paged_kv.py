@@ -8,6 +8,7 @@ may be captured in a CUDA graph:
 
     plan_paged_step   lengths -> blocks, slots, positions, q_indptr
     write_paged_kv    new keys and values into their slots
+    append_paged_kv   the same with the keys (and the queries) rotated on the way; into 8 bits too
     paged_attention   the new tokens' queries over the cache
 
 ``q_indptr`` has the layout of ``KernelInputMetaData.seg_indptr`` with one
@@ -23,6 +24,7 @@ from typing import Dict, List, Optional, Sequence
 import torch
 
 from multi_lora_b200 import _native
+from multi_lora_b200.rotary import RotaryPositions, rotate
 
 # what paged_attention asks of a workspace, whatever the shapes (mlora_paged_attention_workspace_bytes)
 ATTENTION_WORKSPACE_BYTES = 64 << 20
@@ -111,10 +113,39 @@ def write_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
     _native.direct("write_paged_kv")(k, v, k_cache, v_cache, slot_map, status)
 
 
+def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    slot_map: torch.Tensor, *, positions: Optional[torch.Tensor] = None,
+                    rotary: Optional[RotaryPositions] = None, q: Optional[torch.Tensor] = None,
+                    q_out: Optional[torch.Tensor] = None, k_scales: Optional[torch.Tensor] = None,
+                    v_scales: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """:func:`write_paged_kv` with the step's rotation on the way, in one launch: keys go to the cache rotated by
+    ``rotary`` at ``positions`` (int32 [tokens]), values as they are, and the rotated queries ``q`` are
+    returned (in ``q_out`` where it is given, which may be ``q`` itself). Without ``rotary`` nothing is rotated.
+
+    A cache of float8_e4m3fn holds codes: slot s of block b, head h stands for ``code * scales[b, h]``, with
+    ``k_scales`` and ``v_scales`` float32 [num_blocks, kv_heads] of any strides. New rows give their block the scale 2^k of
+    the smallest k (not below -100) for which 448 * 2^k holds their largest finite magnitude. Where they begin behind a block's first slot it
+    is not less than the scale that the block has, and if it grows, the rows before them are rounded again. Infinities are
+    held as +-448 scales. The tokens of a block must be consecutive rows with consecutive slots, what a plan gives
+    them, and blocks have at most 2048 slots. bfloat16, float16 or float32 rows; head_dim up to 512.
+    """
+    _need_cuda(k, "append_paged_kv")
+    if q is not None and rotary is not None and q.requires_grad and torch.is_grad_enabled():
+        # a graph is asked for: the queries go through an operator whose result is part of it, as paged_attention's is
+        out = rotate(q, positions, rotary, out=q_out)
+        append_paged_kv(k, v, k_cache, v_cache, slot_map, positions=positions, rotary=rotary, k_scales=k_scales,
+                        v_scales=v_scales, status=status)
+        return out
+    turns, interleaved, factor = (None, False, 1.0) if rotary is None else (rotary.turns, rotary.interleaved, rotary.factor)
+    return _native.direct("append_paged_kv")(k, v, k_cache, v_cache, slot_map, positions, turns, interleaved, factor, q,
+                                             q_out, k_scales, v_scales, status)
+
+
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
                     kv_lens: torch.Tensor, q_indptr: torch.Tensor, *, max_q_len: int, workspace: torch.Tensor,
                     scale: Optional[float] = None, window: int = 0, out: Optional[torch.Tensor] = None,
-                    status: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    status: Optional[torch.Tensor] = None, k_scales: Optional[torch.Tensor] = None,
+                    v_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of each request's new tokens over its cached keys (its own new ones among them).
 
     q [tokens, q_heads, head_dim]: request i's are rows q_indptr[i] ..
@@ -128,11 +159,20 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``max_q_len`` or with offsets that make no sense are reported in ``status`` and are zeros where they are not
     computed. What a query does not see does not reach it, infinities and NaN included. bfloat16,
     float16 or float32; head_dim a multiple of 8, at most 256; the tensor-core
-    kernels take 16-bit caches with head_dim up to 128 and blocks of a multiple of 8 slots.
+    kernels take 16-bit queries with head_dim up to 128 and blocks of a multiple of 8 slots.
+
+    The cache is of q's dtype, or of float8_e4m3fn codes with ``k_scales`` and ``v_scales`` (:func:`append_paged_kv`; any
+    finite scales that are not negative). Codes are exact in the products and scales multiply in float32, so the result is
+    that of the values which the codes stand for.
     """
     _need_cuda(q, "paged_attention")
     if scale is None:
         scale = q.shape[-1] ** -0.5
+    if k_scales is not None or v_scales is not None:
+        if k_scales is None or v_scales is None:
+            raise ValueError("paged_attention: k_scales and v_scales come together")
+        return _native.direct("paged_attention_8bit")(q, k_cache, v_cache, k_scales, v_scales, block_tables, kv_lens,
+                                                      q_indptr, max_q_len, scale, window, out, workspace, status)
     return _native.direct("paged_attention")(q, k_cache, v_cache, block_tables, kv_lens, q_indptr, max_q_len, scale, window,
                                          out, workspace, status)
 
@@ -145,8 +185,12 @@ class PagedKVCache:
         o = cache.attend(layer, q, max_q_len)
         cache.advance(num_new)                  # tokens that stay (all of them, or those that verification kept)
 
+        q = cache.append(layer, q, k, v, rotary)   # instead of write: q and k rotated at the plan's positions
+
     Blocks are stored head by head ([num_blocks, kv_heads, block_size, head_dim]),
     so that what one head's attention reads of a block is one piece of memory.
+    With ``dtype`` float8_e4m3fn they hold codes, with a scale for each block and head
+    (:func:`append_paged_kv`): half the memory and half the traffic of 16 bits.
     """
 
     def __init__(self, *, layers: int, num_blocks: int, block_size: int, kv_heads: int, head_dim: int,
@@ -155,6 +199,9 @@ class PagedKVCache:
             raise ValueError("PagedKVCache: every size must be positive")
         shape = (layers, 2, num_blocks, kv_heads, block_size, head_dim)
         self.storage = torch.zeros(shape, dtype=dtype, device=device)
+        # of a cache of codes: [layers, 2, num_blocks, kv_heads]
+        self.scale_storage = (torch.zeros(shape[:4], dtype=torch.float32, device=device)
+                              if dtype == torch.float8_e4m3fn else None)
         self.block_size, self.num_blocks, self.device = block_size, num_blocks, torch.device(device)
 
         def i32(*shape, value=0):
@@ -176,6 +223,10 @@ class PagedKVCache:
         """(k_cache, v_cache) of a layer, [num_blocks, block_size, kv_heads, head_dim] views."""
         k, v = self.storage[index]
         return k.transpose(1, 2), v.transpose(1, 2)
+
+    def scales(self, index: int):
+        """(k_scales, v_scales) of a layer, [num_blocks, kv_heads] views; (None, None) where blocks hold no codes."""
+        return (None, None) if self.scale_storage is None else tuple(self.scale_storage[index])
 
     def plan(self, new_lens: torch.Tensor, max_tokens: int) -> PagedStepPlan:
         """Plan a step of ``new_lens`` (int32 [max_requests]) tokens, ``max_tokens`` rows in all; blocks are taken
@@ -200,14 +251,28 @@ class PagedKVCache:
         return self._plan
 
     def write(self, index: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        if self.scale_storage is not None:
+            k_scales, v_scales = self.scales(index)
+            append_paged_kv(k, v, *self.layer(index), self.plan_now.slot_map, k_scales=k_scales, v_scales=v_scales,
+                            status=self.status)
+            return
         write_paged_kv(k, v, *self.layer(index), self.plan_now.slot_map, status=self.status)
+
+    def append(self, index: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rotary: RotaryPositions, *,
+               q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Rotated keys and values into the cache; the rotated queries (:func:`append_paged_kv`)."""
+        plan = self.plan_now
+        k_scales, v_scales = self.scales(index)
+        return append_paged_kv(k, v, *self.layer(index), plan.slot_map, positions=plan.positions, rotary=rotary, q=q,
+                               q_out=q_out, k_scales=k_scales, v_scales=v_scales, status=self.status)
 
     def attend(self, index: int, q: torch.Tensor, max_q_len: int, *, scale: Optional[float] = None, window: int = 0,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
         plan = self.plan_now
+        k_scales, v_scales = self.scales(index)
         return paged_attention(q, *self.layer(index), self.block_tables, plan.kv_lens, plan.q_indptr,
                                max_q_len=max_q_len, workspace=self._workspace, scale=scale, window=window, out=out,
-                               status=self.status)
+                               status=self.status, k_scales=k_scales, v_scales=v_scales)
 
     def advance(self, num_new: torch.Tensor) -> None:
         """``num_new`` (int32 [max_requests]) of the planned tokens stay in the cache; slots behind them are planned

@@ -62,6 +62,52 @@ def attention(q, k_cache, v_cache, tables, kv_lens, q_indptr, scale, window=0):
     return out, mean, spread, seen
 
 
+def rotate(x, positions, radians, interleaved=False, factor=1.0):
+    """x [T, H, D] with pair i of row t turned by positions[t] * radians[i], each pair as a complex number."""
+    out = np.array(x, np.float64)
+    for i, f in enumerate(radians):
+        a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + len(radians))
+        turn = factor * np.exp(1j * np.asarray(positions, np.float64) * f)[:, None]
+        z = (out[..., a] + 1j * out[..., b]) * turn
+        out[..., a], out[..., b] = z.real, z.imag
+    return out
+
+
+def round_e4m3(x):
+    """The nearest of e4m3's values (even on a tie): 1.mmm * 2^e for e from -6 to 8, multiples of 2^-9 below; at most 448."""
+    x = np.asarray(x, np.float64)
+    with np.errstate(divide="ignore", invalid="ignore"):
+        e = np.clip(np.floor(np.log2(np.abs(x))), -6, 8)
+    step = 2.0 ** (np.where(np.isfinite(e), e, 8) - 3)
+    return np.where(np.isnan(x), np.nan, np.clip(np.round(np.clip(x, -448, 448) / step) * step, -448, 448))
+
+
+def append_codes(values, scales, rows, slots, block):
+    """New rows [T, H, D] into a cache of codes: (code values, scales, codes before they are rounded), a block at a time.
+
+    values [num_blocks, block, H, D] are what the codes stand for over their scale, scales [num_blocks, H]."""
+    values, scales, rows = (np.array(t, np.float64) for t in (values, scales, rows))
+    exact = values.copy()
+    slots = np.asarray(slots)
+    for b in np.unique(slots[slots >= 0] // block):
+        mine = np.flatnonzero((slots >= 0) & (slots // block == b))
+        first = int((slots[mine] % block).min())
+        size = np.where(np.isfinite(rows[mine]), np.abs(rows[mine]), 0.0).max((0, 2))
+        for h, most in enumerate(size):
+            k = -100
+            while 448.0 * 2.0 ** k < most:
+                k += 1
+            old, f = scales[b, h], 2.0 ** k
+            if first > 0:
+                f = max(f, old)
+                values[b, :first, h] = round_e4m3(values[b, :first, h] * (old / f))
+                exact[b, :first, h] = values[b, :first, h]
+            scales[b, h] = f
+            exact[b, slots[mine] % block, h] = rows[mine, h] / f
+            values[b, slots[mine] % block, h] = round_e4m3(rows[mine, h] / f)
+    return values, scales, exact
+
+
 def verify(target, draft, draft_tokens, row_indptr, accept_u, sample_u):
     """Emitted tokens (-1 behind the last) and their number, with Python's whole numbers for the 40-bit weights.
 
