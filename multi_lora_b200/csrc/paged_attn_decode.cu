@@ -42,13 +42,14 @@
 #include "device.h"
 #include "kernels.h"
 #include "mma.cuh"
+#include "paged_codes.cuh"
 #include "paged_sched.cuh"
 #include "paged_tma.h"
 #include "tc.cuh"
 
 namespace mlora {
 
-constexpr int kDecTile = 64;  // keys a stage
+constexpr int kDecTile = 64;  // keys a stage; of codes kCodeTile
 constexpr int kDecJoin = 3;   // joining a piece costs about three tiles
 constexpr int kDecItem = 3;   // and so does an item besides its tiles
 using DecodeSplit = PagedSplit<kDecJoin, kDecItem>;
@@ -59,13 +60,14 @@ struct DecodeArgs {
   int box;     // rows of a TMA box
 };
 
-template <int D>
+template <int D, bool CODES>
 struct DecodeCfg {
+  static constexpr int kTile = CODES ? kCodeTile : kDecTile;  // the same bytes
   static constexpr int KG = 4;                    // key groups: warps that share 16 rows
   static constexpr int kWarps = KG;
   static constexpr int kThreads = kWarps * 32 + 32;
   static constexpr int kPerSm = 2;
-  static constexpr int kSide = kDecTile * D * 2;  // bytes of K (or V) in a stage
+  static constexpr int kSide = kTile * D * (CODES ? 1 : 2);  // bytes of K (or V) in a stage
   static constexpr int kStages = 96 * 1024 / (2 * kSide);
   static constexpr int kRowF = D + 4;             // floats of a row in the merge buffer
   static constexpr int kMerge = 16 * kRowF * 4;
@@ -77,29 +79,31 @@ struct DecodeItem {
   int req, head, q0, qn, kv, first, tile0, n;
 };
 
+template <int TILE>
 __device__ __forceinline__ void decode_request(const PagedAttnArgs& p, DecodeItem& it, int req, const PagedRequest& r) {
   it.req = req;
   it.q0 = r.q0;
   it.qn = r.qn;
   it.kv = r.kv;
   it.first = paged_first_key(p, r.kv - r.qn);
-  it.tile0 = it.first / kDecTile;
-  it.n = r.qn > 0 && r.qn * p.group <= kDecodeMaxRows ? max(1, (r.kv + kDecTile - 1) / kDecTile - it.tile0) : 0;
+  it.tile0 = it.first / TILE;
+  it.n = r.qn > 0 && r.qn * p.group <= kDecodeMaxRows ? max(1, (r.kv + TILE - 1) / TILE - it.tile0) : 0;
 }
 
 constexpr int kFewCtas = 8;    // CTAs of a cluster
 constexpr int kFewItems = 16;  // (request, key head)s that clusters are launched for, at most
 constexpr int kFewKeys = 4096; // keys that the block tables have room for, at most
 
-template <typename T, int D, bool CLUSTER>
-__global__ void __launch_bounds__(DecodeCfg<D>::kThreads, DecodeCfg<D>::kPerSm)
+template <typename T, int D, bool CLUSTER, bool CODES>
+__global__ void __launch_bounds__(DecodeCfg<D, CODES>::kThreads, DecodeCfg<D, CODES>::kPerSm)
 paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
-  using C = DecodeCfg<D>;
+  using C = DecodeCfg<D, CODES>;
   constexpr float kUp = Num<T>::is_bf16 ? 0.f : 15.f;  // P is taken times 2^kUp
-  constexpr int NS = C::kStages, SIDE = C::kSide, HALF = kDecTile * 128;
+  constexpr int NS = C::kStages, SIDE = C::kSide, TILE = C::kTile, HALF = kDecTile * 128;
   extern __shared__ __align__(1024) unsigned char s_raw[];
   __shared__ __align__(8) uint64_t full[NS], empty[NS];
   __shared__ float s_m[C::kWarps][16], s_l[C::kWarps][16];
+  __shared__ __align__(16) float s_scale[CODES ? NS : 1][2][TILE / 8];  // of K and V, for each eight keys of a stage
   __shared__ int s_last;
   __shared__ PagedPlace s_place;  // of the item that is being joined
   const PagedAttnArgs& p = args.a;
@@ -134,7 +138,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     // rows beyond what the caller said: reported, and where they do not fit the tile not computed
     if (report && r.qn > p.max_q_len) flag_error(p.status, kErrLength);
     DecodeItem x;
-    decode_request(p, x, i, r);
+    decode_request<TILE>(p, x, i, r);
     skipped |= r.odd || (r.qn > 0 && x.n == 0);
     return x.n > 0 ? (x.n + kDecItem) * p.kv_heads : 0;
   };
@@ -155,7 +159,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     const int item = blockIdx.x / kFewCtas;
     req = item / p.kv_heads;
     units(req, 0, 1, found);
-    decode_request(p, it, req, found);
+    decode_request<TILE>(p, it, req, found);
     if (it.n == 0) {  // the same in the whole cluster
       if (warp == C::kWarps) zero_others();
       return;
@@ -173,7 +177,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       if (warp == C::kWarps) zero_others();
       return;
     }
-    decode_request(p, it, req, found);
+    decode_request<TILE>(p, it, req, found);
     it.head = (cur.pos - before) / (it.n + kDecItem);
     cur.unit = cur.pos - before - it.head * (it.n + kDecItem);
   }
@@ -182,7 +186,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       it.head = 0;
       PagedRequest r;
       const int i = paged_next(p, it.req, kDecodeMaxRows, r);
-      if (i < p.requests) decode_request(p, it, i, r);
+      if (i < p.requests) decode_request<TILE>(p, it, i, r);
     }
   };
   if (!CLUSTER && cur.begin(it.n)) next_item();
@@ -199,26 +203,63 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
   bool ok = true;
 
   if (warp == C::kWarps) {  // ---- producer ----
-    const int boxes = kDecTile / args.box, jobs = boxes * (D / 64) * 2;
-    const int b = lane % boxes, half = (lane / boxes) % (D / 64), side = lane / (boxes * (D / 64));
+    constexpr int HALVES = CODES ? 1 : D / 64;
+    const int boxes = TILE / args.box, jobs = boxes * HALVES * 2;
+    const int b = lane % boxes, half = (lane / boxes) % HALVES, side = lane / (boxes * HALVES);
     int stage = 0, round = 0;
     while (take()) {
       const int32_t* table = p.tables + it.req * p.table_stride;
-      for (int k = 0; k < cur.len; ++k) {
-        const int j = (it.tile0 + cur.tile + k) * kDecTile + b * args.box;
-        int block = (int)p.num_blocks, off = 0;  // out of range: zeros
+      auto box_key = [&](int k) { return (it.tile0 + cur.tile + k) * TILE + b * args.box; };
+      auto lookup = [&](int k, int& block, int& off) {
+        const int j = box_key(k);
+        block = (int)p.num_blocks;  // out of range: zeros
+        off = 0;
         if (lane < jobs && j < it.kv && j + args.box > it.first) {
           const int e = __ldcg(table + j / p.block_size);
           off = j % p.block_size;
           if (e >= 0 && e < p.num_blocks) block = e;
           else flag_error(p.status, kErrKvRange);
         }
+      };
+      // Codes: a tile's scales hang on its table entries, two loads one after the other; the entries are
+      // asked for two tiles ahead and the scales one, so that a tile waits for neither.
+      int next[2] = {(int)p.num_blocks, (int)p.num_blocks}, next_off[2] = {0, 0};
+      float next_scale = 0.f;
+      auto scale_of = [&](int block) {
+        if (block >= p.num_blocks) return 0.f;
+        return __ldcg(side == 0 ? p.k_scale + block * p.ks_block + it.head * p.ks_head
+                                : p.v_scale + block * p.vs_block + it.head * p.vs_head);
+      };
+      if constexpr (CODES) {
+        if (cur.len > 0) lookup(0, next[0], next_off[0]);
+        if (cur.len > 1) lookup(1, next[1], next_off[1]);
+        next_scale = scale_of(next[0]);
+      }
+      for (int k = 0; k < cur.len; ++k) {
+        int block, off;
+        float scale = 0.f;
+        if constexpr (CODES) {
+          block = next[0];
+          off = next_off[0];
+          scale = next_scale;
+          next[0] = next[1];
+          next_off[0] = next_off[1];
+          next_scale = k + 1 < cur.len ? scale_of(next[0]) : 0.f;
+          if (k + 2 < cur.len) lookup(k + 2, next[1], next_off[1]);
+        } else {
+          lookup(k, block, off);
+        }
         if (round > 0) ok = __all_sync(0xffffffffu, ok && mbar_poll(&empty[stage], (round - 1) & 1, p.status));
         if (ok) {
+          if constexpr (CODES) {
+            if (lane < jobs)
+              for (int i = 0; i < args.box / 8; ++i) s_scale[stage][side][b * (args.box / 8) + i] = scale;
+            __syncwarp();
+          }
           if (lane == 0) mbar_arrive_expect_tx(&full[stage], 2 * SIDE);
           __syncwarp();
           if (lane < jobs)
-            tma_load_4d(smem + stage * 2 * SIDE + side * SIDE + half * HALF + b * args.box * 128,
+            tma_load_4d(smem + stage * 2 * SIDE + side * SIDE + half * HALF + b * args.box * (CODES ? D : 128),
                         side == 0 ? &args.k_map : &args.v_map, half * 64, off, it.head, block, &full[stage]);
         }
         if (++stage == NS) {
@@ -248,17 +289,30 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
   constexpr int PART = 16 * (D + 2);  // floats of a piece: sums, maxima, totals
   // Q fragments: rows lane / 4 and + 8, columns (lane % 4) * 2 (+ 8) of each 16
   uint32_t qf[D / 16][4];
+  float row_f[2] = {sl, sl};  // of codes: what the products of the lane's rows are multiplied by
   auto load_q = [&](const DecodeItem& x) {
+    if constexpr (CODES) {
+      auto row = [&](int e) {
+        const int r = (lane >> 2) + e * 8, t = paged_token(p, r);
+        return r < x.qn * group ? static_cast<const T*>(p.q) + (int64_t)(x.q0 + t) * p.q_token +
+                                      (int64_t)(x.head * group + r - t * group) * p.q_head
+                                : nullptr;
+      };
+      code_queries<T, D>(p.dim, row, qf, row_f);
+      row_f[0] *= sl;
+      row_f[1] *= sl;
+    } else {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = (lane >> 2) + e * 8, t = paged_token(p, r);
-      const T* src = static_cast<const T*>(p.q) + (int64_t)(x.q0 + t) * p.q_token +
-                     (int64_t)(x.head * group + r - t * group) * p.q_head + (lane & 3) * 2;
-      const bool real = r < x.qn * group;
+      for (int e = 0; e < 2; ++e) {
+        const int r = (lane >> 2) + e * 8, t = paged_token(p, r);
+        const T* src = static_cast<const T*>(p.q) + (int64_t)(x.q0 + t) * p.q_token +
+                       (int64_t)(x.head * group + r - t * group) * p.q_head + (lane & 3) * 2;
+        const bool real = r < x.qn * group;
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        qf[k][e] = real && k * 16 < p.dim ? __ldcg(reinterpret_cast<const unsigned int*>(src + k * 16)) : 0u;
-        qf[k][2 + e] = real && k * 16 + 8 < p.dim ? __ldcg(reinterpret_cast<const unsigned int*>(src + k * 16 + 8)) : 0u;
+        for (int k = 0; k < D / 16; ++k) {
+          qf[k][e] = real && k * 16 < p.dim ? __ldcg(reinterpret_cast<const unsigned int*>(src + k * 16)) : 0u;
+          qf[k][2 + e] = real && k * 16 + 8 < p.dim ? __ldcg(reinterpret_cast<const unsigned int*>(src + k * 16 + 8)) : 0u;
+        }
       }
     }
   };
@@ -274,10 +328,11 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       limit[e] = r < rows ? pq + 1 : 0;
       floor_[e] = paged_first_key(p, pq);
     }
-    float o[D / 8][4];
-#pragma unroll
-    for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    CodeSums<D> sums;
+    sums.clear();
+    auto& o = sums.o;
+    auto& m = sums.m;
+    auto& l = sums.l;
     const int all_end = it.kv - it.qn + 1, all_first = paged_first_key(p, it.kv - 1);  // keys that every row sees
 
     for (int k = 0; k < cur.len; ++k) {
@@ -285,8 +340,16 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       const int next = stage + 1 < NS ? stage + 1 : 0;
       ready = mbar_test(&full[next], next == 0 ? phase ^ 1 : phase);  // answered while this tile is worked on
       __syncwarp();
-      const int k0 = kg * 16, j0 = (it.tile0 + cur.tile + k) * kDecTile + k0;  // 16 keys
-      if (j0 < it.kv && j0 + 16 > it.first) {
+      constexpr int MINE = TILE / C::KG;
+      const int k0 = kg * MINE, j0 = (it.tile0 + cur.tile + k) * TILE + k0;  // 16 keys, 32 of codes
+      if (CODES && j0 < it.kv && j0 + MINE > it.first) {
+        const uint32_t ks = smem_addr(smem + stage * 2 * SIDE);
+        const CodeSpan span = {it.kv, it.first, all_first, all_end, {limit[0], limit[1]}, {floor_[0], floor_[1]}, it.qn > 1};
+        if constexpr (CODES)
+          code_tile<T, D>(sums, qf, span, ks, ks + SIDE, k0, j0, *reinterpret_cast<const float4*>(&s_scale[stage][0][kg * 4]),
+                          *reinterpret_cast<const float4*>(&s_scale[stage][1][kg * 4]), row_f);
+      }
+      if (!CODES && j0 < it.kv && j0 + 16 > it.first) {
         const uint32_t ks = smem_addr(smem + stage * 2 * SIDE), vs = ks + SIDE;
         // All of K's fragments, then the products as four independent chains.
         uint32_t kf[2][D / 32][4];
@@ -448,6 +511,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     for (int e = 0; e < 2; ++e) {
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+      if constexpr (CODES) l[e] *= 0x1p-15f;  // kCodeUp
       if ((lane & 3) == 0) {
         s_m[warp][(lane >> 2) + e * 8] = m[e];
         s_l[warp][(lane >> 2) + e * 8] = l[e];
@@ -462,10 +526,14 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
 #pragma unroll
       for (int g = 0; g < C::KG; ++g) top = fmaxf(top, s_m[g][r]);
       const float own = top == -INFINITY ? 0.f : exp2_fast(m[e] - top);
+      if constexpr (CODES) {
+        sums.settle(e, own);
+      } else {
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n) {
-        o[n][2 * e] *= own;
-        o[n][2 * e + 1] *= own;
+        for (int n = 0; n < D / 8; ++n) {
+          o[n][2 * e] *= own;
+          o[n][2 * e + 1] *= own;
+        }
       }
     }
     for (int g = 0; g < C::KG; g += slots) {
@@ -474,6 +542,19 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
         for (int e = 0; e < 2; ++e) {
           const int r = (lane >> 2) + e * 8;
           if (r >= rows) continue;
+          if constexpr (CODES) {  // four columns side by side
+            float* d = merge + ((kg - g) * apart + r) * C::kRowF + (lane & 3) * 4;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+              float4 v = make_float4(o[2 * c][2 * e], o[2 * c + 1][2 * e], o[2 * c][2 * e + 1], o[2 * c + 1][2 * e + 1]);
+              if (g > 0) {
+                const float4 u = *reinterpret_cast<const float4*>(d + c * 16);
+                v = make_float4(v.x + u.x, v.y + u.y, v.z + u.z, v.w + u.w);
+              }
+              *reinterpret_cast<float4*>(d + c * 16) = v;
+            }
+            continue;
+          }
           float* d = merge + ((kg - g) * apart + r) * C::kRowF + (lane & 3) * 2;
           if (g > 0) {
             float2 u[D / 8];  // all the loads first
@@ -517,6 +598,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     };
     // What a lane stored in columns from c of row r where it is not finite, though the row's sum is: the whole warp.
     auto settle = [&](auto words, int r, int c, bool odd) {
+      if (CODES) return;  // codes have no infinities
       if (__builtin_expect(__any_sync(0xffffffffu, odd), 0)) {
         paged_settle<T, decltype(words)::value>(p, &s_place, r, c, place(r, c), odd);
       }
@@ -668,10 +750,10 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
 
 namespace {
 
-template <typename T, int D, bool CLUSTER>
+template <typename T, int D, bool CLUSTER, bool CODES>
 cudaError_t launch_decode(const DecodeArgs& a, cudaStream_t st, bool pdl) {
-  using C = DecodeCfg<D>;
-  auto kern = paged_attention_decode_kernel<T, D, CLUSTER>;
+  using C = DecodeCfg<D, CODES>;
+  auto kern = paged_attention_decode_kernel<T, D, CLUSTER, CODES>;
   static SmemLimit limit;
   if (const cudaError_t e = limit.raise(kern, C::kSmem); e != cudaSuccess) return e;
   const int ctas = device_sm_count() * C::kPerSm;
@@ -700,31 +782,38 @@ cudaError_t launch_decode(const DecodeArgs& a, cudaStream_t st, bool pdl) {
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool CODES>
 cudaError_t launch_decode_any(const DecodeArgs& a, cudaStream_t st, bool pdl) {
   // One request of 777 keys, 8 key heads: 6.5 us with clusters, 11.3 without; 4000 keys 12.9 and 18.5. From
   // twice that on an item needs more CTAs than a cluster has. The host knows the lengths' bound only.
   // Without requests there is no item to launch a cluster for: the other kernel's CTAs write the zeros.
   if (a.a.requests > 0 && (long long)a.a.requests * a.a.kv_heads <= kFewItems &&
       (long long)a.a.width * a.a.block_size <= kFewKeys)
-    return launch_decode<T, D, true>(a, st, pdl);
-  return launch_decode<T, D, false>(a, st, pdl);
+    return launch_decode<T, D, true, CODES>(a, st, pdl);
+  return launch_decode<T, D, false, CODES>(a, st, pdl);
+}
+
+template <bool CODES>
+cudaError_t launch_decode_of(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl) {
+  constexpr int TILE = CODES ? kCodeTile : kDecTile;
+  if ((dtype != kBF16 && dtype != kF16) || a.dim > 128) return cudaErrorNotSupported;
+  // units of work (paged_sched.cuh) in 32 bits
+  if ((long long)a.requests * a.kv_heads * ((long long)a.width * a.block_size / TILE + 2 + kDecItem) >= INT_MAX)
+    return cudaErrorNotSupported;
+  DecodeArgs d{};
+  d.a = a;
+  d.box = paged_box(a.block_size, TILE);
+  const int columns = CODES ? (a.dim <= 64 ? 64 : 128) : 64;
+  if (d.box < 8 || !paged_maps(a, CODES ? kPagedCodes : dtype, columns, d.box, &d.k_map, &d.v_map)) return cudaErrorNotSupported;
+  if (dtype == kBF16)
+    return a.dim <= 64 ? launch_decode_any<__nv_bfloat16, 64, CODES>(d, st, pdl) : launch_decode_any<__nv_bfloat16, 128, CODES>(d, st, pdl);
+  return a.dim <= 64 ? launch_decode_any<__half, 64, CODES>(d, st, pdl) : launch_decode_any<__half, 128, CODES>(d, st, pdl);
 }
 
 }  // namespace
 
 cudaError_t launch_paged_attention_decode(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl) {
-  if ((dtype != kBF16 && dtype != kF16) || a.dim > 128) return cudaErrorNotSupported;
-  // units of work (paged_sched.cuh) in 32 bits
-  if ((long long)a.requests * a.kv_heads * ((long long)a.width * a.block_size / kDecTile + 2 + kDecItem) >= INT_MAX)
-    return cudaErrorNotSupported;
-  DecodeArgs d{};
-  d.a = a;
-  d.box = paged_box(a.block_size, kDecTile);
-  if (d.box < 8 || !paged_maps(a, dtype, d.box, &d.k_map, &d.v_map)) return cudaErrorNotSupported;
-  if (dtype == kBF16)
-    return a.dim <= 64 ? launch_decode_any<__nv_bfloat16, 64>(d, st, pdl) : launch_decode_any<__nv_bfloat16, 128>(d, st, pdl);
-  return a.dim <= 64 ? launch_decode_any<__half, 64>(d, st, pdl) : launch_decode_any<__half, 128>(d, st, pdl);
+  return a.k_scale != nullptr ? launch_decode_of<true>(a, dtype, st, pdl) : launch_decode_of<false>(a, dtype, st, pdl);
 }
 
 }  // namespace mlora

@@ -1005,7 +1005,7 @@ cudaError_t launch_paged_attention_chunk(const PagedAttnArgs& a, int dtype, cuda
   ChunkArgs c{};
   c.a = a;
   c.box = paged_box(a.block_size, kChunkKeys);
-  if (c.box < 8 || !paged_maps(a, dtype, c.box, &c.k_map, &c.v_map)) return cudaErrorNotSupported;
+  if (c.box < 8 || !paged_maps(a, dtype, 64, c.box, &c.k_map, &c.v_map)) return cudaErrorNotSupported;
   c.q_tma = paged_q_map(a, dtype, 128, &c.q_map);
   c.out32 = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_token % 16 == 0 && a.out_head % 16 == 0 && a.dim % 16 == 0;
   if (dtype == kBF16)

@@ -374,10 +374,11 @@ int attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int6
   const cudaStream_t st = (cudaStream_t)stream;
   // rows (tokens x group) times group below 2^32: where division by multiplication is exact
   const bool rows_ok = (int64_t)a.tokens * a.group * a.group < (1ll << 32);
-  if (vec && es == 2 && rows_ok && scales == nullptr) {
+  if (vec && es == 2 && rows_ok) {
     const bool few = (int64_t)a.max_q_len * (q_heads / c.kv_heads) <= mlora::kDecodeMaxRows;
-    const cudaError_t e = few ? mlora::launch_paged_attention_decode(a, dtype, st, pdl)
-                              : mlora::launch_paged_attention_chunk(a, dtype, st, pdl);
+    const cudaError_t e = few                 ? mlora::launch_paged_attention_decode(a, dtype, st, pdl)
+                          : scales == nullptr ? mlora::launch_paged_attention_chunk(a, dtype, st, pdl)
+                                              : cudaErrorNotSupported;
     if (e != cudaErrorNotSupported) return launched(e, "paged attention launch");
   }
   return launched(mlora::launch_paged_attention_general(a, dtype, vec, st, pdl), "paged attention launch");

@@ -25,28 +25,31 @@ EncodeTiled encode_tiled() {
 }
 
 bool one_map(CUtensorMap* map, const void* base, int dtype, const PagedAttnArgs& a, int64_t slot, int64_t head,
-             int64_t block, int box) {
+             int64_t block, int columns, int box) {
+  const int es = dtype == kPagedCodes ? 1 : 2;
   const EncodeTiled enc = encode_tiled();
   if (enc == nullptr || a.num_blocks < 1) return false;
   const cuuint64_t dims[4] = {(cuuint64_t)a.dim, (cuuint64_t)a.block_size, (cuuint64_t)a.kv_heads,
                               (cuuint64_t)a.num_blocks};
   // the stride of a dimension of one is never used, but has to be a valid one
-  const auto bytes = [&](int64_t s, cuuint64_t n) { return n > 1 ? (cuuint64_t)s * 2 : (cuuint64_t)a.dim * 2; };
+  const auto bytes = [&](int64_t s, cuuint64_t n) { return n > 1 ? (cuuint64_t)s * es : ((cuuint64_t)a.dim * es + 15) / 16 * 16; };
   const cuuint64_t strides[3] = {bytes(slot, dims[1]), bytes(head, dims[2]), bytes(block, dims[3])};
   for (const cuuint64_t s : strides)
     if (s == 0 || s % 16 != 0 || s >= (1ull << 40)) return false;
-  const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1}, ones[4] = {1, 1, 1, 1};
-  return enc(map, dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-             const_cast<void*>(base), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  const cuuint32_t boxes[4] = {(cuuint32_t)columns, (cuuint32_t)box, 1, 1}, ones[4] = {1, 1, 1, 1};
+  return enc(map, dtype == kPagedCodes ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                  : dtype == kBF16     ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+             4, const_cast<void*>(base), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             columns * es == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace
 
-bool paged_maps(const PagedAttnArgs& a, int dtype, int box, CUtensorMap* k, CUtensorMap* v) {
-  return one_map(k, a.k, dtype, a, a.k_slot, a.k_head, a.k_block, box) &&
-         one_map(v, a.v, dtype, a, a.v_slot, a.v_head, a.v_block, box);
+bool paged_maps(const PagedAttnArgs& a, int dtype, int columns, int box, CUtensorMap* k, CUtensorMap* v) {
+  return one_map(k, a.k, dtype, a, a.k_slot, a.k_head, a.k_block, columns, box) &&
+         one_map(v, a.v, dtype, a, a.v_slot, a.v_head, a.v_block, columns, box);
 }
 
 bool paged_q_map(const PagedAttnArgs& a, int dtype, int rows, CUtensorMap* q) {

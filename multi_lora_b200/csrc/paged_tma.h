@@ -14,9 +14,10 @@ inline int paged_box(int block_size, int tile) {
   return low < tile ? low : tile;
 }
 
-// Maps {dim, slot, head, block} over K and V, box 64 columns x `box` slots,
-// 128-byte swizzle, zeros out of range. False where a map cannot describe the cache.
-bool paged_maps(const PagedAttnArgs& a, int dtype, int box, CUtensorMap* k, CUtensorMap* v);
+// Maps {dim, slot, head, block} over K and V, box `columns` x `box` slots (rows of 64 or 128 bytes, swizzled by as
+// many), zeros out of range. False where a map cannot describe the cache. `dtype`: kPagedCodes for one of codes.
+constexpr int kPagedCodes = 3;
+bool paged_maps(const PagedAttnArgs& a, int dtype, int columns, int box, CUtensorMap* k, CUtensorMap* v);
 
 // Map {dim, head, token} over Q, box 64 columns x group heads x rows / group tokens: a
 // tile of `rows` packed rows (token major, then head). False where group does not divide it.
