@@ -104,6 +104,8 @@ cudaError_t launch_paged_attention_decode(const PagedAttnArgs& a, int dtype, cud
 constexpr int kDecodeMaxRows = 16;
 
 cudaError_t launch_paged_attention_chunk(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl);
+// the same over a cache of codes
+cudaError_t launch_paged_attention_code_chunk(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl);
 
 struct VerifyArgs {
   const void* target;         // [rows, vocab]

@@ -1,0 +1,879 @@
+// Attention of chunks over a paged cache of e4m3 codes, on the fifth-generation tensor cores.
+//
+// Items, halves of tiles, TMEM and the running maximum are those of csrc/paged_attn_tc.cu. What differs is how K and V
+// come to the tensor cores: a warpgroup of its own fetches codes from their pages, a tile ahead of
+// what it works on, and writes them as 16-bit values in the swizzled tiles that the products read: K in the queries'
+// type, V in f16, both exact. Scales stay in fp32 outside the products:
+//   S = Q C_K^T,  x = S f_K - m,  P = exp2(x) f_V / F,  O += P C_V,   F the largest f_V so far
+// with f constant over each eight keys, so a key's scale costs nothing beside the scale that a score has anyway (the
+// maximum is taken of each eight scores first), and a value's one multiplication of two probabilities.
+//
+// P is f16 whatever the queries are: 11 bits, taken times 2^11 (below 2^15, see kRaise), so nothing is
+// coarser than 2^-36 of the largest. For bf16 results, which keep 8 bits, that is one term and half as much work in
+// the second product as the two that bf16 probabilities need; f16 results take two terms.
+//
+// Codes of keys that no row sees become zeros on the way, and NaN of those that only some rows see too, which is
+// added to these rows' outputs at the end (codes have no infinities).
+//
+// What bounds it: the exponentials and the tensor cores (2048 cycles a tile of 128 keys and 256 rows each, f16
+// queries 3072 of the latter).
+#include <climits>
+
+#include "device.h"
+#include "kernels.h"
+#include "paged_chunk.cuh"
+#include "paged_codes.cuh"
+#include "paged_tma.h"
+
+namespace mlora {
+
+constexpr int kCodeThreads = 512;  // Q and tensor cores, two warpgroups of softmax, one of codes
+
+struct CodeChunkArgs {
+  CUtensorMap q_map;
+  PagedAttnArgs a;
+  int q_tma;  // Q tiles are boxes of q_map (group divides 128)
+  int out32;  // rows of the output allow 32-byte stores
+};
+
+template <int D>
+struct CodeChunkCfg {
+  static constexpr int kSlot = kChunkKeys * D * 2;  // K or V of a tile
+  static constexpr int kQ = 128 * D * 2;            // one tile of Q
+  static constexpr int kSlots = 160 * 1024 / kSlot;
+  static constexpr int kSmem = 2 * kQ + kSlots * kSlot + 1024;
+  static constexpr int kPart = 128 * (D + 2);  // floats of a tile's piece
+  // tiles whose scales wait: K of a tile gets its slot when V of the third tile before it (D = 64: scores of the fifth,
+  // so values of the sixth) is done with
+  static constexpr int kScaleTiles = D == 128 ? 4 : 8;
+};
+
+// NaN that was taken out of V, added in TMEM to the outputs of row r, if it sees it: the item's keys of [from, to) that
+// not every row sees, those of every tile's half `half` if that is not negative. Seldom run.
+template <int D>
+__device__ __noinline__ void code_give_back(const PagedAttnArgs& p, uint32_t o_addr, int req, int head, int rt, int qn, int kv, int r,
+                                            int from, int to, int half) {
+  ChunkItem it;
+  it.qn = qn;
+  it.kv = kv;
+  it.rt = rt;
+  it.rows = qn * p.group;
+  int seen_lo, seen_hi;
+  chunk_seen(p, it, seen_lo, seen_hi);
+  const int pos = kv - qn + paged_token(p, r);
+  if (r < it.rows) {
+    from = max(from, paged_first_key(p, pos));
+    to = min(to, pos + 1);
+  } else {
+    to = from;
+  }
+#pragma unroll 1
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t o[32];
+    tmem_ld32_async(o_addr + c * 32, o);
+    tmem_wait_ld();
+    tie32(o);
+#pragma unroll 1
+    for (int j = from; j < to; ++j) {
+      if ((j >= seen_lo && j < seen_hi) || (half >= 0 && ((j / kHalfKeys) & 1) != half)) continue;
+      const int block = __ldcg(p.tables + req * p.table_stride + j / p.block_size);
+      if (block < 0 || block >= p.num_blocks) continue;
+      const unsigned char* src = static_cast<const unsigned char*>(p.v) + block * p.v_block + (j % p.block_size) * p.v_slot +
+                                 head * p.v_head + c * 32;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // a dim is a multiple of 8
+        if (c * 32 + 8 * i >= p.dim) continue;
+        const uint2 u = __ldcg(reinterpret_cast<const uint2*>(src) + i);
+        const uint32_t a = codes_nan(u.x), b = codes_nan(u.y);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (a >> (8 * e + 7) & 1u) o[8 * i + e] = 0x7fc00000u;
+          if (b >> (8 * e + 7) & 1u) o[8 * i + 4 + e] = 0x7fc00000u;
+        }
+      }
+    }
+    __syncwarp();
+    tmem_st32(o_addr + c * 32, o);
+  }
+  tmem_wait_st();
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// Four codes as values of T.
+template <typename T>
+__device__ __forceinline__ uint2 code_values(uint32_t x) {
+  uint32_t a = codes_lo(x), b = codes_hi(x);
+  if constexpr (Num<T>::is_bf16) {
+    a = pack_round2<T>(Pack2<__half>::lo(a), Pack2<__half>::hi(a));
+    b = pack_round2<T>(Pack2<__half>::lo(b), Pack2<__half>::hi(b));
+  }
+  return make_uint2(a, b);
+}
+
+// Pieces of 16 codes (the chunk-th of rows row0, row0 + 512 / D, ..) as values of T, in swizzled rows of 128 bytes.
+template <typename T, int D>
+__device__ __forceinline__ void code_put(unsigned char* to, int chunk, int row0, const uint4 (&u)[D / 16]) {
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    const int row = row0 + i * (512 / D);
+    const uint2 a = code_values<T>(u[i].x), b = code_values<T>(u[i].y), c = code_values<T>(u[i].z), d = code_values<T>(u[i].w);
+    *reinterpret_cast<uint4*>(to + row * 128 + (((chunk * 2) ^ (row & 7)) << 4)) = make_uint4(a.x, a.y, b.x, b.y);
+    *reinterpret_cast<uint4*>(to + row * 128 + (((chunk * 2 + 1) ^ (row & 7)) << 4)) = make_uint4(c.x, c.y, d.x, d.y);
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kCodeThreads, 1)
+paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
+  using C = CodeChunkCfg<D>;
+  constexpr int NS = C::kSlots, HALF = kChunkKeys * 128;
+  constexpr bool TWO = !Num<T>::is_bf16;      // terms of P
+  constexpr float kRaise = 4.f, kUp = 11.f;   // in powers of two
+  constexpr uint32_t S_COL = 0, O_COL = 256;
+  extern __shared__ __align__(1024) unsigned char s_raw[];
+  __shared__ __align__(8) uint64_t full[NS], empty[NS], q_ready[2], q_free[2], s_full[2][2], p_ready[2][2], pv_done[2][2];
+  constexpr int kScaleTiles = C::kScaleTiles;
+  __shared__ __align__(16) float s_scale[kScaleTiles][2][kChunkKeys / 8];  // of K and V, for each eight keys
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_last[2];
+  __shared__ bool s_skipped;
+  __shared__ float2 s_mate[128];  // maximum and sum of the other warpgroup's rows
+  __shared__ float s_mate_most;   // its largest scale of V
+  __shared__ uint32_t s_taken;      // a NaN was taken out of V
+  const PagedAttnArgs& p = args.a;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = same_in_warp(tid >> 5);
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* ring = smem + 2 * C::kQ;
+
+  if (tid == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&full[s], 4);   // the warps that write codes
+      mbar_init(&empty[s], 2);  // both warps of the tensor cores
+    }
+    for (int q = 0; q < 2; ++q) {
+      mbar_init(&q_ready[q], 1);
+      mbar_init(&q_free[q], 2);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&s_full[q][b], 1);
+        mbar_init(&p_ready[q][b], 4);
+        mbar_init(&pv_done[q][b], 1);
+      }
+    }
+    fence_barrier_init();
+    s_taken = 0u;
+    if (args.q_tma) tma_prefetch_map(&args.q_map);
+  }
+  if (warp == 1) tmem_alloc(&s_tmem, 512);
+  tc_fence_before();
+  pdl_wait();
+  pdl_trigger();
+
+  ChunkSplit split;
+  ChunkItem it;
+  int before, in_req;
+  int req;
+  PagedRequest found;
+  bool skipped = false;  // a request that is not computed
+  paged_find<kCodeThreads, 32>(
+      p.requests,
+      [&](int i, int part, int parts, PagedRequest& r) {
+        r = paged_request(p, i, part == 0 && blockIdx.x == 0);
+        skipped |= r.odd;
+        ChunkItem x;
+        chunk_request(p, x, i, r);
+        int n = 0;
+        for (x.rt = part; x.rt * kChunkRows < x.rows; x.rt += parts) {
+          chunk_span(p, x);
+          n += x.n + kChunkItem;
+        }
+        return n * p.kv_heads;
+      },
+      split, req, found, before, in_req);
+  skipped = __syncthreads_or(skipped);  // and the barriers are initialised, and s_tmem is there
+  if (tid == 96) s_skipped = skipped;   // for its own warp, at the end
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  PagedCursor<ChunkSplit> cur(split);
+  auto item_of_request = [&](int rel) {  // the item that holds unit `rel` of request it.req: a lane a tile of rows
+    const int per_head = in_req / p.kv_heads;
+    it.head = rel / per_head;
+    rel -= it.head * per_head;
+    it.rt = 0;
+    for (int rt0 = 0; rt0 * kChunkRows < it.rows; rt0 += 32) {
+      ChunkItem x = it;
+      x.rt = rt0 + lane;
+      int units = 0;
+      if (x.rt * kChunkRows < x.rows) {
+        chunk_span(p, x);
+        units = x.n + kChunkItem;
+      }
+      int upto = units;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += u;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, rel < upto);
+      if (hit != 0u) {
+        const int src = __ffs(hit) - 1;
+        it.rt = rt0 + src;
+        cur.unit = rel - __shfl_sync(0xffffffffu, upto - units, src);
+        break;
+      }
+      rel -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    chunk_span(p, it);
+  };
+  auto next_item = [&]() {
+    if (++it.rt * kChunkRows >= it.rows) {
+      it.rt = 0;
+      if (++it.head == p.kv_heads) {
+        it.head = 0;
+        PagedRequest r;
+        const int i = paged_next(p, it.req, INT_MAX, r);
+        if (i < p.requests) {
+          r.q0 = same_in_warp(r.q0);
+          r.qn = same_in_warp(r.qn);
+          r.kv = same_in_warp(r.kv);
+          chunk_request(p, it, i, r);
+        }
+      }
+    }
+    chunk_span(p, it);
+  };
+  if (cur.pos < cur.end) {
+    chunk_request(p, it, req, found);
+    item_of_request(cur.pos - before);
+    if (cur.begin(it.n)) next_item();
+  }
+  bool ok = true;
+
+  // Registers: 512 threads are launched with 128 each (65536); the warps of Q and the tensor cores keep 64, those of
+  // codes 112, and the softmax warps take 168: 128 * 64 + 128 * 112 + 256 * 168 = 65536.
+  if (warp < 4) {
+    regs_down<64>();
+    if (warp == 1 || warp == 2) {  // ---- tensor cores, a warp a tile of rows: S of a half, then O of the half before ----
+      const int q = warp - 1;
+      constexpr uint32_t idesc_s = umma_idesc_f16(Num<T>::is_bf16, 128, kHalfKeys);
+      constexpr uint32_t idesc_o = umma_idesc_f16(false, 128, D) | (1u << 16);  // B: columns contiguous
+      constexpr uint32_t kStep = kHalfKeys * 128 >> 4;  // a half of a K or V tile
+      const uint32_t ring_lo = smem_addr(ring) >> 4;
+      const uint32_t s_col = tmem + S_COL + q * 128, o_col = tmem + O_COL + q * D;
+      int kslot = 0, k_phase = 0, vslot = 1, v_phase = 0;
+      int n = 0;                 // halves begun
+      int items = 0, pairs = 0;  // items, and those of two tiles of rows
+      auto wait = [&](uint64_t* bar, int parity) { ok = ok && mbar_poll(bar, parity & 1, p.status); };
+      bool held = false, held_first = false, held_last = false;  // the half whose product with V is to come
+      uint32_t held_lo = 0;
+      int held_slot = 0;
+      auto values = [&]() {  // half n - 1 of this tile of rows is the newest, half `number` the held one
+        const int number = n - 1, b = number & 1;
+        wait(&p_ready[q][b], number >> 1);
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t a = s_col + b * 64;
+#pragma unroll
+          for (int i = 0; i < kHalfKeys / 16; ++i) umma_ts(o_col, a + i * 8, held_lo + i * 128, idesc_o, !held_first || i > 0);
+          if (TWO) {
+#pragma unroll
+            for (int i = 0; i < kHalfKeys / 16; ++i) umma_ts(o_col, a + 32 + i * 8, held_lo + i * 128, idesc_o, true);
+          }
+          umma_commit(&pv_done[q][b]);
+          if (held_last) umma_commit(&empty[held_slot]);
+        }
+        held = false;
+      };
+      while (cur.take(it.n)) {
+        const bool solo = chunk_solo(it);  // this warp then has every other half of the one tile
+        const int qs = solo ? 0 : q, h0 = solo ? q : 0;
+        const bool odd = !solo && chunk_odd(it, cur);
+        const uint32_t q_lo = smem_addr(smem + qs * C::kQ) >> 4;
+        if (held) values();  // nothing of the item before waits for this one's Q, or keeps its V from the ring
+#pragma unroll 1
+        for (int k = 0; k < cur.len; ++k) {
+          wait(&full[kslot], k_phase);
+          const int h1 = solo ? q + 1 : odd && k == cur.len - 1 ? 1 : 2;
+#pragma unroll 1
+          for (int h = h0; h < h1; ++h) {
+            const bool first = k == 0 && h == h0, last = h == h1 - 1;
+            if (first) wait(&q_ready[qs], qs == 0 ? items : pairs);
+            const int b = n & 1;
+            if (n > 1) wait(&pv_done[q][b], (n >> 1) - 1);  // P in this buffer has been read
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t kl = ring_lo + kslot * (C::kSlot >> 4) + h * kStep;
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i)
+                umma_ss(s_col + b * 64, q_lo + (i >> 2) * (HALF >> 4) + 2 * (i & 3), kl + (i >> 2) * (HALF >> 4) + 2 * (i & 3),
+                        idesc_s, i > 0);
+              umma_commit(&s_full[q][b]);
+              if (last) umma_commit(&empty[kslot]);
+              if (last && k == cur.len - 1) {  // two arrivals free a tile of Q
+                umma_commit(&q_free[qs]);
+                if (!solo) umma_commit(&q_free[qs]);
+              }
+            }
+            if (held) values();
+            ++n;
+            if (h == h0) wait(&full[vslot], v_phase);
+            held = true;
+            held_first = first;
+            held_last = last;
+            held_lo = ring_lo + vslot * (C::kSlot >> 4) + h * kStep + ((HALF >> 4) << 16);
+            held_slot = vslot;
+          }
+          kslot += 2;
+          if (kslot >= NS) {
+            kslot -= NS;
+            k_phase ^= 1;
+          }
+          vslot += 2;
+          if (vslot >= NS) {
+            vslot -= NS;
+            v_phase ^= 1;
+          }
+        }
+        ++items;
+        pairs += solo ? 0 : 1;
+        if (cur.advance()) next_item();
+      }
+      if (held) values();
+    } else if (warp == 0) {  // ---- Q of each item, as soon as the scores of the item before are done ----
+      int items[2] = {0, 0};
+      while (cur.take(it.n)) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int r0 = it.rt * kChunkRows + q * 128;
+          if (r0 >= it.rows) continue;
+          if (items[q] > 0) ok = __all_sync(0xffffffffu, ok && mbar_poll(&q_free[q], (items[q] - 1) & 1, p.status));
+          ++items[q];
+          if (args.q_tma) {  // rows behind the request's are others', or zeros: no score of theirs is used
+            if (ok && lane == 0) {
+              mbar_arrive_expect_tx(&q_ready[q], C::kQ);
+              for (int c = 0; c < D / 64; ++c)
+                tma_load_3d(smem + q * C::kQ + c * HALF, &args.q_map, c * 64, it.head * p.group, it.q0 + paged_token(p, r0),
+                            &q_ready[q]);
+            }
+            __syncwarp();
+          } else {
+            constexpr int PIECES = D / 8, AT_ONCE = 8;  // 16-byte pieces, swizzled as TMA would
+#pragma unroll 1
+            for (int e0 = lane; e0 < 128 * PIECES; e0 += 32 * AT_ONCE) {
+              uint4 u[AT_ONCE];
+#pragma unroll
+              for (int i = 0; i < AT_ONCE; ++i) {
+                const int e = e0 + i * 32, r = r0 + e / PIECES, c = e % PIECES, t = paged_token(p, r);
+                u[i] = make_uint4(0, 0, 0, 0);
+                if (r < it.rows && c * 8 < p.dim)
+                  u[i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (int64_t)(it.q0 + t) * p.q_token +
+                                                               (int64_t)(it.head * p.group + r - t * p.group) * p.q_head + c * 8));
+              }
+#pragma unroll
+              for (int i = 0; i < AT_ONCE; ++i) {
+                const int e = e0 + i * 32, r = e / PIECES, c = e % PIECES;
+                *reinterpret_cast<uint4*>(smem + q * C::kQ + (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = u[i];
+              }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_ready[q]);
+          }
+        }
+        if (cur.advance()) next_item();
+      }
+    } else {  // ---- rows that nobody has ----
+      __syncwarp();
+      if (s_skipped) paged_zero_uncomputed<T>(p, split.total > 0 ? INT_MAX : -1);
+      else paged_zero_rest<T>(p);
+    }
+  } else if (warp >= 12) {  // ---- codes of K and V, 32 keys of each tile a warp ----
+    regs_down<112>();
+    constexpr int PASSES = D / 16, ROWS = 32 / PASSES;  // pieces of 16 codes a thread, keys at once
+    const int w = warp - 12;
+    // eight lanes side by side store to all banks: of two keys the first four pieces, or the last four
+    const int chunk = (lane & 3) | (D == 128 ? lane >> 4 << 2 : 0), row0 = w * 32 + (D == 128 ? lane >> 2 & 3 : lane >> 2);
+    int slot = 0, round = 0;
+    uint32_t tile_no = 0;
+    while (cur.take(it.n)) {
+      const int32_t* table = p.tables + it.req * p.table_stride;
+      const int j_first = (it.tile0 + cur.tile) * kChunkKeys;
+      int seen_lo, seen_hi;
+      chunk_seen(p, it, seen_lo, seen_hi);
+      // eight keys a lane, of the warp's 32: their block (-1: nothing of it is seen or it is outside the cache) and slot
+      auto lookup = [&](int k, int& block, int& off) {
+        const int j = j_first + k * kChunkKeys + w * 32 + lane * 8;
+        block = -1;
+        off = 0;
+        if (lane < 4 && j < it.end && j + 8 > it.first) {
+          const int e = __ldcg(table + j / p.block_size);
+          off = j % p.block_size;
+          if (e >= 0 && e < p.num_blocks) block = e;
+          else flag_error(p.status, kErrKvRange);
+        }
+      };
+      auto fetch = [&](uint4* u, int k, int block, int off, const void* base, int64_t s_block, int64_t s_slot, int64_t s_head) {
+        const unsigned char* from = static_cast<const unsigned char*>(base) + it.head * s_head + chunk * 16;
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+          const int eight = i * ROWS / 8, row = row0 + i * ROWS, j = j_first + k * kChunkKeys + row;
+          const int b = __shfl_sync(0xffffffffu, block, eight), o = __shfl_sync(0xffffffffu, off, eight) + (row & 7);
+          u[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (b >= 0 && j >= it.first && j < it.end && chunk * 16 < p.dim) {
+            const unsigned char* src = from + b * s_block + o * s_slot;
+            if (chunk * 16 + 16 <= p.dim) {
+              u[i] = __ldcg(reinterpret_cast<const uint4*>(src));
+            } else {
+              const uint2 h = __ldcg(reinterpret_cast<const uint2*>(src));
+              u[i].x = h.x;
+              u[i].y = h.y;
+            }
+          }
+        }
+      };
+      auto scales_of = [&](int block, float& a, float& b) {
+        a = b = 0.f;
+        if (block >= 0) {
+          a = __ldcg(p.k_scale + block * p.ks_block + it.head * p.ks_head);
+          b = __ldcg(p.v_scale + block * p.vs_block + it.head * p.vs_head);
+        }
+      };
+      auto filled = [&]() {  // the slot is
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[slot]);
+        if (++slot == NS) {
+          slot = 0;
+          ++round;
+        }
+      };
+      auto room = [&]() {
+        if (round > 0) ok = __all_sync(0xffffffffu, ok && mbar_poll(&empty[slot], (round - 1) & 1, p.status));
+      };
+      uint4 uk[PASSES], uv[PASSES];
+      int block, off, next_block = -1, next_off = 0;
+      float fk, fv;
+      if (cur.len > 0) {
+        lookup(0, block, off);
+        scales_of(block, fk, fv);
+        fetch(uk, 0, block, off, p.k, p.k_block, p.k_slot, p.k_head);
+        fetch(uv, 0, block, off, p.v, p.v_block, p.v_slot, p.v_head);
+        if (cur.len > 1) lookup(1, next_block, next_off);
+      }
+      for (int k = 0; k < cur.len; ++k) {
+        const int j0 = j_first + k * kChunkKeys;
+        const bool more = k + 1 < cur.len;
+        room();
+        if (lane < 4) {
+          s_scale[tile_no % kScaleTiles][0][w * 4 + lane] = fk;
+          s_scale[tile_no % kScaleTiles][1][w * 4 + lane] = fv;
+        }
+        ++tile_no;
+        code_put<T, D>(ring + slot * C::kSlot + (chunk >> 2) * HALF, chunk & 3, row0, uk);
+        filled();
+        if (more) {
+          scales_of(next_block, fk, fv);
+          fetch(uk, k + 1, next_block, next_off, p.k, p.k_block, p.k_slot, p.k_head);
+        }
+        if (j0 + kChunkKeys > seen_hi || j0 < seen_lo) {  // NaN of keys that not every row sees
+          bool taken = false;
+#pragma unroll
+          for (int i = 0; i < PASSES; ++i) {
+            const int j = j0 + row0 + i * ROWS;
+            if (j >= seen_lo && j < seen_hi) continue;
+            const uint4 nan = make_uint4(codes_nan(uv[i].x), codes_nan(uv[i].y), codes_nan(uv[i].z), codes_nan(uv[i].w));
+            taken |= (nan.x | nan.y | nan.z | nan.w) != 0u;
+            uv[i].x &= ~((nan.x >> 7) * 0xffu);
+            uv[i].y &= ~((nan.y >> 7) * 0xffu);
+            uv[i].z &= ~((nan.z >> 7) * 0xffu);
+            uv[i].w &= ~((nan.w >> 7) * 0xffu);
+          }
+          if (taken) count_store(&s_taken, 1u);
+        }
+        room();
+        code_put<__half, D>(ring + slot * C::kSlot + (chunk >> 2) * HALF, chunk & 3, row0, uv);
+        filled();
+        if (more) {
+          fetch(uv, k + 1, next_block, next_off, p.v, p.v_block, p.v_slot, p.v_head);
+          next_block = -1;
+          if (k + 2 < cur.len) lookup(k + 2, next_block, next_off);
+        }
+      }
+      if (cur.advance()) next_item();
+    }
+  } else {  // ---- softmax: warpgroup q, thread = row ----
+    regs_up<168>();
+    const int q = (warp >> 2) - 1, row = tid & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + lanes + S_COL + q * 128, o_addr = tmem + lanes + O_COL + q * D;
+    const float sl = p.scale * 1.4426950408889634f;  // scores in powers of two
+    uint32_t* tickets = static_cast<uint32_t*>(p.workspace);
+    float* parts = reinterpret_cast<float*>(tickets + kPagedTickets);
+    int n = 0;             // halves done
+    uint32_t tile_no = 0;  // of the current item's first tile
+    bool lent = false;     // the other warpgroup still reads this one's O
+    while (cur.take(it.n)) {
+      const bool solo = chunk_solo(it);  // the warpgroups share its keys, half by half
+      const int r_lo = it.rt * kChunkRows + (solo ? 0 : q * 128), r = r_lo + row;
+      const int pq = it.kv - it.qn + paged_token(p, r);
+      const int limit = r < it.rows ? pq + 1 : 0, floor_ = paged_first_key(p, pq);
+      // key tiles that every row of this tile sees whole need no mask
+      const int r_hi = min(it.rows, r_lo + 128) - 1;
+      const int all_end = it.kv - it.qn + paged_token(p, r_lo) + 1,
+                all_first = paged_first_key(p, it.kv - it.qn + paged_token(p, r_hi));
+      const bool none = r - lane >= it.rows;  // no row in this warp: its lanes of P and O are never looked at
+      float m = -INFINITY, l = 0.f;
+      float most = 0.f, inv_most = 0.f;  // the largest scale of V so far: O is in units of it
+      const int halves = solo ? cur.len : 2 * cur.len - chunk_odd(it, cur);
+      for (int k = 0; k < halves; ++k, ++n) {
+        const int b = n & 1;
+        ok = ok && mbar_poll(&s_full[q][b], (n >> 1) & 1, p.status);
+        __syncwarp();
+        tc_fence_after();
+        if (none) {
+          if (lent) {
+            named_barrier(5, 256);
+            lent = false;
+          }
+          if (lane == 0) mbar_arrive(&p_ready[q][b]);
+          continue;
+        }
+        uint32_t s[2][32];
+        tmem_ld32_async(s_addr + b * 64, s[0]);
+        tmem_ld32_async(s_addr + b * 64 + 32, s[1]);
+        const int half = solo ? 2 * k + q : k;  // of the item
+        float fk[8], fv[8];
+        {
+          const float* f = &s_scale[(tile_no + (half >> 1)) % kScaleTiles][0][(half & 1) * 8];
+          const float4 a = *reinterpret_cast<const float4*>(f), c = *reinterpret_cast<const float4*>(f + 4);
+          const float4 d = *reinterpret_cast<const float4*>(f + kChunkKeys / 8), e = *reinterpret_cast<const float4*>(f + kChunkKeys / 8 + 4);
+          fk[0] = a.x, fk[1] = a.y, fk[2] = a.z, fk[3] = a.w, fk[4] = c.x, fk[5] = c.y, fk[6] = c.z, fk[7] = c.w;
+          fv[0] = d.x, fv[1] = d.y, fv[2] = d.z, fv[3] = d.w, fv[4] = e.x, fv[5] = e.y, fv[6] = e.z, fv[7] = e.w;
+        }
+        // not zero, so that minus infinity stays what it is
+#pragma unroll
+        for (int i = 0; i < 8; ++i) fk[i] = fmaxf(fk[i] * sl, 1e-37f);
+        const float largest = fmaxf(max3(max3(fv[0], fv[1], fv[2]), fv[3], fv[4]), max3(fv[5], fv[6], fv[7]));
+        tmem_wait_ld();
+        tie32(s[0]);
+        tie32(s[1]);
+        const int j0 = (it.tile0 + cur.tile) * kChunkKeys + half * kHalfKeys;
+        if (j0 + kHalfKeys > all_end || j0 < all_first) {
+          const int hi = limit - j0, lo = floor_ - j0;
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c * 32 + i >= hi || c * 32 + i < lo) s[c][i] = 0xff800000u;  // -infinity
+        }
+        float top[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const uint32_t* x = &s[c >> 2][(c & 3) * 8];
+          top[c] = max3(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]));
+          top[c] = max3(top[c], __uint_as_float(x[3]), __uint_as_float(x[4]));
+          top[c] = fmaxf(max3(top[c], __uint_as_float(x[5]), __uint_as_float(x[6])), __uint_as_float(x[7])) * fk[c];
+        }
+        const float mx = fmaxf(max3(max3(top[0], top[1], top[2]), top[3], top[4]), max3(top[5], top[6], top[7]));
+        if (k == 0) {
+          m = mx;
+          most = largest;
+          inv_most = most > 0.f ? 1.f / most : 0.f;
+        } else {
+          const bool raise = mx > m + kRaise, wider = largest > most;
+          if (__any_sync(0xffffffffu, raise || wider)) {
+            // O holds the halves before this one once the last product is done
+            ok = ok && mbar_poll(&pv_done[q][b ^ 1], ((n - 1) >> 1) & 1, p.status);
+            __syncwarp();
+            tc_fence_after();
+            float fix = raise ? exp2_fast(m - mx) : 1.f;
+            if (raise) m = mx;
+            l *= fix;
+            if (wider) {
+              fix *= most / largest;
+              most = largest;
+              inv_most = 1.f / most;
+            }
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32_async(o_addr + c * 32, o);
+              tmem_wait_ld();
+              tie32(o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fix);
+              tmem_st32(o_addr + c * 32, o);
+            }
+          }
+        }
+        const float ref = (m == -INFINITY ? 0.f : m) - kUp;
+        const uint64_t ref2 = pack2(-ref, -ref);
+        uint64_t sum[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {  // 32 keys
+          uint32_t w[16], rest[16];  // P, two keys a column
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const int eight = c * 4 + i / 8;
+            const float f = fk[eight], g = fv[eight] * inv_most;
+            const uint64_t x = fma2(pack2u(s[c][i], s[c][i + 1]), pack2(f, f), ref2);
+            const uint64_t pp = pack2(exp2_fast(lo_of(x)), exp2_fast(hi_of(x)));
+            sum[(i >> 1) & 3] = add2(sum[(i >> 1) & 3], pp);
+            const uint64_t pw = mul2(pp, pack2(g, g));
+            w[i >> 1] = pack_round2<__half>(lo_of(pw), hi_of(pw));
+            if constexpr (TWO)
+              rest[i >> 1] = pack_round2<__half>(lo_of(pw) - Pack2<__half>::lo(w[i >> 1]), hi_of(pw) - Pack2<__half>::hi(w[i >> 1]));
+          }
+          tmem_st16(s_addr + b * 64 + c * 16, w);
+          // over scores that are in registers by now
+          if constexpr (TWO) tmem_st16(s_addr + b * 64 + 32 + c * 16, rest);
+        }
+        const uint64_t both = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+        l += lo_of(both) + hi_of(both);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lent) {  // this half's product overwrites O
+          named_barrier(5, 256);
+          lent = false;
+        }
+        if (lane == 0) mbar_arrive(&p_ready[q][b]);
+      }
+
+      const ChunkItem done = it;
+      const bool whole = cur.whole(it.n);
+      const int item0 = cur.pos - cur.unit;
+      const int tile0 = it.tile0 + cur.tile, tiles = cur.len;
+      tile_no += cur.len;
+      if (cur.advance()) next_item();
+
+      ok = ok && mbar_poll(&pv_done[q][(n - 1) & 1], ((n - 1) >> 1) & 1, p.status);
+      __syncwarp();
+      tc_fence_after();
+      if (__any_sync(0xffffffffu, *const_cast<volatile uint32_t*>(&s_taken) != 0u))
+        code_give_back<D>(p, o_addr, done.req, done.head, done.rt, done.qn, done.kv, r, tile0 * kChunkKeys,
+                          (tile0 + tiles) * kChunkKeys, solo ? q : -1);
+      // An item that both warpgroups worked on: the first one reads the other's O too
+      // (their threads of a row have the same TMEM lane).
+      float own = most, others = 0.f;  // what the two warpgroups' sums are multiplied by
+      if (solo) {
+        if (q == 1) {
+          s_mate[row] = make_float2(m, l);
+          if (!none) s_mate_most = most;  // every warp with rows has the same
+          tc_fence_before();
+          named_arrive(4, 256);
+          lent = true;
+          continue;
+        }
+        named_barrier(4, 256);
+        tc_fence_after();
+        const float2 mate = s_mate[row];
+        const float top = fmaxf(m, mate.x), base = top == -INFINITY ? 0.f : top;
+        const float a = exp2_fast(m - base), c = exp2_fast(mate.x - base);
+        own = a * most;
+        others = c * s_mate_most;
+        l = l * a + mate.y * c;
+        m = top;
+      }
+      const int t = paged_token(p, r);
+      T* dst = static_cast<T*>(p.out) + (int64_t)(done.q0 + t) * p.out_token +
+               (int64_t)(done.head * p.group + r - t * p.group) * p.out_head;
+      auto store = [&](T* dst, int c, const float* v, float inv) {  // 16 columns: a thread a row, so whole sectors
+        uint32_t u[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] = pack_round2<T>(v[2 * i] * inv, v[2 * i + 1] * inv);
+        if (args.out32) {
+          if (c < p.dim) store32(dst + c, u);
+        } else {
+          if (c < p.dim) *reinterpret_cast<uint4*>(dst + c) = make_uint4(u[0], u[1], u[2], u[3]);
+          if (c + 8 < p.dim) *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(u[4], u[5], u[6], u[7]);
+        }
+      };
+      // pieces: [column / 4][row] of four floats, then maxima, then sums
+      auto piece = [&](int cta, int first_cta) {
+        return parts + (((long long)cta * 2 + (cta == first_cta ? 1 : 0)) * 2 + q) * C::kPart;
+      };
+      const int c0 = whole ? 0 : split.first_cta(item0, done.n);
+      float* part = piece(blockIdx.x, c0);
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll 1
+      for (int c = 0; c < (none ? 0 : D / 32); ++c) {
+        uint32_t o[32];
+        tmem_ld32_async(o_addr + c * 32, o);
+        tmem_wait_ld();
+        tie32(o);
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]) * own;
+        if (solo) {
+          tmem_ld32_async(o_addr + D + c * 32, o);
+          tmem_wait_ld();
+          tie32(o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = fmaf(__uint_as_float(o[i]), others, v[i]);
+        }
+        if (whole) {
+          if (r < done.rows) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 16) store(dst, c * 32 + i, v + i, inv);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            __stcg(reinterpret_cast<float4*>(part) + (c * 8 + i / 4) * 128 + row,
+                   make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+        }
+      }
+      tc_fence_before();
+      if (solo) named_arrive(5, 256);
+      if (!whole) {
+        __stcg(part + 128 * D + row, m);
+        __stcg(part + 128 * (D + 1) + row, l);
+        const int c1 = split.last_cta(item0, done.n);
+        const PagedJoin run(c0, c1, blockIdx.x);
+        auto last_of = [&](uint32_t* ticket, int n) {  // whether this warpgroup is the last of n to get here
+          named_barrier(1 + q, 128);
+          if (row == 0) {
+            __threadfence();
+            const bool last = atomicAdd(ticket, 1u) == (uint32_t)(n - 1);
+            if (last) *ticket = 0u;
+            __threadfence();
+            s_last[q] = last;
+          }
+          named_barrier(1 + q, 128);
+          const bool last = s_last[q];
+          named_barrier(1 + q, 128);
+          return last;
+        };
+        // Pieces x0, x0 + by, .. x1 of this tile of rows, to the output or as one piece to x0's
+        // place; one, two or four threads a row, 32 columns of two pieces at once.
+        auto join = [&](int x0, int x1, int by, bool final) {
+          const int live = min(128, done.rows - r_lo), share = live <= 32 ? 4 : live <= 64 ? 2 : 1;
+          const int jr = row & (128 / share - 1), c_from = row / (128 / share) * 32;
+          float top = -INFINITY, total = 0.f;
+          if (jr < live) {
+#pragma unroll 4
+            for (int x = x0; x <= x1; x += by) top = fmaxf(top, __ldcg(piece(x, c0) + 128 * D + jr));
+            const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
+            for (int x = x0; x <= x1; x += by)
+              total = fmaf(__ldcg(piece(x, c0) + 128 * (D + 1) + jr), exp2_fast(__ldcg(piece(x, c0) + 128 * D + jr) - base), total);
+            const float inv_all = total > 0.f || total != total ? 1.f / total : 0.f;
+            const int jt = paged_token(p, r_lo + jr);
+            T* jdst = static_cast<T*>(p.out) + (int64_t)(done.q0 + jt) * p.out_token +
+                      (int64_t)(done.head * p.group + r_lo + jr - jt * p.group) * p.out_head;
+#pragma unroll 1
+            for (int c = c_from; c < D; c += share * 32) {
+              float v[32];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = 0.f;
+#pragma unroll 1
+              for (int x = x0; x <= x1; x += 2 * by) {
+                float4 u[2][8];
+                float w[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  const int xk = x + k * by;
+                  const float* src = piece(xk, c0);
+                  w[k] = xk <= x1 ? exp2_fast(__ldcg(src + 128 * D + jr) - base) : 0.f;
+#pragma unroll
+                  for (int i = 0; i < 8; ++i)
+                    u[k][i] = xk <= x1 ? __ldcg(reinterpret_cast<const float4*>(src) + (c / 4 + i) * 128 + jr)
+                                       : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) {
+                    v[4 * i] = fmaf(u[k][i].x, w[k], v[4 * i]);
+                    v[4 * i + 1] = fmaf(u[k][i].y, w[k], v[4 * i + 1]);
+                    v[4 * i + 2] = fmaf(u[k][i].z, w[k], v[4 * i + 2]);
+                    v[4 * i + 3] = fmaf(u[k][i].w, w[k], v[4 * i + 3]);
+                  }
+              }
+              if (final) {
+                store(jdst, c, v, inv_all);
+                store(jdst, c + 16, v + 16, inv_all);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; i += 4)
+                  __stcg(reinterpret_cast<float4*>(piece(x0, c0)) + (c / 4 + i / 4) * 128 + jr,
+                         make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+              }
+            }
+          }
+          if (!final) {
+            named_barrier(1 + q, 128);  // all threads of a row have read its statistics
+            if (jr < live && c_from == 0) {
+              __stcg(piece(x0, c0) + 128 * D + jr, top);
+              __stcg(piece(x0, c0) + 128 * (D + 1) + jr, total);
+            }
+          }
+        };
+        uint32_t* ticket = tickets + c0 * 2 + q;
+        uint32_t* run_ticket = tickets + gridDim.x * 2 + (run.x0 * 2 + (run.x0 == c0 ? 1 : 0)) * 2 + q;
+        if (run.runs == 1) {
+          if (last_of(ticket, c1 - c0 + 1)) join(c0, c1, 1, true);
+        } else if (last_of(run_ticket, run.x1 - run.x0 + 1)) {
+          join(run.x0, run.x1, 1, false);
+          if (last_of(ticket, run.runs)) join(c0, c1, run.by, true);
+        }
+        __syncwarp();
+      }
+      __syncwarp();
+    }
+    if (lent) named_barrier(5, 256);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_free(tmem, 512);
+}
+
+namespace {
+
+template <typename T, int D>
+cudaError_t launch_code_chunk(const CodeChunkArgs& a, cudaStream_t st, bool pdl) {
+  using C = CodeChunkCfg<D>;
+  static_assert(C::kSmem <= 227 * 1024, "shared memory");
+  auto kern = paged_attention_code_chunk_kernel<T, D>;
+  static SmemLimit limit;
+  if (const cudaError_t e = limit.raise(kern, C::kSmem); e != cudaSuccess) return e;
+  const int ctas = device_sm_count();
+  if (ctas * 6 > kPagedTickets || (size_t)ctas * 4 * C::kPart * 4 + kPagedTickets * 4 > kPagedWorkspaceBytes)
+    return cudaErrorNotSupported;
+  return launch_kernel(kern, dim3(ctas), dim3(kCodeThreads), C::kSmem, st, pdl, a);
+}
+
+}  // namespace
+
+cudaError_t launch_paged_attention_code_chunk(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl) {
+  // a maximum of scores is one of scaled scores for a positive scale only; eight keys lie in one block
+  if ((dtype != kBF16 && dtype != kF16) || a.dim > 128 || a.block_size % 8 != 0 || !(a.scale > 0.f)) return cudaErrorNotSupported;
+  // units of work (paged_sched.cuh) in 32 bits
+  const long long items = (long long)a.tokens * a.group / kChunkRows + a.requests;
+  if (items * a.kv_heads * ((long long)a.width * a.block_size / kChunkKeys + 2 + kChunkItem) >= INT_MAX)
+    return cudaErrorNotSupported;
+  CodeChunkArgs c{};
+  c.a = a;
+  c.q_tma = paged_q_map(a, dtype, 128, &c.q_map);
+  c.out32 = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_token % 16 == 0 && a.out_head % 16 == 0 && a.dim % 16 == 0;
+  if (dtype == kBF16)
+    return a.dim <= 64 ? launch_code_chunk<__nv_bfloat16, 64>(c, st, pdl) : launch_code_chunk<__nv_bfloat16, 128>(c, st, pdl);
+  return a.dim <= 64 ? launch_code_chunk<__half, 64>(c, st, pdl) : launch_code_chunk<__half, 128>(c, st, pdl);
+}
+
+}  // namespace mlora

@@ -378,7 +378,7 @@ int attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int6
     const bool few = (int64_t)a.max_q_len * (q_heads / c.kv_heads) <= mlora::kDecodeMaxRows;
     const cudaError_t e = few                 ? mlora::launch_paged_attention_decode(a, dtype, st, pdl)
                           : scales == nullptr ? mlora::launch_paged_attention_chunk(a, dtype, st, pdl)
-                                              : cudaErrorNotSupported;
+                                              : mlora::launch_paged_attention_code_chunk(a, dtype, st, pdl);
     if (e != cudaErrorNotSupported) return launched(e, "paged attention launch");
   }
   return launched(mlora::launch_paged_attention_general(a, dtype, vec, st, pdl), "paged attention launch");
