@@ -58,6 +58,7 @@ struct PagedAppendArgs {
   PagedSide side[2];          // K and V; their heads are kv_heads (0: there is no cache, and no slot_map)
   const int32_t* slot_map;
   int tokens, q_heads, kv_heads, dim, block_size;
+  int wide;                   // rows and strides are whole pieces of 32 bytes
   int64_t num_blocks;
   // a cache of e4m3 codes: a scale for each block and head
   float* scale[2];

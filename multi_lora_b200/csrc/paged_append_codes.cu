@@ -11,10 +11,14 @@
 //
 // New rows of a block are a run: consecutive tokens with consecutive slots, which begins where the slot is not the
 // one behind its predecessor's or begins a block. A CTA takes the runs that begin in a window of tokens, whole,
-// with some of the heads, K and V: it has every row that a scale depends on, so nothing
-// is agreed on between CTAs. Four units a thread (two vectors each) wait in registers between the maximum and the
-// codes; more are read again. Memory bounds it, with few rows the latency of
-// slots, rows and scales, one after the other.
+// with some of the heads of K or V: it has every row that a scale depends on, so nothing
+// is agreed on between CTAs. A thread goes through every so many rows of one head with one unit of them (two
+// vectors), once for the largest magnitude and back again for the codes: the last row waits in registers, others come
+// out of L2 again. A window's {cos, sin} are made once, for all of the CTA's heads.
+//
+// Measured over sets of inputs larger than L2, bf16 heads of 128, queries rotated beside: 512 tokens of 64 and 8 heads
+// 9.8 us (20 MB), prompts of 4340 tokens, 32 and 8 heads, 32.7 us (98 MB, 3.0 TB/s): about 240 instructions a
+// unit and turn bound it, as the latency of slots, rows and scales, one after the other, does with few rows.
 #include <cuda_fp8.h>
 
 #include <climits>
@@ -26,14 +30,16 @@
 
 namespace mlora {
 
-constexpr int kCodeUnits = 4, kCodeWindow = 32;
+constexpr int kCodeWindow = 32;
 
 // What the host decides about a launch.
 struct CodeShape {
-  int q_ctas, q_per_cta;   // CTAs that rotate queries, tokens each
-  int units;               // of a row
-  int window, parts, part_heads;
-  int max_rows, turn_rows; // rows that runs of a window can have; of those with {cos, sin} in shared memory
+  int code_ctas, q_per_cta;       // CTAs of codes come first; tokens of each that rotates queries
+  int units;                      // of a row
+  int window, parts, part_items;  // an item: a head of K, or of V
+  int step;                       // rows of an item at once
+  int max_rows, turn_rows;        // rows that runs of a window can have; of those with {cos, sin} in shared memory
+  int scale_at;                   // of shared memory
 };
 
 // The scale of rows whose largest magnitude is `most`: 448 = 1.75 * 2^8.
@@ -42,20 +48,18 @@ __device__ __forceinline__ float code_scale(float most) {
   return most > 0.f ? __uint_as_float((uint32_t)(max(k, -100) + 127) << 23) : 0x1p-100f;
 }
 
-// V values over the scale, rounded to codes at dst.
+// V values over the scale, rounded to codes at dst; `inv`: its reciprocal where that is exact, otherwise 0.
 template <int V>
-__device__ __forceinline__ void store_codes(unsigned char* dst, const float (&x)[V], float scale) {
-  float y[V];
-  if ((__float_as_uint(scale) & 0x7fffffu) == 0) {  // a power of two: its reciprocal is exact
-    const float inv = 1.f / scale;
+__device__ __forceinline__ void store_codes(unsigned char* dst, float (&x)[V], float scale, float inv) {
+  if (inv != 0.f) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) y[i] = x[i] * inv;
+    for (int i = 0; i < V; ++i) x[i] *= inv;
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) y[i] = x[i] / scale;
+    for (int i = 0; i < V; ++i) x[i] /= scale;
   }
   if constexpr (V == 1) {
-    *dst = (unsigned char)__nv_cvt_float_to_fp8(y[0], __NV_SATFINITE, __NV_E4M3);
+    *dst = (unsigned char)__nv_cvt_float_to_fp8(x[0], __NV_SATFINITE, __NV_E4M3);
   } else {
     union {
       typename RawBytes<V>::type raw;
@@ -63,41 +67,42 @@ __device__ __forceinline__ void store_codes(unsigned char* dst, const float (&x)
     } u;
 #pragma unroll
     for (int i = 0; i < V; i += 2)
-      u.pair[i / 2] = __nv_cvt_float2_to_fp8x2(make_float2(y[i], y[i + 1]), __NV_SATFINITE, __NV_E4M3);
+      u.pair[i / 2] = __nv_cvt_float2_to_fp8x2(make_float2(x[i], x[i + 1]), __NV_SATFINITE, __NV_E4M3);
     *reinterpret_cast<typename RawBytes<V>::type*>(dst) = u.raw;
   }
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kRotNT) paged_append_codes_kernel(const PagedAppendArgs p, const CodeShape g) {
+__global__ void __launch_bounds__(kRotNT, 4) paged_append_codes_kernel(const PagedAppendArgs p, const CodeShape g) {
   extern __shared__ __align__(16) unsigned char s_dyn[];
   float2* s_turn = reinterpret_cast<float2*>(s_dyn);
   pdl_wait();
   pdl_trigger();
-  if ((int)blockIdx.x < g.q_ctas) {
-    append_rows<T, V>(p, 0, blockIdx.x, g.q_per_cta, g.units, s_turn);
+  if ((int)blockIdx.x >= g.code_ctas) {
+    append_rows<T, V>(p, 0, blockIdx.x - g.code_ctas, g.q_per_cta, g.units, s_turn);
     return;
   }
   __shared__ int s_rows, s_runs, s_grown;
   __shared__ int s_first[kCodeWindow];  // row that a run begins with
-  int* s_slot = reinterpret_cast<int*>(s_turn + g.turn_rows * p.angles.pairs);  // [max_rows], -1: not of a run that begins here
-  short* s_run = reinterpret_cast<short*>(s_slot + g.max_rows);                // [max_rows]
-  uint32_t* s_most = reinterpret_cast<uint32_t*>(s_run + (g.max_rows + 1) / 2 * 2);  // [window][2 part_heads]
-  float* s_scale = reinterpret_cast<float*>(s_most + g.window * 2 * g.part_heads);
-  float* s_ratio = s_scale + g.window * 2 * g.part_heads;
+  int2* s_place = reinterpret_cast<int2*>(s_turn + g.turn_rows * p.angles.pairs);  // [max_rows] block and slot; block -1: not of a run that begins here
+  short* s_run = reinterpret_cast<short*>(s_place + g.max_rows);                   // [max_rows]
+  uint32_t* s_most = reinterpret_cast<uint32_t*>(s_run + (g.max_rows + 1) / 2 * 2);  // [window][part_items]
+  float2* s_scale = reinterpret_cast<float2*>(s_dyn + g.scale_at);                 // and its reciprocal, if that is exact
   const int tid = threadIdx.x, lane = tid & 31;
-  const int cta = blockIdx.x - g.q_ctas, part = cta % g.parts, t0 = cta / g.parts * g.window;
-  const int head0 = part * g.part_heads, heads = min(g.part_heads, p.kv_heads - head0), items = 2 * heads;
+  const int part = blockIdx.x % g.parts, t0 = blockIdx.x / g.parts * g.window;
+  const int item0 = part * g.part_items, items = min(g.part_items, 2 * p.kv_heads - item0);
 
   // ---- the runs that begin in the window ----
   if (tid < 32) {
     auto slot_at = [&](int t) { return t >= 0 && t < p.tokens ? __ldcg(p.slot_map + t) : -1; };
     const int t = t0 + lane, before = lane < g.window ? slot_at(t - 1) : -1;
-    int slot = lane < g.window ? slot_at(t) : -1;
-    bool begins = slot >= 0 && (before < 0 || before + 1 != slot || slot % p.block_size == 0);
-    if (slot >= 0 && slot / p.block_size >= p.num_blocks) {
+    const int slot = lane < g.window ? slot_at(t) : -1;
+    int block = slot >= 0 ? slot / p.block_size : -1;
+    const int off = slot - block * p.block_size;
+    bool begins = slot >= 0 && (before < 0 || before + 1 != slot || off == 0);
+    if (block >= p.num_blocks) {
       if (part == 0) flag_error(p.status, kErrKvRange);
-      slot = -1;
+      block = -1;
       begins = false;
     }
     const unsigned mask = __ballot_sync(0xffffffffu, begins);
@@ -105,21 +110,21 @@ __global__ void __launch_bounds__(kRotNT) paged_append_codes_kernel(const PagedA
     int rows = 0;
     if (mask != 0u) {
       if (lane < g.window) {
-        s_slot[lane] = run >= 0 ? slot : -1;
+        s_place[lane] = make_int2(run >= 0 ? block : -1, off);
         s_run[lane] = (short)run;
       }
       if (begins) s_first[run] = lane;
-      const int last = __shfl_sync(0xffffffffu, slot, g.window - 1), last_run = __shfl_sync(0xffffffffu, run, 31);
+      const int last = __shfl_sync(0xffffffffu, slot, g.window - 1), last_block = __shfl_sync(0xffffffffu, block, g.window - 1),
+                last_off = __shfl_sync(0xffffffffu, off, g.window - 1), last_run = __shfl_sync(0xffffffffu, run, 31);
       rows = min(g.window, p.tokens - t0);
       // the last run behind the window's end: at most the rest of its block
-      for (int most = last >= 0 ? p.block_size - 1 - last % p.block_size : 0; most > 0; most -= 32) {
-        const int r = rows + lane;
-        const int want = last + 1 + r - g.window;
-        const bool goes = lane < most && slot_at(t0 + r) == want;
+      for (int most = last_block >= 0 ? p.block_size - 1 - last_off : 0; most > 0; most -= 32) {
+        const int r = rows + lane, behind = 1 + r - g.window;
+        const bool goes = lane < most && slot_at(t0 + r) == last + behind;
         const unsigned more = __ballot_sync(0xffffffffu, goes);
         const int n = more == 0xffffffffu ? 32 : __ffs(~more) - 1;
         if (lane < n) {
-          s_slot[r] = want;
+          s_place[r] = make_int2(last_block, last_off + behind);
           s_run[r] = (short)last_run;
         }
         rows += n;
@@ -136,118 +141,128 @@ __global__ void __launch_bounds__(kRotNT) paged_append_codes_kernel(const PagedA
   const int rows = s_rows, runs = s_runs;
   if (rows == 0) return;
   for (int i = tid; i < runs * items; i += kRotNT) s_most[i] = 0u;
-  const bool rotated = p.angles.turns != nullptr;
-  const int all = rows * items * g.units, chunks = (all + kRotNT * kCodeUnits - 1) / (kRotNT * kCodeUnits);
 
-  struct Unit {
-    Vec<T, V> x[2];
-    RotaryUnit un;
-    int row, item;  // row < 0: none
+  // the scales that the blocks have, on their way meanwhile
+  auto scale_at = [&](int i, bool& begun) {
+    const int run = i / items, item = item0 + i - run * items, side = item >= p.kv_heads, h = item - side * p.kv_heads;
+    const int2 place = s_place[s_first[run]];
+    begun = place.y > 0;
+    return p.scale[side] + place.x * p.scale_block[side] + h * p.scale_head[side];
   };
-  Unit w[kCodeUnits];
-  auto load = [&](int chunk) {
-#pragma unroll
-    for (int k = 0; k < kCodeUnits; ++k) {
-      const int at = (chunk * kCodeUnits + k) * kRotNT + tid;
-      w[k].row = -1;
-      if (at >= all) continue;
-      const int piece = at / g.units, u = at - piece * g.units, row = piece / items;
-      w[k].item = piece - row * items;
-      if (s_slot[row] < 0) continue;
-      w[k].row = row;
-      const int side = w[k].item >= heads, h = head0 + w[k].item - side * heads;
-      const PagedSide& s = p.side[side];
-      w[k].un = rotary_unit(p.angles, side == 0 && rotated, p.dim, V, u);
-      const T* src = static_cast<const T*>(s.src) + (int64_t)(t0 + row) * s.src_token + h * s.src_head;
-      w[k].x[0].load(src + w[k].un.e0);
-      if (w[k].un.both) w[k].x[1].load(src + w[k].un.e1);
-    }
+  float held_scale = 0.f;
+  if (tid < runs * items) {
+    bool begun;
+    const float* at = scale_at(tid, begun);
+    if (begun) held_scale = __ldcg(at);
+  }
+
+  // A thread has one item, one unit of its rows, and every step-th row.
+  const int lane_row = tid / (g.units * items), mine = lane_row < g.step ? tid - lane_row * g.units * items : -1;
+  const int own = mine >= 0 ? mine / g.units : 0, u = mine - own * g.units;
+  const int side = item0 + own >= p.kv_heads, h = item0 + own - side * p.kv_heads;
+  const bool rotated = p.angles.turns != nullptr && item0 < p.kv_heads;
+  const RotaryUnit un = rotary_unit(p.angles, side == 0 && rotated, p.dim, V, u);
+  const PagedSide& s = p.side[side];
+  const T* from = static_cast<const T*>(s.src) + t0 * s.src_token + h * s.src_head;
+  unsigned char* to = static_cast<unsigned char*>(s.dst) + h * s.head;
+  // its rows, in this order and back again: the last one waits in registers in between
+  auto next = [&](int row, int by) {
+    do row += by;
+    while (row >= 0 && row < rows && s_place[row].x < 0);
+    return row >= 0 && row < rows ? row : -1;
   };
-  auto values = [&](const Unit& w, float (&a)[V], float (&b)[V]) {
-    w.x[0].to_f(a);
-    w.x[1].to_f(b);
-    if (!w.un.turned) return;
-    if (w.row < g.turn_rows) {
-      rotary_apply<V>(p.angles.interleaved != 0, s_turn + w.row * p.angles.pairs + w.un.pair, a, b);
+  auto load = [&](int row, Vec<T, V> (&x)[2]) {
+    const T* src = from + row * s.src_token;
+    x[0].load(src + un.e0);
+    if (un.both) x[1].load(src + un.e1);
+  };
+  auto values = [&](int row, const Vec<T, V> (&x)[2], float (&a)[V], float (&b)[V]) {
+    x[0].to_f(a);
+    x[1].to_f(b);
+    if (!un.turned) return;
+    float2 turn[V];
+    if (row < g.turn_rows) {
+      rotary_row<V>(p.angles, s_turn + row * p.angles.pairs, un.pair, turn);
     } else {
-      float2 cs[V];
-      const int position = __ldcg(p.angles.positions + t0 + w.row);
+      const int position = __ldcg(p.angles.positions + t0 + row);
 #pragma unroll
-      for (int i = 0; i < V; ++i) cs[i] = rotary_turn(__ldg(p.angles.turns + w.un.pair + i), position, p.angles.factor);
-      rotary_apply<V>(p.angles.interleaved != 0, cs, a, b);
+      for (int i = 0; i < V; ++i) turn[i] = rotary_turn(__ldg(p.angles.turns + un.pair + i), position, p.angles.factor);
     }
+    rotary_apply<V>(p.angles.interleaved != 0, turn, a, b);
   };
-
-  load(0);
-  if (rotated) rotary_table(p.angles, t0, min(rows, g.turn_rows), s_turn);
+  Vec<T, V> x[2];
+  int row = mine >= 0 ? next(lane_row - g.step, g.step) : -1;
+  if (row >= 0) load(row, x);
+  if (rotated) rotary_table<V>(p.angles, t0, min(rows, g.turn_rows), s_turn);
   __syncthreads();
-  // ---- the largest magnitudes ----
-  const bool lanes_share = (g.units & (g.units - 1)) == 0 && g.units <= 32;  // a row's units lie in aligned lanes
-  for (int c = 0; c < chunks; ++c) {
-    if (c > 0) load(c);
+  // ---- the largest magnitudes, as whole numbers in the same order ----
+  if (row >= 0) {
+    uint32_t most = 0u;
+    while (true) {
+      const int after = next(row, g.step);
+      Vec<T, V> y[2];
+      if (after >= 0) load(after, y);
+      float a[V], b[V];
+      values(row, x, a, b);
 #pragma unroll
-    for (int k = 0; k < kCodeUnits; ++k) {
-      uint32_t most = 0u;  // of magnitudes as whole numbers, in the same order
-      if (w[k].row >= 0) {
-        float a[V], b[V];
-        values(w[k], a, b);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const uint32_t ua = __float_as_uint(a[i]) & 0x7fffffffu, ub = __float_as_uint(b[i]) & 0x7fffffffu;
-          if (ua < 0x7f800000u) most = max(most, ua);
-          if (ub < 0x7f800000u && w[k].un.both) most = max(most, ub);
-        }
+      for (int i = 0; i < V; ++i) {
+        const uint32_t ua = __float_as_uint(a[i]) & 0x7fffffffu, ub = __float_as_uint(b[i]) & 0x7fffffffu;
+        if (ua < 0x7f800000u) most = max(most, ua);
+        if (ub < 0x7f800000u && un.both) most = max(most, ub);
       }
-      if (lanes_share)
-        for (int o = g.units >> 1; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-      if (w[k].row >= 0 && most != 0u && (!lanes_share || (lane & (g.units - 1)) == 0))
-        atomicMax(s_most + s_run[w[k].row] * items + w[k].item, most);
+      if (after < 0 || s_run[after] != s_run[row]) {
+        if (most != 0u) atomicMax(s_most + s_run[row] * items + own, most);
+        most = 0u;
+      }
+      if (after < 0) break;
+      row = after;
+      x[0] = y[0];
+      x[1] = y[1];
     }
   }
   __syncthreads();
   // ---- the scales ----
   for (int i = tid; i < runs * items; i += kRotNT) {
-    const int run = i / items, item = i - run * items, side = item >= heads, h = head0 + item - side * heads;
-    const int slot = s_slot[s_first[run]], block = slot / p.block_size;
-    float* at = p.scale[side] + block * p.scale_block[side] + h * p.scale_head[side];
+    bool begun;
+    float* at = scale_at(i, begun);
     float scale = code_scale(__uint_as_float(s_most[i])), ratio = 1.f;
-    if (slot - block * p.block_size > 0) {
-      const float old = __ldcg(at);
+    if (begun) {
+      const float old = i == tid ? held_scale : __ldcg(at);
       if (old < scale) ratio = old / scale;
       scale = fmaxf(scale, old);
     }
     *at = scale;
-    s_scale[i] = scale;
-    s_ratio[i] = ratio;
+    s_scale[i] = make_float2(scale, (__float_as_uint(scale) & 0x7fffffu) == 0 ? 1.f / scale : 0.f);
+    s_most[i] = __float_as_uint(ratio);
     if (ratio != 1.f) s_grown = 1;
   }
   __syncthreads();
   // ---- the codes ----
-  for (int c = chunks - 1; c >= 0; --c) {
-    if (c < chunks - 1) load(c);
-#pragma unroll
-    for (int k = 0; k < kCodeUnits; ++k) {
-      if (w[k].row < 0) continue;
-      float a[V], b[V];
-      values(w[k], a, b);
-      const int slot = s_slot[w[k].row], block = slot / p.block_size, off = slot - block * p.block_size;
-      const int side = w[k].item >= heads, h = head0 + w[k].item - side * heads;
-      const PagedSide& s = p.side[side];
-      unsigned char* dst = static_cast<unsigned char*>(s.dst) + block * s.block + off * s.slot + h * s.head;
-      const float scale = s_scale[s_run[w[k].row] * items + w[k].item];
-      store_codes<V>(dst + w[k].un.e0, a, scale);
-      if (w[k].un.both) store_codes<V>(dst + w[k].un.e1, b, scale);
-    }
+  while (row >= 0) {
+    const int after = next(row, -g.step);
+    Vec<T, V> y[2];
+    if (after >= 0) load(after, y);
+    float a[V], b[V];
+    values(row, x, a, b);
+    const int2 place = s_place[row];
+    unsigned char* dst = to + place.x * s.block + place.y * s.slot;
+    const float2 scale = s_scale[s_run[row] * items + own];
+    store_codes<V>(dst + un.e0, a, scale.x, scale.y);
+    if (un.both) store_codes<V>(dst + un.e1, b, scale.x, scale.y);
+    row = after;
+    x[0] = y[0];
+    x[1] = y[1];
   }
   if (s_grown == 0) return;
   // ---- older rows of blocks whose scales have grown ----
   for (int i = 0; i < runs * items; ++i) {
-    const float ratio = s_ratio[i];
+    const float ratio = __uint_as_float(s_most[i]);
     if (ratio == 1.f) continue;
-    const int run = i / items, item = i - run * items, side = item >= heads, h = head0 + item - side * heads;
-    const int slot = s_slot[s_first[run]], block = slot / p.block_size, off = slot - block * p.block_size;
+    const int run = i / items, item = item0 + i - run * items, side = item >= p.kv_heads, h = item - side * p.kv_heads;
+    const int2 place = s_place[s_first[run]];
+    const int off = place.y;
     const PagedSide& s = p.side[side];
-    unsigned char* base = static_cast<unsigned char*>(s.dst) + block * s.block + h * s.head;
+    unsigned char* base = static_cast<unsigned char*>(s.dst) + place.x * s.block + h * s.head;
     const int pieces = p.dim / V;
     for (int e = tid; e < off * pieces; e += kRotNT) {
       const int row = e / pieces;
@@ -260,7 +275,7 @@ __global__ void __launch_bounds__(kRotNT) paged_append_codes_kernel(const PagedA
       float x[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) x[j] = __half2float(__half(__nv_cvt_fp8_to_halfraw(u.code[j], __NV_E4M3))) * ratio;
-      store_codes<V>(at, x, 1.f);
+      store_codes<V>(at, x, 1.f, 1.f);
     }
   }
 }
@@ -271,26 +286,34 @@ template <typename T, int V>
 cudaError_t codes_v(const PagedAppendArgs& a, cudaStream_t st, bool pdl) {
   CodeShape g{};
   g.units = (a.dim + 2 * V - 1) / (2 * V);
-  g.q_per_cta = a.q_heads > 0 ? tokens_per_cta(a, a.q_heads, g.units) : 1;
-  g.q_ctas = a.q_heads > 0 ? (a.tokens + g.q_per_cta - 1) / g.q_per_cta : 0;
-  // heads for which a whole block's rows wait in registers; windows that leave every SM about eight CTAs
-  const int block = a.block_size < a.tokens ? a.block_size : a.tokens;
-  const int64_t per_head = 2ll * block * g.units, room = (int64_t)kRotNT * kCodeUnits / per_head;
-  g.part_heads = room < 1 ? 1 : room > a.kv_heads ? a.kv_heads : (int)room;
-  g.parts = (a.kv_heads + g.part_heads - 1) / g.part_heads;
-  const int64_t want = (int64_t)a.tokens * g.parts / (8 * device_sm_count());
-  g.window = want < 1 ? 1 : want > kCodeWindow ? kCodeWindow : (int)want;
+  g.q_per_cta = a.q_heads > 0 ? tokens_per_cta(a, g.units) : 1;
+  const int q_ctas = a.q_heads > 0 ? (a.tokens + g.q_per_cta - 1) / g.q_per_cta : 0;
+  // Items for which a whole block's rows are four units a thread, and windows of as many tokens (a window's
+  // runs have as many rows as it has tokens, more or less), but no more than leave every SM two CTAs. (Prompts of 4340
+  // tokens 32.7 us; two units a thread 38.1, eight 37.1; 512 single tokens 9.8, 9.9 and 11.2, four CTAs an SM 14.6.)
+  const int block = a.block_size < a.tokens ? a.block_size : a.tokens, all_items = 2 * a.kv_heads;
+  const int64_t full = 4 * kRotNT / g.units, room = full / block;
+  g.part_items = room < 1 ? 1 : room > all_items ? all_items : (int)room;
+  if (g.part_items > kRotNT / g.units) g.part_items = kRotNT / g.units;
+  g.step = kRotNT / (g.units * g.part_items);
+  g.parts = (all_items + g.part_items - 1) / g.part_items;
+  const int64_t even = (int64_t)a.tokens * g.parts / (2 * device_sm_count()), rows = full / g.part_items;
+  const int64_t window = even < rows ? even : rows;
+  g.window = window < 1 ? 1 : window > kCodeWindow ? kCodeWindow : (int)window;
   g.max_rows = g.window + a.block_size;
   if (a.angles.turns != nullptr) {
     const int most = 48 * 1024 / (a.angles.pairs * (int)sizeof(float2));
     g.turn_rows = g.max_rows < most ? g.max_rows : most;
-    if (g.q_per_cta > g.turn_rows && g.q_ctas > 0) g.turn_rows = g.q_per_cta;
+    if (g.q_per_cta > g.turn_rows) g.turn_rows = g.q_per_cta;
   }
-  const size_t smem = (size_t)g.turn_rows * a.angles.pairs * sizeof(float2) + g.max_rows * sizeof(int) +
-                      (g.max_rows + 1) / 2 * 2 * sizeof(short) + (size_t)g.window * 2 * g.part_heads * 3 * sizeof(float);
-  const int64_t ctas = ((int64_t)a.tokens + g.window - 1) / g.window * g.parts + g.q_ctas;
+  const size_t most_at = (size_t)g.turn_rows * a.angles.pairs * sizeof(float2) + g.max_rows * sizeof(int2) +
+                         (g.max_rows + 1) / 2 * 2 * sizeof(short);
+  g.scale_at = (int)((most_at + (size_t)g.window * g.part_items * sizeof(uint32_t) + 7) / 8 * 8);
+  const size_t smem = g.scale_at + (size_t)g.window * g.part_items * sizeof(float2);
+  const int64_t code_ctas = ((int64_t)a.tokens + g.window - 1) / g.window * g.parts, ctas = code_ctas + q_ctas;
+  g.code_ctas = (int)code_ctas;
   if (a.block_size > kAppendMaxBlock || ctas > INT_MAX || smem > 160 * 1024 ||
-      (int64_t)g.max_rows * 2 * g.part_heads * g.units > INT_MAX)
+      (int64_t)g.max_rows * g.part_items * g.units > INT_MAX)
     return cudaErrorInvalidValue;
   auto kern = paged_append_codes_kernel<T, V>;
   static SmemLimit limit;

@@ -84,10 +84,11 @@ int append_common(mlora::PagedAppendArgs& a, const mlora_rotary_t* rotary, const
   return MLORA_OK;
 }
 
-// Elements at once that the rows of q, out, k and v allow: 16 bytes, 8 or one element.
-int append_vec(const mlora::PagedAppendArgs& a, int es, bool codes) {
-  for (int bytes = 16; bytes >= 8; bytes /= 2) {
-    const int v = bytes / es;
+// Elements at once that the rows of q, out, k and v allow: 16 bytes, 8 or one element; `wide`: 32 bytes where a
+// unit's two vectors lie side by side.
+int append_vec(mlora::PagedAppendArgs& a, int es, bool codes) {
+  for (int bytes = 32; bytes >= 8; bytes /= 2) {
+    const int v = (bytes < 16 ? bytes : 16) / es;
     if (v < 2 || a.dim % v != 0 || a.angles.pairs % v != 0) continue;
     if (a.q_heads > 0 && !(pieces(a.q, es, a.q_token, a.q_head, 0, bytes) && pieces(a.out, es, a.out_token, a.out_head, 0, bytes)))
       continue;
@@ -96,6 +97,7 @@ int append_vec(const mlora::PagedAppendArgs& a, int es, bool codes) {
       if (a.kv_heads > 0)
         ok = ok && pieces(s.src, es, s.src_token, s.src_head, 0, bytes) &&
              pieces(s.dst, codes ? 1 : es, s.block, s.slot, s.head, codes ? v : bytes);
+    a.wide = ok && bytes == 32;
     if (ok) return v;
   }
   return 1;

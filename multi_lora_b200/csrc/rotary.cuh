@@ -64,12 +64,29 @@ struct Vec {
   __device__ __forceinline__ void load(const T* p) { raw = __ldcg(reinterpret_cast<const Raw*>(p)); }
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Raw*>(p) = raw; }
   __device__ __forceinline__ void to_f(float (&f)[V]) const {
+    if constexpr (sizeof(T) == 2 && V > 1) {
+      uint32_t w[V / 2];
+      memcpy(w, &raw, sizeof(raw));
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = Num<T>::to_f(at[i]);
+      for (int i = 0; i < V; i += 2) {
+        f[i] = Pack2<T>::lo(w[i / 2]);
+        f[i + 1] = Pack2<T>::hi(w[i / 2]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = Num<T>::to_f(at[i]);
+    }
   }
   __device__ __forceinline__ void from_f(const float (&f)[V]) {
+    if constexpr (sizeof(T) == 2 && V > 1) {  // two roundings an instruction
+      uint32_t w[V / 2];
 #pragma unroll
-    for (int i = 0; i < V; ++i) at[i] = Num<T>::from_f(f[i]);
+      for (int i = 0; i < V; i += 2) w[i / 2] = pack_round2<T>(f[i], f[i + 1]);
+      memcpy(&raw, w, sizeof(raw));
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) at[i] = Num<T>::from_f(f[i]);
+    }
   }
 };
 
@@ -95,35 +112,49 @@ __device__ __forceinline__ RotaryUnit rotary_unit(const RotaryAngles& a, bool ro
   return r;
 }
 
-// The two vectors of a rotated unit, `cs` the {cos, sin} of its pairs.
+// A unit's two vectors where they lie side by side and 32 bytes allow it: whole sectors at once.
+template <typename T, int V>
+__device__ __forceinline__ void load_both(Vec<T, V> (&x)[2], const T* p) {
+  static_assert(V * sizeof(T) == 16, "32 bytes");
+  uint4 a, b;
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+               : "l"(p)
+               : "memory");
+  x[0].raw = a;
+  x[1].raw = b;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_both(T* p, const Vec<T, V> (&x)[2]) {
+  static_assert(V * sizeof(T) == 16, "32 bytes");
+  const uint4 a = x[0].raw, b = x[1].raw;
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w),
+               "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
+
+// One pair; the same roundings in every kernel and width.
+__device__ __forceinline__ void rotary_pair(float2 t, float& a, float& b) {
+  const float x = __fmaf_rn(a, t.x, -__fmul_rn(b, t.y));
+  b = __fmaf_rn(b, t.x, __fmul_rn(a, t.y));
+  a = x;
+}
+
+// The two vectors of a rotated unit, `t` the {cos, sin} of its pairs.
 template <int V>
-__device__ __forceinline__ void rotary_apply(bool interleaved, const float2* cs, float (&a)[V], float (&b)[V]) {
-  float2 t[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) t[i] = cs[i];
-  if (interleaved) {
-    if constexpr (V == 1) {
-      const float x = a[0] * t[0].x - b[0] * t[0].y;
-      b[0] = b[0] * t[0].x + a[0] * t[0].y;
-      a[0] = x;
-    } else {
+__device__ __forceinline__ void rotary_apply(bool interleaved, const float2 (&t)[V], float (&a)[V], float (&b)[V]) {
+  if constexpr (V > 1) {
+    if (interleaved) {
 #pragma unroll
       for (int i = 0; i < V; i += 2) {
-        const float x = a[i] * t[i / 2].x - a[i + 1] * t[i / 2].y, y = b[i] * t[V / 2 + i / 2].x - b[i + 1] * t[V / 2 + i / 2].y;
-        a[i + 1] = a[i + 1] * t[i / 2].x + a[i] * t[i / 2].y;
-        b[i + 1] = b[i + 1] * t[V / 2 + i / 2].x + b[i] * t[V / 2 + i / 2].y;
-        a[i] = x;
-        b[i] = y;
+        rotary_pair(t[i / 2], a[i], a[i + 1]);
+        rotary_pair(t[V / 2 + i / 2], b[i], b[i + 1]);
       }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float x = a[i] * t[i].x - b[i] * t[i].y;
-      b[i] = b[i] * t[i].x + a[i] * t[i].y;
-      a[i] = x;
+      return;
     }
   }
+#pragma unroll
+  for (int i = 0; i < V; ++i) rotary_pair(t[i], a[i], b[i]);
 }
 
 }  // namespace mlora
