@@ -1,9 +1,10 @@
 // Attention of chunks over a paged cache of e4m3 codes, on the fifth-generation tensor cores.
 //
 // Items, halves of tiles, TMEM and the running maximum are those of csrc/paged_attn_tc.cu. What differs is how K and V
-// come to the tensor cores: a warpgroup of its own fetches codes from their pages, a tile ahead of
-// what it works on, and writes them as 16-bit values in the swizzled tiles that the products read: K in the queries'
-// type, V in f16, both exact. Scales stay in fp32 outside the products:
+// come to the tensor cores: TMA brings the codes' pages, and a warpgroup of its own
+// writes them as 16-bit values into the swizzled tiles that the products read: K in the queries'
+// type, V in f16, both exact. (It takes codes to registers before it waits for room to write, so its registers are a
+// stage of the pipeline too.) Scales stay in fp32 outside the products:
 //   S = Q C_K^T,  x = S f_K - m,  P = exp2(x) f_V / F,  O += P C_V,   F the largest f_V so far
 // with f constant over each eight keys, so a key's scale costs nothing beside the scale that a score has anyway (the
 // maximum is taken of each eight scores first), and a value's one multiplication of two probabilities.
@@ -30,8 +31,9 @@ namespace mlora {
 constexpr int kCodeThreads = 512;  // Q and tensor cores, two warpgroups of softmax, one of codes
 
 struct CodeChunkArgs {
-  CUtensorMap q_map;
+  CUtensorMap k_map, v_map, q_map;
   PagedAttnArgs a;
+  int box;    // rows of a TMA box of codes
   int q_tma;  // Q tiles are boxes of q_map (group divides 128)
   int out32;  // rows of the output allow 32-byte stores
 };
@@ -40,11 +42,13 @@ template <int D>
 struct CodeChunkCfg {
   static constexpr int kSlot = kChunkKeys * D * 2;  // K or V of a tile
   static constexpr int kQ = 128 * D * 2;            // one tile of Q
-  static constexpr int kSlots = 160 * 1024 / kSlot;
-  static constexpr int kSmem = 2 * kQ + kSlots * kSlot + 1024;
+  static constexpr int kRaw = kChunkKeys * D;       // codes of K or V of a tile
+  static constexpr int kRaws = D == 128 ? 2 : 4;
+  static constexpr int kSlots = D == 128 ? 4 : 8;
+  static constexpr int kSmem = 2 * kQ + kSlots * kSlot + kRaws * kRaw + 1024;
   static constexpr int kPart = 128 * (D + 2);  // floats of a tile's piece
-  // tiles whose scales wait: K of a tile gets its slot when V of the third tile before it (D = 64: scores of the fifth,
-  // so values of the sixth) is done with
+  // tiles whose scales wait: K of a tile gets its slot when the scores of the second (D = 64: fourth) tile before it are
+  // done, so all of the one before that is
   static constexpr int kScaleTiles = D == 128 ? 4 : 8;
 };
 
@@ -124,30 +128,27 @@ __device__ __forceinline__ uint2 code_values(uint32_t x) {
   return make_uint2(a, b);
 }
 
-// Pieces of 16 codes (the chunk-th of rows row0, row0 + 512 / D, ..) as values of T, in swizzled rows of 128 bytes.
-template <typename T, int D>
-__device__ __forceinline__ void code_put(unsigned char* to, int chunk, int row0, const uint4 (&u)[D / 16]) {
-#pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
-    const int row = row0 + i * (512 / D);
-    const uint2 a = code_values<T>(u[i].x), b = code_values<T>(u[i].y), c = code_values<T>(u[i].z), d = code_values<T>(u[i].w);
-    *reinterpret_cast<uint4*>(to + row * 128 + (((chunk * 2) ^ (row & 7)) << 4)) = make_uint4(a.x, a.y, b.x, b.y);
-    *reinterpret_cast<uint4*>(to + row * 128 + (((chunk * 2 + 1) ^ (row & 7)) << 4)) = make_uint4(c.x, c.y, d.x, d.y);
-  }
+// 16 codes as values of T: the chunk-th piece of a swizzled row of 128 bytes.
+template <typename T>
+__device__ __forceinline__ void code_put(unsigned char* row_at, int row, int chunk, const uint4& u) {
+  const uint2 a = code_values<T>(u.x), b = code_values<T>(u.y), c = code_values<T>(u.z), d = code_values<T>(u.w);
+  *reinterpret_cast<uint4*>(row_at + (((chunk * 2) ^ (row & 7)) << 4)) = make_uint4(a.x, a.y, b.x, b.y);
+  *reinterpret_cast<uint4*>(row_at + (((chunk * 2 + 1) ^ (row & 7)) << 4)) = make_uint4(c.x, c.y, d.x, d.y);
 }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kCodeThreads, 1)
 paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
   using C = CodeChunkCfg<D>;
-  constexpr int NS = C::kSlots, HALF = kChunkKeys * 128;
+  constexpr int NS = C::kSlots, NR = C::kRaws, HALF = kChunkKeys * 128;
   constexpr bool TWO = !Num<T>::is_bf16;      // terms of P
   constexpr float kRaise = 4.f, kUp = 11.f;   // in powers of two
   constexpr uint32_t S_COL = 0, O_COL = 256;
   extern __shared__ __align__(1024) unsigned char s_raw[];
-  __shared__ __align__(8) uint64_t full[NS], empty[NS], q_ready[2], q_free[2], s_full[2][2], p_ready[2][2], pv_done[2][2];
+  __shared__ __align__(8) uint64_t full[NS], empty[NS], raw_full[NR], raw_empty[NR], q_ready[2], q_free[2], s_full[2][2], p_ready[2][2], pv_done[2][2];
   constexpr int kScaleTiles = C::kScaleTiles;
   __shared__ __align__(16) float s_scale[kScaleTiles][2][kChunkKeys / 8];  // of K and V, for each eight keys
+  __shared__ __align__(16) float s_raw_scale[NR / 2][2][kChunkKeys / 8];  // of a tile whose codes have come, with K
   __shared__ uint32_t s_tmem;
   __shared__ int s_last[2];
   __shared__ bool s_skipped;
@@ -158,12 +159,16 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = same_in_warp(tid >> 5);
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~uintptr_t(1023));
-  unsigned char* ring = smem + 2 * C::kQ;
+  unsigned char *ring = smem + 2 * C::kQ, *raw = ring + NS * C::kSlot;
 
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&full[s], 4);   // the warps that write codes
       mbar_init(&empty[s], 2);  // both warps of the tensor cores
+    }
+    for (int s = 0; s < NR; ++s) {
+      mbar_init(&raw_full[s], 1);
+      mbar_init(&raw_empty[s], 4);
     }
     for (int q = 0; q < 2; ++q) {
       mbar_init(&q_ready[q], 1);
@@ -176,6 +181,8 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
     }
     fence_barrier_init();
     s_taken = 0u;
+    tma_prefetch_map(&args.k_map);
+    tma_prefetch_map(&args.v_map);
     if (args.q_tma) tma_prefetch_map(&args.q_map);
   }
   if (warp == 1) tmem_alloc(&s_tmem, 512);
@@ -205,7 +212,7 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
       },
       split, req, found, before, in_req);
   skipped = __syncthreads_or(skipped);  // and the barriers are initialised, and s_tmem is there
-  if (tid == 96) s_skipped = skipped;   // for its own warp, at the end
+  if (tid == 0) s_skipped = skipped;    // for its own warp, at the end
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   PagedCursor<ChunkSplit> cur(split);
@@ -266,7 +273,7 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
   // Registers: 512 threads are launched with 128 each (65536); the warps of Q and the tensor cores keep 64, those of
   // codes 112, and the softmax warps take 168: 128 * 64 + 128 * 112 + 256 * 168 = 65536.
   if (warp < 4) {
-    regs_down<64>();
+    regs_down<80>();
     if (warp == 1 || warp == 2) {  // ---- tensor cores, a warp a tile of rows: S of a half, then O of the half before ----
       const int q = warp - 1;
       constexpr uint32_t idesc_s = umma_idesc_f16(Num<T>::is_bf16, 128, kHalfKeys);
@@ -396,122 +403,137 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
         }
         if (cur.advance()) next_item();
       }
-    } else {  // ---- rows that nobody has ----
       __syncwarp();
       if (s_skipped) paged_zero_uncomputed<T>(p, split.total > 0 ? INT_MAX : -1);
       else paged_zero_rest<T>(p);
-    }
-  } else if (warp >= 12) {  // ---- codes of K and V, 32 keys of each tile a warp ----
-    regs_down<112>();
-    constexpr int PASSES = D / 16, ROWS = 32 / PASSES;  // pieces of 16 codes a thread, keys at once
-    const int w = warp - 12;
-    // eight lanes side by side store to all banks: of two keys the first four pieces, or the last four
-    const int chunk = (lane & 3) | (D == 128 ? lane >> 4 << 2 : 0), row0 = w * 32 + (D == 128 ? lane >> 2 & 3 : lane >> 2);
-    int slot = 0, round = 0;
-    uint32_t tile_no = 0;
-    while (cur.take(it.n)) {
-      const int32_t* table = p.tables + it.req * p.table_stride;
-      const int j_first = (it.tile0 + cur.tile) * kChunkKeys;
-      int seen_lo, seen_hi;
-      chunk_seen(p, it, seen_lo, seen_hi);
-      // eight keys a lane, of the warp's 32: their block (-1: nothing of it is seen or it is outside the cache) and slot
-      auto lookup = [&](int k, int& block, int& off) {
-        const int j = j_first + k * kChunkKeys + w * 32 + lane * 8;
-        block = -1;
-        off = 0;
-        if (lane < 4 && j < it.end && j + 8 > it.first) {
-          const int e = __ldcg(table + j / p.block_size);
-          off = j % p.block_size;
-          if (e >= 0 && e < p.num_blocks) block = e;
-          else flag_error(p.status, kErrKvRange);
-        }
-      };
-      auto fetch = [&](uint4* u, int k, int block, int off, const void* base, int64_t s_block, int64_t s_slot, int64_t s_head) {
-        const unsigned char* from = static_cast<const unsigned char*>(base) + it.head * s_head + chunk * 16;
+    } else {  // ---- codes of K and V of each tile, a box of a page a lane, and their scales ----
+      const int boxes = kChunkKeys / args.box, eights = args.box / 8;
+      int slot = 0, round = 0;
+      while (cur.take(it.n)) {
+        const int32_t* table = p.tables + it.req * p.table_stride;
+        auto lookup = [&](int k, int& block, int& off) {
+          const int j = (it.tile0 + cur.tile + k) * kChunkKeys + lane * args.box;
+          block = (int)p.num_blocks;  // out of range: zeros
+          off = 0;
+          if (lane < boxes && j < it.end && j + args.box > it.first) {
+            const int e = __ldcg(table + j / p.block_size);
+            off = j % p.block_size;
+            if (e >= 0 && e < p.num_blocks) block = e;
+            else flag_error(p.status, kErrKvRange);
+          }
+        };
+        auto scales_of = [&](int block, float& a, float& b) {
+          a = b = 0.f;
+          if (block < p.num_blocks) {
+            a = __ldcg(p.k_scale + block * p.ks_block + it.head * p.ks_head);
+            b = __ldcg(p.v_scale + block * p.vs_block + it.head * p.vs_head);
+          }
+        };
+        // table entries are asked for two tiles ahead, the scales that hang on them one
+        int next[2] = {(int)p.num_blocks, (int)p.num_blocks}, next_off[2] = {0, 0};
+        float next_k, next_v;
+        lookup(0, next[0], next_off[0]);
+        if (cur.len > 1) lookup(1, next[1], next_off[1]);
+        scales_of(next[0], next_k, next_v);
+        for (int k = 0; k < cur.len; ++k) {
+          const int block = next[0], off = next_off[0];
+          const float fk = next_k, fv = next_v;
+          next[0] = next[1];
+          next_off[0] = next_off[1];
+          if (k + 1 < cur.len) scales_of(next[0], next_k, next_v);
+          if (k + 2 < cur.len) lookup(k + 2, next[1], next_off[1]);
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-          const int eight = i * ROWS / 8, row = row0 + i * ROWS, j = j_first + k * kChunkKeys + row;
-          const int b = __shfl_sync(0xffffffffu, block, eight), o = __shfl_sync(0xffffffffu, off, eight) + (row & 7);
-          u[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (b >= 0 && j >= it.first && j < it.end && chunk * 16 < p.dim) {
-            const unsigned char* src = from + b * s_block + o * s_slot;
-            if (chunk * 16 + 16 <= p.dim) {
-              u[i] = __ldcg(reinterpret_cast<const uint4*>(src));
-            } else {
-              const uint2 h = __ldcg(reinterpret_cast<const uint2*>(src));
-              u[i].x = h.x;
-              u[i].y = h.y;
+          for (int side = 0; side < 2; ++side) {
+            if (round > 0) ok = __all_sync(0xffffffffu, ok && mbar_poll(&raw_empty[slot], (round - 1) & 1, p.status));
+            if (ok) {
+              if (side == 0 && lane < boxes)
+                for (int i = 0; i < eights; ++i) {
+                  s_raw_scale[slot / 2][0][lane * eights + i] = fk;
+                  s_raw_scale[slot / 2][1][lane * eights + i] = fv;
+                }
+              __syncwarp();
+              if (lane == 0) mbar_arrive_expect_tx(&raw_full[slot], C::kRaw);
+              __syncwarp();
+              if (lane < boxes)
+                tma_load_4d(raw + slot * C::kRaw + lane * args.box * D, side == 0 ? &args.k_map : &args.v_map, 0, off, it.head,
+                            block, &raw_full[slot]);
+            }
+            if (++slot == NR) {
+              slot = 0;
+              ++round;
             }
           }
         }
-      };
-      auto scales_of = [&](int block, float& a, float& b) {
-        a = b = 0.f;
-        if (block >= 0) {
-          a = __ldcg(p.k_scale + block * p.ks_block + it.head * p.ks_head);
-          b = __ldcg(p.v_scale + block * p.vs_block + it.head * p.vs_head);
-        }
-      };
-      auto filled = [&]() {  // the slot is
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&full[slot]);
-        if (++slot == NS) {
-          slot = 0;
-          ++round;
-        }
-      };
-      auto room = [&]() {
-        if (round > 0) ok = __all_sync(0xffffffffu, ok && mbar_poll(&empty[slot], (round - 1) & 1, p.status));
-      };
-      uint4 uk[PASSES], uv[PASSES];
-      int block, off, next_block = -1, next_off = 0;
-      float fk, fv;
-      if (cur.len > 0) {
-        lookup(0, block, off);
-        scales_of(block, fk, fv);
-        fetch(uk, 0, block, off, p.k, p.k_block, p.k_slot, p.k_head);
-        fetch(uv, 0, block, off, p.v, p.v_block, p.v_slot, p.v_head);
-        if (cur.len > 1) lookup(1, next_block, next_off);
+        if (cur.advance()) next_item();
       }
+    }
+  } else if (warp >= 12) {  // ---- codes to values, 32 keys of each tile a warp ----
+    regs_down<96>();
+    constexpr int PASSES = D / 16, ROWS = 32 / PASSES;  // pieces of 16 codes a thread, keys at once
+    const int w = warp - 12;
+    // Eight lanes side by side read and write all banks: the first four pieces of one key and the last four of
+    // the next (D = 64: the four pieces of two keys).
+    const int sub = lane >> 2 & 1, chunk = D == 128 ? (lane & 3) + 4 * sub : lane & 3;
+    const int row0 = w * 32 + (D == 128 ? (lane >> 4) * 2 + (sub ^ (lane >> 3 & 1)) : lane >> 2);
+    int slot = 0, round = 0, raw_slot = 0, raw_phase = 0;
+    uint32_t tile_no = 0;
+    float f = 0.f;  // scales of eight keys: K's in four lanes, V's in four
+    uint4 u[PASSES];
+    auto take = [&]() {  // the next codes
+      ok = __all_sync(0xffffffffu, ok && mbar_poll(&raw_full[raw_slot], raw_phase, p.status));
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i)
+        u[i] = *reinterpret_cast<const uint4*>(raw + raw_slot * C::kRaw + code_at<D>(row0 + i * ROWS, chunk));
+      if ((raw_slot & 1) == 0) f = s_raw_scale[raw_slot / 2][lane >> 2 & 1][w * 4 + (lane & 3)];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&raw_empty[raw_slot]);
+      if (++raw_slot == NR) {
+        raw_slot = 0;
+        raw_phase ^= 1;
+      }
+      if (round > 0) ok = __all_sync(0xffffffffu, ok && mbar_poll(&empty[slot], (round - 1) & 1, p.status));
+      return ring + slot * C::kSlot + (chunk >> 2) * HALF;
+    };
+    auto filled = [&]() {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[slot]);
+      if (++slot == NS) {
+        slot = 0;
+        ++round;
+      }
+    };
+    while (cur.take(it.n)) {
+      int seen_lo, seen_hi;
+      chunk_seen(p, it, seen_lo, seen_hi);
       for (int k = 0; k < cur.len; ++k) {
-        const int j0 = j_first + k * kChunkKeys;
-        const bool more = k + 1 < cur.len;
-        room();
-        if (lane < 4) {
-          s_scale[tile_no % kScaleTiles][0][w * 4 + lane] = fk;
-          s_scale[tile_no % kScaleTiles][1][w * 4 + lane] = fv;
-        }
+        const int j0 = (it.tile0 + cur.tile + k) * kChunkKeys;
+        unsigned char* to = take();
+        if (lane < 8) s_scale[tile_no % kScaleTiles][lane >> 2][w * 4 + (lane & 3)] = f;
         ++tile_no;
-        code_put<T, D>(ring + slot * C::kSlot + (chunk >> 2) * HALF, chunk & 3, row0, uk);
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) code_put<T>(to + (row0 + i * ROWS) * 128, row0 + i * ROWS, chunk & 3, u[i]);
         filled();
-        if (more) {
-          scales_of(next_block, fk, fv);
-          fetch(uk, k + 1, next_block, next_off, p.k, p.k_block, p.k_slot, p.k_head);
-        }
-        if (j0 + kChunkKeys > seen_hi || j0 < seen_lo) {  // NaN of keys that not every row sees
+        to = take();
+        if (j0 + kChunkKeys > seen_hi || j0 < seen_lo) {  // keys that not every row sees
           bool taken = false;
 #pragma unroll
           for (int i = 0; i < PASSES; ++i) {
             const int j = j0 + row0 + i * ROWS;
             if (j >= seen_lo && j < seen_hi) continue;
-            const uint4 nan = make_uint4(codes_nan(uv[i].x), codes_nan(uv[i].y), codes_nan(uv[i].z), codes_nan(uv[i].w));
-            taken |= (nan.x | nan.y | nan.z | nan.w) != 0u;
-            uv[i].x &= ~((nan.x >> 7) * 0xffu);
-            uv[i].y &= ~((nan.y >> 7) * 0xffu);
-            uv[i].z &= ~((nan.z >> 7) * 0xffu);
-            uv[i].w &= ~((nan.w >> 7) * 0xffu);
+            const uint4 nan = make_uint4(codes_nan(u[i].x), codes_nan(u[i].y), codes_nan(u[i].z), codes_nan(u[i].w));
+            const bool some = j >= it.first && j < it.end;
+            taken |= some && (nan.x | nan.y | nan.z | nan.w) != 0u;
+            u[i].x &= some ? ~((nan.x >> 7) * 0xffu) : 0u;
+            u[i].y &= some ? ~((nan.y >> 7) * 0xffu) : 0u;
+            u[i].z &= some ? ~((nan.z >> 7) * 0xffu) : 0u;
+            u[i].w &= some ? ~((nan.w >> 7) * 0xffu) : 0u;
           }
           if (taken) count_store(&s_taken, 1u);
         }
-        room();
-        code_put<__half, D>(ring + slot * C::kSlot + (chunk >> 2) * HALF, chunk & 3, row0, uv);
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) code_put<__half>(to + (row0 + i * ROWS) * 128, row0 + i * ROWS, chunk & 3, u[i]);
         filled();
-        if (more) {
-          fetch(uv, k + 1, next_block, next_off, p.v, p.v_block, p.v_slot, p.v_head);
-          next_block = -1;
-          if (k + 2 < cur.len) lookup(k + 2, next_block, next_off);
-        }
       }
       if (cur.advance()) next_item();
     }
@@ -861,14 +883,16 @@ cudaError_t launch_code_chunk(const CodeChunkArgs& a, cudaStream_t st, bool pdl)
 }  // namespace
 
 cudaError_t launch_paged_attention_code_chunk(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl) {
-  // a maximum of scores is one of scaled scores for a positive scale only; eight keys lie in one block
-  if ((dtype != kBF16 && dtype != kF16) || a.dim > 128 || a.block_size % 8 != 0 || !(a.scale > 0.f)) return cudaErrorNotSupported;
+  // a maximum of scores is one of scaled scores for a positive scale only
+  if ((dtype != kBF16 && dtype != kF16) || a.dim > 128 || !(a.scale > 0.f)) return cudaErrorNotSupported;
   // units of work (paged_sched.cuh) in 32 bits
   const long long items = (long long)a.tokens * a.group / kChunkRows + a.requests;
   if (items * a.kv_heads * ((long long)a.width * a.block_size / kChunkKeys + 2 + kChunkItem) >= INT_MAX)
     return cudaErrorNotSupported;
   CodeChunkArgs c{};
   c.a = a;
+  c.box = paged_box(a.block_size, kChunkKeys);
+  if (c.box < 8 || !paged_maps(a, kPagedCodes, a.dim <= 64 ? 64 : 128, c.box, &c.k_map, &c.v_map)) return cudaErrorNotSupported;
   c.q_tma = paged_q_map(a, dtype, 128, &c.q_map);
   c.out32 = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_token % 16 == 0 && a.out_head % 16 == 0 && a.dim % 16 == 0;
   if (dtype == kBF16)
