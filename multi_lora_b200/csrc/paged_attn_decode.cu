@@ -60,15 +60,20 @@ struct DecodeArgs {
   int box;     // rows of a TMA box
 };
 
-template <int D, bool CODES>
+// What the cache holds: values, codes, or codes for at most eight rows an item.
+enum DecodeKind { kDecValues, kDecCodes, kDecCodesFew };
+
+template <int D, DecodeKind KIND>
 struct DecodeCfg {
+  static constexpr bool CODES = KIND != kDecValues, FEW = KIND == kDecCodesFew;
   static constexpr int kTile = CODES ? kCodeTile : kDecTile;  // the same bytes
+  static constexpr int kMaxRows = FEW ? 8 : kDecodeMaxRows;
   static constexpr int KG = 4;                    // key groups: warps that share 16 rows
   static constexpr int kWarps = KG;
   static constexpr int kThreads = kWarps * 32 + 32;
-  static constexpr int kPerSm = 2;
+  static constexpr int kPerSm = FEW ? 3 : 2;
   static constexpr int kSide = kTile * D * (CODES ? 1 : 2);  // bytes of K (or V) in a stage
-  static constexpr int kStages = 96 * 1024 / (2 * kSide);
+  static constexpr int kStages = (FEW ? 64 : 96) * 1024 / (2 * kSide);
   static constexpr int kRowF = D + 4;             // floats of a row in the merge buffer
   static constexpr int kMerge = 16 * kRowF * 4;
   static constexpr int kSmem = kStages * 2 * kSide + kMerge + 1024;
@@ -79,7 +84,7 @@ struct DecodeItem {
   int req, head, q0, qn, kv, first, tile0, n;
 };
 
-template <int TILE>
+template <int TILE, int MOST>
 __device__ __forceinline__ void decode_request(const PagedAttnArgs& p, DecodeItem& it, int req, const PagedRequest& r) {
   it.req = req;
   it.q0 = r.q0;
@@ -87,17 +92,18 @@ __device__ __forceinline__ void decode_request(const PagedAttnArgs& p, DecodeIte
   it.kv = r.kv;
   it.first = paged_first_key(p, r.kv - r.qn);
   it.tile0 = it.first / TILE;
-  it.n = r.qn > 0 && r.qn * p.group <= kDecodeMaxRows ? max(1, (r.kv + TILE - 1) / TILE - it.tile0) : 0;
+  it.n = r.qn > 0 && r.qn * p.group <= MOST ? max(1, (r.kv + TILE - 1) / TILE - it.tile0) : 0;
 }
 
 constexpr int kFewCtas = 8;    // CTAs of a cluster
 constexpr int kFewItems = 16;  // (request, key head)s that clusters are launched for, at most
 constexpr int kFewKeys = 4096; // keys that the block tables have room for, at most
 
-template <typename T, int D, bool CLUSTER, bool CODES>
-__global__ void __launch_bounds__(DecodeCfg<D, CODES>::kThreads, DecodeCfg<D, CODES>::kPerSm)
+template <typename T, int D, bool CLUSTER, DecodeKind KIND>
+__global__ void __launch_bounds__(DecodeCfg<D, KIND>::kThreads, DecodeCfg<D, KIND>::kPerSm)
 paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
-  using C = DecodeCfg<D, CODES>;
+  using C = DecodeCfg<D, KIND>;
+  constexpr bool CODES = C::CODES, FEW = C::FEW;
   constexpr float kUp = Num<T>::is_bf16 ? 0.f : 15.f;  // P is taken times 2^kUp
   constexpr int NS = C::kStages, SIDE = C::kSide, TILE = C::kTile, HALF = kDecTile * 128;
   extern __shared__ __align__(1024) unsigned char s_raw[];
@@ -138,7 +144,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     // rows beyond what the caller said: reported, and where they do not fit the tile not computed
     if (report && r.qn > p.max_q_len) flag_error(p.status, kErrLength);
     DecodeItem x;
-    decode_request<TILE>(p, x, i, r);
+    decode_request<TILE, C::kMaxRows>(p, x, i, r);
     skipped |= r.odd || (r.qn > 0 && x.n == 0);
     return x.n > 0 ? (x.n + kDecItem) * p.kv_heads : 0;
   };
@@ -152,14 +158,14 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       if (lane < p.requests) units(lane, 0, 1, r);
       skipped = __any_sync(0xffffffffu, skipped);
     }
-    if (skipped) paged_zero_uncomputed<T>(p, kDecodeMaxRows);
+    if (skipped) paged_zero_uncomputed<T>(p, C::kMaxRows);
     else paged_zero_rest<T>(p);
   };
   if constexpr (CLUSTER) {
     const int item = blockIdx.x / kFewCtas;
     req = item / p.kv_heads;
     units(req, 0, 1, found);
-    decode_request<TILE>(p, it, req, found);
+    decode_request<TILE, C::kMaxRows>(p, it, req, found);
     if (it.n == 0) {  // the same in the whole cluster
       if (warp == C::kWarps) zero_others();
       return;
@@ -177,7 +183,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       if (warp == C::kWarps) zero_others();
       return;
     }
-    decode_request<TILE>(p, it, req, found);
+    decode_request<TILE, C::kMaxRows>(p, it, req, found);
     it.head = (cur.pos - before) / (it.n + kDecItem);
     cur.unit = cur.pos - before - it.head * (it.n + kDecItem);
   }
@@ -185,8 +191,8 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     if (++it.head == p.kv_heads) {
       it.head = 0;
       PagedRequest r;
-      const int i = paged_next(p, it.req, kDecodeMaxRows, r);
-      if (i < p.requests) decode_request<TILE>(p, it, i, r);
+      const int i = paged_next(p, it.req, C::kMaxRows, r);
+      if (i < p.requests) decode_request<TILE, C::kMaxRows>(p, it, i, r);
     }
   };
   if (!CLUSTER && cur.begin(it.n)) next_item();
@@ -288,7 +294,9 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
   float* parts = reinterpret_cast<float*>(tickets + kPagedTickets);
   constexpr int PART = 16 * (D + 2);  // floats of a piece: sums, maxima, totals
   // Q fragments: rows lane / 4 and + 8, columns (lane % 4) * 2 (+ 8) of each 16
-  uint32_t qf[D / 16][4];
+  uint32_t qf[D / 16][FEW ? 2 : 4];
+  // rows of the lane's statistics: lane / 4 and + 8, or (lane % 4) * 2 and + 1
+  auto row_of = [&](int e) { return FEW ? (lane & 3) * 2 + e : (lane >> 2) + e * 8; };
   float row_f[2] = {sl, sl};  // of codes: what the products of the lane's rows are multiplied by
   auto load_q = [&](const DecodeItem& x) {
     if constexpr (CODES) {
@@ -298,7 +306,8 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
                                       (int64_t)(x.head * group + r - t * group) * p.q_head
                                 : nullptr;
       };
-      code_queries<T, D>(p.dim, row, qf, row_f);
+      if constexpr (FEW) code_queries_few<T, D>(p.dim, row(0), qf, row_f);
+      else code_queries<T, D>(p.dim, row, qf, row_f);
       row_f[0] *= sl;
       row_f[1] *= sl;
     } else {
@@ -323,12 +332,12 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     int limit[2], floor_[2];  // keys below `limit` and at or above `floor_` are seen
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int r = (lane >> 2) + e * 8;
+      const int r = row_of(e);
       const int pq = it.kv - it.qn + paged_token(p, r);
       limit[e] = r < rows ? pq + 1 : 0;
       floor_[e] = paged_first_key(p, pq);
     }
-    CodeSums<D> sums;
+    typename std::conditional<FEW, CodeSumsFew<D>, CodeSums<D>>::type sums;
     sums.clear();
     auto& o = sums.o;
     auto& m = sums.m;
@@ -345,11 +354,12 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       if (CODES && j0 < it.kv && j0 + MINE > it.first) {
         const uint32_t ks = smem_addr(smem + stage * 2 * SIDE);
         const CodeSpan span = {it.kv, it.first, all_first, all_end, {limit[0], limit[1]}, {floor_[0], floor_[1]}, it.qn > 1};
-        if constexpr (CODES)
-          code_tile<T, D>(sums, qf, span, ks, ks + SIDE, k0, j0, *reinterpret_cast<const float4*>(&s_scale[stage][0][kg * 4]),
-                          *reinterpret_cast<const float4*>(&s_scale[stage][1][kg * 4]), row_f);
+        const float4 key_f = *reinterpret_cast<const float4*>(&s_scale[CODES ? stage : 0][0][CODES ? kg * 4 : 0]),
+                     value_f = *reinterpret_cast<const float4*>(&s_scale[CODES ? stage : 0][1][CODES ? kg * 4 : 0]);
+        if constexpr (FEW) code_tile_few<T, D>(sums, qf, span, ks, ks + SIDE, k0, j0, key_f, value_f, row_f);
+        else if constexpr (CODES) code_tile<T, D>(sums, qf, span, ks, ks + SIDE, k0, j0, key_f, value_f, row_f);
       }
-      if (!CODES && j0 < it.kv && j0 + 16 > it.first) {
+      if constexpr (!CODES) if (j0 < it.kv && j0 + 16 > it.first) {
         const uint32_t ks = smem_addr(smem + stage * 2 * SIDE), vs = ks + SIDE;
         // All of K's fragments, then the products as four independent chains.
         uint32_t kf[2][D / 32][4];
@@ -509,19 +519,20 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
     // merge buffer where the rows are few, further ones are added in turn ----
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], FEW ? 4 : 1);
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], FEW ? 8 : 2);
+      if constexpr (FEW) l[e] += __shfl_xor_sync(0xffffffffu, l[e], 16);
       if constexpr (CODES) l[e] *= 0x1p-15f;  // kCodeUp
-      if ((lane & 3) == 0) {
-        s_m[warp][(lane >> 2) + e * 8] = m[e];
-        s_l[warp][(lane >> 2) + e * 8] = l[e];
+      if (FEW ? lane < 4 : (lane & 3) == 0) {
+        s_m[warp][row_of(e)] = m[e];
+        s_l[warp][row_of(e)] = l[e];
       }
     }
     const int slots = rows <= 4 ? C::KG : rows <= 8 ? 2 : 1, apart = 16 / (rows <= 4 ? 4 : slots);
     named_barrier(1, C::kWarps * 32);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int r = (lane >> 2) + e * 8;
+      const int r = row_of(e);
       float top = -INFINITY;
 #pragma unroll
       for (int g = 0; g < C::KG; ++g) top = fmaxf(top, s_m[g][r]);
@@ -540,9 +551,20 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       if (kg >= g && kg < g + slots) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int r = (lane >> 2) + e * 8;
+          const int r = row_of(e);
           if (r >= rows) continue;
-          if constexpr (CODES) {  // four columns side by side
+          if constexpr (FEW) {  // two columns side by side
+            float* d = merge + ((kg - g) * apart + r) * C::kRowF + (lane >> 2) * 2;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+              float2 v = make_float2(o[c][e], o[c][2 + e]);
+              if (g > 0) {
+                const float2 u = *reinterpret_cast<const float2*>(d + c * 16);
+                v = make_float2(v.x + u.x, v.y + u.y);
+              }
+              *reinterpret_cast<float2*>(d + c * 16) = v;
+            }
+          } else if constexpr (CODES) {  // four columns side by side
             float* d = merge + ((kg - g) * apart + r) * C::kRowF + (lane & 3) * 4;
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
@@ -553,8 +575,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
               }
               *reinterpret_cast<float4*>(d + c * 16) = v;
             }
-            continue;
-          }
+          } else {
           float* d = merge + ((kg - g) * apart + r) * C::kRowF + (lane & 3) * 2;
           if (g > 0) {
             float2 u[D / 8];  // all the loads first
@@ -569,6 +590,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
 #pragma unroll
           for (int n = 0; n < D / 8; ++n)
             *reinterpret_cast<float2*>(d + n * 8) = make_float2(o[n][2 * e], o[n][2 * e + 1]);
+          }
         }
       }
       named_barrier(1, C::kWarps * 32);
@@ -736,7 +758,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
           }
         }
       };
-      uint32_t* run_ticket = tickets + gridDim.x + run.x0 * 2 + (run.x0 == c0 ? 1 : 0);
+      uint32_t* run_ticket = (FEW ? paged_more_tickets(p) : tickets + gridDim.x) + run.x0 * 2 + (run.x0 == c0 ? 1 : 0);
       if (run.runs == 1) {
         if (last_of(tickets + c0, c1 - c0 + 1)) join(c0, c1, 1, true);
       } else if (last_of(run_ticket, run.x1 - run.x0 + 1)) {
@@ -750,16 +772,16 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
 
 namespace {
 
-template <typename T, int D, bool CLUSTER, bool CODES>
+template <typename T, int D, bool CLUSTER, DecodeKind KIND>
 cudaError_t launch_decode(const DecodeArgs& a, cudaStream_t st, bool pdl) {
-  using C = DecodeCfg<D, CODES>;
-  auto kern = paged_attention_decode_kernel<T, D, CLUSTER, CODES>;
+  using C = DecodeCfg<D, KIND>;
+  auto kern = paged_attention_decode_kernel<T, D, CLUSTER, KIND>;
   static SmemLimit limit;
   if (const cudaError_t e = limit.raise(kern, C::kSmem); e != cudaSuccess) return e;
   const int ctas = device_sm_count() * C::kPerSm;
   static_assert(C::kSmem <= 227 * 1024, "shared memory");
-  if (ctas * 3 > kPagedTickets ||
-      (size_t)ctas * 2 * 16 * (D + 2) * 4 + kPagedTickets * 4 > kPagedWorkspaceBytes)
+  if ((C::FEW ? ctas * 2 : ctas * 3) > kPagedTickets ||
+      (size_t)ctas * 2 * 16 * (D + 2) * 4 + 2 * kPagedTickets * 4 > kPagedWorkspaceBytes)
     return cudaErrorNotSupported;
   if constexpr (!CLUSTER) {
     return launch_kernel(kern, dim3(ctas), dim3(C::kThreads), C::kSmem, st, pdl, a);
@@ -782,19 +804,20 @@ cudaError_t launch_decode(const DecodeArgs& a, cudaStream_t st, bool pdl) {
   }
 }
 
-template <typename T, int D, bool CODES>
+template <typename T, int D, DecodeKind KIND>
 cudaError_t launch_decode_any(const DecodeArgs& a, cudaStream_t st, bool pdl) {
   // One request of 777 keys, 8 key heads: 6.5 us with clusters, 11.3 without; 4000 keys 12.9 and 18.5. From
   // twice that on an item needs more CTAs than a cluster has. The host knows the lengths' bound only.
   // Without requests there is no item to launch a cluster for: the other kernel's CTAs write the zeros.
   if (a.a.requests > 0 && (long long)a.a.requests * a.a.kv_heads <= kFewItems &&
       (long long)a.a.width * a.a.block_size <= kFewKeys)
-    return launch_decode<T, D, true, CODES>(a, st, pdl);
-  return launch_decode<T, D, false, CODES>(a, st, pdl);
+    return launch_decode<T, D, true, KIND>(a, st, pdl);
+  return launch_decode<T, D, false, KIND>(a, st, pdl);
 }
 
-template <bool CODES>
+template <DecodeKind KIND>
 cudaError_t launch_decode_of(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl) {
+  constexpr bool CODES = KIND != kDecValues;
   constexpr int TILE = CODES ? kCodeTile : kDecTile;
   if ((dtype != kBF16 && dtype != kF16) || a.dim > 128) return cudaErrorNotSupported;
   // units of work (paged_sched.cuh) in 32 bits
@@ -806,14 +829,16 @@ cudaError_t launch_decode_of(const PagedAttnArgs& a, int dtype, cudaStream_t st,
   const int columns = CODES ? (a.dim <= 64 ? 64 : 128) : 64;
   if (d.box < 8 || !paged_maps(a, CODES ? kPagedCodes : dtype, columns, d.box, &d.k_map, &d.v_map)) return cudaErrorNotSupported;
   if (dtype == kBF16)
-    return a.dim <= 64 ? launch_decode_any<__nv_bfloat16, 64, CODES>(d, st, pdl) : launch_decode_any<__nv_bfloat16, 128, CODES>(d, st, pdl);
-  return a.dim <= 64 ? launch_decode_any<__half, 64, CODES>(d, st, pdl) : launch_decode_any<__half, 128, CODES>(d, st, pdl);
+    return a.dim <= 64 ? launch_decode_any<__nv_bfloat16, 64, KIND>(d, st, pdl) : launch_decode_any<__nv_bfloat16, 128, KIND>(d, st, pdl);
+  return a.dim <= 64 ? launch_decode_any<__half, 64, KIND>(d, st, pdl) : launch_decode_any<__half, 128, KIND>(d, st, pdl);
 }
 
 }  // namespace
 
 cudaError_t launch_paged_attention_decode(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl) {
-  return a.k_scale != nullptr ? launch_decode_of<true>(a, dtype, st, pdl) : launch_decode_of<false>(a, dtype, st, pdl);
+  if (a.k_scale == nullptr) return launch_decode_of<kDecValues>(a, dtype, st, pdl);
+  return (int64_t)a.max_q_len * a.group <= 8 ? launch_decode_of<kDecCodesFew>(a, dtype, st, pdl)
+                                             : launch_decode_of<kDecCodes>(a, dtype, st, pdl);
 }
 
 }  // namespace mlora

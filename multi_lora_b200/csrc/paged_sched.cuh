@@ -506,5 +506,9 @@ struct PagedJoin {
 
 constexpr int kPagedTickets = 1024;  // words at the start of the workspace, zero between calls
 constexpr size_t kPagedWorkspaceBytes = (size_t)64 << 20;
+// As many more at its end, for a launch with more CTAs than those have room for.
+__device__ __forceinline__ uint32_t* paged_more_tickets(const PagedAttnArgs& p) {
+  return reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(p.workspace) + kPagedWorkspaceBytes) - kPagedTickets;
+}
 
 }  // namespace mlora

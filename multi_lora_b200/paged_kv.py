@@ -55,7 +55,7 @@ def check_status(status: torch.Tensor) -> None:
 
 def attention_workspace(device: torch.device) -> torch.Tensor:
     """A workspace for :func:`paged_attention`; calls that may overlap on the GPU need one each. Its
-    first 4 KiB are counters, zero between calls; they are to be zeroed again after a call that reported a
+    first and last 4 KiB are counters, zero between calls; they are to be zeroed again after a call that reported a
     copy that did not complete in time."""
     return torch.zeros(ATTENTION_WORKSPACE_BYTES, dtype=torch.uint8, device=device)
 

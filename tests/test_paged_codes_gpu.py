@@ -217,7 +217,7 @@ def test_requests_longer_than_the_host_said(cuda_dev, workspace, q_lens, dtype):
     at, gone = 0, 0
     for q in q_lens:
         rows = slice(at, at + q)
-        if q * 4 > 16 and (out[rows] == 0).all():  # more than the kernel that `max_q_len` = 1 chooses has room for
+        if q > 1 and (out[rows] == 0).all():  # more than the kernel that `max_q_len` = 1 chooses has room for
             gone += 1
         else:
             torch.testing.assert_close(out[rows].float(), want[rows].float(), rtol=2.0 ** -7, atol=2.0 ** -7)
