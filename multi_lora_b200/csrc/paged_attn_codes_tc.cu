@@ -28,7 +28,7 @@
 
 namespace mlora {
 
-constexpr int kCodeThreads = 512;  // Q and tensor cores, two warpgroups of softmax, one of codes
+constexpr int kCodeThreads = 768;  // Q, TMA and tensor cores; four warpgroups of softmax; one of codes
 
 struct CodeChunkArgs {
   CUtensorMap k_map, v_map, q_map;
@@ -45,18 +45,57 @@ struct CodeChunkCfg {
   static constexpr int kRaw = kChunkKeys * D;       // codes of K or V of a tile
   static constexpr int kRaws = D == 128 ? 2 : 4;
   static constexpr int kSlots = D == 128 ? 4 : 8;
-  static constexpr int kSmem = 2 * kQ + kSlots * kSlot + kRaws * kRaw + 1024;
+  static constexpr int kSmem = 2 * kQ + kSlots * kSlot + kRaws * kRaw;
   static constexpr int kPart = 128 * (D + 2);  // floats of a tile's piece
   // tiles whose scales wait: K of a tile gets its slot when the scores of the second (D = 64: fourth) tile before it are
   // done, so all of the one before that is
   static constexpr int kScaleTiles = D == 128 ? 4 : 8;
 };
 
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+// 16 columns, waited for.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// Whether any of the 64 threads at barrier `id` says so; all of them wait for one another.
+__device__ __forceinline__ bool barrier_any(int id, bool mine) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %1, 0;\n\t"
+      "bar.red.or.pred p, %2, 64, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(any)
+      : "r"((uint32_t)mine), "r"(id)
+      : "memory");
+  return any != 0u;
+}
+
 // NaN that was taken out of V, added in TMEM to the outputs of row r, if it sees it: the item's keys of [from, to) that
 // not every row sees, those of every tile's half `half` if that is not negative. Seldom run.
 template <int D>
-__device__ __noinline__ void code_give_back(const PagedAttnArgs& p, uint32_t o_addr, int req, int head, int rt, int qn, int kv, int r,
-                                            int from, int to, int half) {
+__device__ __noinline__ void code_give_back(const PagedAttnArgs& p, uint32_t o_addr, int column, int req, int head, int rt, int qn,
+                                            int kv, int r, int from, int to, int half) {
   ChunkItem it;
   it.qn = qn;
   it.kv = kv;
@@ -72,21 +111,19 @@ __device__ __noinline__ void code_give_back(const PagedAttnArgs& p, uint32_t o_a
     to = from;
   }
 #pragma unroll 1
-  for (int c = 0; c < D / 32; ++c) {
-    uint32_t o[32];
-    tmem_ld32_async(o_addr + c * 32, o);
-    tmem_wait_ld();
-    tie32(o);
+  for (int c = 0; c < D / 2; c += 16) {  // of the columns from `column` on
+    uint32_t o[16];
+    tmem_ld16(o_addr + c, o);
 #pragma unroll 1
     for (int j = from; j < to; ++j) {
       if ((j >= seen_lo && j < seen_hi) || (half >= 0 && ((j / kHalfKeys) & 1) != half)) continue;
       const int block = __ldcg(p.tables + req * p.table_stride + j / p.block_size);
       if (block < 0 || block >= p.num_blocks) continue;
       const unsigned char* src = static_cast<const unsigned char*>(p.v) + block * p.v_block + (j % p.block_size) * p.v_slot +
-                                 head * p.v_head + c * 32;
+                                 head * p.v_head + column + c;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {  // a dim is a multiple of 8
-        if (c * 32 + 8 * i >= p.dim) continue;
+      for (int i = 0; i < 2; ++i) {  // a dim is a multiple of 8
+        if (column + c + 8 * i >= p.dim) continue;
         const uint2 u = __ldcg(reinterpret_cast<const uint2*>(src) + i);
         const uint32_t a = codes_nan(u.x), b = codes_nan(u.y);
 #pragma unroll
@@ -97,18 +134,9 @@ __device__ __noinline__ void code_give_back(const PagedAttnArgs& p, uint32_t o_a
       }
     }
     __syncwarp();
-    tmem_st32(o_addr + c * 32, o);
+    tmem_st16(o_addr + c, o);
   }
   tmem_wait_st();
-}
-
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
 }
 
 __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
@@ -152,13 +180,19 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
   __shared__ uint32_t s_tmem;
   __shared__ int s_last[2];
   __shared__ bool s_skipped;
-  __shared__ float2 s_mate[128];  // maximum and sum of the other warpgroup's rows
-  __shared__ float s_mate_most;   // its largest scale of V
+  // What the threads of a row tell one another: a maximum or a sum of each half of the columns; and, where both tiles'
+  // warpgroups work on one, the second's maximum and sum.
+  __shared__ float s_part[2][2][128];
+  __shared__ float s_mate_most;  // the largest scale of V beside these
   __shared__ uint32_t s_taken;      // a NaN was taken out of V
   const PagedAttnArgs& p = args.a;
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = same_in_warp(tid >> 5);
-  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* smem = s_raw;  // there is no room to align it in: it is, and if it were not nothing would be read or written
+  if ((smem_addr(s_raw) & 1023u) != 0u) {
+    if (tid == 0) flag_error(p.status, kErrTimeout);
+    return;
+  }
   unsigned char *ring = smem + 2 * C::kQ, *raw = ring + NS * C::kSlot;
 
   if (tid == 0) {
@@ -175,7 +209,7 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
       mbar_init(&q_free[q], 2);
       for (int b = 0; b < 2; ++b) {
         mbar_init(&s_full[q][b], 1);
-        mbar_init(&p_ready[q][b], 4);
+        mbar_init(&p_ready[q][b], 8);
         mbar_init(&pv_done[q][b], 1);
       }
     }
@@ -270,10 +304,10 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
   }
   bool ok = true;
 
-  // Registers: 512 threads are launched with 128 each (65536); the warps of Q and the tensor cores keep 64, those of
-  // codes 112, and the softmax warps take 168: 128 * 64 + 128 * 112 + 256 * 168 = 65536.
+  // Registers: 768 threads are launched with 80 each (61440); the warps of Q, TMA and the tensor cores keep 72, those of
+  // codes take 88, and the softmax warps stay: 128 * 72 + 128 * 88 + 512 * 80 = 61440.
   if (warp < 4) {
-    regs_down<80>();
+    regs_down<72>();
     if (warp == 1 || warp == 2) {  // ---- tensor cores, a warp a tile of rows: S of a half, then O of the half before ----
       const int q = warp - 1;
       constexpr uint32_t idesc_s = umma_idesc_f16(Num<T>::is_bf16, 128, kHalfKeys);
@@ -467,10 +501,10 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
         if (cur.advance()) next_item();
       }
     }
-  } else if (warp >= 12) {  // ---- codes to values, 32 keys of each tile a warp ----
-    regs_down<96>();
+  } else if (warp >= 20) {  // ---- codes to values, 32 keys of each tile a warp ----
+    regs_up<88>();
     constexpr int PASSES = D / 16, ROWS = 32 / PASSES;  // pieces of 16 codes a thread, keys at once
-    const int w = warp - 12;
+    const int w = warp - 20;
     // Eight lanes side by side read and write all banks: the first four pieces of one key and the last four of
     // the next (D = 64: the four pieces of two keys).
     const int sub = lane >> 2 & 1, chunk = D == 128 ? (lane & 3) + 4 * sub : lane & 3;
@@ -485,6 +519,8 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
       for (int i = 0; i < PASSES; ++i)
         u[i] = *reinterpret_cast<const uint4*>(raw + raw_slot * C::kRaw + code_at<D>(row0 + i * ROWS, chunk));
       if ((raw_slot & 1) == 0) f = s_raw_scale[raw_slot / 2][lane >> 2 & 1][w * 4 + (lane & 3)];
+      // These loads may still be under way when an arrival is not: without the fence the next codes came over them.
+      fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&raw_empty[raw_slot]);
       if (++raw_slot == NR) {
@@ -537,143 +573,139 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
       }
       if (cur.advance()) next_item();
     }
-  } else {  // ---- softmax: warpgroup q, thread = row ----
-    regs_up<168>();
-    const int q = (warp >> 2) - 1, row = tid & 127;
+  } else {  // ---- softmax: two warpgroups a tile of rows, a thread half of a row's columns ----
+    const int group = (warp >> 2) - 1, q = group >> 1, side = group & 1, row = tid & 127;
+    const int pair = 6 + q * 4 + (warp & 3);  // barrier of the two warps that share 32 rows
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + S_COL + q * 128, o_addr = tmem + lanes + O_COL + q * D;
+    const uint32_t s_addr = tmem + lanes + S_COL + q * 128, o_addr = tmem + lanes + O_COL + q * D + side * (D / 2);
     const float sl = p.scale * 1.4426950408889634f;  // scores in powers of two
     uint32_t* tickets = static_cast<uint32_t*>(p.workspace);
     float* parts = reinterpret_cast<float*>(tickets + kPagedTickets);
     int n = 0;             // halves done
     uint32_t tile_no = 0;  // of the current item's first tile
-    bool lent = false;     // the other warpgroup still reads this one's O
+    bool lent = false;     // the other tile's warpgroups still read this one's O and sums
     while (cur.take(it.n)) {
-      const bool solo = chunk_solo(it);  // the warpgroups share its keys, half by half
+      if (lent) named_barrier(5, 512);
+      lent = false;
+      const bool solo = chunk_solo(it);  // the tiles' warpgroups share its keys, half by half
       const int r_lo = it.rt * kChunkRows + (solo ? 0 : q * 128), r = r_lo + row;
-      const int pq = it.kv - it.qn + paged_token(p, r);
-      const int limit = r < it.rows ? pq + 1 : 0, floor_ = paged_first_key(p, pq);
-      // key tiles that every row of this tile sees whole need no mask
-      const int r_hi = min(it.rows, r_lo + 128) - 1;
-      const int all_end = it.kv - it.qn + paged_token(p, r_lo) + 1,
-                all_first = paged_first_key(p, it.kv - it.qn + paged_token(p, r_hi));
       const bool none = r - lane >= it.rows;  // no row in this warp: its lanes of P and O are never looked at
       float m = -INFINITY, l = 0.f;
       float most = 0.f, inv_most = 0.f;  // the largest scale of V so far: O is in units of it
-      const int halves = solo ? cur.len : 2 * cur.len - chunk_odd(it, cur);
-      for (int k = 0; k < halves; ++k, ++n) {
-        const int b = n & 1;
-        ok = ok && mbar_poll(&s_full[q][b], (n >> 1) & 1, p.status);
-        __syncwarp();
-        tc_fence_after();
-        if (none) {
-          if (lent) {
-            named_barrier(5, 256);
-            lent = false;
+      {
+        const int pq = it.kv - it.qn + paged_token(p, r);
+        const int limit = r < it.rows ? pq + 1 : 0, floor_ = paged_first_key(p, pq);
+        // key tiles that every row of this tile sees whole need no mask
+        const int r_hi = min(it.rows, r_lo + 128) - 1;
+        const int all_end = it.kv - it.qn + paged_token(p, r_lo) + 1,
+                  all_first = paged_first_key(p, it.kv - it.qn + paged_token(p, r_hi));
+        const int halves = solo ? cur.len : 2 * cur.len - chunk_odd(it, cur);
+        const int key0 = (it.tile0 + cur.tile) * kChunkKeys;
+#pragma unroll 1
+        for (int k = 0; k < halves; ++k, ++n) {
+          const int b = n & 1;
+          ok = ok && mbar_poll(&s_full[q][b], (n >> 1) & 1, p.status);
+          __syncwarp();
+          tc_fence_after();
+          if (none) {
+            if (lane == 0) mbar_arrive(&p_ready[q][b]);
+            continue;
           }
-          if (lane == 0) mbar_arrive(&p_ready[q][b]);
-          continue;
-        }
-        uint32_t s[2][32];
-        tmem_ld32_async(s_addr + b * 64, s[0]);
-        tmem_ld32_async(s_addr + b * 64 + 32, s[1]);
-        const int half = solo ? 2 * k + q : k;  // of the item
-        float fk[8], fv[8];
-        {
+          uint32_t s[32];
+          tmem_ld32_async(s_addr + b * 64 + side * 32, s);
+          const int half = solo ? 2 * k + q : k;  // of the item
           const float* f = &s_scale[(tile_no + (half >> 1)) % kScaleTiles][0][(half & 1) * 8];
-          const float4 a = *reinterpret_cast<const float4*>(f), c = *reinterpret_cast<const float4*>(f + 4);
-          const float4 d = *reinterpret_cast<const float4*>(f + kChunkKeys / 8), e = *reinterpret_cast<const float4*>(f + kChunkKeys / 8 + 4);
-          fk[0] = a.x, fk[1] = a.y, fk[2] = a.z, fk[3] = a.w, fk[4] = c.x, fk[5] = c.y, fk[6] = c.z, fk[7] = c.w;
-          fv[0] = d.x, fv[1] = d.y, fv[2] = d.z, fv[3] = d.w, fv[4] = e.x, fv[5] = e.y, fv[6] = e.z, fv[7] = e.w;
-        }
-        // not zero, so that minus infinity stays what it is
-#pragma unroll
-        for (int i = 0; i < 8; ++i) fk[i] = fmaxf(fk[i] * sl, 1e-37f);
-        const float largest = fmaxf(max3(max3(fv[0], fv[1], fv[2]), fv[3], fv[4]), max3(fv[5], fv[6], fv[7]));
-        tmem_wait_ld();
-        tie32(s[0]);
-        tie32(s[1]);
-        const int j0 = (it.tile0 + cur.tile) * kChunkKeys + half * kHalfKeys;
-        if (j0 + kHalfKeys > all_end || j0 < all_first) {
-          const int hi = limit - j0, lo = floor_ - j0;
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
+          const float4 fa = *reinterpret_cast<const float4*>(f + kChunkKeys / 8), fb = *reinterpret_cast<const float4*>(f + kChunkKeys / 8 + 4);
+          const float largest = fmaxf(max3(max3(fa.x, fa.y, fa.z), fa.w, fb.x), max3(fb.y, fb.z, fb.w));
+          const float4 f4 = *reinterpret_cast<const float4*>(f + side * 4), g4 = side == 0 ? fa : fb;
+          // not zero, so that minus infinity stays what it is
+          const float fk[4] = {fmaxf(f4.x * sl, 1e-37f), fmaxf(f4.y * sl, 1e-37f), fmaxf(f4.z * sl, 1e-37f), fmaxf(f4.w * sl, 1e-37f)};
+          tmem_wait_ld();
+          tie32(s);
+          const int j0 = key0 + half * kHalfKeys + side * 32;
+          if (j0 + 32 > all_end || j0 < all_first) {
+            const int hi = limit - j0, lo = floor_ - j0;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (c * 32 + i >= hi || c * 32 + i < lo) s[c][i] = 0xff800000u;  // -infinity
-        }
-        float top[8];
+              if (i >= hi || i < lo) s[i] = 0xff800000u;  // -infinity
+          }
+          float top[4];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const uint32_t* x = &s[c >> 2][(c & 3) * 8];
-          top[c] = max3(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]));
-          top[c] = max3(top[c], __uint_as_float(x[3]), __uint_as_float(x[4]));
-          top[c] = fmaxf(max3(top[c], __uint_as_float(x[5]), __uint_as_float(x[6])), __uint_as_float(x[7])) * fk[c];
-        }
-        const float mx = fmaxf(max3(max3(top[0], top[1], top[2]), top[3], top[4]), max3(top[5], top[6], top[7]));
-        if (k == 0) {
-          m = mx;
-          most = largest;
-          inv_most = most > 0.f ? 1.f / most : 0.f;
-        } else {
-          const bool raise = mx > m + kRaise, wider = largest > most;
-          if (__any_sync(0xffffffffu, raise || wider)) {
-            // O holds the halves before this one once the last product is done
-            ok = ok && mbar_poll(&pv_done[q][b ^ 1], ((n - 1) >> 1) & 1, p.status);
-            __syncwarp();
-            tc_fence_after();
-            float fix = raise ? exp2_fast(m - mx) : 1.f;
-            if (raise) m = mx;
-            l *= fix;
-            if (wider) {
-              fix *= most / largest;
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t* x = &s[c * 8];
+            top[c] = max3(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]));
+            top[c] = max3(top[c], __uint_as_float(x[3]), __uint_as_float(x[4]));
+            top[c] = fmaxf(max3(top[c], __uint_as_float(x[5]), __uint_as_float(x[6])), __uint_as_float(x[7])) * fk[c];
+          }
+          float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]);
+          // Both warps of the rows go by the same maximum. Seldom does one of them have to raise it; and neither writes P
+          // before the other one has its scores.
+          if (barrier_any(pair, k == 0 || mx > m + kRaise || largest > most)) {
+            s_part[q][side][row] = mx;
+            named_barrier(pair, 64);
+            mx = fmaxf(mx, s_part[q][side ^ 1][row]);
+            if (k == 0) {
+              m = mx;
               most = largest;
-              inv_most = 1.f / most;
-            }
+              inv_most = most > 0.f ? 1.f / most : 0.f;
+            } else {
+              // O holds the halves before this one once the last product is done
+              ok = ok && mbar_poll(&pv_done[q][b ^ 1], ((n - 1) >> 1) & 1, p.status);
+              __syncwarp();
+              tc_fence_after();
+              const bool raise = mx > m + kRaise;
+              float fix = raise ? exp2_fast(m - mx) : 1.f;
+              if (raise) m = mx;
+              l *= fix;
+              if (largest > most) {
+                fix *= most / largest;
+                most = largest;
+                inv_most = 1.f / most;
+              }
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32_async(o_addr + c * 32, o);
-              tmem_wait_ld();
-              tie32(o);
+              for (int c = 0; c < D / 2; c += 16) {
+                uint32_t o[16];
+                tmem_ld16(o_addr + c, o);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fix);
-              tmem_st32(o_addr + c * 32, o);
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fix);
+                tmem_st16(o_addr + c, o);
+              }
             }
           }
-        }
-        const float ref = (m == -INFINITY ? 0.f : m) - kUp;
-        const uint64_t ref2 = pack2(-ref, -ref);
-        uint64_t sum[4] = {0, 0, 0, 0};
+          const float ref = (m == -INFINITY ? 0.f : m) - kUp;
+          const uint64_t ref2 = pack2(-ref, -ref);
+          const float gk[4] = {g4.x * inv_most, g4.y * inv_most, g4.z * inv_most, g4.w * inv_most};
+          uint64_t sum[2] = {0, 0};
+          constexpr int AT_ONCE = TWO ? 16 : 32;  // keys
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {  // 32 keys
-          uint32_t w[16], rest[16];  // P, two keys a column
+          for (int c = 0; c < 32; c += AT_ONCE) {
+            uint32_t w[AT_ONCE / 2], rest[AT_ONCE / 2];  // P, two keys a column
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const int eight = c * 4 + i / 8;
-            const float f = fk[eight], g = fv[eight] * inv_most;
-            const uint64_t x = fma2(pack2u(s[c][i], s[c][i + 1]), pack2(f, f), ref2);
-            const uint64_t pp = pack2(exp2_fast(lo_of(x)), exp2_fast(hi_of(x)));
-            sum[(i >> 1) & 3] = add2(sum[(i >> 1) & 3], pp);
-            const uint64_t pw = mul2(pp, pack2(g, g));
-            w[i >> 1] = pack_round2<__half>(lo_of(pw), hi_of(pw));
-            if constexpr (TWO)
-              rest[i >> 1] = pack_round2<__half>(lo_of(pw) - Pack2<__half>::lo(w[i >> 1]), hi_of(pw) - Pack2<__half>::hi(w[i >> 1]));
+            for (int i = 0; i < AT_ONCE; i += 2) {
+              const float f = fk[(c + i) / 8], g = gk[(c + i) / 8];
+              const uint64_t x = fma2(pack2u(s[c + i], s[c + i + 1]), pack2(f, f), ref2);
+              const uint64_t pp = pack2(exp2_fast(lo_of(x)), exp2_fast(hi_of(x)));
+              sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pp);
+              const uint64_t pw = mul2(pp, pack2(g, g));
+              w[i >> 1] = pack_round2<__half>(lo_of(pw), hi_of(pw));
+              if constexpr (TWO)
+                rest[i >> 1] = pack_round2<__half>(lo_of(pw) - Pack2<__half>::lo(w[i >> 1]), hi_of(pw) - Pack2<__half>::hi(w[i >> 1]));
+            }
+            const uint32_t to = s_addr + b * 64 + (side * 32 + c) / 2;
+            if constexpr (TWO) {
+              tmem_st8(to, w);
+              tmem_st8(to + 32, rest);
+            } else {
+              tmem_st16(to, w);
+            }
           }
-          tmem_st16(s_addr + b * 64 + c * 16, w);
-          // over scores that are in registers by now
-          if constexpr (TWO) tmem_st16(s_addr + b * 64 + 32 + c * 16, rest);
+          const uint64_t both = add2(sum[0], sum[1]);
+          l += lo_of(both) + hi_of(both);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_ready[q][b]);
         }
-        const uint64_t both = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
-        l += lo_of(both) + hi_of(both);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lent) {  // this half's product overwrites O
-          named_barrier(5, 256);
-          lent = false;
-        }
-        if (lane == 0) mbar_arrive(&p_ready[q][b]);
       }
 
       const ChunkItem done = it;
@@ -683,32 +715,41 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
       tile_no += cur.len;
       if (cur.advance()) next_item();
 
+      if (!none) {  // the row's sum
+        named_barrier(pair, 64);  // the other warp has read what it was told last
+        s_part[q][side][row] = l;
+        named_barrier(pair, 64);
+        l += s_part[q][side ^ 1][row];
+      }
       ok = ok && mbar_poll(&pv_done[q][(n - 1) & 1], ((n - 1) >> 1) & 1, p.status);
       __syncwarp();
       tc_fence_after();
       if (__any_sync(0xffffffffu, *const_cast<volatile uint32_t*>(&s_taken) != 0u))
-        code_give_back<D>(p, o_addr, done.req, done.head, done.rt, done.qn, done.kv, r, tile0 * kChunkKeys,
+        code_give_back<D>(p, o_addr, side * (D / 2), done.req, done.head, done.rt, done.qn, done.kv, r, tile0 * kChunkKeys,
                           (tile0 + tiles) * kChunkKeys, solo ? q : -1);
-      // An item that both warpgroups worked on: the first one reads the other's O too
+      // An item that all four warpgroups worked on: the first two read the others' O too
       // (their threads of a row have the same TMEM lane).
-      float own = most, others = 0.f;  // what the two warpgroups' sums are multiplied by
+      float own = most, others = 0.f;  // what the two tiles' sums are multiplied by
       if (solo) {
         if (q == 1) {
-          s_mate[row] = make_float2(m, l);
-          if (!none) s_mate_most = most;  // every warp with rows has the same
+          if (!none) {
+            named_barrier(pair, 64);  // both have the row's sum
+            s_part[1][side][row] = side == 0 ? m : l;
+            s_mate_most = most;  // every warp with rows has the same
+          }
           tc_fence_before();
-          named_arrive(4, 256);
+          named_arrive(4, 512);
           lent = true;
           continue;
         }
-        named_barrier(4, 256);
+        named_barrier(4, 512);
         tc_fence_after();
-        const float2 mate = s_mate[row];
-        const float top = fmaxf(m, mate.x), base = top == -INFINITY ? 0.f : top;
-        const float a = exp2_fast(m - base), c = exp2_fast(mate.x - base);
+        const float mate = s_part[1][0][row];
+        const float top = fmaxf(m, mate), base = top == -INFINITY ? 0.f : top;
+        const float a = exp2_fast(m - base), c = exp2_fast(mate - base);
         own = a * most;
         others = c * s_mate_most;
-        l = l * a + mate.y * c;
+        l = l * a + s_part[1][1][row] * c;
         m = top;
       }
       const int t = paged_token(p, r);
@@ -733,59 +774,54 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
       float* part = piece(blockIdx.x, c0);
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll 1
-      for (int c = 0; c < (none ? 0 : D / 32); ++c) {
-        uint32_t o[32];
-        tmem_ld32_async(o_addr + c * 32, o);
-        tmem_wait_ld();
-        tie32(o);
-        float v[32];
+      for (int c = 0; c < (none ? 0 : D / 2); c += 16) {
+        uint32_t o[16];
+        tmem_ld16(o_addr + c, o);
+        float v[16];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]) * own;
+        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(o[i]) * own;
         if (solo) {
-          tmem_ld32_async(o_addr + D + c * 32, o);
-          tmem_wait_ld();
-          tie32(o);
+          tmem_ld16(o_addr + D + c, o);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = fmaf(__uint_as_float(o[i]), others, v[i]);
+          for (int i = 0; i < 16; ++i) v[i] = fmaf(__uint_as_float(o[i]), others, v[i]);
         }
+        const int col = side * (D / 2) + c;
         if (whole) {
-          if (r < done.rows) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 16) store(dst, c * 32 + i, v + i, inv);
-          }
+          if (r < done.rows) store(dst, col, v, inv);
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            __stcg(reinterpret_cast<float4*>(part) + (c * 8 + i / 4) * 128 + row,
-                   make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+          for (int i = 0; i < 16; i += 4)
+            __stcg(reinterpret_cast<float4*>(part) + ((col + i) / 4) * 128 + row, make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
         }
       }
       tc_fence_before();
-      if (solo) named_arrive(5, 256);
+      if (solo) named_arrive(5, 512);
       if (!whole) {
-        __stcg(part + 128 * D + row, m);
-        __stcg(part + 128 * (D + 1) + row, l);
+        if (side == 0) {
+          __stcg(part + 128 * D + row, m);
+          __stcg(part + 128 * (D + 1) + row, l);
+        }
         const int c1 = split.last_cta(item0, done.n);
         const PagedJoin run(c0, c1, blockIdx.x);
-        auto last_of = [&](uint32_t* ticket, int n) {  // whether this warpgroup is the last of n to get here
-          named_barrier(1 + q, 128);
-          if (row == 0) {
+        auto last_of = [&](uint32_t* ticket, int n) {  // whether this tile's warpgroups are the last of n to get here
+          named_barrier(1 + q, 256);
+          if (row == 0 && side == 0) {
             __threadfence();
             const bool last = atomicAdd(ticket, 1u) == (uint32_t)(n - 1);
             if (last) *ticket = 0u;
             __threadfence();
             s_last[q] = last;
           }
-          named_barrier(1 + q, 128);
+          named_barrier(1 + q, 256);
           const bool last = s_last[q];
-          named_barrier(1 + q, 128);
+          named_barrier(1 + q, 256);
           return last;
         };
         // Pieces x0, x0 + by, .. x1 of this tile of rows, to the output or as one piece to x0's
-        // place; one, two or four threads a row, 32 columns of two pieces at once.
+        // place; two, four or eight threads a row, 16 columns of two pieces at once.
         auto join = [&](int x0, int x1, int by, bool final) {
           const int live = min(128, done.rows - r_lo), share = live <= 32 ? 4 : live <= 64 ? 2 : 1;
-          const int jr = row & (128 / share - 1), c_from = row / (128 / share) * 32;
+          const int jr = row & (128 / share - 1), c_from = (side * share + row / (128 / share)) * 16;
           float top = -INFINITY, total = 0.f;
           if (jr < live) {
 #pragma unroll 4
@@ -800,12 +836,12 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
                       (int64_t)(done.head * p.group + r_lo + jr - jt * p.group) * p.out_head;
 #pragma unroll 1
             for (int c = c_from; c < D; c += share * 32) {
-              float v[32];
+              float v[16];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = 0.f;
+              for (int i = 0; i < 16; ++i) v[i] = 0.f;
 #pragma unroll 1
               for (int x = x0; x <= x1; x += 2 * by) {
-                float4 u[2][8];
+                float4 u[2][4];
                 float w[2];
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
@@ -813,14 +849,14 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
                   const float* src = piece(xk, c0);
                   w[k] = xk <= x1 ? exp2_fast(__ldcg(src + 128 * D + jr) - base) : 0.f;
 #pragma unroll
-                  for (int i = 0; i < 8; ++i)
+                  for (int i = 0; i < 4; ++i)
                     u[k][i] = xk <= x1 ? __ldcg(reinterpret_cast<const float4*>(src) + (c / 4 + i) * 128 + jr)
                                        : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
 #pragma unroll
-                  for (int i = 0; i < 8; ++i) {
+                  for (int i = 0; i < 4; ++i) {
                     v[4 * i] = fmaf(u[k][i].x, w[k], v[4 * i]);
                     v[4 * i + 1] = fmaf(u[k][i].y, w[k], v[4 * i + 1]);
                     v[4 * i + 2] = fmaf(u[k][i].z, w[k], v[4 * i + 2]);
@@ -829,17 +865,16 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
               }
               if (final) {
                 store(jdst, c, v, inv_all);
-                store(jdst, c + 16, v + 16, inv_all);
               } else {
 #pragma unroll
-                for (int i = 0; i < 32; i += 4)
+                for (int i = 0; i < 16; i += 4)
                   __stcg(reinterpret_cast<float4*>(piece(x0, c0)) + (c / 4 + i / 4) * 128 + jr,
                          make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
               }
             }
           }
           if (!final) {
-            named_barrier(1 + q, 128);  // all threads of a row have read its statistics
+            named_barrier(1 + q, 256);  // all threads of a row have read its statistics
             if (jr < live && c_from == 0) {
               __stcg(piece(x0, c0) + 128 * D + jr, top);
               __stcg(piece(x0, c0) + 128 * (D + 1) + jr, total);
@@ -858,7 +893,7 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
       }
       __syncwarp();
     }
-    if (lent) named_barrier(5, 256);
+    if (lent) named_barrier(5, 512);
   }
   tc_fence_before();
   __syncthreads();

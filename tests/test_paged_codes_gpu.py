@@ -112,6 +112,22 @@ def test_attention_with_many_items_and_tiles_a_cta(cuda_dev, workspace, q_lens, 
     assert torch.equal(attend(pr, workspace), got)
 
 
+@pytest.mark.parametrize("q_lens, kv_lens, dtype", [
+    ([900, 130, 257, 700, 64, 1000], [900, 1300, 257, 2700, 3000, 1000], "bf16"),
+    ([400] * 6, [5000, 400, 3000, 401, 900, 2000], "f16"), ([1, 1, 1, 1] * 12, [3000, 17, 900, 5000] * 12, "bf16"),
+])
+def test_many_calls_give_the_same_bits(cuda_dev, workspace, q_lens, kv_lens, dtype):  # noqa: F811
+    """Every CTA at work over many tiles, again and again: what a stage hands on it has read whole."""
+    pr = problem(cuda_dev, 14, q_lens, kv_lens, 32, 8, 128, dtype, 16)
+    want = attend(pr, workspace)
+    out = torch.empty_like(want)
+    wrong = torch.zeros((), dtype=torch.bool, device=cuda_dev)
+    for _ in range(60):
+        attend(pr, workspace, out=out.fill_(float("nan")))
+        wrong |= (out != want).any()
+    assert not wrong
+
+
 @pytest.mark.parametrize("dim, block, dtype, layout", [
     (128, 16, "f32", "head"), (64, 5, "f32", "token"), (128, 1, "bf16", "token"), (96, 16, "bf16", "head"),
     (112, 16, "f16", "head"), (40, 24, "bf16", "token"), (256, 12, "f16", "token"), (8, 3, "f16", "head"),
