@@ -5,14 +5,16 @@ its drafts, packed into one batch:
 
     plan_paged_step   blocks, slots, positions; its q_indptr routes the LoRA segments too
     apply_lora_group  the adapters' deltas on the fused q/k/v projection (and on o)
-    write / attend    new keys and values into the cache, attention over it
+    append / attend   queries and keys rotated, new keys and values into the cache, attention over it
     verify_draft      which drafts stay, and the token behind them
     advance           the tokens that stay
 
 The weights are random and the drafter is a table of next-token logits, so the text means
 nothing; the emitted tokens are distributed as the decoder's own, drafts or not.
 
-    python examples/speculative_decode.py [--requests 8] [--steps 32] [--drafts 4]
+    python examples/speculative_decode.py [--requests 8] [--steps 32] [--drafts 4] [--codes]
+
+With --codes the cache holds keys and values as e4m3 codes, in half the memory.
 """
 
 from __future__ import annotations
@@ -31,6 +33,7 @@ from multi_lora_b200 import KernelInputMetaData  # noqa: E402
 from multi_lora_b200.backend import get_lora_backend  # noqa: E402
 from multi_lora_b200.paged_kv import PagedKVCache  # noqa: E402
 from multi_lora_b200.rmsnorm import rmsnorm_fwd  # noqa: E402
+from multi_lora_b200.rotary import RotaryPositions  # noqa: E402
 from multi_lora_b200.speculative import verify_draft  # noqa: E402
 
 
@@ -58,19 +61,16 @@ class LoRADecoder:
         self.ranks = torch.full((slots,), rank, dtype=torch.int32, device=device)
         self.scalings = torch.ones(slots, dtype=dtype, device=device)
         self.freqs = 10000.0 ** (-torch.arange(self.dim // 2, device=device) / (self.dim // 2))
+        self.rotary = RotaryPositions.from_frequencies(self.freqs.tolist(), device)
         self.dtype, self.device, self.vocab = dtype, torch.device(device), vocab
         self.backend = get_lora_backend("cuda")
 
-    def cache(self, requests: int, max_tokens: int, block_size: int = 16) -> PagedKVCache:
+    def cache(self, requests: int, max_tokens: int, block_size: int = 16,
+              dtype: Optional[torch.dtype] = None) -> PagedKVCache:
         blocks = -(-max_tokens // block_size)
         return PagedKVCache(layers=len(self.layers), num_blocks=requests * blocks, block_size=block_size,
                             kv_heads=self.kv_heads, head_dim=self.dim, max_requests=requests, max_blocks=blocks,
-                            dtype=self.dtype, device=self.device)
-
-    def _rotate(self, x: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
-        angle = positions[:, None, None] * self.freqs
-        a, b = x.float().chunk(2, -1)
-        return torch.cat([a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()], -1).to(x.dtype)
+                            dtype=dtype or self.dtype, device=self.device)
 
     def forward(self, ids: torch.Tensor, cache: PagedKVCache, new_lens: torch.Tensor, max_q_len: int,
                 slots: torch.Tensor) -> torch.Tensor:
@@ -85,20 +85,21 @@ class LoRADecoder:
             qkv = F.linear(x, w["qkv"])
             self.backend.apply_lora_group(x, w["a"][:3], w["b"][:3], list(qkv.split(self.outs, -1)))
             q, k, v = (t.unflatten(-1, (-1, self.dim)) for t in qkv.split(self.outs, -1))
-            cache.write(i, self._rotate(k, plan.positions), v)
-            o = cache.attend(i, self._rotate(q, plan.positions), max_q_len).flatten(1)
+            q = cache.append(i, q, k, v, self.rotary)
+            o = cache.attend(i, q, max_q_len).flatten(1)
             h = h + self.backend.apply_lora(o, w["a"][3], w["b"][3], F.linear(o, w["o"]))
         return F.linear(rmsnorm_fwd(h, self.norm, 1e-6), self.head)
 
 
 @torch.inference_mode()
 def generate(model: LoRADecoder, prompts: List[List[int]], slots: List[int], steps: int, drafts: int,
-             drafter: Optional[torch.Tensor], temperature: float = 1.0, seed: int = 0):
+             drafter: Optional[torch.Tensor], temperature: float = 1.0, seed: int = 0,
+             cache_dtype: Optional[torch.dtype] = None):
     """``steps`` steps behind the prompts. ``drafter`` [vocab, vocab]: next-token logits of the draft model (None with
     ``drafts`` = 0). Returns the emitted tokens per request and the share of drafts that was kept."""
     dev, r = model.device, len(prompts)
     g = torch.Generator(device=dev).manual_seed(seed)
-    cache = model.cache(r, max(map(len, prompts)) + steps * (drafts + 1) + 1)
+    cache = model.cache(r, max(map(len, prompts)) + steps * (drafts + 1) + 1, dtype=cache_dtype)
     slot_ids = torch.tensor(slots, dtype=torch.int32, device=dev)
 
     def probs(logits):
@@ -138,13 +139,15 @@ def main() -> None:
     ap.add_argument("--requests", type=int, default=8)
     ap.add_argument("--steps", type=int, default=32)
     ap.add_argument("--drafts", type=int, default=4)
+    ap.add_argument("--codes", action="store_true", help="a cache of e4m3 codes")
     args = ap.parse_args()
     model = LoRADecoder()
     g = torch.Generator().manual_seed(1)
     prompts = [torch.randint(0, model.vocab, (int(n),), generator=g).tolist()
                for n in torch.randint(3, 200, (args.requests,), generator=g)]
     drafter = (model.embed @ model.head.T).float()  # what the decoder would say without its layers
-    out, share = generate(model, prompts, [i % 4 for i in range(args.requests)], args.steps, args.drafts, drafter)
+    out, share = generate(model, prompts, [i % 4 for i in range(args.requests)], args.steps, args.drafts, drafter,
+                          cache_dtype=torch.float8_e4m3fn if args.codes else None)
     total = sum(map(len, out))
     print(f"{total} tokens in {args.steps} steps of {args.requests} requests: "
           f"{total / (args.steps * args.requests):.2f} a step, {100 * share:.0f} % of the drafts kept")

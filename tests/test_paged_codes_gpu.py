@@ -8,12 +8,14 @@ from __future__ import annotations
 import numpy as np
 import pytest
 import torch
+from torch.utils._python_dispatch import TorchDispatchMode
 
+from test_paged_decode_gpu import example
 from test_paged_gpu import DTYPES, SHAPES, host, i32, status_word, workspace  # noqa: F401  (a fixture)
 from test_rotary_gpu import E4M3, HALF
 
 from multi_lora_b200 import paged_kv as P
-from multi_lora_b200.rotary import RotaryPositions
+from multi_lora_b200.rotary import RotaryPositions, rotate
 from oracle import paged_oracle as O
 
 pytestmark = pytest.mark.gpu
@@ -114,7 +116,9 @@ def test_attention_with_many_items_and_tiles_a_cta(cuda_dev, workspace, q_lens, 
 
 @pytest.mark.parametrize("q_lens, kv_lens, dtype", [
     ([900, 130, 257, 700, 64, 1000], [900, 1300, 257, 2700, 3000, 1000], "bf16"),
-    ([400] * 6, [5000, 400, 3000, 401, 900, 2000], "f16"), ([1, 1, 1, 1] * 12, [3000, 17, 900, 5000] * 12, "bf16"),
+    ([400] * 6, [5000, 400, 3000, 401, 900, 2000], "f16"),
+    ([5, 6, 8, 7] * 40, [85, 120, 100, 700, 90, 128, 129, 300] * 20, "f16"),  # many short items a CTA, of one tile of keys and of two
+    ([1, 1, 1, 1] * 12, [3000, 17, 900, 5000] * 12, "bf16"),
 ])
 def test_many_calls_give_the_same_bits(cuda_dev, workspace, q_lens, kv_lens, dtype):  # noqa: F811
     """Every CTA at work over many tiles, again and again: what a stage hands on it has read whole."""
@@ -126,6 +130,8 @@ def test_many_calls_give_the_same_bits(cuda_dev, workspace, q_lens, kv_lens, dty
         attend(pr, workspace, out=out.fill_(float("nan")))
         wrong |= (out != want).any()
     assert not wrong
+    if max(q_lens) < 10:  # the oracle takes its time over the others
+        assert_attention(want, pr, dtype)
 
 
 @pytest.mark.parametrize("dim, block, dtype, layout", [
@@ -395,3 +401,95 @@ def test_cache_object_over_steps(cuda_dev, codes):
                 past[layer][i] = kv[:, :kv.shape[1] - new[i] + keep[i]]
         cache.advance(i32(keep, cuda_dev))
         cache.check()
+
+
+def test_a_captured_step_is_replayed_between_prompts_of_other_sizes(cuda_dev):
+    """A cache of codes: a step that plans, appends and attends, as a graph, next to one that does it call by call."""
+    r, heads, kv_heads, dim = 3, 4, 2, 64
+    g = torch.Generator(device=cuda_dev).manual_seed(12)
+    rotary = RotaryPositions.new(dim, cuda_dev)
+
+    class Side:
+        def __init__(self):
+            self.cache = P.PagedKVCache(layers=2, num_blocks=60, block_size=16, kv_heads=kv_heads, head_dim=dim, max_requests=r,
+                                        max_blocks=30, dtype=E4M3, device=cuda_dev)
+            self.new = i32([2] * r, cuda_dev)
+            self.qkv = torch.zeros(2 * r, heads + 2 * kv_heads, dim, dtype=torch.bfloat16, device=cuda_dev)
+            self.out = [torch.zeros(2 * r, heads, dim, dtype=torch.bfloat16, device=cuda_dev) for _ in range(2)]
+
+        def step(self, new, qkv, most, outs):
+            self.cache.plan(new, qkv.shape[0])
+            for layer, out in enumerate(outs):
+                q = self.cache.append(layer, *qkv.split([heads, kv_heads, kv_heads], 1), rotary)
+                self.cache.attend(layer, q, most, out=out)
+            self.cache.advance(new)
+
+    eager, captured = Side(), Side()
+    for side in (eager, captured):
+        side.step(side.new, side.qkv, 2, side.out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured.step(captured.new, captured.qkv, 2, captured.out)
+    for lens in ([40, 0, 3], None, [0, 130, 1], [5, 5, 5], None):
+        if lens is not None:
+            qkv = torch.randn(sum(lens), heads + 2 * kv_heads, dim, generator=g, device=cuda_dev).bfloat16()
+            outs = [[torch.empty_like(qkv[:, :heads]) for _ in range(2)] for _ in range(2)]
+            for side, out in zip((eager, captured), outs):
+                side.step(i32(lens, cuda_dev), qkv, max(lens), out)
+            assert all(torch.equal(a, b) for a, b in zip(*outs))
+        qkv = torch.randn(eager.qkv.shape, generator=g, device=cuda_dev)
+        for side in (eager, captured):
+            side.qkv.copy_(qkv)
+        eager.step(eager.new, eager.qkv, 2, eager.out)
+        graph.replay()
+        for a, b in zip([*eager.out, eager.cache.ctx_lens, eager.cache.storage.view(torch.uint8), eager.cache.scale_storage],
+                        [*captured.out, captured.cache.ctx_lens, captured.cache.storage.view(torch.uint8),
+                         captured.cache.scale_storage]):
+            assert torch.equal(a, b)
+    eager.cache.check()
+    captured.cache.check()
+
+
+def test_dispatch_modes_and_profilers_see_the_operators(cuda_dev, workspace):  # noqa: F811
+    pr = problem(cuda_dev, 2, [1, 2], [20, 30], 4, 2, 64, "bf16", 16)
+    rotary, at = RotaryPositions.new(64, cuda_dev), i32([1, 2, 3], cuda_dev)
+    slots = i32([0, 1, 2], cuda_dev)
+    calls = {
+        "rotate": lambda: rotate(pr["q"], at, rotary),
+        "append_paged_kv": lambda: P.append_paged_kv(pr["q"][:, :2], pr["q"][:, 2:], pr["k"], pr["v"], slots, positions=at, rotary=rotary,
+                                                     q=pr["q"], k_scales=pr["ks"], v_scales=pr["vs"]),
+        "paged_attention_8bit": lambda: attend(pr, workspace),
+    }
+    seen = []
+
+    class Names(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    for name, call in calls.items():
+        plain = call()
+        with Names():
+            again = call()
+        assert any(s.startswith(f"mlora.{name}") for s in seen), (name, seen)
+        assert torch.equal(plain, again)
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        for call in calls.values():
+            call()
+    assert {f"mlora::{name}" for name in calls} <= {e.name for e in prof.events()}
+
+
+def test_the_decoder_with_a_cache_of_codes(cuda_dev):
+    """The example's decoder: with drafts and a cache of codes it runs, and its first logits, whose attention reads the
+    codes of the prompt alone, are near those of its own 16-bit cache (an error of 2^-4 a value, averaged over a sum)."""
+    model = example.LoRADecoder()
+    slots, lens = i32([0, 3], cuda_dev), [40, 90]
+    new = i32(lens, cuda_dev)
+    ids = torch.arange(sum(lens), device=cuda_dev)
+    with torch.inference_mode():
+        values, codes = (model.forward(ids, model.cache(2, 100, dtype=t), new, max(lens), slots).double() for t in (None, E4M3))
+    assert 0 < (values - codes).norm() < 2.0 ** -3 * values.norm()
+    out, _ = example.generate(model, [[1, 2, 3], [4] * 20], [1, 2], 6, 2, torch.zeros(model.vocab, model.vocab, device=cuda_dev),
+                              cache_dtype=E4M3)
+    assert all(7 <= len(row) <= 19 for row in out)
