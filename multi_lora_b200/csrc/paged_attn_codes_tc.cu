@@ -38,14 +38,17 @@ struct CodeChunkArgs {
   int out32;  // rows of the output allow 32-byte stores
 };
 
-template <int D>
+// ROWS: of an item, as of what paged_chunk.cuh has. Where no request has more than 128, the second tile of Q is room
+// for two more tiles of codes on their way: they are what such a call, with little to compute a key, waits for.
+template <int D, int ROWS>
 struct CodeChunkCfg {
   static constexpr int kSlot = kChunkKeys * D * 2;  // K or V of a tile
   static constexpr int kQ = 128 * D * 2;            // one tile of Q
   static constexpr int kRaw = kChunkKeys * D;       // codes of K or V of a tile
-  static constexpr int kRaws = D == 128 ? 2 : 4;
+  static constexpr int kTiles = ROWS / 128;         // of Q
+  static constexpr int kRaws = (D == 128 ? 2 : 4) + (2 - kTiles) * kQ / kRaw;
   static constexpr int kSlots = D == 128 ? 4 : 8;
-  static constexpr int kSmem = 2 * kQ + kSlots * kSlot + kRaws * kRaw;
+  static constexpr int kSmem = kTiles * kQ + kSlots * kSlot + kRaws * kRaw;
   static constexpr int kPart = 128 * (D + 2);  // floats of a tile's piece
   // tiles whose scales wait: K of a tile gets its slot when the scores of the second (D = 64: fourth) tile before it are
   // done, so all of the one before that is
@@ -93,7 +96,7 @@ __device__ __forceinline__ bool barrier_any(int id, bool mine) {
 
 // NaN that was taken out of V, added in TMEM to the outputs of row r, if it sees it: the item's keys of [from, to) that
 // not every row sees, those of every tile's half `half` if that is not negative. Seldom run.
-template <int D>
+template <int D, int ROWS>
 __device__ __noinline__ void code_give_back(const PagedAttnArgs& p, uint32_t o_addr, int column, int req, int head, int rt, int qn,
                                             int kv, int r, int from, int to, int half) {
   ChunkItem it;
@@ -102,7 +105,7 @@ __device__ __noinline__ void code_give_back(const PagedAttnArgs& p, uint32_t o_a
   it.rt = rt;
   it.rows = qn * p.group;
   int seen_lo, seen_hi;
-  chunk_seen(p, it, seen_lo, seen_hi);
+  chunk_seen<ROWS>(p, it, seen_lo, seen_hi);
   const int pos = kv - qn + paged_token(p, r);
   if (r < it.rows) {
     from = max(from, paged_first_key(p, pos));
@@ -164,22 +167,21 @@ __device__ __forceinline__ void code_put(unsigned char* row_at, int row, int chu
   *reinterpret_cast<uint4*>(row_at + (((chunk * 2 + 1) ^ (row & 7)) << 4)) = make_uint4(c.x, c.y, d.x, d.y);
 }
 
-template <typename T, int D>
+template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(kCodeThreads, 1)
 paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
-  using C = CodeChunkCfg<D>;
+  using C = CodeChunkCfg<D, ROWS>;
   constexpr int NS = C::kSlots, NR = C::kRaws, HALF = kChunkKeys * 128;
   constexpr bool TWO = !Num<T>::is_bf16;      // terms of P
   constexpr float kRaise = 4.f, kUp = 11.f;   // in powers of two
   constexpr uint32_t S_COL = 0, O_COL = 256;
   extern __shared__ __align__(1024) unsigned char s_raw[];
-  __shared__ __align__(8) uint64_t full[NS], empty[NS], raw_full[NR], raw_empty[NR], q_ready[2], q_free[2], s_full[2][2], p_ready[2][2], pv_done[2][2];
+  __shared__ __align__(8) uint64_t full[NS], empty[NS], raw_full[NR], raw_empty[NR], q_ready[C::kTiles], q_free[C::kTiles], s_full[2][2], p_ready[2][2], pv_done[2][2];
   constexpr int kScaleTiles = C::kScaleTiles;
   __shared__ __align__(16) float s_scale[kScaleTiles][2][kChunkKeys / 8];  // of K and V, for each eight keys
   __shared__ __align__(16) float s_raw_scale[NR / 2][2][kChunkKeys / 8];  // of a tile whose codes have come, with K
   __shared__ uint32_t s_tmem;
-  __shared__ int s_last[2];
-  __shared__ bool s_skipped;
+  __shared__ bool s_last[2], s_skipped;
   // What the threads of a row tell one another: a maximum or a sum of each half of the columns; and, where both tiles'
   // warpgroups work on one, the second's maximum and sum.
   __shared__ float s_part[2][2][128];
@@ -193,7 +195,7 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
     if (tid == 0) flag_error(p.status, kErrTimeout);
     return;
   }
-  unsigned char *ring = smem + 2 * C::kQ, *raw = ring + NS * C::kSlot;
+  unsigned char *ring = smem + C::kTiles * C::kQ, *raw = ring + NS * C::kSlot;
 
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
@@ -205,8 +207,10 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
       mbar_init(&raw_empty[s], 4);
     }
     for (int q = 0; q < 2; ++q) {
-      mbar_init(&q_ready[q], 1);
-      mbar_init(&q_free[q], 2);
+      if (q < C::kTiles) {
+        mbar_init(&q_ready[q], 1);
+        mbar_init(&q_free[q], 2);
+      }
       for (int b = 0; b < 2; ++b) {
         mbar_init(&s_full[q][b], 1);
         mbar_init(&p_ready[q][b], 8);
@@ -230,16 +234,17 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
   int req;
   PagedRequest found;
   bool skipped = false;  // a request that is not computed
-  paged_find<kCodeThreads, 32>(
-      p.requests,
+  static_assert(sizeof(PagedFindRoom<kCodeThreads>) <= sizeof(s_part), "shared memory");
+  paged_find_in<kCodeThreads, 32>(
+      reinterpret_cast<PagedFindRoom<kCodeThreads>&>(s_part), p.requests,
       [&](int i, int part, int parts, PagedRequest& r) {
         r = paged_request(p, i, part == 0 && blockIdx.x == 0);
         skipped |= r.odd;
         ChunkItem x;
         chunk_request(p, x, i, r);
         int n = 0;
-        for (x.rt = part; x.rt * kChunkRows < x.rows; x.rt += parts) {
-          chunk_span(p, x);
+        for (x.rt = part; x.rt * ROWS < x.rows; x.rt += parts) {
+          chunk_span<ROWS>(p, x);
           n += x.n + kChunkItem;
         }
         return n * p.kv_heads;
@@ -255,12 +260,12 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
     it.head = rel / per_head;
     rel -= it.head * per_head;
     it.rt = 0;
-    for (int rt0 = 0; rt0 * kChunkRows < it.rows; rt0 += 32) {
+    for (int rt0 = 0; rt0 * ROWS < it.rows; rt0 += 32) {
       ChunkItem x = it;
       x.rt = rt0 + lane;
       int units = 0;
-      if (x.rt * kChunkRows < x.rows) {
-        chunk_span(p, x);
+      if (x.rt * ROWS < x.rows) {
+        chunk_span<ROWS>(p, x);
         units = x.n + kChunkItem;
       }
       int upto = units;
@@ -278,10 +283,10 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
       }
       rel -= __shfl_sync(0xffffffffu, upto, 31);
     }
-    chunk_span(p, it);
+    chunk_span<ROWS>(p, it);
   };
   auto next_item = [&]() {
-    if (++it.rt * kChunkRows >= it.rows) {
+    if (++it.rt * ROWS >= it.rows) {
       it.rt = 0;
       if (++it.head == p.kv_heads) {
         it.head = 0;
@@ -295,7 +300,7 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
         }
       }
     }
-    chunk_span(p, it);
+    chunk_span<ROWS>(p, it);
   };
   if (cur.pos < cur.end) {
     chunk_request(p, it, req, found);
@@ -340,7 +345,7 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
         held = false;
       };
       while (cur.take(it.n)) {
-        const bool solo = chunk_solo(it);  // this warp then has every other half of the one tile
+        const bool solo = chunk_solo<ROWS>(it);  // this warp then has every other half of the one tile
         const int qs = solo ? 0 : q, h0 = solo ? q : 0;
         const bool odd = !solo && chunk_odd(it, cur);
         const uint32_t q_lo = smem_addr(smem + qs * C::kQ) >> 4;
@@ -398,8 +403,8 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
       int items[2] = {0, 0};
       while (cur.take(it.n)) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int r0 = it.rt * kChunkRows + q * 128;
+        for (int q = 0; q < C::kTiles; ++q) {
+          const int r0 = it.rt * ROWS + q * 128;
           if (r0 >= it.rows) continue;
           if (items[q] > 0) ok = __all_sync(0xffffffffu, ok && mbar_poll(&q_free[q], (items[q] - 1) & 1, p.status));
           ++items[q];
@@ -503,7 +508,7 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
     }
   } else if (warp >= 20) {  // ---- codes to values, 32 keys of each tile a warp ----
     regs_up<88>();
-    constexpr int PASSES = D / 16, ROWS = 32 / PASSES;  // pieces of 16 codes a thread, keys at once
+    constexpr int PASSES = D / 16, KEYS = 32 / PASSES;  // pieces of 16 codes a thread, keys at once
     const int w = warp - 20;
     // Eight lanes side by side read and write all banks: the first four pieces of one key and the last four of
     // the next (D = 64: the four pieces of two keys).
@@ -513,12 +518,7 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
     uint32_t tile_no = 0;
     float f = 0.f;  // scales of eight keys: K's in four lanes, V's in four
     uint4 u[PASSES];
-    auto take = [&]() {  // the next codes
-      ok = __all_sync(0xffffffffu, ok && mbar_poll(&raw_full[raw_slot], raw_phase, p.status));
-#pragma unroll
-      for (int i = 0; i < PASSES; ++i)
-        u[i] = *reinterpret_cast<const uint4*>(raw + raw_slot * C::kRaw + code_at<D>(row0 + i * ROWS, chunk));
-      if ((raw_slot & 1) == 0) f = s_raw_scale[raw_slot / 2][lane >> 2 & 1][w * 4 + (lane & 3)];
+    auto let_go = [&]() {  // of codes that have been read
       // These loads may still be under way when an arrival is not: without the fence the next codes came over them.
       fence_proxy_async_smem();
       __syncwarp();
@@ -527,12 +527,24 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
         raw_slot = 0;
         raw_phase ^= 1;
       }
+    };
+    auto take = [&]() {  // the next codes
+      ok = __all_sync(0xffffffffu, ok && mbar_poll(&raw_full[raw_slot], raw_phase, p.status));
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i)
+        u[i] = *reinterpret_cast<const uint4*>(raw + raw_slot * C::kRaw + code_at<D>(row0 + i * KEYS, chunk));
+      if ((raw_slot & 1) == 0) f = s_raw_scale[raw_slot / 2][lane >> 2 & 1][w * 4 + (lane & 3)];
+      if (C::kTiles == 2) let_go();
       if (round > 0) ok = __all_sync(0xffffffffu, ok && mbar_poll(&empty[slot], (round - 1) & 1, p.status));
       return ring + slot * C::kSlot + (chunk >> 2) * HALF;
     };
     auto filled = [&]() {
-      fence_proxy_async_smem();
-      __syncwarp();
+      if (C::kTiles == 2) {
+        fence_proxy_async_smem();
+        __syncwarp();
+      } else {
+        let_go();  // there are others to go on with, and one fence does
+      }
       if (lane == 0) mbar_arrive(&full[slot]);
       if (++slot == NS) {
         slot = 0;
@@ -541,21 +553,21 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
     };
     while (cur.take(it.n)) {
       int seen_lo, seen_hi;
-      chunk_seen(p, it, seen_lo, seen_hi);
+      chunk_seen<ROWS>(p, it, seen_lo, seen_hi);
       for (int k = 0; k < cur.len; ++k) {
         const int j0 = (it.tile0 + cur.tile + k) * kChunkKeys;
         unsigned char* to = take();
         if (lane < 8) s_scale[tile_no % kScaleTiles][lane >> 2][w * 4 + (lane & 3)] = f;
         ++tile_no;
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) code_put<T>(to + (row0 + i * ROWS) * 128, row0 + i * ROWS, chunk & 3, u[i]);
+        for (int i = 0; i < PASSES; ++i) code_put<T>(to + (row0 + i * KEYS) * 128, row0 + i * KEYS, chunk & 3, u[i]);
         filled();
         to = take();
         if (j0 + kChunkKeys > seen_hi || j0 < seen_lo) {  // keys that not every row sees
           bool taken = false;
 #pragma unroll
           for (int i = 0; i < PASSES; ++i) {
-            const int j = j0 + row0 + i * ROWS;
+            const int j = j0 + row0 + i * KEYS;
             if (j >= seen_lo && j < seen_hi) continue;
             const uint4 nan = make_uint4(codes_nan(u[i].x), codes_nan(u[i].y), codes_nan(u[i].z), codes_nan(u[i].w));
             const bool some = j >= it.first && j < it.end;
@@ -568,7 +580,7 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
           if (taken) count_store(&s_taken, 1u);
         }
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) code_put<__half>(to + (row0 + i * ROWS) * 128, row0 + i * ROWS, chunk & 3, u[i]);
+        for (int i = 0; i < PASSES; ++i) code_put<__half>(to + (row0 + i * KEYS) * 128, row0 + i * KEYS, chunk & 3, u[i]);
         filled();
       }
       if (cur.advance()) next_item();
@@ -587,8 +599,8 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
     while (cur.take(it.n)) {
       if (lent) named_barrier(5, 512);
       lent = false;
-      const bool solo = chunk_solo(it);  // the tiles' warpgroups share its keys, half by half
-      const int r_lo = it.rt * kChunkRows + (solo ? 0 : q * 128), r = r_lo + row;
+      const bool solo = chunk_solo<ROWS>(it);  // the tiles' warpgroups share its keys, half by half
+      const int r_lo = it.rt * ROWS + (solo ? 0 : q * 128), r = r_lo + row;
       const bool none = r - lane >= it.rows;  // no row in this warp: its lanes of P and O are never looked at
       float m = -INFINITY, l = 0.f;
       float most = 0.f, inv_most = 0.f;  // the largest scale of V so far: O is in units of it
@@ -653,7 +665,8 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
               ok = ok && mbar_poll(&pv_done[q][b ^ 1], ((n - 1) >> 1) & 1, p.status);
               __syncwarp();
               tc_fence_after();
-              const bool raise = mx > m + kRaise;
+              // every row's, while O is rescaled anyway: the next time is further off
+              const bool raise = mx > m;
               float fix = raise ? exp2_fast(m - mx) : 1.f;
               if (raise) m = mx;
               l *= fix;
@@ -725,7 +738,7 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
       __syncwarp();
       tc_fence_after();
       if (__any_sync(0xffffffffu, *const_cast<volatile uint32_t*>(&s_taken) != 0u))
-        code_give_back<D>(p, o_addr, side * (D / 2), done.req, done.head, done.rt, done.qn, done.kv, r, tile0 * kChunkKeys,
+        code_give_back<D, ROWS>(p, o_addr, side * (D / 2), done.req, done.head, done.rt, done.qn, done.kv, r, tile0 * kChunkKeys,
                           (tile0 + tiles) * kChunkKeys, solo ? q : -1);
       // An item that all four warpgroups worked on: the first two read the others' O too
       // (their threads of a row have the same TMEM lane).
@@ -902,11 +915,11 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
 
 namespace {
 
-template <typename T, int D>
+template <typename T, int D, int ROWS>
 cudaError_t launch_code_chunk(const CodeChunkArgs& a, cudaStream_t st, bool pdl) {
-  using C = CodeChunkCfg<D>;
+  using C = CodeChunkCfg<D, ROWS>;
   static_assert(C::kSmem <= 227 * 1024, "shared memory");
-  auto kern = paged_attention_code_chunk_kernel<T, D>;
+  auto kern = paged_attention_code_chunk_kernel<T, D, ROWS>;
   static SmemLimit limit;
   if (const cudaError_t e = limit.raise(kern, C::kSmem); e != cudaSuccess) return e;
   const int ctas = device_sm_count();
@@ -915,13 +928,20 @@ cudaError_t launch_code_chunk(const CodeChunkArgs& a, cudaStream_t st, bool pdl)
   return launch_kernel(kern, dim3(ctas), dim3(kCodeThreads), C::kSmem, st, pdl, a);
 }
 
+template <typename T>
+cudaError_t launch_code_chunk(const CodeChunkArgs& a, cudaStream_t st, bool pdl) {
+  const bool one = (int64_t)a.a.max_q_len * a.a.group <= 128;  // tile of rows a request
+  if (a.a.dim <= 64) return one ? launch_code_chunk<T, 64, 128>(a, st, pdl) : launch_code_chunk<T, 64, kChunkRows>(a, st, pdl);
+  return one ? launch_code_chunk<T, 128, 128>(a, st, pdl) : launch_code_chunk<T, 128, kChunkRows>(a, st, pdl);
+}
+
 }  // namespace
 
 cudaError_t launch_paged_attention_code_chunk(const PagedAttnArgs& a, int dtype, cudaStream_t st, bool pdl) {
   // a maximum of scores is one of scaled scores for a positive scale only
   if ((dtype != kBF16 && dtype != kF16) || a.dim > 128 || !(a.scale > 0.f)) return cudaErrorNotSupported;
   // units of work (paged_sched.cuh) in 32 bits
-  const long long items = (long long)a.tokens * a.group / kChunkRows + a.requests;
+  const long long items = (long long)a.tokens * a.group / 128 + a.requests;
   if (items * a.kv_heads * ((long long)a.width * a.block_size / kChunkKeys + 2 + kChunkItem) >= INT_MAX)
     return cudaErrorNotSupported;
   CodeChunkArgs c{};
@@ -930,9 +950,7 @@ cudaError_t launch_paged_attention_code_chunk(const PagedAttnArgs& a, int dtype,
   if (c.box < 8 || !paged_maps(a, kPagedCodes, a.dim <= 64 ? 64 : 128, c.box, &c.k_map, &c.v_map)) return cudaErrorNotSupported;
   c.q_tma = paged_q_map(a, dtype, 128, &c.q_map);
   c.out32 = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_token % 16 == 0 && a.out_head % 16 == 0 && a.dim % 16 == 0;
-  if (dtype == kBF16)
-    return a.dim <= 64 ? launch_code_chunk<__nv_bfloat16, 64>(c, st, pdl) : launch_code_chunk<__nv_bfloat16, 128>(c, st, pdl);
-  return a.dim <= 64 ? launch_code_chunk<__half, 64>(c, st, pdl) : launch_code_chunk<__half, 128>(c, st, pdl);
+  return dtype == kBF16 ? launch_code_chunk<__nv_bfloat16>(c, st, pdl) : launch_code_chunk<__half>(c, st, pdl);
 }
 
 }  // namespace mlora

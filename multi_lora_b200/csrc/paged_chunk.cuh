@@ -20,8 +20,10 @@ struct ChunkItem {
   int tile0, n;
 };
 
+// ROWS: of an item, kChunkRows or 128 (of which each is one tile).
+template <int ROWS = kChunkRows>
 __device__ __forceinline__ void chunk_span(const PagedAttnArgs& p, ChunkItem& it) {
-  const int r0 = it.rt * kChunkRows, r1 = min(it.rows, r0 + kChunkRows);
+  const int r0 = it.rt * ROWS, r1 = min(it.rows, r0 + ROWS);
   const int base = it.kv - it.qn;
   it.first = paged_first_key(p, base + paged_token(p, r0));
   it.end = max(0, base + paged_token(p, r1 - 1) + 1);
@@ -30,15 +32,19 @@ __device__ __forceinline__ void chunk_span(const PagedAttnArgs& p, ChunkItem& it
 }
 
 // Keys [lo, hi) that every row of the item sees (none when lo >= hi).
+template <int ROWS = kChunkRows>
 __device__ __forceinline__ void chunk_seen(const PagedAttnArgs& p, const ChunkItem& it, int& lo, int& hi) {
-  const int r0 = it.rt * kChunkRows, r1 = min(it.rows, r0 + kChunkRows);
+  const int r0 = it.rt * ROWS, r1 = min(it.rows, r0 + ROWS);
   const int base = it.kv - it.qn;
   lo = paged_first_key(p, base + paged_token(p, r1 - 1));
   hi = max(0, base + paged_token(p, r0) + 1);
 }
 
 // One tile of rows only: the warps of both tiles work on it, each on every other half of the keys.
-__device__ __forceinline__ bool chunk_solo(const ChunkItem& it) { return it.rows - it.rt * kChunkRows <= 128; }
+template <int ROWS = kChunkRows>
+__device__ __forceinline__ bool chunk_solo(const ChunkItem& it) {
+  return ROWS == 128 || it.rows - it.rt * ROWS <= 128;
+}
 
 __device__ __forceinline__ void chunk_request(const PagedAttnArgs& p, ChunkItem& it, int req, const PagedRequest& r) {
   it.req = req;

@@ -168,17 +168,21 @@ __device__ __forceinline__ void paged_find_warp(int requests, F units, S& split,
   found.kv = __shfl_sync(0xffffffffu, last.kv, src);
 }
 
+// What its threads tell one another, in shared memory.
+template <int NT>
+struct PagedFindRoom {
+  int warp[NT / 32];
+  int before, sum, req;
+  PagedRequest found;
+};
+
 template <int NT, int MAX_PARTS, typename F, typename S>
-__device__ __forceinline__ void paged_find(int requests, F units, S& split, int& req, PagedRequest& found,
-                                           int& before, int& in_req) {
+__device__ __forceinline__ void paged_find_in(PagedFindRoom<NT>& room, int requests, F units, S& split, int& req,
+                                              PagedRequest& found, int& before, int& in_req) {
   if (requests <= 32) {  // every warp for itself, without a barrier
     paged_find_warp<MAX_PARTS>(requests, units, split, req, found, before, in_req);
     return;
   }
-  __shared__ int s_warp[NT / 32];
-  __shared__ int s_before, s_sum;
-  __shared__ int s_req;
-  __shared__ PagedRequest s_found;
   PagedRequest last = {0, 0, 0, false};
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int parts = 1;
@@ -196,13 +200,13 @@ __device__ __forceinline__ void paged_find(int requests, F units, S& split, int&
     const int w = __shfl_xor_sync(0xffffffffu, all_parts, o);
     if (o < parts) all_parts = paged_sum(all_parts, w);
   }
-  if (lane == 31) s_warp[warp] = incl;
-  if (tid == 0) s_req = requests;
+  if (lane == 31) room.warp[warp] = incl;
+  if (tid == 0) room.req = requests;
   __syncthreads();
   int total = 0, upto = incl - mine;
 #pragma unroll
   for (int w = 0; w < NT / 32; ++w) {
-    const int u = s_warp[w];
+    const int u = room.warp[w];
     upto += w < warp ? u : 0;
     total = paged_sum(total, u);
   }
@@ -214,18 +218,25 @@ __device__ __forceinline__ void paged_find(int requests, F units, S& split, int&
       for (all_parts = units(i, 0, 1, last); a >= upto + all_parts && i + 1 < r1; all_parts = units(++i, 0, 1, last))
         upto += all_parts;
     }
-    s_req = i;
-    s_before = upto;
-    s_sum = all_parts;
-    s_found = last;
+    room.req = i;
+    room.before = upto;
+    room.sum = all_parts;
+    room.found = last;
   }
   __syncthreads();
-  req = same_in_warp(s_req);
-  before = same_in_warp(s_before);
-  in_req = same_in_warp(s_sum);
-  found.q0 = same_in_warp(s_found.q0);
-  found.qn = same_in_warp(s_found.qn);
-  found.kv = same_in_warp(s_found.kv);
+  req = same_in_warp(room.req);
+  before = same_in_warp(room.before);
+  in_req = same_in_warp(room.sum);
+  found.q0 = same_in_warp(room.found.q0);
+  found.qn = same_in_warp(room.found.qn);
+  found.kv = same_in_warp(room.found.kv);
+}
+
+template <int NT, int MAX_PARTS, typename F, typename S>
+__device__ __forceinline__ void paged_find(int requests, F units, S& split, int& req, PagedRequest& found,
+                                           int& before, int& in_req) {
+  __shared__ PagedFindRoom<NT> room;
+  paged_find_in<NT, MAX_PARTS>(room, requests, units, split, req, found, before, in_req);
 }
 
 // The first request from i on with rows, at most `most` of them (tokens x group), in the rare case that there
