@@ -174,6 +174,7 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
   constexpr int NS = C::kSlots, NR = C::kRaws, HALF = kChunkKeys * 128;
   constexpr bool TWO = !Num<T>::is_bf16;      // terms of P
   constexpr float kRaise = 4.f, kUp = 11.f;   // in powers of two
+  constexpr float kLeast = 0x1p-149f;         // positive
   constexpr uint32_t S_COL = 0, O_COL = 256;
   extern __shared__ __align__(1024) unsigned char s_raw[];
   __shared__ __align__(8) uint64_t full[NS], empty[NS], raw_full[NR], raw_empty[NR], q_ready[C::kTiles], q_free[C::kTiles], s_full[2][2], p_ready[2][2], pv_done[2][2];
@@ -631,7 +632,7 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
           const float largest = fmaxf(max3(max3(fa.x, fa.y, fa.z), fa.w, fb.x), max3(fb.y, fb.z, fb.w));
           const float4 f4 = *reinterpret_cast<const float4*>(f + side * 4), g4 = side == 0 ? fa : fb;
           // not zero, so that minus infinity stays what it is
-          const float fk[4] = {fmaxf(f4.x * sl, 1e-37f), fmaxf(f4.y * sl, 1e-37f), fmaxf(f4.z * sl, 1e-37f), fmaxf(f4.w * sl, 1e-37f)};
+          const float fk[4] = {fmaxf(f4.x * sl, kLeast), fmaxf(f4.y * sl, kLeast), fmaxf(f4.z * sl, kLeast), fmaxf(f4.w * sl, kLeast)};
           tmem_wait_ld();
           tie32(s);
           const int j0 = key0 + half * kHalfKeys + side * 32;
