@@ -36,12 +36,20 @@ bool one_map(CUtensorMap* map, const void* base, int dtype, const PagedAttnArgs&
   const cuuint64_t strides[3] = {bytes(slot, dims[1]), bytes(head, dims[2]), bytes(block, dims[3])};
   for (const cuuint64_t s : strides)
     if (s == 0 || s % 16 != 0 || s >= (1ull << 40)) return false;
+  // What L2 fetches at once is no more than a head's rows have side by side: behind them lies another head's, which is read
+  // by another CTA at another time. Caches stored token by token, 96 requests to 4095 keys of 32 heads and 4 to 131071 of 8,
+  // codes: heads of 128 bytes, 128 at once 312 and 126 us, 256 at once 376 and 159; of 64 bytes, 64 at once 291 and 80 us, 128 at
+  // once 301 and 107, 256 at once 324 and 114.
+  const int64_t row = (int64_t)a.dim * es;
+  const CUtensorMapL2promotion promotion = slot == a.dim || row >= 256 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B
+                                           : row >= 128                ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B
+                                                                       : CU_TENSOR_MAP_L2_PROMOTION_L2_64B;
   const cuuint32_t boxes[4] = {(cuuint32_t)columns, (cuuint32_t)box, 1, 1}, ones[4] = {1, 1, 1, 1};
   return enc(map, dtype == kPagedCodes ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                   : dtype == kBF16     ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                        : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
              4, const_cast<void*>(base), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             columns * es == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             columns * es == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, promotion,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
