@@ -22,6 +22,8 @@
 // heads): 64 requests of 2000 keys 298 us, 3.5 TB/s of keys and values; one of 60000
 // keys 475 us; 512 new tokens 256 us. A warp a (token, query head) and a lane a key
 // took 2596, 72700 and 948 us.
+// Over codes (64 requests of 2000 keys) fp32 queries take 282 us, and 16 bits with blocks of 12 slots as many: it is
+// the work a key and query head, not the bytes.
 #include <cuda_fp8.h>
 
 #include <algorithm>

@@ -1,10 +1,10 @@
 // Attention of chunks over a paged cache of e4m3 codes, on the fifth-generation tensor cores.
 //
 // Items, halves of tiles, TMEM and the running maximum are those of csrc/paged_attn_tc.cu. What differs is how K and V
-// come to the tensor cores: TMA brings the codes' pages, and a warpgroup of its own
-// writes them as 16-bit values into the swizzled tiles that the products read: K in the queries'
-// type, V in f16, both exact. (It takes codes to registers before it waits for room to write, so its registers are a
-// stage of the pipeline too.) Scales stay in fp32 outside the products:
+// come to the tensor cores: TMA brings the codes' pages, and a warpgroup of its own writes them as 16-bit values into
+// the swizzled tiles that the products read: K in the queries' type, V in f16, both exact. (It takes codes to registers
+// before it waits for room to write, so its registers are a stage of the pipeline too.) Scales stay in fp32 outside
+// the products:
 //   S = Q C_K^T,  x = S f_K - m,  P = exp2(x) f_V / F,  O += P C_V,   F the largest f_V so far
 // with f constant over each eight keys, so a key's scale costs nothing beside the scale that a score has anyway (the
 // maximum is taken of each eight scores first), and a value's one multiplication of two probabilities.
@@ -16,8 +16,16 @@
 // Codes of keys that no row sees become zeros on the way, and NaN of those that only some rows see too, which is
 // added to these rows' outputs at the end (codes have no infinities).
 //
-// What bounds it: the exponentials and the tensor cores (2048 cycles a tile of 128 keys and 256 rows each, f16
-// queries 3072 of the latter).
+// A tile of 128 rows has two warpgroups, a thread half of a row's columns: with one, and twice the registers, drafts
+// took 168 us where they take 121, prompts 105 for 98, and 2048 tokens over 16384 keys 673 for 685.
+//
+// What bounds it: for 256 rows the exponentials (2048 cycles a tile of 128 keys) and the tensor cores (2048, and for f16
+// queries half as much again) beside all else that a softmax issues: a tile takes 5200 cycles, the tensor pipe is busy for two fifths of
+// them and the schedulers for a half. For few rows it is the way of a half tile from its scores to its output and back,
+// 4500 cycles for two of them, 2 TB/s. Beginnings and ends of short items cost 10 000 cycles each.
+//
+// Measured, heads of 128: 2048 tokens over 16384 keys, 32 heads over 8, 677 to 705 us in bf16 (0.58 TFLOP, counted without what is
+// masked), 798 in f16; 8 prompts of 128 to 1024 tokens 97; 32 requests with 1 to 6 drafts to 8192 keys, 64 heads over 8, f16, 121.
 #include <climits>
 
 #include "device.h"
@@ -38,8 +46,9 @@ struct CodeChunkArgs {
   int out32;  // rows of the output allow 32-byte stores
 };
 
-// ROWS: of an item, as of what paged_chunk.cuh has. Where no request has more than 128, the second tile of Q is room
-// for two more tiles of codes on their way: they are what such a call, with little to compute a key, waits for.
+// ROWS: of an item. Where no request has more than 128, the second tile of Q is room for two more tiles of codes on
+// their way: they are what such a call, with little to compute a key, waits for. (64 requests of 2000 keys, 8 key heads: 48
+// rows in f16 136 us with it and 149 without, 128 rows 151 and 162, 16 rows in bf16 143 and 150.)
 template <int D, int ROWS>
 struct CodeChunkCfg {
   static constexpr int kSlot = kChunkKeys * D * 2;  // K or V of a tile
