@@ -17,7 +17,7 @@
 // added to these rows' outputs at the end (codes have no infinities).
 //
 // A tile of 128 rows has two warpgroups, a thread half of a row's columns: with one, and twice the registers, drafts
-// took 168 us where they take 121, prompts 105 for 98, and 2048 tokens over 16384 keys 673 for 685.
+// took 168 us where two take 134, prompts 105 and 100, and 2048 tokens over 16384 keys 673 and 690.
 //
 // What bounds it: for 256 rows the exponentials (2048 cycles a tile of 128 keys) and the tensor cores (2048, and for f16
 // queries half as much again) beside all else that a softmax issues: a tile takes 5200 cycles, the tensor pipe is busy for two fifths of
@@ -25,7 +25,7 @@
 // 4500 cycles for two of them, 2 TB/s. Beginnings and ends of short items cost 10 000 cycles each.
 //
 // Measured, heads of 128: 2048 tokens over 16384 keys, 32 heads over 8, 677 to 705 us in bf16 (0.58 TFLOP, counted without what is
-// masked), 798 in f16; 8 prompts of 128 to 1024 tokens 97; 32 requests with 1 to 6 drafts to 8192 keys, 64 heads over 8, f16, 121.
+// masked), 798 in f16; 8 prompts of 128 to 1024 tokens 97; 32 requests with 1 to 6 drafts to 8192 keys, 64 heads over 8, f16, 113 to 115.
 #include <climits>
 
 #include "device.h"
@@ -37,6 +37,14 @@
 namespace mlora {
 
 constexpr int kCodeThreads = 768;  // Q, TMA and tensor cores; four warpgroups of softmax; one of codes
+
+// Where a CTA begins.
+struct CodeStart {
+  ChunkSplit split;
+  ChunkItem it;
+  int pos, unit;  // of the cursor
+};
+constexpr int kStartAt = 256;  // in shared memory, behind what paged_find_in has there
 
 struct CodeChunkArgs {
   CUtensorMap k_map, v_map, q_map;
@@ -238,32 +246,34 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
   pdl_wait();
   pdl_trigger();
 
-  ChunkSplit split;
+  // Where requests have one tile of rows, where this CTA begins is found once, by warp 3 (with many requests by all), and read
+  // by the others: 24 warps that each look for themselves take turns at every instruction, 6000 cycles (drafts 119 us, 113
+  // so). With two tiles it won prompts 1 us of 97 but cost the long loop of the softmax registers: 2048 over 16384 707 us, 676.
+  constexpr bool ONCE = ROWS == 128;
+  ChunkSplit split = {0, 0, 0, 0};
   ChunkItem it;
   int before, in_req;
   int req;
   PagedRequest found;
   bool skipped = false;  // a request that is not computed
-  static_assert(sizeof(PagedFindRoom<kCodeThreads>) <= sizeof(s_part), "shared memory");
-  paged_find_in<kCodeThreads, 32>(
-      reinterpret_cast<PagedFindRoom<kCodeThreads>&>(s_part), p.requests,
-      [&](int i, int part, int parts, PagedRequest& r) {
-        r = paged_request(p, i, part == 0 && blockIdx.x == 0);
-        skipped |= r.odd;
-        ChunkItem x;
-        chunk_request(p, x, i, r);
-        int n = 0;
-        for (x.rt = part; x.rt * ROWS < x.rows; x.rt += parts) {
-          chunk_span<ROWS>(p, x);
-          n += x.n + kChunkItem;
-        }
-        return n * p.kv_heads;
-      },
-      split, req, found, before, in_req);
-  skipped = __syncthreads_or(skipped);  // and the barriers are initialised, and s_tmem is there
-  if (tid == 0) s_skipped = skipped;    // for its own warp, at the end
-  tc_fence_after();
-  const uint32_t tmem = s_tmem;
+  static_assert(kStartAt >= sizeof(PagedFindRoom<kCodeThreads>) && kStartAt + sizeof(CodeStart) <= sizeof(s_part), "shared memory");
+  CodeStart& start = *reinterpret_cast<CodeStart*>(reinterpret_cast<unsigned char*>(s_part) + kStartAt);
+  if (!ONCE || warp == 3 || p.requests > 32)
+    paged_find_in<kCodeThreads, 32>(
+        reinterpret_cast<PagedFindRoom<kCodeThreads>&>(s_part), p.requests,
+        [&](int i, int part, int parts, PagedRequest& r) {
+          r = paged_request(p, i, part == 0 && blockIdx.x == 0);
+          skipped |= r.odd;
+          ChunkItem x;
+          chunk_request(p, x, i, r);
+          int n = 0;
+          for (x.rt = part; x.rt * ROWS < x.rows; x.rt += parts) {
+            chunk_span<ROWS>(p, x);
+            n += x.n + kChunkItem;
+          }
+          return n * p.kv_heads;
+        },
+        split, req, found, before, in_req);
   PagedCursor<ChunkSplit> cur(split);
   auto item_of_request = [&](int rel) {  // the item that holds unit `rel` of request it.req: a lane a tile of rows
     const int per_head = in_req / p.kv_heads;
@@ -312,10 +322,32 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
     }
     chunk_span<ROWS>(p, it);
   };
-  if (cur.pos < cur.end) {
-    chunk_request(p, it, req, found);
-    item_of_request(cur.pos - before);
-    if (cur.begin(it.n)) next_item();
+  auto begin = [&]() {
+    if (cur.pos < cur.end) {
+      chunk_request(p, it, req, found);
+      item_of_request(cur.pos - before);
+      if (cur.begin(it.n)) next_item();
+    }
+  };
+  if (ONCE && warp == 3) {
+    begin();
+    if (lane == 0) start = {split, it, cur.pos, cur.unit};
+  }
+  skipped = __syncthreads_or(skipped);  // and the barriers are initialised, and s_tmem and `start` are there
+  if (tid == 0) s_skipped = skipped;    // for its own warp, at the end
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  if constexpr (ONCE) {  // as values that the compiler knows to be uniform
+    split = {same_in_warp(start.split.total), same_in_warp(start.split.base), same_in_warp(start.split.rem), same_in_warp(start.split.T)};
+    it = {same_in_warp(start.it.req),   same_in_warp(start.it.head), same_in_warp(start.it.rt),    same_in_warp(start.it.q0),
+          same_in_warp(start.it.qn),    same_in_warp(start.it.kv),   same_in_warp(start.it.rows),  same_in_warp(start.it.first),
+          same_in_warp(start.it.end),   same_in_warp(start.it.tile0), same_in_warp(start.it.n)};
+    cur.pos = same_in_warp(start.pos);
+    cur.unit = same_in_warp(start.unit);
+    cur.end = split.start(blockIdx.x + 1);
+    __syncthreads();  // s_part is used again
+  } else {
+    begin();
   }
   bool ok = true;
 
