@@ -493,3 +493,36 @@ def test_the_decoder_with_a_cache_of_codes(cuda_dev):
     out, _ = example.generate(model, [[1, 2, 3], [4] * 20], [1, 2], 6, 2, torch.zeros(model.vocab, model.vocab, device=cuda_dev),
                               cache_dtype=E4M3)
     assert all(7 <= len(row) <= 19 for row in out)
+
+
+def test_two_streams_at_once(cuda_dev, workspace):  # noqa: F811
+    """Chunks and decode steps side by side, each stream with its own workspace."""
+    other = P.attention_workspace(cuda_dev)
+    problems = [problem(cuda_dev, 5, [300, 40, 129], [900, 700, 400], 8, 2, 128, "bf16", 16),
+                problem(cuda_dev, 6, [1] * 40, list(range(100, 2100, 50)), 8, 2, 128, "f16", 32),
+                problem(cuda_dev, 7, [5] * 9, list(range(300, 1200, 100)), 8, 2, 64, "bf16", 16)]
+    want = [attend(pr, workspace).clone() for pr in problems]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(10):
+        for s, stream, room in ((0, streams[0], workspace), (1, streams[1], other)):
+            with torch.cuda.stream(stream):
+                for pr in problems[::1 - 2 * s]:
+                    got[s].append(attend(pr, room))
+    torch.cuda.synchronize()
+    for s in range(2):
+        for i, out in enumerate(got[s]):
+            assert torch.equal(out, want[::1 - 2 * s][i % 3])
+
+
+@pytest.mark.parametrize("dim", [64, 80, 96, 112, 128])
+@pytest.mark.parametrize("q_len", [1, 3, 20, 70])
+def test_heads_that_lie_side_by_side(cuda_dev, workspace, dim, q_len):  # noqa: F811
+    """Token by token: behind a head's row lies the next head's, whose codes may be NaN."""
+    pr = problem(cuda_dev, dim + q_len, [q_len] * 3, [q_len + 5, 200, 513], 8, 4, dim, "bf16", 16, layout="token")
+    want = attend(pr, workspace)
+    assert_attention(want, pr, "bf16")
+    for cache in (pr["k"], pr["v"]):
+        cache.view(torch.uint8)[:, :, 1::2] = 0x7F
+    got = attend(pr, workspace)
+    assert torch.equal(got.view(3 * q_len, 4, 2, dim)[:, ::2], want.view(3 * q_len, 4, 2, dim)[:, ::2])
