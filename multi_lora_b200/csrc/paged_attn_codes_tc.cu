@@ -24,8 +24,8 @@
 // them and the schedulers for a half. For few rows it is the way of a half tile from its scores to its output and back,
 // 4500 cycles for two of them, 2 TB/s. Beginnings and ends of short items cost 10 000 cycles each.
 //
-// Measured, heads of 128: 2048 tokens over 16384 keys, 32 heads over 8, 677 to 705 us in bf16 (0.58 TFLOP, counted without what is
-// masked), 798 in f16; 8 prompts of 128 to 1024 tokens 97; 32 requests with 1 to 6 drafts to 8192 keys, 64 heads over 8, f16, 113 to 115.
+// Measured, heads of 128: 2048 tokens over 16384 keys, 32 heads over 8, 685 to 705 us in bf16 (0.58 TFLOP, counted without what is
+// masked), 798 in f16; 8 prompts of 128 to 1024 tokens 96; 32 requests with 1 to 6 drafts to 8192 keys, 64 heads over 8, f16, 113 to 115.
 #include <climits>
 
 #include "device.h"
@@ -43,6 +43,8 @@ struct CodeStart {
   ChunkSplit split;
   ChunkItem it;
   int pos, unit;  // of the cursor
+  PagedRequest found;
+  int req, before, in_req;
 };
 constexpr int kStartAt = 256;  // in shared memory, behind what paged_find_in has there
 
@@ -246,9 +248,10 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
   pdl_wait();
   pdl_trigger();
 
-  // Where requests have one tile of rows, where this CTA begins is found once, by warp 3 (with many requests by all), and read
-  // by the others: 24 warps that each look for themselves take turns at every instruction, 6000 cycles (drafts 119 us, 113
-  // so). With two tiles it won prompts 1 us of 97 but cost the long loop of the softmax registers: 2048 over 16384 707 us, 676.
+  // Where this CTA begins is found once, by warp 3 (with many requests by all), and read by the others: 24 warps that each
+  // look for themselves take turns at every instruction, 6000 cycles. With two tiles of rows an item every warp still goes
+  // from the request to the item by itself. (Drafts 119 us, 113 so; prompts 99 and 96; the item too would be another 1 us of
+  // these, but costs the softmax registers: 2048 over 16384 707 us, 685 so, and 677 where every warp finds all.)
   constexpr bool ONCE = ROWS == 128;
   ChunkSplit split = {0, 0, 0, 0};
   ChunkItem it;
@@ -258,7 +261,7 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
   bool skipped = false;  // a request that is not computed
   static_assert(kStartAt >= sizeof(PagedFindRoom<kCodeThreads>) && kStartAt + sizeof(CodeStart) <= sizeof(s_part), "shared memory");
   CodeStart& start = *reinterpret_cast<CodeStart*>(reinterpret_cast<unsigned char*>(s_part) + kStartAt);
-  if (!ONCE || warp == 3 || p.requests > 32)
+  if (warp == 3 || p.requests > 32)
     paged_find_in<kCodeThreads, 32>(
         reinterpret_cast<PagedFindRoom<kCodeThreads>&>(s_part), p.requests,
         [&](int i, int part, int parts, PagedRequest& r) {
@@ -329,9 +332,9 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
       if (cur.begin(it.n)) next_item();
     }
   };
-  if (ONCE && warp == 3) {
-    begin();
-    if (lane == 0) start = {split, it, cur.pos, cur.unit};
+  if (warp == 3) {
+    if (ONCE) begin();
+    if (lane == 0) start = {split, it, cur.pos, cur.unit, found, req, before, in_req};
   }
   skipped = __syncthreads_or(skipped);  // and the barriers are initialised, and s_tmem and `start` are there
   if (tid == 0) s_skipped = skipped;    // for its own warp, at the end
@@ -345,10 +348,17 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
     cur.pos = same_in_warp(start.pos);
     cur.unit = same_in_warp(start.unit);
     cur.end = split.start(blockIdx.x + 1);
-    __syncthreads();  // s_part is used again
   } else {
+    split = {same_in_warp(start.split.total), same_in_warp(start.split.base), same_in_warp(start.split.rem), same_in_warp(start.split.T)};
+    found = {same_in_warp(start.found.q0), same_in_warp(start.found.qn), same_in_warp(start.found.kv), false};
+    req = same_in_warp(start.req);
+    before = same_in_warp(start.before);
+    in_req = same_in_warp(start.in_req);
+    cur.pos = split.start(blockIdx.x);
+    cur.end = split.start(blockIdx.x + 1);
     begin();
   }
+  __syncthreads();  // s_part is used again
   bool ok = true;
 
   // Registers: 768 threads are launched with 80 each (61440); the warps of Q, TMA and the tensor cores keep 72, those of
