@@ -13,11 +13,11 @@
 // one behind its predecessor's or begins a block. A CTA takes the runs that begin in a window of tokens, whole,
 // with some of the heads of K or V: it has every row that a scale depends on, so nothing
 // is agreed on between CTAs. A thread goes through every so many rows of one head with one unit of them (two
-// vectors), once for the largest magnitude and back again for the codes: the last row waits in registers, others come
+// vectors), once for the largest magnitude and again for the codes: the first two wait in registers, others come
 // out of L2 again. A window's {cos, sin} are made once, for all of the CTA's heads.
 //
 // Measured over sets of inputs larger than L2, bf16 heads of 128, queries rotated beside: 512 tokens of 64 and 8 heads
-// 9.8 us (20 MB), prompts of 4340 tokens, 32 and 8 heads, 32.7 us (98 MB, 3.0 TB/s): about 240 instructions a
+// 9.4 us (20 MB), prompts of 4340 tokens, 32 and 8 heads, 32.7 us (98 MB, 3.0 TB/s): about 240 instructions a
 // unit and turn bound it, as the latency of slots, rows and scales, one after the other, does with few rows.
 #include <cuda_fp8.h>
 
@@ -31,6 +31,9 @@
 namespace mlora {
 
 constexpr int kCodeWindow = 32;
+// Rows of a thread that wait in registers between the two turns. (Four, and the three CTAs an SM that this leaves: prompts of
+// 4340 tokens 40 us, 512 single tokens 11.2, where two and four CTAs take 32.8 and 9.4; one row, forth and back, 33.0 and 9.9.)
+constexpr int kKept = 2;
 
 // What the host decides about a launch.
 struct CodeShape {
@@ -165,12 +168,7 @@ __global__ void __launch_bounds__(kRotNT, 4) paged_append_codes_kernel(const Pag
   const PagedSide& s = p.side[side];
   const T* from = static_cast<const T*>(s.src) + t0 * s.src_token + h * s.src_head;
   unsigned char* to = static_cast<unsigned char*>(s.dst) + h * s.head;
-  // its rows, in this order and back again: the last one waits in registers in between
-  auto next = [&](int row, int by) {
-    do row += by;
-    while (row >= 0 && row < rows && s_place[row].x < 0);
-    return row >= 0 && row < rows ? row : -1;
-  };
+  auto there = [&](int row) { return mine >= 0 && row < rows && s_place[row].x >= 0; };
   auto load = [&](int row, Vec<T, V> (&x)[2]) {
     const T* src = from + row * s.src_token;
     x[0].load(src + un.e0);
@@ -190,36 +188,43 @@ __global__ void __launch_bounds__(kRotNT, 4) paged_append_codes_kernel(const Pag
     }
     rotary_apply<V>(p.angles.interleaved != 0, turn, a, b);
   };
-  Vec<T, V> x[2];
-  int row = mine >= 0 ? next(lane_row - g.step, g.step) : -1;
-  if (row >= 0) load(row, x);
+  // The first rows stay in registers, those behind them come out of L2 again.
+  Vec<T, V> x[kKept][2];
+#pragma unroll
+  for (int i = 0; i < kKept; ++i)
+    if (there(lane_row + i * g.step)) load(lane_row + i * g.step, x[i]);
   if (rotated) rotary_table<V>(p.angles, t0, min(rows, g.turn_rows), s_turn);
   __syncthreads();
   // ---- the largest magnitudes, as whole numbers in the same order ----
-  if (row >= 0) {
-    uint32_t most = 0u;
-    while (true) {
-      const int after = next(row, g.step);
-      Vec<T, V> y[2];
-      if (after >= 0) load(after, y);
-      float a[V], b[V];
-      values(row, x, a, b);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const uint32_t ua = __float_as_uint(a[i]) & 0x7fffffffu, ub = __float_as_uint(b[i]) & 0x7fffffffu;
-        if (ua < 0x7f800000u) most = max(most, ua);
-        if (ub < 0x7f800000u && un.both) most = max(most, ub);
-      }
-      if (after < 0 || s_run[after] != s_run[row]) {
-        if (most != 0u) atomicMax(s_most + s_run[row] * items + own, most);
-        most = 0u;
-      }
-      if (after < 0) break;
-      row = after;
-      x[0] = y[0];
-      x[1] = y[1];
+  uint32_t most = 0u;
+  int most_run = -1;
+  auto count = [&](int row, const Vec<T, V> (&x)[2]) {
+    float a[V], b[V];
+    values(row, x, a, b);
+    const int run = s_run[row];
+    if (run != most_run) {
+      if (most != 0u) atomicMax(s_most + most_run * items + own, most);
+      most = 0u;
+      most_run = run;
     }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const uint32_t ua = __float_as_uint(a[i]) & 0x7fffffffu, ub = __float_as_uint(b[i]) & 0x7fffffffu;
+      if (ua < 0x7f800000u) most = max(most, ua);
+      if (ub < 0x7f800000u && un.both) most = max(most, ub);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kKept; ++i)
+    if (there(lane_row + i * g.step)) count(lane_row + i * g.step, x[i]);
+#pragma unroll 1
+  for (int row = lane_row + kKept * g.step; row < rows; row += g.step) {
+    if (!there(row)) continue;
+    Vec<T, V> y[2];
+    load(row, y);
+    count(row, y);
   }
+  if (most != 0u) atomicMax(s_most + most_run * items + own, most);
   __syncthreads();
   // ---- the scales ----
   for (int i = tid; i < runs * items; i += kRotNT) {
@@ -238,10 +243,7 @@ __global__ void __launch_bounds__(kRotNT, 4) paged_append_codes_kernel(const Pag
   }
   __syncthreads();
   // ---- the codes ----
-  while (row >= 0) {
-    const int after = next(row, -g.step);
-    Vec<T, V> y[2];
-    if (after >= 0) load(after, y);
+  auto put = [&](int row, const Vec<T, V> (&x)[2]) {
     float a[V], b[V];
     values(row, x, a, b);
     const int2 place = s_place[row];
@@ -249,9 +251,16 @@ __global__ void __launch_bounds__(kRotNT, 4) paged_append_codes_kernel(const Pag
     const float2 scale = s_scale[s_run[row] * items + own];
     store_codes<V>(dst + un.e0, a, scale.x, scale.y);
     if (un.both) store_codes<V>(dst + un.e1, b, scale.x, scale.y);
-    row = after;
-    x[0] = y[0];
-    x[1] = y[1];
+  };
+#pragma unroll
+  for (int i = 0; i < kKept; ++i)
+    if (there(lane_row + i * g.step)) put(lane_row + i * g.step, x[i]);
+#pragma unroll 1
+  for (int row = lane_row + kKept * g.step; row < rows; row += g.step) {
+    if (!there(row)) continue;
+    Vec<T, V> y[2];
+    load(row, y);
+    put(row, y);
   }
   if (s_grown == 0) return;
   // ---- older rows of blocks whose scales have grown ----
