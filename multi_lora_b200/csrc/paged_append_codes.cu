@@ -17,7 +17,7 @@
 // out of L2 again. A window's {cos, sin} are made once, for all of the CTA's heads.
 //
 // Measured over sets of inputs larger than L2, bf16 heads of 128, queries rotated beside: 512 tokens of 64 and 8 heads
-// 9.4 us (20 MB), prompts of 4340 tokens, 32 and 8 heads, 32.7 us (98 MB, 3.0 TB/s): about 240 instructions a
+// 7.6 us (20 MB, 2.6 TB/s), prompts of 4340 tokens, 32 and 8 heads, 32.3 us (98 MB, 3.0 TB/s): about 240 instructions a
 // unit and turn bound it, as the latency of slots, rows and scales, one after the other, does with few rows.
 #include <cuda_fp8.h>
 
@@ -263,28 +263,37 @@ __global__ void __launch_bounds__(kRotNT, 4) paged_append_codes_kernel(const Pag
     put(row, y);
   }
   if (s_grown == 0) return;
-  // ---- older rows of blocks whose scales have grown ----
-  for (int i = 0; i < runs * items; ++i) {
+  // ---- older rows of blocks whose scales have grown: a warp a block and head, four pieces a lane on their way ----
+  const int pieces = p.dim / V;
+  for (int i = tid >> 5; i < runs * items; i += kRotNT / 32) {
     const float ratio = __uint_as_float(s_most[i]);
     if (ratio == 1.f) continue;
     const int run = i / items, item = item0 + i - run * items, side = item >= p.kv_heads, h = item - side * p.kv_heads;
     const int2 place = s_place[s_first[run]];
-    const int off = place.y;
     const PagedSide& s = p.side[side];
     unsigned char* base = static_cast<unsigned char*>(s.dst) + place.x * s.block + h * s.head;
-    const int pieces = p.dim / V;
-    for (int e = tid; e < off * pieces; e += kRotNT) {
-      const int row = e / pieces;
-      unsigned char* at = base + row * s.slot + (e - row * pieces) * V;
+    const int all = place.y * pieces;
+    constexpr int AT_ONCE = 4;
+    for (int e0 = lane; e0 < all; e0 += 32 * AT_ONCE) {
       union {
         typename RawBytes<V>::type raw;
         unsigned char code[V];
-      } u;
-      u.raw = *reinterpret_cast<const typename RawBytes<V>::type*>(at);
-      float x[V];
+      } u[AT_ONCE];
+      auto at = [&](int k) {
+        const int e = e0 + 32 * k, row = e / pieces;
+        return base + row * s.slot + (e - row * pieces) * V;
+      };
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[j] = __half2float(__half(__nv_cvt_fp8_to_halfraw(u.code[j], __NV_E4M3))) * ratio;
-      store_codes<V>(at, x, 1.f, 1.f);
+      for (int k = 0; k < AT_ONCE; ++k)
+        if (e0 + 32 * k < all) u[k].raw = *reinterpret_cast<const typename RawBytes<V>::type*>(at(k));
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) {
+        if (e0 + 32 * k >= all) continue;
+        float x[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[j] = __half2float(__half(__nv_cvt_fp8_to_halfraw(u[k].code[j], __NV_E4M3))) * ratio;
+        store_codes<V>(at(k), x, 1.f, 1.f);
+      }
     }
   }
 }
@@ -299,7 +308,9 @@ cudaError_t codes_v(const PagedAppendArgs& a, cudaStream_t st, bool pdl) {
   const int q_ctas = a.q_heads > 0 ? (a.tokens + g.q_per_cta - 1) / g.q_per_cta : 0;
   // Items for which a whole block's rows are four units a thread, and windows of as many tokens (a window's
   // runs have as many rows as it has tokens, more or less), but no more than leave every SM two CTAs. (Prompts of 4340
-  // tokens 32.7 us; two units a thread 38.1, eight 37.1; 512 single tokens 9.8, 9.9 and 11.2, four CTAs an SM 14.6.)
+  // tokens 32.3 us; three units a thread 37.9, six 36.3; four CTAs an SM for 512 single tokens 14.6 and not 9.3.)
+  // Then, as long as its rows go through the threads in one turn, a window takes more tokens until all CTAs are at work
+  // at once, those of the queries among them (512 single tokens 7.6 us, 9.3 without; 400 5.6 and 7.2, 256 5.6 and 6.5).
   const int block = a.block_size < a.tokens ? a.block_size : a.tokens, all_items = 2 * a.kv_heads;
   const int64_t full = 4 * kRotNT / g.units, room = full / block;
   g.part_items = room < 1 ? 1 : room > all_items ? all_items : (int)room;
@@ -307,8 +318,10 @@ cudaError_t codes_v(const PagedAppendArgs& a, cudaStream_t st, bool pdl) {
   g.step = kRotNT / (g.units * g.part_items);
   g.parts = (all_items + g.part_items - 1) / g.part_items;
   const int64_t even = (int64_t)a.tokens * g.parts / (2 * device_sm_count()), rows = full / g.part_items;
-  const int64_t window = even < rows ? even : rows;
-  g.window = window < 1 ? 1 : window > kCodeWindow ? kCodeWindow : (int)window;
+  int64_t window = even < rows ? even : rows;
+  if (window < 1) window = 1;
+  while (window < g.step && window < rows && (a.tokens + window - 1) / window * g.parts + q_ctas > 4 * device_sm_count()) ++window;
+  g.window = window > kCodeWindow ? kCodeWindow : (int)window;
   g.max_rows = g.window + a.block_size;
   if (a.angles.turns != nullptr) {
     const int most = 48 * 1024 / (a.angles.pairs * (int)sizeof(float2));
