@@ -58,7 +58,7 @@ struct CodeChunkArgs {
 
 // ROWS: of an item. Where no request has more than 128, the second tile of Q is room for two more tiles of codes on
 // their way: they are what such a call, with little to compute a key, waits for. (64 requests of 2000 keys, 8 key heads: 48
-// rows in f16 136 us with it and 149 without, 128 rows 151 and 162, 16 rows in bf16 143 and 150.)
+// rows in f16 129 us with it and 148 without, 128 rows 147 and 159, 48 rows in bf16 146 and 155.)
 template <int D, int ROWS>
 struct CodeChunkCfg {
   static constexpr int kSlot = kChunkKeys * D * 2;  // K or V of a tile

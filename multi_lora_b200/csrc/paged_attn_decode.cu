@@ -844,7 +844,7 @@ cudaError_t launch_paged_attention_decode(const PagedAttnArgs& a, int dtype, cud
   // Codes take half the bytes, so the work a key has to halve too: eight rows are the columns of a product whose
   // rows are keys, and three CTAs of it fit an SM (96 requests of 33 to 4095 keys, one row: 303 us, and 410 with sixteen rows; 64
   // requests of 2000 keys, eight rows: 61 and 81). More than sixteen rows go to the chunk kernel (64 x 2000, sixteen rows
-  // of bf16: 88 here and 143 there; f16 96 and 132).
+  // of bf16: 88 here and 143 there; f16 96 and 126).
   return (int64_t)a.max_q_len * a.group <= 8 ? launch_decode_of<kDecCodesFew>(a, dtype, st, pdl)
                                              : launch_decode_of<kDecCodes>(a, dtype, st, pdl);
 }
