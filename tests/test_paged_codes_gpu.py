@@ -526,3 +526,30 @@ def test_heads_that_lie_side_by_side(cuda_dev, workspace, dim, q_len):  # noqa: 
         cache.view(torch.uint8)[:, :, 1::2] = 0x7F
     got = attend(pr, workspace)
     assert torch.equal(got.view(3 * q_len, 4, 2, dim)[:, ::2], want.view(3 * q_len, 4, 2, dim)[:, ::2])
+
+
+@pytest.mark.parametrize("requests, active, heads", [
+    (40, {0: 1, 39: 2}, (8, 2)), (1500, {0: 1, 31: 1, 32: 4, 33: 1, 64: 2, 500: 1, 1499: 2}, (8, 2)),  # decode kernels
+    (30, {3: 7, 29: 9}, (8, 2)), (40, {0: 7, 39: 30}, (8, 2)), (1200, {i: 1 + i % 30 for i in range(0, 1200, 97)}, (8, 2)),
+    (30, {3: 70, 29: 40}, (8, 2)), (300, {0: 30, 150: 200, 299: 5}, (8, 2)),  # chunk kernels
+])
+def test_few_active_among_many(cuda_dev, workspace, requests, active, heads):  # noqa: F811
+    q_lens = [active.get(i, 0) for i in range(requests)]
+    kv_lens = [q + 37 * i % 900 if q else 5 * (i % 3) for i, q in enumerate(q_lens)]
+    pr = problem(cuda_dev, 91, q_lens, kv_lens, *heads, 64, "bf16", 16, spare_rows=2)
+    status = status_word(cuda_dev)
+    got = attend(pr, workspace, status=status)
+    assert status.item() == 0
+    assert (got[sum(q_lens):] == 0).all()
+    assert_attention(got, pr, "bf16")
+
+
+@pytest.mark.parametrize("width", [0, 4, 2000])
+@pytest.mark.parametrize("rows, most", [(1, 1), (7, 0), (7, 3), (60, 20), (300, 40)])
+def test_no_requests_and_rows(cuda_dev, workspace, rows, most, width):  # noqa: F811
+    pr = problem(cuda_dev, 1, [1], [20], 8, 2, 128, "bf16", 16)
+    q = torch.randn(rows, 8, 128, device=cuda_dev).bfloat16()
+    out, status = torch.full_like(q, float("nan")), status_word(cuda_dev)
+    attend(dict(pr, q=q, tables=torch.zeros(0, width, dtype=torch.int32, device=cuda_dev), kv_lens=i32([], cuda_dev),
+                indptr=i32([0], cuda_dev), max_q_len=most), workspace, out=out, status=status)
+    assert (out == 0).all() and status.item() == 0
