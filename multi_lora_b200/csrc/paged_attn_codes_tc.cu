@@ -680,7 +680,7 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
           const int half = solo ? 2 * k + q : k;  // of the item
           const float* f = &s_scale[(tile_no + (half >> 1)) % kScaleTiles][0][(half & 1) * 8];
           const float4 fa = *reinterpret_cast<const float4*>(f + kChunkKeys / 8), fb = *reinterpret_cast<const float4*>(f + kChunkKeys / 8 + 4);
-          const float largest = fmaxf(max3(max3(fa.x, fa.y, fa.z), fa.w, fb.x), max3(fb.y, fb.z, fb.w));
+          const float largest = fmaxf(max3(max3(fa.x, fa.y, fa.z), fa.w, fb.x), fmaxf(max3(fb.y, fb.z, fb.w), kCodeLeast));
           const float4 f4 = *reinterpret_cast<const float4*>(f + side * 4), g4 = side == 0 ? fa : fb;
           // not zero, so that minus infinity stays what it is
           const float fk[4] = {fmaxf(f4.x * sl, kLeast), fmaxf(f4.y * sl, kLeast), fmaxf(f4.z * sl, kLeast), fmaxf(f4.w * sl, kLeast)};
@@ -711,7 +711,7 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
             if (k == 0) {
               m = mx;
               most = largest;
-              inv_most = most > 0.f ? 1.f / most : 0.f;
+              inv_most = 1.f / most;
             } else {
               // O holds the halves before this one once the last product is done
               ok = ok && mbar_poll(&pv_done[q][b ^ 1], ((n - 1) >> 1) & 1, p.status);
@@ -794,7 +794,7 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
                           (tile0 + tiles) * kChunkKeys, solo ? q : -1);
       // An item that all four warpgroups worked on: the first two read the others' O too
       // (their threads of a row have the same TMEM lane).
-      float own = most, others = 0.f;  // what the two tiles' sums are multiplied by
+      float own = 1.f, others = 0.f, mate_most = 1.f;  // what the two tiles' sums are multiplied by, besides their scales of V
       if (solo) {
         if (q == 1) {
           if (!none) {
@@ -812,8 +812,9 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
         const float mate = s_part[1][0][row];
         const float top = fmaxf(m, mate), base = top == -INFINITY ? 0.f : top;
         const float a = exp2_fast(m - base), c = exp2_fast(mate - base);
-        own = a * most;
-        others = c * s_mate_most;
+        own = a;
+        others = c;
+        mate_most = s_mate_most;
         l = l * a + s_part[1][1][row] * c;
         m = top;
       }
@@ -844,11 +845,11 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
         tmem_ld16(o_addr + c, o);
         float v[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(o[i]) * own;
+        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(o[i]) * own * most;
         if (solo) {
           tmem_ld16(o_addr + D + c, o);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = fmaf(__uint_as_float(o[i]), others, v[i]);
+          for (int i = 0; i < 16; ++i) v[i] = fmaf(__uint_as_float(o[i]) * others, mate_most, v[i]);
         }
         const int col = side * (D / 2) + c;
         if (whole) {

@@ -20,6 +20,7 @@ namespace mlora {
 
 constexpr int kCodeTile = 128;  // keys a stage: 32 of them a warp
 constexpr float kCodeUp = 15.f; // P is taken times 2^15
+constexpr float kCodeLeast = 0x1p-126f;  // what scales of V are taken relative to is no less: its reciprocal is finite
 
 // Codes 0 and 1 (2 and 3) of a word as a pair of f16.
 __device__ __forceinline__ uint32_t codes_lo(uint32_t x) {
@@ -100,11 +101,11 @@ struct CodeSums {
   }
   // In units of one, without the power of two; `weight`: of row e besides.
   __device__ __forceinline__ void settle(int e, float weight) {
-    const float f = weight * 0x1p-15f * most;
+    const float f = weight * 0x1p-15f;  // not times `most`: it may be as small as a normal number can
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) {
-      o[n][2 * e] *= f;
-      o[n][2 * e + 1] *= f;
+      o[n][2 * e] = o[n][2 * e] * f * most;
+      o[n][2 * e + 1] = o[n][2 * e + 1] * f * most;
     }
   }
 };
@@ -161,7 +162,7 @@ __device__ __forceinline__ void code_tile(CodeSums<D>& z, const uint32_t (&qf)[D
       }
   }
   // the scales of V relative to the largest so far
-  const float most = fmaxf(fmaxf(vf4[0], vf4[1]), fmaxf(vf4[2], vf4[3]));
+  const float most = fmaxf(fmaxf(fmaxf(vf4[0], vf4[1]), fmaxf(vf4[2], vf4[3])), kCodeLeast);
   if (most > z.most) {  // the whole warp
     const float f = z.most / most;
 #pragma unroll
@@ -338,11 +339,11 @@ struct CodeSumsFew {
     }
   }
   __device__ __forceinline__ void settle(int e, float weight) {
-    const float f = weight * 0x1p-15f * most;
+    const float f = weight * 0x1p-15f;
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) {
-      o[c][e] *= f;
-      o[c][2 + e] *= f;
+      o[c][e] = o[c][e] * f * most;
+      o[c][2 + e] = o[c][2 + e] * f * most;
     }
   }
 };
@@ -395,7 +396,7 @@ __device__ __forceinline__ void code_tile_few(CodeSumsFew<D>& z, const uint32_t 
         if (j >= it.limit[e] || j < it.floor_[e]) x[n][e] = -INFINITY;
       }
     }
-  const float most = fmaxf(fmaxf(vf4[0], vf4[1]), fmaxf(vf4[2], vf4[3]));
+  const float most = fmaxf(fmaxf(fmaxf(vf4[0], vf4[1]), fmaxf(vf4[2], vf4[3])), kCodeLeast);
   if (most > z.most) {  // the whole warp
     const float f = z.most / most;
     z.scale(f, f);
