@@ -430,8 +430,11 @@ int mlora_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
 size_t mlora_paged_attention_workspace_bytes(void);
 
 /*
- * The same over a cache of MLORA_E4M3 codes with scales: K and V are the values that the codes stand for, to
- * fp32's accuracy (codes enter the products as they are, scales in fp32). `dtype` is that of q and out.
+ * The same over a cache of MLORA_E4M3 codes with scales: K and V are the values that the codes stand for (codes enter the
+ * products as they are, scales in fp32). `dtype` is that of q and out. Scores, their softmax and all sums are fp32; a
+ * key's probability times its value's scale enters the product with V in 11 bits for MLORA_BF16 (whose results have 8), in 21 for
+ * MLORA_F16 and in fp32 for MLORA_F32, and in 16 bits it is no coarser than 2^-33 of the largest such product among the
+ * keys that the row sees.
  */
 int mlora_paged_attention_8bit(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,
                                int32_t q_heads, int32_t dtype, const mlora_paged_cache_t* cache,

@@ -5,13 +5,15 @@
 // the swizzled tiles that the products read: K in the queries' type, V in f16, both exact. (It takes codes to registers
 // before it waits for room to write, so its registers are a stage of the pipeline too.) Scales stay in fp32 outside
 // the products:
-//   S = Q C_K^T,  x = S f_K - m,  P = exp2(x) f_V / F,  O += P C_V,   F the largest f_V so far
+//   S = Q C_K^T,  x = S f_K - m,  P = exp2(x) f_V u,  O += P C_V,   1 / u the unit of the row's sums
 // with f constant over each eight keys, so a key's scale costs nothing beside the scale that a score has anyway (the
 // maximum is taken of each eight scores first), and a value's one multiplication of two probabilities.
 //
-// P is f16 whatever the queries are: 11 bits, taken times 2^11 (below 2^15, see kRaise), so nothing is
-// coarser than 2^-36 of the largest. For bf16 results, which keep 8 bits, that is one term and half as much work in
-// the second product as the two that bf16 probabilities need; f16 results take two terms.
+// P is f16 whatever the queries are: 11 bits of it, and nothing coarser than 2^-33 of the largest exp2(x) f_V that the
+// row has met, which is 2^8 when u is chosen (paged_codes.cuh). For bf16 results, which keep 8 bits, that is one term and
+// half as much work in the second product as the two that bf16 probabilities need; f16 results take two terms. (2^11 leaves
+// less room above, and O is multiplied more often: drafts 124 us where 2^8 takes 119, prompts 103 and 98, 2048 tokens over
+// 16384 keys 706 and 696.)
 //
 // Codes of keys that no row sees become zeros on the way, and NaN of those that only some rows see too, which is
 // added to these rows' outputs at the end (codes have no infinities).
@@ -161,10 +163,11 @@ __device__ __noinline__ void code_give_back(const PagedAttnArgs& p, uint32_t o_a
   tmem_wait_st();
 }
 
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
+// Sizes as whole numbers: 2^23 + 2^8 (code_log(f) + 127), and what 2^8 (x - m) and it may have as their sum.
+constexpr float kCodeFine = 256.f;
+__device__ __forceinline__ float code_size(float f) { return __uint_as_float((__float_as_uint(f) >> 15) + 0x4b000000u); }
+__device__ __forceinline__ float code_size_limit(float up) {
+  return __uint_as_float(0x4b000000u + (uint32_t)((kCodeTop + 254.f) * kCodeFine) - (__float_as_uint(up) >> 15));
 }
 
 // Four codes as values of T.
@@ -192,7 +195,6 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
   using C = CodeChunkCfg<D, ROWS>;
   constexpr int NS = C::kSlots, NR = C::kRaws, HALF = kChunkKeys * 128;
   constexpr bool TWO = !Num<T>::is_bf16;      // terms of P
-  constexpr float kRaise = 4.f, kUp = 11.f;   // in powers of two
   constexpr float kLeast = 0x1p-149f;         // positive
   constexpr uint32_t S_COL = 0, O_COL = 256;
   extern __shared__ __align__(1024) unsigned char s_raw[];
@@ -202,10 +204,9 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
   __shared__ __align__(16) float s_raw_scale[NR / 2][2][kChunkKeys / 8];  // of a tile whose codes have come, with K
   __shared__ uint32_t s_tmem;
   __shared__ bool s_last[2], s_skipped;
-  // What the threads of a row tell one another: a maximum or a sum of each half of the columns; and, where both tiles'
-  // warpgroups work on one, the second's maximum and sum.
+  // What the threads of a row tell one another: maximum, size or sum of each half of the columns; and, where both tiles'
+  // warpgroups work on one, the second's maximum and sum, and its unit in the first's place.
   __shared__ float s_part[2][2][128];
-  __shared__ float s_mate_most;  // the largest scale of V beside these
   __shared__ uint32_t s_taken;      // a NaN was taken out of V
   const PagedAttnArgs& p = args.a;
   const int tid = threadIdx.x, lane = tid & 31;
@@ -528,7 +529,7 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
         scales_of(next[0], next_k, next_v);
         for (int k = 0; k < cur.len; ++k) {
           const int block = next[0], off = next_off[0];
-          const float fk = next_k, fv = next_v;
+          const float fk = next_k, fv = next_v + 0.f;  // no minus zero: code_size reads its bits
           next[0] = next[1];
           next_off[0] = next_off[1];
           if (k + 1 < cur.len) scales_of(next[0], next_k, next_v);
@@ -654,8 +655,8 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
       const bool solo = chunk_solo<ROWS>(it);  // the tiles' warpgroups share its keys, half by half
       const int r_lo = it.rt * ROWS + (solo ? 0 : q * 128), r = r_lo + row;
       const bool none = r - lane >= it.rows;  // no row in this warp: its lanes of P and O are never looked at
-      float m = -INFINITY, l = 0.f;
-      float most = 0.f, inv_most = 0.f;  // the largest scale of V so far: O is in units of it
+      float m = kCodeNone, l = 0.f;
+      float up = kCodeMostUp;  // O is in units of 1 / up (paged_codes.cuh)
       {
         const int pq = it.kv - it.qn + paged_token(p, r);
         const int limit = r < it.rows ? pq + 1 : 0, floor_ = paged_first_key(p, pq);
@@ -678,12 +679,10 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
           uint32_t s[32];
           tmem_ld32_async(s_addr + b * 64 + side * 32, s);
           const int half = solo ? 2 * k + q : k;  // of the item
-          const float* f = &s_scale[(tile_no + (half >> 1)) % kScaleTiles][0][(half & 1) * 8];
-          const float4 fa = *reinterpret_cast<const float4*>(f + kChunkKeys / 8), fb = *reinterpret_cast<const float4*>(f + kChunkKeys / 8 + 4);
-          const float largest = fmaxf(max3(max3(fa.x, fa.y, fa.z), fa.w, fb.x), fmaxf(max3(fb.y, fb.z, fb.w), kCodeLeast));
-          const float4 f4 = *reinterpret_cast<const float4*>(f + side * 4), g4 = side == 0 ? fa : fb;
+          const float* f = &s_scale[(tile_no + (half >> 1)) % kScaleTiles][0][(half & 1) * 8 + side * 4];
+          const float4 f4 = *reinterpret_cast<const float4*>(f), g4 = *reinterpret_cast<const float4*>(f + kChunkKeys / 8);
           // not zero, so that minus infinity stays what it is
-          const float fk[4] = {fmaxf(f4.x * sl, kLeast), fmaxf(f4.y * sl, kLeast), fmaxf(f4.z * sl, kLeast), fmaxf(f4.w * sl, kLeast)};
+          float fk[4] = {fmaxf(f4.x * sl, kLeast), fmaxf(f4.y * sl, kLeast), fmaxf(f4.z * sl, kLeast), fmaxf(f4.w * sl, kLeast)};
           tmem_wait_ld();
           tie32(s);
           const int j0 = key0 + half * kHalfKeys + side * 32;
@@ -693,40 +692,46 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
             for (int i = 0; i < 32; ++i)
               if (i >= hi || i < lo) s[i] = 0xff800000u;  // -infinity
           }
-          float top[4];
+          const float g[4] = {g4.x, g4.y, g4.z, g4.w};
+          float top[4], over[4], size[4];  // of each eight scores: the largest; above m; and with the size of V's scale
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const uint32_t* x = &s[c * 8];
             top[c] = max3(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]));
             top[c] = max3(top[c], __uint_as_float(x[3]), __uint_as_float(x[4]));
-            top[c] = fmaxf(max3(top[c], __uint_as_float(x[5]), __uint_as_float(x[6])), __uint_as_float(x[7])) * fk[c];
+            top[c] = fmaxf(max3(top[c], __uint_as_float(x[5]), __uint_as_float(x[6])), __uint_as_float(x[7]));
+            over[c] = fmaf(top[c], fk[c], -m);
+            size[c] = fmaf(over[c], kCodeFine, code_size(g[c]));
           }
-          float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]);
-          // Both warps of the rows go by the same maximum. Seldom does one of them have to raise it; and neither writes P
-          // before the other one has its scores.
-          if (barrier_any(pair, k == 0 || mx > m + kRaise || largest > most)) {
-            s_part[q][side][row] = mx;
+          // Both warps of the rows go by the same maximum and unit. Seldom has one of them a row that needs others; and
+          // neither writes P before the other one has its scores.
+          const bool mine = fmaxf(max3(over[0], over[1], over[2]), over[3]) > kCodeRaise ||
+                            fmaxf(max3(size[0], size[1], size[2]), size[3]) > code_size_limit(up);
+          if (barrier_any(pair, mine)) {
+            // What a row goes by must not hang on scores of others, which may be of keys that it does not see: its own
+            // need is the lowest bit of what its threads tell one another.
+            const float mx = fmaxf(max3(top[0] * fk[0], top[1] * fk[1], top[2] * fk[2]), top[3] * fk[3]);
+            const uint32_t word = (__float_as_uint(mx) & ~1u) | (uint32_t)mine;
+            s_part[q][side][row] = __uint_as_float(word);
             named_barrier(pair, 64);
-            mx = fmaxf(mx, s_part[q][side ^ 1][row]);
-            if (k == 0) {
-              m = mx;
-              most = largest;
-              inv_most = 1.f / most;
-            } else {
+            const uint32_t other = __float_as_uint(s_part[q][side ^ 1][row]);
+            const bool again = ((word | other) & 1u) != 0u;
+            const float most = fmaxf(__uint_as_float(word & ~1u), __uint_as_float(other & ~1u));
+            const float raised = again && most > m ? most - m : 0.f, back = exp2_fast(-raised);
+            if (again) m = fmaxf(m, most);
+            float largest = 0.f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) largest = fmaxf(largest, g[c] * exp2_fast(fmaf(top[c], fk[c], -m)));
+            s_part[q][side ^ 1][row] = largest;  // in the place that it has just read
+            named_barrier(pair, 64);
+            const float next = again ? code_new_up(0x1p8f, up, raised, fmaxf(largest, s_part[q][side][row])) : up;
+            if (k > 0) {
               // O holds the halves before this one once the last product is done
               ok = ok && mbar_poll(&pv_done[q][b ^ 1], ((n - 1) >> 1) & 1, p.status);
               __syncwarp();
               tc_fence_after();
-              // every row's, while O is rescaled anyway: the next time is further off
-              const bool raise = mx > m;
-              float fix = raise ? exp2_fast(m - mx) : 1.f;
-              if (raise) m = mx;
-              l *= fix;
-              if (largest > most) {
-                fix *= most / largest;
-                most = largest;
-                inv_most = 1.f / most;
-              }
+              const float fix = again ? code_rescale(back, up, next) : 1.f;
+              l *= back;
 #pragma unroll 1
               for (int c = 0; c < D / 2; c += 16) {
                 uint32_t o[16];
@@ -736,10 +741,10 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
                 tmem_st16(o_addr + c, o);
               }
             }
+            up = next;
           }
-          const float ref = (m == -INFINITY ? 0.f : m) - kUp;
-          const uint64_t ref2 = pack2(-ref, -ref);
-          const float gk[4] = {g4.x * inv_most, g4.y * inv_most, g4.z * inv_most, g4.w * inv_most};
+          const uint64_t m2 = pack2(-m, -m);
+          const float gk[4] = {code_weight(g[0], up), code_weight(g[1], up), code_weight(g[2], up), code_weight(g[3], up)};
           uint64_t sum[2] = {0, 0};
           constexpr int AT_ONCE = TWO ? 16 : 32;  // keys
 #pragma unroll
@@ -747,11 +752,11 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
             uint32_t w[AT_ONCE / 2], rest[AT_ONCE / 2];  // P, two keys a column
 #pragma unroll
             for (int i = 0; i < AT_ONCE; i += 2) {
-              const float f = fk[(c + i) / 8], g = gk[(c + i) / 8];
-              const uint64_t x = fma2(pack2u(s[c + i], s[c + i + 1]), pack2(f, f), ref2);
+              const float f = fk[(c + i) / 8], w_f = gk[(c + i) / 8];
+              const uint64_t x = fma2(pack2u(s[c + i], s[c + i + 1]), pack2(f, f), m2);
               const uint64_t pp = pack2(exp2_fast(lo_of(x)), exp2_fast(hi_of(x)));
               sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pp);
-              const uint64_t pw = mul2(pp, pack2(g, g));
+              const uint64_t pw = mul2(pp, pack2(w_f, w_f));
               w[i >> 1] = pack_round2<__half>(lo_of(pw), hi_of(pw));
               if constexpr (TWO)
                 rest[i >> 1] = pack_round2<__half>(lo_of(pw) - Pack2<__half>::lo(w[i >> 1]), hi_of(pw) - Pack2<__half>::hi(w[i >> 1]));
@@ -794,27 +799,27 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
                           (tile0 + tiles) * kChunkKeys, solo ? q : -1);
       // An item that all four warpgroups worked on: the first two read the others' O too
       // (their threads of a row have the same TMEM lane).
-      float own = 1.f, others = 0.f, mate_most = 1.f;  // what the two tiles' sums are multiplied by, besides their scales of V
+      float own = code_inverse(up), others = 0.f;  // what the two tiles' sums are multiplied by
       if (solo) {
         if (q == 1) {
           if (!none) {
             named_barrier(pair, 64);  // both have the row's sum
             s_part[1][side][row] = side == 0 ? m : l;
-            s_mate_most = most;  // every warp with rows has the same
           }
+          named_barrier(14, 512);  // the first tile's warpgroups have their sums
+          if (!none && side == 0) s_part[0][0][row] = up;
           tc_fence_before();
           named_arrive(4, 512);
           lent = true;
           continue;
         }
+        named_arrive(14, 512);
         named_barrier(4, 512);
         tc_fence_after();
         const float mate = s_part[1][0][row];
-        const float top = fmaxf(m, mate), base = top == -INFINITY ? 0.f : top;
-        const float a = exp2_fast(m - base), c = exp2_fast(mate - base);
-        own = a;
-        others = c;
-        mate_most = s_mate_most;
+        const float top = fmaxf(m, mate), a = exp2_fast(m - top), c = exp2_fast(mate - top);
+        own *= a;
+        others = c * code_inverse(s_part[0][0][row]);
         l = l * a + s_part[1][1][row] * c;
         m = top;
       }
@@ -845,11 +850,11 @@ paged_attention_code_chunk_kernel(const __grid_constant__ CodeChunkArgs args) {
         tmem_ld16(o_addr + c, o);
         float v[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(o[i]) * own * most;
+        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(o[i]) * own;
         if (solo) {
           tmem_ld16(o_addr + D + c, o);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = fmaf(__uint_as_float(o[i]) * others, mate_most, v[i]);
+          for (int i = 0; i < 16; ++i) v[i] = fmaf(__uint_as_float(o[i]), others, v[i]);
         }
         const int col = side * (D / 2) + c;
         if (whole) {

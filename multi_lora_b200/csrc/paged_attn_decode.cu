@@ -113,7 +113,7 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
   extern __shared__ __align__(1024) unsigned char s_raw[];
   __shared__ __align__(8) uint64_t full[NS], empty[NS];
   __shared__ float s_m[C::kWarps][16], s_l[C::kWarps][16];
-  __shared__ __align__(16) float s_scale[CODES ? NS : 1][2][TILE / 8];  // of K and V, for each eight keys of a stage
+  __shared__ __align__(16) float s_scale[CODES ? NS : 1][3][TILE / 8];  // of K and V, and code_log of the latter, for each eight keys of a stage
   __shared__ int s_last;
   __shared__ PagedPlace s_place;  // of the item that is being joined
   const PagedAttnArgs& p = args.a;
@@ -263,7 +263,10 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
         if (ok) {
           if constexpr (CODES) {
             if (lane < jobs)
-              for (int i = 0; i < args.box / 8; ++i) s_scale[stage][side][b * (args.box / 8) + i] = scale;
+              for (int i = 0; i < args.box / 8; ++i) {
+                s_scale[stage][side][b * (args.box / 8) + i] = scale;
+                if (side == 1) s_scale[stage][2][b * (args.box / 8) + i] = code_log(scale);
+              }
             __syncwarp();
           }
           if (lane == 0) mbar_arrive_expect_tx(&full[stage], 2 * SIDE);
@@ -359,9 +362,10 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
         const uint32_t ks = smem_addr(smem + stage * 2 * SIDE);
         const CodeSpan span = {it.kv, it.first, all_first, all_end, {limit[0], limit[1]}, {floor_[0], floor_[1]}, it.qn > 1};
         const float4 key_f = *reinterpret_cast<const float4*>(&s_scale[CODES ? stage : 0][0][CODES ? kg * 4 : 0]),
-                     value_f = *reinterpret_cast<const float4*>(&s_scale[CODES ? stage : 0][1][CODES ? kg * 4 : 0]);
-        if constexpr (FEW) code_tile_few<T, D>(sums, qf, span, ks, ks + SIDE, k0, j0, key_f, value_f, row_f);
-        else if constexpr (CODES) code_tile<T, D>(sums, qf, span, ks, ks + SIDE, k0, j0, key_f, value_f, row_f);
+                     value_f = *reinterpret_cast<const float4*>(&s_scale[CODES ? stage : 0][1][CODES ? kg * 4 : 0]),
+                     value_log = *reinterpret_cast<const float4*>(&s_scale[CODES ? stage : 0][2][CODES ? kg * 4 : 0]);
+        if constexpr (FEW) code_tile_few<T, D>(sums, qf, span, ks, ks + SIDE, k0, j0, key_f, value_f, value_log, row_f);
+        else if constexpr (CODES) code_tile<T, D>(sums, qf, span, ks, ks + SIDE, k0, j0, key_f, value_f, value_log, row_f);
       }
       if constexpr (!CODES) if (j0 < it.kv && j0 + 16 > it.first) {
         const uint32_t ks = smem_addr(smem + stage * 2 * SIDE), vs = ks + SIDE;
@@ -526,7 +530,6 @@ paged_attention_decode_kernel(const __grid_constant__ DecodeArgs args) {
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], FEW ? 4 : 1);
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], FEW ? 8 : 2);
       if constexpr (FEW) l[e] += __shfl_xor_sync(0xffffffffu, l[e], 16);
-      if constexpr (CODES) l[e] *= 0x1p-15f;  // kCodeUp
       if (FEW ? lane < 4 : (lane & 3) == 0) {
         s_m[warp][row_of(e)] = m[e];
         s_l[warp][row_of(e)] = l[e];

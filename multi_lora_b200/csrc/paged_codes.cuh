@@ -5,22 +5,55 @@
 //   * Q is taken in f16. f16 queries are; a bf16 row is multiplied by the power of two that brings its largest
 //     element to 2^14 .. 2^15 (undone on the score), which keeps its 8 bits down to 2^-29 of that
 //     element and anything below to 2^-40 of it.
-//   * P times the value's scale is taken in f16 relative to the largest scale so far (per warp) and times 2^15:
-//     11 bits of it (of f16 queries, whose result has as many, two terms: 21 bits), and
-//     nothing coarser than 2^-40 of the largest scale.
+//   * P times the value's scale is taken in f16 in a unit of the row's own, in which the largest such product
+//     that the row has met is 2^11 or more: 11 bits of it (of f16 queries, whose result has as many, two
+//     terms: 21 bits), and nothing coarser than 2^-36 of the row's largest. (In units of the largest scale of a tile,
+//     values behind or beside a block of much larger ones lost their bits, for rows that do not see that block too.)
 // Four codes of a register are two operands of the product as they lie: of a row of K the dimension may be taken in any order
 // (Q in the same), and of V, transposed in pairs of columns, the even columns make one tile of eight and
 // the odd ones another, so that a thread ends up with four columns side by side.
 #pragma once
 
+#include "float2.cuh"
 #include "mma.cuh"
 #include "paged_sched.cuh"
 
 namespace mlora {
 
 constexpr int kCodeTile = 128;  // keys a stage: 32 of them a warp
-constexpr float kCodeUp = 15.f; // P is taken times 2^15
-constexpr float kCodeLeast = 0x1p-126f;  // what scales of V are taken relative to is no less: its reciprocal is finite
+
+// What enters the second product for a score x and the scale f of its value is w = exp2(x - m) f up, with a running maximum m
+// and a unit 1 / up of the row's own. `up` makes the largest exp2(x - m) f of the tile that it was chosen for a small power of
+// two (with nothing of it lost), and stays until a w would pass 2^kCodeTop or a score is kCodeRaise above m: then both
+// are chosen again. So sums seldom have to be multiplied, and w is in f16's range. What a row goes by hangs on nothing
+// but scores and scales of keys that it sees. up is at most 2^126, whose reciprocal is a normal number.
+constexpr float kCodeTop = 15.75f, kCodeRaise = 24.f;
+constexpr float kCodeNone = -0x1.fffffep127f;  // the maximum of a row that has met nothing: finite, differences are no NaN
+constexpr float kCodeMostUp = 0x1p126f;
+constexpr float kCodeWide = 0x1p18f;  // a larger maximum is chosen again at every tile: sums with it are too coarse
+
+// log2 f, taken as linear between powers of two: too small by at most 0.09. f >= 0; -127 of zero and minus zero.
+__device__ __forceinline__ float code_log(float f) { return fmaf((float)(__float_as_uint(f) & 0x7fffffffu), 0x1p-23f, -127.f); }
+// What a score and code_log of its value's scale may have as their sum: w is below 2^(kCodeTop + 0.14) then (0.05 are
+// lost to rounding), and f16 ends at 2^15.99.
+__device__ __forceinline__ float code_limit(float m, float up) {
+  return fabsf(m) < kCodeWide ? m + (kCodeTop - __log2f(up)) : -INFINITY;
+}
+// f up, finite: a probability that it meets may be zero.
+__device__ __forceinline__ float code_weight(float f, float up) { return fminf(f * up, 0x1.fffffep127f); }
+__device__ __forceinline__ float code_inverse(float x) {  // two units off at most; infinity below 2^-128
+  float y;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The unit in which `largest` is `as`, where the maximum was raised by `raised`: sums so far are not made larger.
+__device__ __forceinline__ float code_new_up(float as, float up, float raised, float largest) {
+  return fminf(fminf(as * code_inverse(largest), up * exp2_fast(raised)), kCodeMostUp);
+}
+// What sums in the old unit are multiplied by; `fix`: exp2(-raised).
+__device__ __forceinline__ float code_rescale(float fix, float up, float next) {
+  return fix * fminf(next * code_inverse(up), 0x1.fffffep127f);
+}
 
 // Codes 0 and 1 (2 and 3) of a word as a pair of f16.
 __device__ __forceinline__ uint32_t codes_lo(uint32_t x) {
@@ -90,22 +123,33 @@ __device__ __forceinline__ void code_queries(int dim, Row row, uint32_t (&qf)[D 
 template <int D>
 struct CodeSums {
   float o[D / 8][4];     // tiles 2c and 2c + 1: even and odd columns of 16 c .. 16 c + 15
-  float m[2], l[2];      // maximum and sum, the latter times 2^kCodeUp
-  float most, inv_most;  // o is in units of the largest scale of V so far, times 2^kCodeUp
+  float m[2], l[2];      // maximum and sum
+  float up[2];           // o is in units of 1 / up
+  float limit[2];        // code_limit
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-    m[0] = m[1] = -INFINITY;
+    m[0] = m[1] = kCodeNone;
     l[0] = l[1] = 0.f;
-    most = inv_most = 0.f;
+    up[0] = up[1] = kCodeMostUp;
+    limit[0] = limit[1] = -INFINITY;
   }
-  // In units of one, without the power of two; `weight`: of row e besides.
-  __device__ __forceinline__ void settle(int e, float weight) {
-    const float f = weight * 0x1p-15f;  // not times `most`: it may be as small as a normal number can
+  __device__ __forceinline__ void scale(float a, float b) {
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) {
-      o[n][2 * e] = o[n][2 * e] * f * most;
-      o[n][2 * e + 1] = o[n][2 * e + 1] * f * most;
+      o[n][0] *= a;
+      o[n][1] *= a;
+      o[n][2] *= b;
+      o[n][3] *= b;
+    }
+  }
+  // Row e in units of one, and times `weight`. (Where that product is subnormal, another part of the row is 2^-24 or more.)
+  __device__ __forceinline__ void settle(int e, float weight) {
+    const float f = weight * code_inverse(up[e]);
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) {
+      o[n][2 * e] *= f;
+      o[n][2 * e + 1] *= f;
     }
   }
 };
@@ -118,11 +162,43 @@ struct CodeSpan {
   bool several;            // tokens
 };
 
-// 32 keys from j0 on, at row k0 of a tile of K at `ks` and of V at `vs`; key_f, value_f: the scales of each eight of them;
+// New maxima and units of those of a warp's rows that need them, from 32 keys: `top`, a score or the larger of two of eight keys
+// each, and the scales of their values; lanes A, B (and C) apart have the other keys of a row.
+// What a row goes by hangs on its own scores alone: others' may be of keys that it does not see.
+template <int A, int B, int C = 0, typename Sums>
+__device__ __forceinline__ void code_raise(Sums& z, const float (&top)[4][2], const float (&f)[4], const bool (&need)[2]) {
+  auto over_lanes = [](float x) {
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, A));
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, B));
+    return C > 0 ? fmaxf(x, __shfl_xor_sync(0xffffffffu, x, C)) : x;
+  };
+  const int lane = threadIdx.x & 31;
+  const uint32_t row = C > 0 ? 0x11111111u << (lane & 3) : 0xfu << (lane & 28);  // its lanes
+  float fix[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const bool again = (__ballot_sync(0xffffffffu, need[e]) & row) != 0u;
+    const float most = over_lanes(fmaxf(fmaxf(top[0][e], top[1][e]), fmaxf(top[2][e], top[3][e])));
+    const float raised = again && most > z.m[e] ? most - z.m[e] : 0.f, back = exp2_fast(-raised);
+    if (again) z.m[e] = fmaxf(z.m[e], most);
+    float largest = 0.f;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) largest = fmaxf(largest, f[n] * exp2_fast(top[n][e] - z.m[e]));
+    largest = over_lanes(largest);
+    const float up = again ? code_new_up(0x1p11f, z.up[e], raised, largest) : z.up[e];
+    z.l[e] *= back;
+    fix[e] = again ? code_rescale(back, z.up[e], up) : 1.f;
+    z.up[e] = up;
+    z.limit[e] = code_limit(z.m[e], up);
+  }
+  z.scale(fix[0], fix[1]);
+}
+
+// 32 keys from j0 on, at row k0 of a tile of K at `ks` and of V at `vs`; key_f, value_f: the scales of each eight of them, value_log: code_log of the latter;
 // row_f: what a row's products are multiplied by besides.
 template <typename T, int D>
 __device__ __forceinline__ void code_tile(CodeSums<D>& z, const uint32_t (&qf)[D / 16][4], const CodeSpan& it, uint32_t ks,
-                                          uint32_t vs, int k0, int j0, const float4& key_f, const float4& value_f,
+                                          uint32_t vs, int k0, int j0, const float4& key_f, const float4& value_f, const float4& value_log,
                                           const float (&row_f)[2]) {
   constexpr bool TWO = !Num<T>::is_bf16;  // terms of P
   const int lane = threadIdx.x & 31;
@@ -142,7 +218,7 @@ __device__ __forceinline__ void code_tile(CodeSums<D>& z, const uint32_t (&qf)[D
         mma_16816<__half>(s[n], qf[c0 + c][0], qf[c0 + c][1], qf[c0 + c][2], qf[c0 + c][3], codes_lo(kf[n][c]), codes_hi(kf[n][c]));
   }
   const float kf4[4] = {key_f.x, key_f.y, key_f.z, key_f.w};
-  float vf4[4] = {value_f.x, value_f.y, value_f.z, value_f.w};
+  const float vf4[4] = {value_f.x, value_f.y, value_f.z, value_f.w};
   const bool edge = j0 + 32 > it.all_end || j0 < it.all_first;
 #pragma unroll
   for (int n = 0; n < 4; ++n) {
@@ -161,54 +237,32 @@ __device__ __forceinline__ void code_tile(CodeSums<D>& z, const uint32_t (&qf)[D
         if (j >= it.limit[e >> 1] || j < it.floor_[e >> 1]) s[n][e] = -INFINITY;
       }
   }
-  // the scales of V relative to the largest so far
-  const float most = fmaxf(fmaxf(fmaxf(vf4[0], vf4[1]), fmaxf(vf4[2], vf4[3])), kCodeLeast);
-  if (most > z.most) {  // the whole warp
-    const float f = z.most / most;
-#pragma unroll
-    for (int n = 0; n < D / 8; ++n) {
-      z.o[n][0] *= f;
-      z.o[n][1] *= f;
-      z.o[n][2] *= f;
-      z.o[n][3] *= f;
-    }
-    z.most = most;
-    z.inv_most = 1.f / most;
-  }
-#pragma unroll
-  for (int n = 0; n < 4; ++n) vf4[n] *= z.inv_most;
-  uint32_t pf[2][4], pr[2][4];
-  float fix[2];
+  float top[4][2];  // the larger of the lane's scores of eight keys
+  bool need[2];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    float top = fmaxf(fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1])),
-                      fmaxf(fmaxf(s[2][2 * e], s[2][2 * e + 1]), fmaxf(s[3][2 * e], s[3][2 * e + 1])));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const float m_new = fmaxf(z.m[e], top), ref = m_new == -INFINITY ? 0.f : m_new;
-    fix[e] = exp2_fast(z.m[e] - ref);
-    z.m[e] = m_new;
-    const float base = ref - kCodeUp;
-    float sum[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) top[n][e] = fmaxf(s[n][2 * e], s[n][2 * e + 1]);
+    need[e] = fmaxf(max3(top[0][e], top[1][e], top[2][e]), top[3][e]) > z.m[e] + kCodeRaise ||
+             fmaxf(max3(top[0][e] + value_log.x, top[1][e] + value_log.y, top[2][e] + value_log.z), top[3][e] + value_log.w) > z.limit[e];
+  }
+  if (__any_sync(0xffffffffu, need[0] || need[1])) code_raise<1, 2>(z, top, vf4, need);
+  uint32_t pf[2][4], pr[2][4];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const uint64_t m2 = pack2(-z.m[e], -z.m[e]), up2 = pack2(z.up[e], z.up[e]);
+    uint64_t sum = 0;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-      const float p0 = exp2_fast(s[n][2 * e] - base), p1 = exp2_fast(s[n][2 * e + 1] - base);
-      sum[n] = p0 + p1;
-      const float w0 = p0 * vf4[n], w1 = p1 * vf4[n];
+      const uint64_t x = add2(pack2(s[n][2 * e], s[n][2 * e + 1]), m2), p = pack2(exp2_fast(lo_of(x)), exp2_fast(hi_of(x)));
+      sum = add2(sum, p);
+      // f first: it and the unit may be far apart, with a probability of zero between them
+      const uint64_t w = mul2(mul2(p, pack2(vf4[n], vf4[n])), up2);
       uint32_t& hi = pf[n >> 1][(n & 1) * 2 + e];
-      hi = pack_round2<__half>(w0, w1);
-      if (TWO) pr[n >> 1][(n & 1) * 2 + e] = pack_round2<__half>(w0 - Pack2<__half>::lo(hi), w1 - Pack2<__half>::hi(hi));
+      hi = pack_round2<__half>(lo_of(w), hi_of(w));
+      if (TWO) pr[n >> 1][(n & 1) * 2 + e] = pack_round2<__half>(lo_of(w) - Pack2<__half>::lo(hi), hi_of(w) - Pack2<__half>::hi(hi));
     }
-    z.l[e] = z.l[e] * fix[e] + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-  }
-  if (__any_sync(0xffffffffu, fix[0] != 1.f || fix[1] != 1.f)) {
-#pragma unroll
-    for (int n = 0; n < D / 8; ++n) {
-      z.o[n][0] *= fix[0];
-      z.o[n][1] *= fix[0];
-      z.o[n][2] *= fix[1];
-      z.o[n][3] *= fix[1];
-    }
+    z.l[e] += lo_of(sum) + hi_of(sum);
   }
   const bool clear = j0 + 32 > it.kv || j0 < it.first, mixed = edge && it.several;
 #pragma unroll
@@ -321,13 +375,14 @@ template <int D>
 struct CodeSumsFew {
   float o[D / 16][4];    // columns 16 c + (lane / 4) * 2 and + 1 of the two rows: {first, second} of the even one, of the odd one
   float m[2], l[2];      // as in CodeSums, of rows (lane % 4) * 2 and + 1; l of the lane's keys
-  float most, inv_most;
+  float up[2], limit[2];
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
-    m[0] = m[1] = -INFINITY;
+    m[0] = m[1] = kCodeNone;
     l[0] = l[1] = 0.f;
-    most = inv_most = 0.f;
+    up[0] = up[1] = kCodeMostUp;
+    limit[0] = limit[1] = -INFINITY;
   }
   __device__ __forceinline__ void scale(float a, float b) {
 #pragma unroll
@@ -339,11 +394,11 @@ struct CodeSumsFew {
     }
   }
   __device__ __forceinline__ void settle(int e, float weight) {
-    const float f = weight * 0x1p-15f;
+    const float f = weight * code_inverse(up[e]);
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) {
-      o[c][e] = o[c][e] * f * most;
-      o[c][2 + e] = o[c][2 + e] * f * most;
+      o[c][e] *= f;
+      o[c][2 + e] *= f;
     }
   }
 };
@@ -351,7 +406,7 @@ struct CodeSumsFew {
 // As code_tile.
 template <typename T, int D>
 __device__ __forceinline__ void code_tile_few(CodeSumsFew<D>& z, const uint32_t (&qf)[D / 16][2], const CodeSpan& it, uint32_t ks,
-                                              uint32_t vs, int k0, int j0, const float4& key_f, const float4& value_f,
+                                              uint32_t vs, int k0, int j0, const float4& key_f, const float4& value_f, const float4& value_log,
                                               const float (&row_f)[2]) {
   constexpr bool TWO = !Num<T>::is_bf16;
   const int lane = threadIdx.x & 31;
@@ -383,7 +438,7 @@ __device__ __forceinline__ void code_tile_few(CodeSumsFew<D>& z, const uint32_t 
   };
   load_v(0);
   const float kf4[4] = {key_f.x, key_f.y, key_f.z, key_f.w};
-  float vf4[4] = {value_f.x, value_f.y, value_f.z, value_f.w};
+  const float vf4[4] = {value_f.x, value_f.y, value_f.z, value_f.w};
   const bool edge = j0 + 32 > it.all_end || j0 < it.all_first;
   float x[4][2];  // eight keys a step, rows
 #pragma unroll
@@ -396,42 +451,31 @@ __device__ __forceinline__ void code_tile_few(CodeSumsFew<D>& z, const uint32_t 
         if (j >= it.limit[e] || j < it.floor_[e]) x[n][e] = -INFINITY;
       }
     }
-  const float most = fmaxf(fmaxf(fmaxf(vf4[0], vf4[1]), fmaxf(vf4[2], vf4[3])), kCodeLeast);
-  if (most > z.most) {  // the whole warp
-    const float f = z.most / most;
-    z.scale(f, f);
-    z.most = most;
-    z.inv_most = 1.f / most;
-  }
-#pragma unroll
-  for (int n = 0; n < 4; ++n) vf4[n] *= z.inv_most;
-  float fix[2], base[2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    float top = fmaxf(fmaxf(x[0][e], x[1][e]), fmaxf(x[2][e], x[3][e]));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-    const float m_new = fmaxf(z.m[e], top), ref = m_new == -INFINITY ? 0.f : m_new;
-    fix[e] = exp2_fast(z.m[e] - ref);
-    z.m[e] = m_new;
-    base[e] = ref - kCodeUp;
-  }
-  if (__any_sync(0xffffffffu, fix[0] != 1.f || fix[1] != 1.f)) z.scale(fix[0], fix[1]);
-  uint32_t pf[4], pr[4];  // of eight keys each, transposed: the lane's keys are (lane % 4) * 2 and + 1, its row lane / 4
-  float sum[2] = {0.f, 0.f};
+  uint64_t size[4];
 #pragma unroll
   for (int n = 0; n < 4; ++n) {
-    const float p0 = exp2_fast(x[n][0] - base[0]), p1 = exp2_fast(x[n][1] - base[1]);
-    sum[0] += p0;
-    sum[1] += p1;
-    const float w0 = p0 * vf4[n], w1 = p1 * vf4[n];
-    const uint32_t hi = pack_round2<__half>(w0, w1);
-    pf[n] = transpose_8x8(hi);
-    if (TWO) pr[n] = transpose_8x8(pack_round2<__half>(w0 - Pack2<__half>::lo(hi), w1 - Pack2<__half>::hi(hi)));
+    const float f = n == 0 ? value_log.x : n == 1 ? value_log.y : n == 2 ? value_log.z : value_log.w;
+    size[n] = add2(pack2(x[n][0], x[n][1]), pack2(f, f));
   }
-  z.l[0] = z.l[0] * fix[0] + sum[0];
-  z.l[1] = z.l[1] * fix[1] + sum[1];
+  const bool need[2] = {fmaxf(max3(x[0][0], x[1][0], x[2][0]), x[3][0]) > z.m[0] + kCodeRaise ||
+                            fmaxf(max3(lo_of(size[0]), lo_of(size[1]), lo_of(size[2])), lo_of(size[3])) > z.limit[0],
+                        fmaxf(max3(x[0][1], x[1][1], x[2][1]), x[3][1]) > z.m[1] + kCodeRaise ||
+                            fmaxf(max3(hi_of(size[0]), hi_of(size[1]), hi_of(size[2])), hi_of(size[3])) > z.limit[1]};
+  if (__any_sync(0xffffffffu, need[0] || need[1])) code_raise<4, 8, 16>(z, x, vf4, need);
+  const uint64_t m2 = pack2(-z.m[0], -z.m[1]), up2 = pack2(z.up[0], z.up[1]);
+  uint32_t pf[4], pr[4];  // of eight keys each, transposed: the lane's keys are (lane % 4) * 2 and + 1, its row lane / 4
+  uint64_t sum = 0;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const uint64_t d = add2(pack2(x[n][0], x[n][1]), m2), p = pack2(exp2_fast(lo_of(d)), exp2_fast(hi_of(d)));
+    sum = add2(sum, p);
+    const uint64_t w = mul2(mul2(p, pack2(vf4[n], vf4[n])), up2);
+    const uint32_t hi = pack_round2<__half>(lo_of(w), hi_of(w));
+    pf[n] = transpose_8x8(hi);
+    if (TWO) pr[n] = transpose_8x8(pack_round2<__half>(lo_of(w) - Pack2<__half>::lo(hi), hi_of(w) - Pack2<__half>::hi(hi)));
+  }
+  z.l[0] += lo_of(sum);
+  z.l[1] += hi_of(sum);
   const bool clear = j0 + 32 > it.kv || j0 < it.first, mixed = edge && it.several;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {

@@ -163,7 +163,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     The cache is of q's dtype, or of float8_e4m3fn codes with ``k_scales`` and ``v_scales`` (:func:`append_paged_kv`; any
     finite scales that are not negative). Codes are exact in the products and scales multiply in float32, so the result is
-    that of the values which the codes stand for.
+    that of the values which the codes stand for. Scores, softmax and sums are float32; a key's probability times its
+    value's scale enters the product with V in 11 bits for bfloat16 results (which have 8), in 21 for float16 and in float32
+    for float32, and in 16 bits no coarser than 2^-33 of the largest one among the keys that the row sees.
     """
     _need_cuda(q, "paged_attention")
     if scale is None:
