@@ -395,7 +395,9 @@ typedef struct mlora_paged_scales {
  * most 2048 slots. Its scale becomes f = 2^k with the smallest k >= -100 for which the largest finite magnitude of the new
  * rows is at most 448 * 2^k; where they begin behind the block's first slot, not less than the
  * scale it has, and the rows before them are rounded again (to nearest even) if it grows. A code is the value over f
- * rounded to nearest even, +-448 for infinities. Rows behind the new ones stay as they are.
+ * rounded to nearest even, +-448 for infinities. Rows behind the new ones stay as they are. Scales are written: each block and
+ * head of K and of V has one of its own (a stride of 0, fine for attention, is refused where its dimension is larger
+ * than one).
  */
 int mlora_append_paged_kv(const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t q_heads, void* q_out,
                           int64_t q_out_token_stride, int64_t q_out_head_stride, const void* k, int64_t k_token_stride,

@@ -59,6 +59,24 @@ int check_scales(const mlora_paged_scales_t* s) {
   return MLORA_OK;
 }
 
+// Two dimensions of pieces of `size` elements, none on another: the pieces side by side along the one with the smaller stride, and
+// runs of them along the other.
+bool apart(int64_t n0, int64_t stride0, int64_t n1, int64_t stride1, int64_t size) {
+  if (n0 <= 1) return n1 <= 1 || stride1 >= size;
+  if (n1 <= 1) return stride0 >= size;
+  const int64_t near = stride0 < stride1 ? stride0 : stride1, far = stride0 < stride1 ? stride1 : stride0,
+                n = stride0 < stride1 ? n0 : n1;
+  return near >= size && (far - size) / near >= n - 1;
+}
+
+// Scales that are written: each block and head has one of its own.
+int check_scales_apart(const mlora_paged_scales_t* s, const mlora_paged_cache_t& c) {
+  if (!apart(c.num_blocks, s->k_block_stride, c.kv_heads, s->k_head_stride, 1) ||
+      !apart(c.num_blocks, s->v_block_stride, c.kv_heads, s->v_head_stride, 1))
+    return refuse(MLORA_ERR_INVALID_ARGUMENT, "scales that blocks or heads share cannot be appended to");
+  return MLORA_OK;
+}
+
 int check_rotary(const mlora_rotary_t* r, const int32_t* positions, int32_t head_dim) {
   if (r->pairs < 1 || r->pairs > head_dim / 2)
     return refuse(MLORA_ERR_INVALID_ARGUMENT, "%d pairs of a head_dim of %d", r->pairs, head_dim);
@@ -239,8 +257,10 @@ int mlora_append_paged_kv(const void* q, int64_t q_token_stride, int64_t q_head_
   if (int rc = check_cache(cache, codes)) return rc;
   const mlora_paged_cache_t& c = *cache;
   if (codes) {
-    if (c.num_blocks > 0)
+    if (c.num_blocks > 0) {
       if (int rc = check_scales(scales)) return rc;
+      if (int rc = check_scales_apart(scales, c)) return rc;
+    }
     if (c.block_size > mlora::kAppendMaxBlock)
       return refuse(MLORA_ERR_INVALID_ARGUMENT, "blocks of %d codes: at most %d are appended to", c.block_size, mlora::kAppendMaxBlock);
   } else if (c.dtype != dtype) {

@@ -272,7 +272,10 @@ at::Tensor append_paged_kv(const at::Tensor& k, const at::Tensor& v, at::Tensor 
     at_positions = i32(*positions, "positions", n, dev);
   }
   mlora_paged_scales_t f{};
-  if (codes) f = scales_of(*k_scales, *v_scales, c, dev);
+  if (codes) {
+    f = scales_of(*k_scales, *v_scales, c, dev);
+    TORCH_CHECK(f.k != f.v || f.k == nullptr, "mlora: k_scales and v_scales are written and must not be the same");
+  }
   at::Tensor out;
   int64_t qt = 0, qh = 0, ot = 0, oh = 0;
   if (q.has_value()) {

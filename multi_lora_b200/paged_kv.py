@@ -123,7 +123,8 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     returned (in ``q_out`` where it is given, which may be ``q`` itself). Without ``rotary`` nothing is rotated.
 
     A cache of float8_e4m3fn holds codes: slot s of block b, head h stands for ``code * scales[b, h]``, with
-    ``k_scales`` and ``v_scales`` float32 [num_blocks, kv_heads] of any strides. New rows give their block the scale 2^k of
+    ``k_scales`` and ``v_scales`` float32 [num_blocks, kv_heads], strided or not, each entry in a place of its own
+    (expanded scales are refused: they are written). New rows give their block the scale 2^k of
     the smallest k (not below -100) for which 448 * 2^k holds their largest finite magnitude. Where they begin behind a block's first slot it
     is not less than the scale that the block has, and if it grows, the rows before them are rounded again. Infinities are
     held as +-448 scales. The tokens of a block must be consecutive rows with consecutive slots, what a plan gives
