@@ -88,7 +88,7 @@ constexpr int32_t kAppendMaxDim = 512;
 
 // Rows that are written: they must not overlap one another.
 bool rows_apart(int64_t tokens, int64_t token_stride, int64_t heads, int64_t head_stride, int64_t dim) {
-  return token_stride >= 0 && head_stride >= 0 && (tokens <= 1 || token_stride >= dim) && (heads <= 1 || head_stride >= dim);
+  return token_stride >= 0 && head_stride >= 0 && apart(tokens, token_stride, heads, head_stride, dim);
 }
 
 // What is checked and set alike for a rotation and an append.
