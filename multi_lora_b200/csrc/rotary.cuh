@@ -2,8 +2,8 @@
 //
 // Pair i of a row at position t is turned by the angle t * f_i. f_i is held as a whole
 // number of 2^-64 turns, so that the product modulo one turn is a 64-bit integer multiplication,
-// exact at every position; its upper 32 bits as a float of half turns go to sincospif
-// (1.5e-9 radians from the truncation, 2^-24 relative from the float).
+// exact at every position; its upper 32 bits, rounded, go to sincospif as a float of half turns
+// (at most 2^-33 turns, 7.4e-10 radians, from the rounding, and 2^-24 relative from the float).
 #pragma once
 
 #include <stdint.h>

@@ -6,8 +6,9 @@ t * f_i radians and multiplied by a factor:
 
     (a, b) -> factor * (a cos - b sin, b cos + a sin)
 
-:class:`RotaryPositions` keeps the frequencies as whole numbers of 2^-64 turns a position, so that angles are
-exact modulo a turn at every position, however far; no table of cosines bounds the length.
+:class:`RotaryPositions` keeps the frequencies as whole numbers of 2^-64 turns a position, so that angles of the
+frequencies as they are held are exact modulo a turn at every position, however far; no table of cosines bounds the
+length. A frequency up to one radian is held to 2^-55 turns a position, what a quotient of doubles leaves.
 """
 
 from __future__ import annotations
