@@ -44,30 +44,40 @@ class RotaryPositions:
 
     @classmethod
     def new(cls, rotary_dim: int, device: torch.device, *, base: float = 10000.0, interleaved: bool = False,
-            scaling: Optional[Mapping[str, object]] = None) -> "RotaryPositions":
+            scaling: Optional[Mapping[str, object]] = None,
+            max_position_embeddings: Optional[int] = None) -> "RotaryPositions":
         """Pair i of ``rotary_dim // 2`` turns by base^(-2i / rotary_dim) radians a position, changed for long contexts by
         ``scaling``, a model configuration's ``rope_scaling`` of ``rope_type`` (or ``type``) "default", "linear",
-        "llama3" or "yarn"."""
+        "llama3" or "yarn". ``max_position_embeddings``, the configuration's own, is the trained length where a
+        "llama3" or "yarn" scaling has no ``original_max_position_embeddings``."""
         if rotary_dim < 2 or rotary_dim % 2:
             raise ValueError(f"RotaryPositions: rotary_dim {rotary_dim}: an even number is wanted")
         freqs = [base ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)]
-        freqs, factor = _scaled(freqs, rotary_dim, base, dict(scaling or {}))
+        freqs, factor = _scaled(freqs, rotary_dim, base, dict(scaling or {}), max_position_embeddings)
         return cls.from_frequencies(freqs, device, interleaved=interleaved, factor=factor)
 
 
-def _scaled(freqs: List[float], dim: int, base: float, scaling: dict):
+def _scaled(freqs: List[float], dim: int, base: float, scaling: dict, longest: Optional[int]):
     kind = scaling.get("rope_type", scaling.get("type", "default"))
     if kind == "default":
         return freqs, 1.0
     if kind not in ("linear", "llama3", "yarn"):
         raise ValueError(f"RotaryPositions: unknown rope_type {kind!r}")
-    factor = float(scaling["factor"])
+
+    def wanted(name: str, otherwise=None) -> float:
+        value = scaling.get(name)
+        value = otherwise if value is None else value
+        if value is None:
+            raise ValueError(f"RotaryPositions: a scaling of rope_type {kind!r} without {name!r}")
+        return float(value)
+
+    factor = wanted("factor")
     if kind == "linear":
         return [f / factor for f in freqs], 1.0
-    trained = float(scaling["original_max_position_embeddings"])
+    trained = wanted("original_max_position_embeddings", longest)
     if kind == "llama3":
         # by the turns that a pair makes over the trained length: many, left alone; few, slowed down; a blend between
-        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        low, high = wanted("low_freq_factor"), wanted("high_freq_factor")
         keep = [(trained * f / (2 * math.pi) - low) / (high - low) for f in freqs]
         attention = 1.0
     else:
