@@ -433,7 +433,8 @@ size_t mlora_paged_attention_workspace_bytes(void);
 
 /*
  * The same over a cache of MLORA_E4M3 codes with scales: K and V are the values that the codes stand for (codes enter the
- * products as they are, scales in fp32). `dtype` is that of q and out. Scores, their softmax and all sums are fp32; a
+ * products as they are, scales in fp32; scales of V up to 2^100, since sums are fp32). `dtype` is that of q and out.
+ * Elements of a MLORA_BF16 query below 2^-29 of its largest lose bits to f16. Scores, their softmax and all sums are fp32; a
  * key's probability times its value's scale enters the product with V in 11 bits for MLORA_BF16 (whose results have 8), in 21 for
  * MLORA_F16 and in fp32 for MLORA_F32, and in 16 bits it is no coarser than 2^-33 of the largest such product among the
  * keys that the row sees.

@@ -18,7 +18,10 @@
 //
 // Measured over sets of inputs larger than L2, bf16 heads of 128, queries rotated beside: 512 tokens of 64 and 8 heads
 // 7.6 us (20 MB, 2.6 TB/s), prompts of 4340 tokens, 32 and 8 heads, 32.3 us (98 MB, 3.0 TB/s): about 240 instructions a
-// unit and turn bound it, as the latency of slots, rows and scales, one after the other, does with few rows.
+// unit and turn bound it, as the latency of slots, rows and scales, one after the other, does with few rows. Calls that find the
+// scales which they leave behind, as these do from the second on, round no older rows again. With the scales put back
+// before every call (less 2 us for that; inputs partly in L2): 512 tokens whose scales do not grow 6.3 us, a third of them do
+// 13.0, all 16.9; the prompts, whose blocks are new, 32.4. fp32 rows of the same prompts: 49.8.
 #include <cuda_fp8.h>
 
 #include <climits>

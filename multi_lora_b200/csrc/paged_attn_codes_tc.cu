@@ -19,15 +19,16 @@
 // added to these rows' outputs at the end (codes have no infinities).
 //
 // A tile of 128 rows has two warpgroups, a thread half of a row's columns: with one, and twice the registers, drafts
-// took 168 us where two take 134, prompts 105 and 100, and 2048 tokens over 16384 keys 673 and 690.
+// took 168 us where two took 134, prompts 105 and 100, and 2048 tokens over 16384 keys 673 and 690.
 //
 // What bounds it: for 256 rows the exponentials (2048 cycles a tile of 128 keys) and the tensor cores (2048, and for f16
-// queries half as much again) beside all else that a softmax issues: a tile takes 5200 cycles, the tensor pipe is busy for two fifths of
-// them and the schedulers for a half. For few rows it is the way of a half tile from its scores to its output and back,
+// queries half as much again) beside all else that a softmax issues: a tile takes 5200 cycles, the tensor pipe is busy for two
+// fifths of them and the schedulers for a half. For few rows it is the way of a half tile from its scores to its output and back,
 // 4500 cycles for two of them, 2 TB/s. Beginnings and ends of short items cost 10 000 cycles each.
 //
-// Measured, heads of 128: 2048 tokens over 16384 keys, 32 heads over 8, 685 to 705 us in bf16 (0.58 TFLOP, counted without what is
-// masked), 798 in f16; 8 prompts of 128 to 1024 tokens 96; 32 requests with 1 to 6 drafts to 8192 keys, 64 heads over 8, f16, 113 to 115.
+// Measured, heads of 128: 2048 tokens over 16384 keys, 32 heads over 8, 692 to 708 us in bf16 (0.58 TFLOP, counted without
+// what is masked), 798 to 807 in f16; 8 prompts of 128 to 1024 tokens 95 to 98; 32 requests with 1 to 6 drafts to 8192
+// keys, 64 heads over 8, f16 119 to 122, bf16 133.
 #include <climits>
 
 #include "device.h"
@@ -60,7 +61,7 @@ struct CodeChunkArgs {
 
 // ROWS: of an item. Where no request has more than 128, the second tile of Q is room for two more tiles of codes on
 // their way: they are what such a call, with little to compute a key, waits for. (64 requests of 2000 keys, 8 key heads: 48
-// rows in f16 129 us with it and 148 without, 128 rows 147 and 159, 48 rows in bf16 146 and 155.)
+// rows in f16 134 us with it and 151 without, 128 rows 149 and 160, 48 rows in bf16 151 and 156.)
 template <int D, int ROWS>
 struct CodeChunkCfg {
   static constexpr int kSlot = kChunkKeys * D * 2;  // K or V of a tile

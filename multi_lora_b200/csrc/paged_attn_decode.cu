@@ -39,8 +39,9 @@
 // 1000, 8 key heads: 60 us, 4.4 TB/s.
 //
 // Over a cache of e4m3 codes the same with tiles of 128 keys (paged_codes.cuh), whose scales the producer's lanes fetch
-// beside the boxes: 96 requests of 33 to 4095 keys, 32 heads: 303 to 317 us, 5.1 to 5.3 TB/s; 4 requests of 40000 to 131071 keys, 64
-// heads over 8: 108 to 114 us, 6.2 to 6.5 TB/s; one request of 900 keys 6.5 us; with a window of 1000 as above 41.
+// beside the boxes: 96 requests of 33 to 4095 keys, 32 heads: 302 to 316 us, 5.1 to 5.3 TB/s; 4 requests of 40000 to
+// 131071 keys, 64 heads over 8: 110 to 116 us, 5.3 to 5.6 TB/s; one request of 900 keys 6.7 us; with a window of 1000 as
+// above 40.
 #include <climits>
 
 #include "device.h"
@@ -846,8 +847,8 @@ cudaError_t launch_paged_attention_decode(const PagedAttnArgs& a, int dtype, cud
   if (a.k_scale == nullptr) return launch_decode_of<kDecValues>(a, dtype, st, pdl);
   // Codes take half the bytes, so the work a key has to halve too: eight rows are the columns of a product whose
   // rows are keys, and three CTAs of it fit an SM (96 requests of 33 to 4095 keys, one row: 303 us, and 410 with sixteen rows; 64
-  // requests of 2000 keys, eight rows: 61 and 81). More than sixteen rows go to the chunk kernel (64 x 2000, sixteen rows
-  // of bf16: 88 here and 143 there; f16 96 and 126).
+  // requests of 2000 keys, eight rows: 61 and 76). More than sixteen rows go to the chunk kernel (64 x 2000, sixteen rows
+  // of bf16: 82 here and 147 there; f16 94 and 131).
   return (int64_t)a.max_q_len * a.group <= 8 ? launch_decode_of<kDecCodesFew>(a, dtype, st, pdl)
                                              : launch_decode_of<kDecCodes>(a, dtype, st, pdl);
 }
