@@ -164,8 +164,8 @@ __device__ __noinline__ void code_give_back(const PagedAttnArgs& p, uint32_t o_a
   tmem_wait_st();
 }
 
-// Sizes as whole numbers: 2^23 + 2^8 (code_log(f) + 127), and what 2^8 (x - m) and it may have as their sum: both logarithms, of f and
-// of up, are too small by at most 0.09, so a w is below 2^(kCodeTop + 0.19).
+// Sizes as whole numbers: 2^23 + 2^8 (code_log(f) + 127), and what 2^8 (x - m) and it may have as their sum: both
+// logarithms, of f and of up, are too small by at most 0.09, so a w is below 2^(kCodeTop + 0.19).
 constexpr float kCodeFine = 256.f;
 __device__ __forceinline__ float code_size(float f) { return __uint_as_float((__float_as_uint(f) >> 15) + 0x4b000000u); }
 __device__ __forceinline__ float code_size_limit(float up) {

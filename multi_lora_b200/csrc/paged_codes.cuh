@@ -194,12 +194,12 @@ __device__ __forceinline__ void code_raise(Sums& z, const float (&top)[4][2], co
   z.scale(fix[0], fix[1]);
 }
 
-// 32 keys from j0 on, at row k0 of a tile of K at `ks` and of V at `vs`; key_f, value_f: the scales of each eight of them, value_log: code_log of the latter;
-// row_f: what a row's products are multiplied by besides.
+// 32 keys from j0 on, at row k0 of a tile of K at `ks` and of V at `vs`; key_f, value_f: the scales of each eight of them,
+// value_log: code_log of the latter; row_f: what a row's products are multiplied by besides.
 template <typename T, int D>
 __device__ __forceinline__ void code_tile(CodeSums<D>& z, const uint32_t (&qf)[D / 16][4], const CodeSpan& it, uint32_t ks,
-                                          uint32_t vs, int k0, int j0, const float4& key_f, const float4& value_f, const float4& value_log,
-                                          const float (&row_f)[2]) {
+                                          uint32_t vs, int k0, int j0, const float4& key_f, const float4& value_f,
+                                          const float4& value_log, const float (&row_f)[2]) {
   constexpr bool TWO = !Num<T>::is_bf16;  // terms of P
   const int lane = threadIdx.x & 31;
   float s[4][4];
@@ -244,7 +244,8 @@ __device__ __forceinline__ void code_tile(CodeSums<D>& z, const uint32_t (&qf)[D
 #pragma unroll
     for (int n = 0; n < 4; ++n) top[n][e] = fmaxf(s[n][2 * e], s[n][2 * e + 1]);
     need[e] = fmaxf(max3(top[0][e], top[1][e], top[2][e]), top[3][e]) > z.m[e] + kCodeRaise ||
-             fmaxf(max3(top[0][e] + value_log.x, top[1][e] + value_log.y, top[2][e] + value_log.z), top[3][e] + value_log.w) > z.limit[e];
+              fmaxf(max3(top[0][e] + value_log.x, top[1][e] + value_log.y, top[2][e] + value_log.z), top[3][e] + value_log.w) >
+                  z.limit[e];
   }
   if (__any_sync(0xffffffffu, need[0] || need[1])) code_raise<1, 2>(z, top, vf4, need);
   uint32_t pf[2][4], pr[2][4];
@@ -406,8 +407,8 @@ struct CodeSumsFew {
 // As code_tile.
 template <typename T, int D>
 __device__ __forceinline__ void code_tile_few(CodeSumsFew<D>& z, const uint32_t (&qf)[D / 16][2], const CodeSpan& it, uint32_t ks,
-                                              uint32_t vs, int k0, int j0, const float4& key_f, const float4& value_f, const float4& value_log,
-                                              const float (&row_f)[2]) {
+                                              uint32_t vs, int k0, int j0, const float4& key_f, const float4& value_f,
+                                              const float4& value_log, const float (&row_f)[2]) {
   constexpr bool TWO = !Num<T>::is_bf16;
   const int lane = threadIdx.x & 31;
   // scores of keys lane / 4 (+ 8 n) for rows (lane % 4) * 2 and + 1; two chains a tile of 16 keys
